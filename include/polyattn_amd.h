@@ -474,6 +474,110 @@ typedef struct pa_attn_bwd_args {
 
 int pa_attn_bwd(const pa_attn_bwd_args* args, void* stream);
 
+/* ---- a paged cache for a batch of requests (no counterpart in the reference, which has no
+ * serving path) -------------------------------------------------------------------------
+ * K and V of a layer are n_pages pages of page_size rows (a power of two, 16 to 256) per KV
+ * head: row `off` of head h of page p is D contiguous elements at p * c_sp + h * c_sh +
+ * off * c_sn (elements, the same in k and v).  Request r's token at position t is row t %
+ * page_size of page tables[r * pitch + t / page_size]; a slot is page * page_size + row.
+ * Positions stay below 2^30 - 1, slots below 2^31.  Everything below takes sizes that change
+ * from step to step (lengths, new tokens, tables) from the device, so a step can be captured
+ * in a graph and replayed for other lengths.
+ *
+ * pa_page_tables: request r holds before[r] tokens and is to get fresh[r] more.  The pages
+ * that takes, in order of (request, page), come from the end of the free list
+ * (free_list[free_count - 1] first) and are written into tables.  lengths[r] = before[r] +
+ * fresh[r]; q_start [R + 1] = exclusive sums of fresh; row i of the packed new tokens gets
+ * its slot and (positions not NULL) its position, both -1 for rows from q_start[R] to
+ * tokens - 1; *free_left = pages still free.  *status is 0, or the sum of
+ *   1  fewer free pages than needed (or a free_count outside 0..n_pages)
+ *   2  a request longer than cols * page_size, or a negative before or fresh
+ *   4  more new tokens than rows (`tokens`)
+ * and then nothing is taken: tables stay, lengths = before, q_start is all 0, the slots and
+ * positions -1, *free_left = free_count.  lengths may be `before` and free_left may be
+ * free_count.  A token whose page is none of the cache gets slot -1.  workspace: int32 [3 R +
+ * 2].
+ *
+ * pa_page_release: pages first[r] .. last[r] - 1 of request r's table (clamped to the table;
+ * entries that are none of the cache are skipped) go back to the end of the free list in order
+ * of (request, page), and their entries become -1.  *status 0, or 1 when the list would pass
+ * n_pages (nothing is done then).  free_left may be free_count.  workspace: int32 [R].
+ *
+ * pa_paged_append: row i of k_new / v_new [T, Hkv, D] (n_st, n_sh: token and head strides in
+ * elements) is written to slot slots[i]; a slot outside the cache (-1) is skipped.  Slots are
+ * distinct.
+ *
+ * pa_paged_attn: rows q_start[r] .. q_start[r + 1] - 1 of q [T, Hq, D] are request r's newest
+ * tokens, at positions lengths[r] - n .. lengths[r] - 1.  Query head h reads KV head h / (Hq /
+ * Hkv).  o = softmax over the cached keys t < lengths[r] that are live under `mask` (evaluated
+ * at positions; any kind but PA_DENSE, perm_q / perm_kv NULL) of scale q . k_t, applied to
+ * v_t; a row with no live key gives 0 and lse -inf.  Keys that are dead for a row contribute
+ * nothing to it, whatever their K and V hold; a live key whose page is none of the cache
+ * counts as dead.  Rows of no request are left as they are.  lse may be NULL (natural log,
+ * [T, Hq] at lse_st, lse_sh).  max_fresh: the most new tokens of a request (a hint: it selects
+ * kernels and moves no result beyond rounding).  D = 64 or 128, f32 / f16 / bf16, scale > 0.
+ * workspace: the bytes pa_paged_workspace gives for the same sizes, 256-byte aligned, not
+ * shared by calls that overlap. */
+typedef struct pa_tables_args {
+  const int32_t* before;
+  const int32_t* fresh;
+  int32_t R;
+  const int32_t* free_list;
+  const int32_t* free_count;
+  int64_t n_pages;
+  int32_t page_size;
+  int32_t* tables;
+  int64_t pitch;
+  int32_t cols;
+  int64_t tokens;
+  int32_t* lengths;
+  int32_t* q_start;
+  int32_t* slots;
+  int32_t* positions;
+  int32_t* free_left;
+  int32_t* status;
+  int32_t* workspace;
+} pa_tables_args;
+
+int pa_page_tables(const pa_tables_args* args, void* stream);
+
+int pa_page_release(const int32_t* first, const int32_t* last, int32_t R, int32_t* tables, int64_t pitch, int32_t cols,
+                    int32_t* free_list, const int32_t* free_count, int64_t n_pages, int32_t* free_left, int32_t* status,
+                    int32_t* workspace, void* stream);
+
+int pa_paged_append(const void* k_new, const void* v_new, int64_t n_st, int64_t n_sh, const int32_t* slots, int64_t T,
+                    void* k, void* v, int64_t c_sp, int64_t c_sh, int64_t c_sn, int64_t n_pages, int32_t page_size,
+                    int32_t Hkv, int32_t D, int32_t dtype, void* stream);
+
+typedef struct pa_paged_args {
+  const void* q;
+  int64_t q_st, q_sh;
+  const void* k;
+  const void* v;
+  int64_t c_sp, c_sh, c_sn;
+  int64_t n_pages;
+  int32_t page_size;
+  const int32_t* tables;
+  int64_t pitch;
+  int32_t cols;
+  const int32_t* lengths;
+  const int32_t* q_start;
+  int32_t R;
+  int64_t T, max_fresh;
+  int32_t Hq, Hkv, D, dtype;
+  float scale;
+  pa_mask mask;
+  void* o;
+  int64_t o_st, o_sh;
+  float* lse;
+  int64_t lse_st, lse_sh;
+  void* workspace;
+  int64_t workspace_bytes;
+} pa_paged_args;
+
+int pa_paged_workspace(const pa_paged_args* args, int64_t* bytes);
+int pa_paged_attn(const pa_paged_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

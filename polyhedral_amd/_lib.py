@@ -14,7 +14,7 @@ LIB_PATH = pathlib.Path(__file__).resolve().parent / "_lib" / "libpolyattn_amd.s
 PA_OK, PA_E_INVALID, PA_E_HIP, PA_E_UNSUPPORTED = 0, -1, -2, -3
 PA_F32, PA_F16, PA_BF16 = 0, 1, 2
 MAX_TERMS = 8
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 c_i32, c_i64, c_f32, c_vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
@@ -74,6 +74,22 @@ class PaAttnBwdArgs(ctypes.Structure):
                 ("mask", PaMask)]
 
 
+class PaTablesArgs(ctypes.Structure):
+    _fields_ = [("before", c_vp), ("fresh", c_vp), ("R", c_i32), ("free_list", c_vp), ("free_count", c_vp),
+                ("n_pages", c_i64), ("page_size", c_i32), ("tables", c_vp), ("pitch", c_i64), ("cols", c_i32),
+                ("tokens", c_i64), ("lengths", c_vp), ("q_start", c_vp), ("slots", c_vp), ("positions", c_vp),
+                ("free_left", c_vp), ("status", c_vp), ("workspace", c_vp)]
+
+
+class PaPagedArgs(ctypes.Structure):
+    _fields_ = [("q", c_vp), ("q_st", c_i64), ("q_sh", c_i64), ("k", c_vp), ("v", c_vp), ("c_sp", c_i64),
+                ("c_sh", c_i64), ("c_sn", c_i64), ("n_pages", c_i64), ("page_size", c_i32), ("tables", c_vp),
+                ("pitch", c_i64), ("cols", c_i32), ("lengths", c_vp), ("q_start", c_vp), ("R", c_i32), ("T", c_i64),
+                ("max_fresh", c_i64), ("Hq", c_i32), ("Hkv", c_i32), ("D", c_i32), ("dtype", c_i32), ("scale", c_f32),
+                ("mask", PaMask), ("o", c_vp), ("o_st", c_i64), ("o_sh", c_i64), ("lse", c_vp), ("lse_st", c_i64),
+                ("lse_sh", c_i64), ("workspace", c_vp), ("workspace_bytes", c_i64)]
+
+
 # name -> (restype, argtypes); every symbol of include/polyattn_amd.h
 SIGNATURES = {
     "pa_last_error": (ctypes.c_char_p, []),
@@ -107,6 +123,12 @@ SIGNATURES = {
                                           c_vp]),
     "pa_index_bits_transpose": (ctypes.c_int, [c_vp, c_i32, c_i64, c_vp, c_vp, c_vp]),
     "pa_attn_bwd": (ctypes.c_int, [ctypes.POINTER(PaAttnBwdArgs), c_vp]),
+    "pa_page_tables": (ctypes.c_int, [ctypes.POINTER(PaTablesArgs), c_vp]),
+    "pa_page_release": (ctypes.c_int, [c_vp, c_vp, c_i32, c_vp, c_i64, c_i32, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp]),
+    "pa_paged_append": (ctypes.c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64,
+                                       c_i32, c_i32, c_i32, c_i32, c_vp]),
+    "pa_paged_workspace": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), ctypes.POINTER(c_i64)]),
+    "pa_paged_attn": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), c_vp]),
 }
 
 _LIB = None

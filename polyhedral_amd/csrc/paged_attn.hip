@@ -1,0 +1,123 @@
+// Attention over a paged cache: the entry points' checks, the workspace and the choice of kernels.
+#include <limits.h>
+#include <math.h>
+
+#include "paged_attn.hpp"
+
+namespace pa {
+namespace {
+
+constexpr int kTarget = 512;   // units that the splits of a call aim for
+
+struct PagedPlan {
+  int page_lg;
+  int64_t max_tiles;  // 16-row tiles of all requests, at most
+  int64_t slots;
+  int64_t part_bytes, bytes;
+};
+
+int plan_of(const pa_paged_args* x, PagedPlan* p) {
+  PA_CHECK_ARG(x, "pa_paged_attn: null arguments");
+  if (int rc = check_pages("pa_paged_attn", x->n_pages, x->page_size, &p->page_lg)) return rc;
+  PA_CHECK_ARG(x->dtype == PA_BF16 || x->dtype == PA_F16 || x->dtype == PA_F32, "pa_paged_attn: dtype %d", x->dtype);
+  PA_CHECK_ARG(x->D == 64 || x->D == 128, "pa_paged_attn: D=%d (64 or 128)", x->D);
+  PA_CHECK_ARG(x->Hkv >= 1 && x->Hq >= x->Hkv && x->Hq % x->Hkv == 0 && x->Hq <= 65535,
+               "pa_paged_attn: %d query heads and %d KV heads (a multiple, at most 65535)", x->Hq, x->Hkv);
+  PA_CHECK_ARG(x->R >= 0 && x->T >= 0 && x->T * x->Hq <= kMaxPosition, "pa_paged_attn: R=%d T=%lld Hq=%d (T Hq < 2^30)",
+               x->R, (long long)x->T, x->Hq);
+  PA_CHECK_ARG(x->max_fresh >= 0, "pa_paged_attn: max_fresh=%lld", (long long)x->max_fresh);
+  PA_CHECK_ARG(x->cols >= 0 && ((int64_t)x->cols << p->page_lg) <= kMaxPosition && x->pitch >= x->cols,
+               "pa_paged_attn: %d columns of %d, pitch %lld", x->cols, x->page_size, (long long)x->pitch);
+  PA_CHECK_ARG(x->scale > 0.f && x->scale < INFINITY, "pa_paged_attn: scale=%g must be positive", (double)x->scale);
+  const int64_t some = x->T < x->R ? x->T : x->R;  // requests with rows, at most
+  p->max_tiles = x->T * (x->Hq / x->Hkv) / 16 + some;
+  const int64_t units = kTarget + p->max_tiles * x->Hkv;
+  // (a tile is split into two shares at least, and then has less than twice the shares that its
+  // blocks fill)
+  p->slots = 2 * kTarget < units ? 2 * kTarget : units;
+  p->part_bytes = p->slots * 16 * x->D * 4;
+  p->bytes = p->part_bytes + p->slots * 16 * 2 * 4;
+  return PA_OK;
+}
+
+}  // namespace
+}  // namespace pa
+
+extern "C" int pa_paged_workspace(const pa_paged_args* x, int64_t* bytes) {
+  pa::PagedPlan p;
+  if (int rc = pa::plan_of(x, &p)) return rc;
+  PA_CHECK_ARG(bytes, "pa_paged_workspace: null output");
+  *bytes = p.bytes;
+  return PA_OK;
+}
+
+extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
+  using namespace pa;
+  PagedPlan p;
+  if (int rc = plan_of(x, &p)) return rc;
+  PA_CHECK_ARG(!x->mask.perm_q && !x->mask.perm_kv, "pa_paged_attn: the mask takes no permutation tables");
+  for (int i = 0; i < x->mask.n_include + x->mask.n_exclude && i < PA_MAX_TERMS; ++i)
+    PA_CHECK_ARG(x->mask.terms[i].kind != PA_DENSE, "pa_paged_attn: PA_DENSE has no meaning here");
+  if (int rc = check_mask(&x->mask, 0)) return rc;
+  if (x->R == 0 || x->T == 0) return PA_OK;
+  PA_CHECK_ARG(x->q && x->o && x->lengths && x->q_start, "pa_paged_attn: null q / o / lengths / q_start");
+  PA_CHECK_ARG(x->cols == 0 || x->tables, "pa_paged_attn: null tables");
+  PA_CHECK_ARG(x->n_pages == 0 || (x->k && x->v), "pa_paged_attn: null k / v");
+  const int64_t esz = x->dtype == PA_F32 ? 4 : 2;
+  auto al = [&](const void* q, int64_t s0, int64_t s1, int64_t s2) {
+    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (s0 * esz) % 16 == 0 && (s1 * esz) % 16 == 0 && (s2 * esz) % 16 == 0;
+  };
+  PA_CHECK_ARG(al(x->q, x->q_st, x->q_sh, 0) && al(x->o, x->o_st, x->o_sh, 0) && al(x->k, x->c_sp, x->c_sh, x->c_sn) &&
+                   al(x->v, x->c_sp, x->c_sh, x->c_sn),
+               "pa_paged_attn: rows must be 16-byte aligned");
+  PA_CHECK_ARG(x->q_st >= 0 && x->q_sh >= 0 && x->o_st >= 0 && x->o_sh >= 0 && x->c_sp >= 0 && x->c_sh >= 0 &&
+                   x->c_sn >= x->D && x->c_sn <= (1 << 21),
+               "pa_paged_attn: negative strides, or cache rows closer than D or further than 2^21");
+  PA_CHECK_ARG(x->workspace && reinterpret_cast<uintptr_t>(x->workspace) % 256 == 0 && x->workspace_bytes >= p.bytes,
+               "pa_paged_attn: needs a 256-byte aligned workspace of %lld bytes", (long long)p.bytes);
+  PagedK a;
+  a.q = static_cast<const char*>(x->q);
+  a.q_st = x->q_st * esz;
+  a.q_sh = x->q_sh * esz;
+  a.k = static_cast<const char*>(x->k);
+  a.v = static_cast<const char*>(x->v);
+  a.c_sp = x->c_sp * esz;
+  a.c_sh = x->c_sh * esz;
+  a.c_sn = x->c_sn * esz;
+  a.n_pages = x->n_pages;
+  a.page_lg = p.page_lg;
+  a.cols = x->cols;
+  a.tables = x->tables;
+  a.pitch = x->pitch;
+  a.lengths = x->lengths;
+  a.q_start = x->q_start;
+  a.R = x->R;
+  a.T = (int32_t)x->T;
+  a.Hkv = x->Hkv;
+  a.G = x->Hq / x->Hkv;
+  a.c = x->scale * 1.4426950408889634f;
+  a.mask.n_include = x->mask.n_include;
+  a.mask.n_exclude = x->mask.n_exclude;
+  for (int i = 0; i < PA_MAX_TERMS; ++i) {
+    pa_term t = x->mask.terms[i];
+    // (no distance reaches the clamp)
+    t.p0 = imin(t.p0, kMaxPosition);
+    t.p1 = imin(t.p1, kMaxPosition);
+    t.p2 = imin(t.p2, kMaxPosition);
+    a.mask.terms[i] = t;
+  }
+  a.o = static_cast<char*>(x->o);
+  a.o_st = x->o_st * esz;
+  a.o_sh = x->o_sh * esz;
+  a.lse = x->lse;
+  a.lse_st = x->lse_st;
+  a.lse_sh = x->lse_sh;
+  a.part_o = static_cast<float*>(x->workspace);
+  a.part_ml = reinterpret_cast<float*>(static_cast<char*>(x->workspace) + p.part_bytes);
+  a.slots = (int32_t)p.slots;
+  a.target = kTarget;
+  a.least = 8;
+  a.row_min = 0;
+  a.row_max = INT_MAX;
+  return launch_paged_rows(a, x->dtype, x->D, p.max_tiles, static_cast<hipStream_t>(stream));
+}

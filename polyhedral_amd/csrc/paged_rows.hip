@@ -1,0 +1,529 @@
+// Attention of few query rows over a paged cache: tiles of 16 rows (single tokens, drafts; every
+// float32 call), the keys split over work-groups and over their four waves.
+//
+// With S^T = K Q^T on 16x16 MFMAs lane (q = l % 16, g = l / 16) holds scores of keys 4 g + 0..3
+// of a 16-key segment for row q, and P^T is in its registers as the B operand of O^T += V^T P^T.
+//  * f16 / bf16: a wave's step is 32 keys (two segments, 16x16x32).  K rows go straight into the
+//    A operand's registers, V rows by LDS DMA into the wave's own two-stage ring, from which
+//    transposed reads take V^T (swizzled 16-byte units, as in attn_narrow.hip).
+//  * f32: a step is 16 keys (16x16x4).  Contraction index g of the j-th product of a segment is
+//    element 4 g + j for the scores and key 4 g + j for the sums, so K is read 16 bytes a lane and
+//    V 4, both straight into registers.
+// Each wave takes every fourth block of the unit's share, its loads a step ahead of its products,
+// with nothing shared between waves until the end.  Segments never straddle pages (a page is a
+// multiple of 16 rows), so a segment is one 64-bit offset.
+//
+// Scores, maxima, sums and O are float32; P is rounded to 16 bits as an MFMA operand only, its
+// sum taken before.
+//
+// A dead key contributes nothing whatever its K and V hold: its score is replaced by -inf, and
+// where a step is masked for some row and its V rows hold an infinity or NaN, the products are
+// taken key by key and added to the rows that the key is live for (a product with a zero would be
+// NaN).
+#include <math.h>
+
+#include <type_traits>
+
+#include "paged_attn.hpp"
+
+namespace pa {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ f32x4 mma16x32(typename Mma<T>::frag a, typename Mma<T>::frag b, f32x4 c) {
+  if constexpr (__is_same(T, __bf16))
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16x4(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// max / sum over the four lanes l % 16 + 16 g that hold one query row
+__device__ __forceinline__ float quad_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(int, x), __builtin_bit_cast(int, x), false, false);
+  return row_nan_max(nan_max(__builtin_bit_cast(float, (int)r[0]), __builtin_bit_cast(float, (int)r[1])));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(int, x), __builtin_bit_cast(int, x), false, false);
+  return row_sum(__builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]));
+}
+
+constexpr int kRows = 16;   // query rows of a tile
+constexpr int kWaves = 4;
+
+// The maximum m of a row's scores so far as the base of its exponentials: 0 for -inf (no live key
+// so far; every score is -inf then).  Maxima are kept unscaled and p = exp2((x - m) c): a maximum
+// that is rounded after its scaling would leave its own p at any power of two where scores are huge.
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+// Bits of the words that hold an infinity or NaN in some half (f16 / bf16): the largest magnitude
+// of each half against the type's first one that is not finite.
+template <typename T>
+struct Finite16 {
+  uint32_t lo = 0u, hi = 0u;
+  __device__ void add(uint32_t w) {
+    lo = max(lo, w & 0x7fffu);
+    hi = max(hi, w & 0x7fff0000u);
+  }
+  __device__ bool all() const {
+    constexpr uint32_t inf = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+    return lo < inf && hi < (inf << 16);
+  }
+};
+
+template <typename T, int D>
+struct RowsShape {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int NS = F32 ? 1 : 2;           // 16-key segments of a step
+  static constexpr int LG = F32 ? 4 : 5;           // log2 keys of a step
+  static constexpr int PER = 64 / NS;              // steps held at a time, a segment per lane
+  static constexpr int ROW = D * (int)sizeof(T);   // bytes of a row
+  static constexpr int RING = F32 ? 0 : kWaves * 2 * 2 * 16 * ROW;
+  static constexpr int OP = D + 4;                 // floats of a row of a wave's O at the end
+  static constexpr int ENDS = kWaves * kRows * (OP + 2) * 4;
+  static constexpr int SMEM = RING > ENDS ? RING : ENDS;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2)))
+void paged_rows_kernel(const PagedK a) {
+  using S = RowsShape<T, D>;
+  constexpr bool F32 = S::F32;
+  constexpr int NS = S::NS, PER = S::PER, ROW = S::ROW, ESZ = sizeof(T);
+  constexpr int NB = D / 16;                       // blocks of 16 output columns
+  constexpr int NK = F32 ? D / 16 : D / 32;        // 16-byte units of a K or Q row that a lane holds
+  constexpr int SEG = 16 * ROW, STAGE = 2 * SEG;
+
+  __shared__ __attribute__((aligned(256))) char smem[S::SMEM];
+
+  const int tid = threadIdx.x, lane = tid & 63, q16 = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  const Unit u = find_unit<kRows, S::LG, false>(a, (int32_t)blockIdx.x, lane);
+  if (!u.found) return;
+
+  // ---- the tile's rows -----------------------------------------------------------
+  const int rows = u.rq.n * a.G;
+  const int i0 = u.tile * kRows;
+  const int n_rows = imin(rows - i0, kRows);
+  const int i = imin(i0 + q16, rows - 1);          // (a lane past the rows repeats the last)
+  const int tok = i / a.G, head = u.h * a.G + (i - tok * a.G);
+  const int pos0 = u.rq.len - u.rq.n;
+  const int q_pos = pos0 + tok;
+  const int q_lo = pos0 + i0 / a.G, q_hi = pos0 + (i0 + n_rows - 1) / a.G;
+  const int len = u.rq.len;
+
+  u32x4 qf[NK];
+  {
+    const char* qrow = a.q + (int64_t)(u.rq.start + tok) * a.q_st + (int64_t)head * a.q_sh + 16 * g;
+#pragma unroll
+    for (int kc = 0; kc < NK; ++kc) qf[kc] = *reinterpret_cast<const u32x4*>(qrow + 64 * kc);
+  }
+
+  // ---- the keys of this share ------------------------------------------------------
+  const KeyList kl = key_list(a.mask, q_lo, q_hi, len, S::LG);
+  int32_t j0, j1;
+  share_of(kl.count(), u.split, u.splits, &j0, &j1);
+  const int n_steps = j1 - j0 > w ? (j1 - j0 - w + kWaves - 1) / kWaves : 0;
+  const int32_t* table = a.tables + (int64_t)u.r * a.pitch;
+  const char* kbase = a.k + u.h * a.c_sh;
+  const char* vbase = a.v + u.h * a.c_sh;
+
+  // PER steps at a time: lane l holds segment l, its first key and its offset in the cache; bit l
+  // of live / full: some pair of it may be live / all are.  The next ones' pages are loaded
+  // halfway through these.
+  int32_t c_key = 0, r_page = -1;
+  int64_t c_off = 0;
+  uint64_t c_live = 0ull, c_full = 0ull;
+  auto key_of = [&](int c) __attribute__((always_inline)) -> int32_t {
+    const int st = c * PER + lane / NS;
+    return st < n_steps ? (kl.block(j0 + w + kWaves * st) << S::LG) + (NS == 2 ? 16 * (lane & 1) : 0) : len;
+  };
+  auto load_raw = [&](int c) __attribute__((always_inline)) {
+    const int32_t key = key_of(c);
+    r_page = key < len ? table[key >> a.page_lg] : -1;
+  };
+  auto take_raw = [&](int c) __attribute__((always_inline)) {
+    const int32_t key = key_of(c);
+    const int32_t page = checked_page(r_page, a.n_pages);
+    int v = kDead;
+    if (key < len && page >= 0) {
+      v = mask_verdict(a.mask, q_lo, q_hi, key, key + 15);
+      if (v == kFull && key + 15 >= len) v = kPartial;
+    }
+    c_live = __ballot(v != kDead);
+    c_full = __ballot(v == kFull);
+    c_key = key;
+    c_off = (int64_t)imax(page, 0) * a.c_sp + (int64_t)(key & ((1 << a.page_lg) - 1)) * a.c_sn;
+    if constexpr (NS == 2) {
+      // (a dead segment of a live step holds the other one's rows again)
+      const bool dead = !((c_live >> lane) & 1ull);
+      const int32_t lo = __shfl_xor((int32_t)c_off, 1), hi = __shfl_xor((int32_t)(c_off >> 32), 1);
+      if (dead) c_off = (int64_t)((uint64_t)(uint32_t)lo | ((uint64_t)(uint32_t)hi << 32));
+    }
+  };
+
+  const uint32_t koff = (uint32_t)(q16 * (int32_t)a.c_sn) + 16u * (uint32_t)g;
+  uint32_t voff[F32 ? 4 : Rows<D>::NI];
+  if constexpr (F32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) voff[j] = (uint32_t)((4 * g + j) * (int32_t)a.c_sn) + 4u * (uint32_t)q16;
+  } else {
+    using R = Rows<D>;
+#pragma unroll
+    for (int j = 0; j < R::NI; ++j) {
+      const int r = R::RPI * j + lane / R::UPR;
+      const int sw = D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
+      voff[j] = (uint32_t)(r * (int32_t)a.c_sn) + 16u * (uint32_t)((lane % R::UPR) ^ sw);
+    }
+  }
+  const uint32_t ring0 = (uint32_t)(uintptr_t)(lds_char_t*)smem + (uint32_t)(w * 2 * STAGE);
+  lds_cptr vptr[F32 ? 1 : NB];
+  if constexpr (!F32) {
+    // transposed reads of 16 columns (block db) of rows 4 g + q16 / 4 of a segment
+#pragma unroll
+    for (int db = 0; db < NB; ++db) {
+      const int r = 4 * g + (q16 >> 2);
+      const int sw = D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
+      vptr[db] = (lds_cptr)smem + w * 2 * STAGE + r * ROW + 16 * ((2 * db + ((q16 & 3) >> 1)) ^ sw) + 8 * (q16 & 1);
+      asm volatile("" : "+v"(vptr[db]));
+    }
+  }
+
+  struct Step {
+    int key;
+    uint32_t live, full;  // NS bits each
+  };
+  struct Data {  // what a step needs in registers
+    u32x4 k[NS][NK];
+    float v[F32 ? 4 : 1][F32 ? NB : 1];
+  };
+  auto prefetch = [&](int st, int SB, Step& s, Data& d) __attribute__((always_inline)) {
+    if (st % PER == 0) take_raw(st / PER);
+    if (st % PER == PER / 2) load_raw(st / PER + 1);
+    const int l0 = NS * (st % PER);
+    s.live = (uint32_t)(c_live >> l0) & ((1u << NS) - 1u);
+    s.full = (uint32_t)(c_full >> l0) & ((1u << NS) - 1u);
+    s.key = __builtin_amdgcn_readlane(c_key, l0);
+    if (s.live == 0u) return;
+#pragma unroll
+    for (int t = 0; t < NS; ++t) {
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)c_off, l0 + t);
+      const int32_t hi = __builtin_amdgcn_readlane((int)(c_off >> 32), l0 + t);
+      const int64_t off = (int64_t)((uint64_t)lo | ((uint64_t)(uint32_t)hi << 32));
+      const char* kp = kbase + off;
+      const char* vp = vbase + off;
+#pragma unroll
+      for (int kc = 0; kc < NK; ++kc) d.k[t][kc] = *reinterpret_cast<const u32x4*>(kp + koff + 64 * kc);
+      if constexpr (F32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int db = 0; db < NB; ++db) d.v[j][db] = *reinterpret_cast<const float*>(vp + voff[j] + 64 * db);
+      } else {
+#pragma unroll
+        for (int j = 0; j < Rows<D>::NI; ++j) dma_x4(ring0 + SB * STAGE + t * SEG + j * 1024, vp, voff[j]);
+      }
+    }
+  };
+
+  f32x4 acc[NB];
+#pragma unroll
+  for (int db = 0; db < NB; ++db) acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY, l_part = 0.f;
+
+  auto compute = [&](int SB, const Step& s, const Data& d) __attribute__((always_inline)) {
+    if (s.live == 0u) return;
+    constexpr uint32_t ALL = (1u << NS) - 1u;
+    f32x4 x[NS];
+#pragma unroll
+    for (int t = 0; t < NS; ++t) {
+      x[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kc = 0; kc < NK; ++kc) {
+        if constexpr (F32) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t kx = d.k[t][kc][j], qx = qf[kc][j];
+            x[t] = mma16x4(__builtin_bit_cast(float, kx), __builtin_bit_cast(float, qx), x[t]);
+          }
+        } else {
+          using Frag = typename Mma<T>::frag;
+          x[t] = mma16x32<T>(__builtin_bit_cast(Frag, d.k[t][kc]), __builtin_bit_cast(Frag, qf[kc]), x[t]);
+        }
+      }
+    }
+    uint32_t word = 0xffffffffu;  // the step's keys live for this lane's row
+    if (s.full != ALL) {
+      word = mask_word(a.mask, q_pos, s.key, len);
+      if (!(s.live & 1u)) word &= 0xffff0000u;
+      if (NS == 1 || !(s.live & 2u)) word &= 0x0000ffffu;
+#pragma unroll
+      for (int t = 0; t < NS; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!((word >> (16 * t + 4 * g + e)) & 1u)) x[t][e] = -INFINITY;
+    }
+    float mx = nan_max(nan_max(x[0][0], x[0][1]), nan_max(x[0][2], x[0][3]));
+    if constexpr (NS == 2) mx = nan_max(mx, nan_max(nan_max(x[1][0], x[1][1]), nan_max(x[1][2], x[1][3])));
+    const float m_new = nan_max(m_run, quad_max(mx));
+    // (a NaN maximum makes the row NaN by its own probabilities; nothing needs a rescale)
+    if (__ballot((m_new - m_run) * a.c > kLazy) != 0ull) {
+      const float alpha = __builtin_amdgcn_exp2f((m_run - base_of(m_new)) * a.c);
+      m_run = m_new;
+      l_part *= alpha;
+#pragma unroll
+      for (int db = 0; db < NB; ++db) acc[db] *= alpha;
+    }
+    const float m_base = base_of(m_run);
+    float p[4 * NS];
+#pragma unroll
+    for (int e = 0; e < 4 * NS; ++e) {
+      p[e] = __builtin_amdgcn_exp2f((x[e >> 2][e & 3] - m_base) * a.c);
+      l_part += p[e];
+    }
+    if constexpr (F32) {
+      bool fin = true;
+      if (s.full != ALL) {
+        float big = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int db = 0; db < NB; ++db) big = nan_max(big, __builtin_fabsf(d.v[j][db]));
+        fin = __ballot(!(big < INFINITY)) == 0ull;
+      }
+      if (fin) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int db = 0; db < NB; ++db) acc[db] = mma16x4(d.v[j][db], p[j], acc[db]);
+      } else {
+#pragma unroll 1
+        for (int gg = 0; gg < 4; ++gg)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool on = (word >> (4 * gg + j)) & 1u;
+#pragma unroll
+            for (int db = 0; db < NB; ++db) {
+              const f32x4 y = mma16x4(g == gg ? d.v[j][db] : 0.f, g == gg ? p[j] : 0.f, f32x4{0.f, 0.f, 0.f, 0.f});
+              if (on) acc[db] += y;
+            }
+          }
+      }
+    } else {
+      using Frag = typename Mma<T>::frag;
+      f32x8 pv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pv[e] = p[e];
+      const Frag pf = Mma<T>::cvt(pv);
+      auto v_frag = [&](int db) __attribute__((always_inline)) -> u32x4 {
+        const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vptr[db] + SB * STAGE));
+        const s16x4 x2 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vptr[db] + SB * STAGE + SEG));
+        return u32x4{__builtin_bit_cast(uint2, x1).x, __builtin_bit_cast(uint2, x1).y, __builtin_bit_cast(uint2, x2).x,
+                     __builtin_bit_cast(uint2, x2).y};
+      };
+      bool fin = true;
+      if (s.full != ALL) {
+        Finite16<T> f;
+#pragma unroll
+        for (int db = 0; db < NB; ++db) {
+          const u32x4 vx = v_frag(db);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f.add(vx[e]);
+        }
+        fin = __ballot(!f.all()) == 0ull;
+      }
+      if (fin) {
+#pragma unroll
+        for (int db = 0; db < NB; ++db) acc[db] = mma16x32<T>(__builtin_bit_cast(Frag, v_frag(db)), pf, acc[db]);
+      } else {
+        // key x of segment t is contraction index 4 t + x % 4 of lane group x / 4
+        const u32x4 pw = __builtin_bit_cast(u32x4, pf);
+#pragma unroll 1
+        for (int key = 0; key < 32; ++key) {
+          const int e = 4 * (key >> 4) + (key & 3), gg = (key >> 2) & 3;
+          const uint32_t half = g == gg ? ((e & 1) ? 0xffff0000u : 0x0000ffffu) : 0u;
+          u32x4 keep;
+#pragma unroll
+          for (int z = 0; z < 4; ++z) keep[z] = z == (e >> 1) ? half : 0u;
+          const bool on = (word >> key) & 1u;
+#pragma unroll
+          for (int db = 0; db < NB; ++db) {
+            const f32x4 y = mma16x32<T>(__builtin_bit_cast(Frag, v_frag(db) & keep), __builtin_bit_cast(Frag, pw & keep),
+                                        f32x4{0.f, 0.f, 0.f, 0.f});
+            if (on) acc[db] += y;
+          }
+        }
+      }
+    }
+  };
+
+  Step s0{}, s1{};
+  Data d0{}, d1{};
+  // The step's V rows are in LDS and its K rows in registers once everything issued is done.
+  // The memory clobber keeps the ring's reads on their side of the wait (no barrier does),
+  // and the last step's are done before the next DMA into their stage; the uses make the
+  // compiler's own wait fall here, before the next step's loads.
+  auto arrive = [&](const Data& d) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < NS; ++t)
+#pragma unroll
+      for (int kc = 0; kc < NK; ++kc) asm volatile("" ::"v"(d.k[t][kc]));
+    if constexpr (F32) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int db = 0; db < NB; ++db) asm volatile("" ::"v"(d.v[j][db]));
+    }
+    asm volatile("" ::"v"(r_page));
+  };
+  if (n_steps > 0) {
+    load_raw(0);
+    prefetch(0, 0, s0, d0);
+  }
+  int st = 0;
+  for (; st + 1 < n_steps; st += 2) {
+    arrive(d0);
+    prefetch(st + 1, 1, s1, d1);
+    compute(0, s0, d0);
+    arrive(d1);
+    if (st + 2 < n_steps) prefetch(st + 2, 0, s0, d0);
+    compute(1, s1, d1);
+  }
+  if (st < n_steps) {
+    arrive(d0);
+    compute(0, s0, d0);
+  }
+
+  // ---- the waves' states become one ------------------------------------------------
+  const float l_own = quad_sum(l_part);
+  __syncthreads();  // every wave is past its ring
+  float* red_o = reinterpret_cast<float*>(smem);                 // [wave][row][OP]
+  float* red_ml = red_o + kWaves * kRows * S::OP;                // [wave][row][2]
+#pragma unroll
+  for (int db = 0; db < NB; ++db)
+    *reinterpret_cast<f32x4*>(red_o + (w * kRows + q16) * S::OP + 16 * db + 4 * g) = acc[db];
+  if (g == 0) {
+    red_ml[2 * (w * kRows + q16)] = m_run;
+    red_ml[2 * (w * kRows + q16) + 1] = l_own;
+  }
+  __syncthreads();
+  // thread: a row and D / 16 of its columns
+  constexpr int CPT = D / 16;
+  const int row = tid >> 4, c0 = (tid & 15) * CPT;
+  if (row >= n_rows) return;
+  float mw[kWaves], M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int x = 0; x < kWaves; ++x) {
+    mw[x] = red_ml[2 * (x * kRows + row)];
+    M = nan_max(M, mw[x]);
+  }
+  float out[CPT];
+#pragma unroll
+  for (int e = 0; e < CPT; ++e) out[e] = 0.f;
+#pragma unroll
+  for (int x = 0; x < kWaves; ++x) {
+    const float f = __builtin_amdgcn_exp2f((mw[x] - base_of(M)) * a.c);
+    L += f * red_ml[2 * (x * kRows + row) + 1];
+#pragma unroll
+    for (int e = 0; e < CPT; ++e) out[e] += f * red_o[(x * kRows + row) * S::OP + c0 + e];
+  }
+  if (u.splits > 1) {
+    if (u.slot >= a.slots) return;  // (not reached by starts in order)
+    float* po = a.part_o + ((int64_t)u.slot * kRows + row) * D + c0;
+#pragma unroll
+    for (int e = 0; e < CPT; e += 4) *reinterpret_cast<f32x4*>(po + e) = f32x4{out[e], out[e + 1], out[e + 2], out[e + 3]};
+    if (c0 == 0) {
+      float* ml = a.part_ml + 2 * ((int64_t)u.slot * kRows + row);
+      ml[0] = M;
+      ml[1] = L;
+    }
+    return;
+  }
+  const int ir = i0 + row, t_r = ir / a.G, h_r = u.h * a.G + (ir - t_r * a.G);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  char* orow = a.o + (int64_t)(u.rq.start + t_r) * a.o_st + (int64_t)h_r * a.o_sh;
+#pragma unroll
+  for (int e = 0; e < CPT; e += 4)
+    Mma<T>::store4(orow + (c0 + e) * ESZ, f32x4{out[e], out[e + 1], out[e + 2], out[e + 3]} * inv);
+  if (a.lse && c0 == 0)
+    a.lse[(int64_t)(u.rq.start + t_r) * a.lse_st + (int64_t)h_r * a.lse_sh] = L == 0.f ? -INFINITY : (M * a.c + log2f(L)) * kLn2;
+}
+
+// The shares of a split tile become its rows: a wave per row, a share's maximum and sum per lane
+// for the weights, then the shares' rows, lanes along the columns.  The order of the sums is that of
+// the shares.
+template <typename T, int D, int LG>
+__global__ __launch_bounds__(64 * kRows) void paged_merge_kernel(const PagedK a) {
+  constexpr int CPL = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int row = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Unit u = find_unit<kRows, LG, true>(a, (int32_t)blockIdx.x, lane);
+  if (!u.found || u.slot + u.splits > a.slots) return;
+  const int ir = u.tile * kRows + row;
+  if (ir >= u.rq.n * a.G) return;
+  typedef float fv __attribute__((ext_vector_type(CPL)));
+  const float* ml = a.part_ml + 2 * ((int64_t)u.slot * kRows + row);
+  const float* po = a.part_o + ((int64_t)u.slot * kRows + row) * D + CPL * lane;
+  float M = -INFINITY, L = 0.f;
+  for (int s = lane; s < u.splits; s += 64) M = nan_max(M, ml[(int64_t)s * 2 * kRows]);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) M = nan_max(M, __shfl_xor(M, o));
+  fv out = {};
+  for (int s0 = 0; s0 < u.splits; s0 += 64) {
+    const int s = s0 + lane;
+    float f = 0.f;
+    if (s < u.splits) {
+      f = __builtin_amdgcn_exp2f((ml[(int64_t)s * 2 * kRows] - base_of(M)) * a.c);
+      L += f * ml[(int64_t)s * 2 * kRows + 1];
+    }
+    const int n = imin(u.splits - s0, 64);
+    for (int b = 0; b < n; b += 16) {
+      fv x[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        x[e] = b + e < n ? *reinterpret_cast<const fv*>(po + (int64_t)(s0 + b + e) * kRows * D) : fv{};
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        out += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), (b + e) & 63)) * x[e];
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) L += __shfl_xor(L, o);
+  const int tok = ir / a.G, head = u.h * a.G + (ir - tok * a.G);
+  out *= L == 0.f ? 0.f : 1.f / L;
+  T* orow = reinterpret_cast<T*>(a.o + (int64_t)(u.rq.start + tok) * a.o_st + (int64_t)head * a.o_sh) + CPL * lane;
+#pragma unroll
+  for (int e = 0; e < CPL; ++e) orow[e] = (T)out[e];
+  if (a.lse && lane == 0)
+    a.lse[(int64_t)(u.rq.start + tok) * a.lse_st + (int64_t)head * a.lse_sh] = L == 0.f ? -INFINITY : (M * a.c + log2f(L)) * kLn2;
+}
+
+template <typename T, int D>
+int launch_rows_t(const PagedK& a, int64_t max_tiles, hipStream_t s) {
+  // (units: at most target, and one more for every tile and KV head)
+  const int64_t grid = a.target + max_tiles * a.Hkv;
+  PA_CHECK_ARG(grid <= 0x7fffffffll, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)grid);
+  hipLaunchKernelGGL((paged_rows_kernel<T, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
+  PA_LAUNCH_CHECK("paged_rows_kernel");
+  // (a split tile has two shares at least)
+  const int64_t groups = max_tiles * a.Hkv < a.target ? max_tiles * a.Hkv : a.target;
+  hipLaunchKernelGGL((paged_merge_kernel<T, D, RowsShape<T, D>::LG>), dim3((unsigned)groups), dim3(64 * kRows), 0, s, a);
+  PA_LAUNCH_CHECK("paged_merge_kernel");
+  return PA_OK;
+}
+
+}  // namespace
+
+int launch_paged_rows(PagedK a, int dtype, int D, int64_t max_tiles, hipStream_t s) {
+  if (dtype == PA_BF16)
+    return D == 64 ? launch_rows_t<__bf16, 64>(a, max_tiles, s) : launch_rows_t<__bf16, 128>(a, max_tiles, s);
+  if (dtype == PA_F16)
+    return D == 64 ? launch_rows_t<_Float16, 64>(a, max_tiles, s) : launch_rows_t<_Float16, 128>(a, max_tiles, s);
+  return D == 64 ? launch_rows_t<float, 64>(a, max_tiles, s) : launch_rows_t<float, 128>(a, max_tiles, s);
+}
+
+}  // namespace pa
