@@ -50,6 +50,19 @@ struct TileReads {
     asm volatile("v_xor_b32 %0, 0x80, %1" : "=v"(x) : "v"((uint32_t)(uintptr_t)p));
     return (lds_cptr)(uintptr_t)x;
   }
+  // The reads of the other of two slots SLOT bytes apart (a power of two, the pair aligned to both).
+  template <int SLOT>
+  __device__ __forceinline__ void turn_rows() {
+#pragma unroll
+    for (int i = 0; i < NR; ++i) row_[i] = (lds_cptr)(uintptr_t)((uint32_t)(uintptr_t)row_[i] ^ SLOT);
+  }
+  template <int SLOT>
+  __device__ __forceinline__ void turn_tr() {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) tr_[i][s] = (lds_cptr)(uintptr_t)((uint32_t)(uintptr_t)tr_[i][s] ^ SLOT);
+  }
   __device__ __forceinline__ lds_cptr row(int kc) const { return kc < NR ? row_[kc] : flip(row_[kc - NR]); }
   __device__ __forceinline__ lds_cptr tr(int db, int s) const { return db < NT ? tr_[db][s] : flip(tr_[db - NT][s]); }
 };

@@ -20,10 +20,14 @@ namespace pa {
 
 constexpr int32_t kMaxPosition = (1 << 30) - 1;  // positions and lengths stay at or below it
 
-// The terms of a pa_mask without tables.
+// The terms of a pa_mask without tables.  They are walked in rolled loops through a pointer (on the
+// device one into the kernel's arguments, read by scalar loads): one copy of each term's code, and
+// no registers held for terms that are not there.
+template <typename Ptr>
 struct PageMask {
   int32_t n_include, n_exclude;
-  pa_term terms[PA_MAX_TERMS];
+  Ptr terms;
+  PA_HD pa_term term(int i) const { return pa_term{terms[i].kind, terms[i].p0, terms[i].p1, terms[i].p2}; }
 };
 
 enum Verdict { kDead = 0, kPartial = 1, kFull = 2 };
@@ -65,19 +69,17 @@ PA_HD int term_verdict(const pa_term& t, int32_t q0, int32_t q1, int32_t k0, int
   }
 }
 
-// The mask on the same pairs.  (Unrolled over the fixed capacity: a runtime index would put a
-// kernel's argument block into scratch memory.)
-PA_HD int mask_verdict(const PageMask& m, int32_t q0, int32_t q1, int32_t k0, int32_t k1) {
+// The mask on the same pairs.
+template <typename Ptr>
+PA_HD int mask_verdict(const PageMask<Ptr>& m, int32_t q0, int32_t q1, int32_t k0, int32_t k1) {
   int inc = kDead, exc = kDead;
-#pragma unroll
-  for (int i = 0; i < PA_MAX_TERMS; ++i) {
-    if (i < m.n_include + m.n_exclude) {
-      const int v = term_verdict(m.terms[i], q0, q1, k0, k1);
-      if (i < m.n_include)
-        inc = imax(inc, v);
-      else
-        exc = imax(exc, v);
-    }
+#pragma unroll 1
+  for (int i = 0; i < m.n_include + m.n_exclude; ++i) {
+    const int v = term_verdict(m.term(i), q0, q1, k0, k1);
+    if (i < m.n_include)
+      inc = imax(inc, v);
+    else
+      exc = imax(exc, v);
   }
   if (inc == kDead || exc == kFull) return kDead;
   return exc == kDead ? inc : (int)kPartial;
@@ -125,17 +127,16 @@ PA_HD uint32_t term_word(const pa_term& t, int32_t q, int32_t k0) {
 }
 
 // Bit b: key k0 + b is cached (below len) and live for query q.
-PA_HD uint32_t mask_word(const PageMask& m, int32_t q, int32_t k0, int32_t len) {
+template <typename Ptr>
+PA_HD uint32_t mask_word(const PageMask<Ptr>& m, int32_t q, int32_t k0, int32_t len) {
   uint32_t inc = 0u, exc = 0u;
-#pragma unroll
-  for (int i = 0; i < PA_MAX_TERMS; ++i) {
-    if (i < m.n_include + m.n_exclude) {
-      const uint32_t w = term_word(m.terms[i], q, k0);
-      if (i < m.n_include)
-        inc |= w;
-      else
-        exc |= w;
-    }
+#pragma unroll 1
+  for (int i = 0; i < m.n_include + m.n_exclude; ++i) {
+    const uint32_t w = term_word(m.term(i), q, k0);
+    if (i < m.n_include)
+      inc |= w;
+    else
+      exc |= w;
   }
   return inc & ~exc & range_word(0, len, k0);
 }
@@ -149,38 +150,37 @@ struct KeyList {
   PA_HD int32_t block(int32_t j) const { return j < low ? j : first + j - low; }
 };
 
-PA_HD KeyList key_list(const PageMask& m, int32_t q0, int32_t q1, int32_t len, int lg) {
+template <typename Ptr>
+PA_HD KeyList key_list(const PageMask<Ptr>& m, int32_t q0, int32_t q1, int32_t len, int lg) {
   int32_t a = 0, b = len, e = 0;  // [0, a) and [b, e)
   const int32_t qc = imax(q0, 0);  // (a query before the first token sees what none of these adds)
-#pragma unroll
-  for (int i = 0; i < PA_MAX_TERMS; ++i) {
-    if (i < m.n_include) {
-      const pa_term& t = m.terms[i];
-      int32_t lo = 0, hi = q1 + 1;
-      switch (t.kind) {
-        case PA_WINDOW:
-          lo = qc - t.p0 + 1;
-          break;
-        case PA_SINKS:
-          lo = qc - t.p0 + 1;
-          a = imax(a, imin(t.p1, hi));
-          break;
-        case PA_TWOBAND:
-          lo = qc - imax(t.p0, t.p2 > 0 ? t.p1 + t.p2 : 0) + 1;
-          break;
-        case PA_PREFIX_LM:
-          if (q0 < t.p0) hi = imax(hi, t.p0);
-          break;
-        case PA_FULL:
-          hi = len;
-          break;
-        default:
-          break;
-      }
-      if (lo < hi) {
-        b = imin(b, imax(lo, 0));
-        e = imax(e, hi);
-      }
+#pragma unroll 1
+  for (int i = 0; i < m.n_include; ++i) {
+    const pa_term t = m.term(i);
+    int32_t lo = 0, hi = q1 + 1;
+    switch (t.kind) {
+      case PA_WINDOW:
+        lo = qc - t.p0 + 1;
+        break;
+      case PA_SINKS:
+        lo = qc - t.p0 + 1;
+        a = imax(a, imin(t.p1, hi));
+        break;
+      case PA_TWOBAND:
+        lo = qc - imax(t.p0, t.p2 > 0 ? t.p1 + t.p2 : 0) + 1;
+        break;
+      case PA_PREFIX_LM:
+        if (q0 < t.p0) hi = imax(hi, t.p0);
+        break;
+      case PA_FULL:
+        hi = len;
+        break;
+      default:
+        break;
+    }
+    if (lo < hi) {
+      b = imin(b, imax(lo, 0));
+      e = imax(e, hi);
     }
   }
   a = imin(imax(a, 0), len);

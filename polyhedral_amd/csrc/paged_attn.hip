@@ -8,13 +8,32 @@ namespace pa {
 namespace {
 
 constexpr int kTarget = 512;   // units that the splits of a call aim for
+constexpr int kFewRows = 32;   // rows of a request (new tokens times heads of a group) up to which
+                               // the 16-row kernel takes it
+
+struct Part {           // one kernel's share of a call
+  int64_t max_tiles;    // tiles of all requests, at most
+  int64_t slots, o_bytes, bytes;
+};
 
 struct PagedPlan {
   int page_lg;
-  int64_t max_tiles;  // 16-row tiles of all requests, at most
-  int64_t slots;
-  int64_t part_bytes, bytes;
+  bool tile;            // some request may have more than kFewRows rows, for paged_tile_kernel
+  Part rows, tiles;
 };
+
+Part part_of(const pa_paged_args* x, int BM) {
+  Part p;
+  const int64_t some = x->T < x->R ? x->T : x->R;  // requests with rows, at most
+  p.max_tiles = x->T * (x->Hq / x->Hkv) / BM + some;
+  const int64_t units = kTarget + p.max_tiles * x->Hkv;
+  // (a tile is split into two shares at least, and then has less than twice the shares that its
+  // blocks fill)
+  p.slots = 2 * kTarget < units ? 2 * kTarget : units;
+  p.o_bytes = p.slots * BM * x->D * 4;
+  p.bytes = p.o_bytes + p.slots * BM * 2 * 4;
+  return p;
+}
 
 int plan_of(const pa_paged_args* x, PagedPlan* p) {
   PA_CHECK_ARG(x, "pa_paged_attn: null arguments");
@@ -29,16 +48,14 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   PA_CHECK_ARG(x->cols >= 0 && ((int64_t)x->cols << p->page_lg) <= kMaxPosition && x->pitch >= x->cols,
                "pa_paged_attn: %d columns of %d, pitch %lld", x->cols, x->page_size, (long long)x->pitch);
   PA_CHECK_ARG(x->scale > 0.f && x->scale < INFINITY, "pa_paged_attn: scale=%g must be positive", (double)x->scale);
-  const int64_t some = x->T < x->R ? x->T : x->R;  // requests with rows, at most
-  p->max_tiles = x->T * (x->Hq / x->Hkv) / 16 + some;
-  const int64_t units = kTarget + p->max_tiles * x->Hkv;
-  // (a tile is split into two shares at least, and then has less than twice the shares that its
-  // blocks fill)
-  p->slots = 2 * kTarget < units ? 2 * kTarget : units;
-  p->part_bytes = p->slots * 16 * x->D * 4;
-  p->bytes = p->part_bytes + p->slots * 16 * 2 * 4;
+  p->tile = x->dtype != PA_F32 && x->n_pages > 0 && x->max_fresh * (x->Hq / x->Hkv) > kFewRows;
+  p->rows = part_of(x, kRows);
+  p->tiles = part_of(x, kTileRows);
   return PA_OK;
 }
+
+// (the kernels of a call run one after the other and share the workspace)
+int64_t bytes_of(const PagedPlan& p) { return p.tile && p.tiles.bytes > p.rows.bytes ? p.tiles.bytes : p.rows.bytes; }
 
 }  // namespace
 }  // namespace pa
@@ -47,7 +64,7 @@ extern "C" int pa_paged_workspace(const pa_paged_args* x, int64_t* bytes) {
   pa::PagedPlan p;
   if (int rc = pa::plan_of(x, &p)) return rc;
   PA_CHECK_ARG(bytes, "pa_paged_workspace: null output");
-  *bytes = p.bytes;
+  *bytes = pa::bytes_of(p);
   return PA_OK;
 }
 
@@ -73,8 +90,8 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
   PA_CHECK_ARG(x->q_st >= 0 && x->q_sh >= 0 && x->o_st >= 0 && x->o_sh >= 0 && x->c_sp >= 0 && x->c_sh >= 0 &&
                    x->c_sn >= x->D && x->c_sn <= (1 << 21),
                "pa_paged_attn: negative strides, or cache rows closer than D or further than 2^21");
-  PA_CHECK_ARG(x->workspace && reinterpret_cast<uintptr_t>(x->workspace) % 256 == 0 && x->workspace_bytes >= p.bytes,
-               "pa_paged_attn: needs a 256-byte aligned workspace of %lld bytes", (long long)p.bytes);
+  PA_CHECK_ARG(x->workspace && reinterpret_cast<uintptr_t>(x->workspace) % 256 == 0 && x->workspace_bytes >= bytes_of(p),
+               "pa_paged_attn: needs a 256-byte aligned workspace of %lld bytes", (long long)bytes_of(p));
   PagedK a;
   a.q = static_cast<const char*>(x->q);
   a.q_st = x->q_st * esz;
@@ -96,15 +113,15 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
   a.Hkv = x->Hkv;
   a.G = x->Hq / x->Hkv;
   a.c = x->scale * 1.4426950408889634f;
-  a.mask.n_include = x->mask.n_include;
-  a.mask.n_exclude = x->mask.n_exclude;
+  a.n_include = x->mask.n_include;
+  a.n_exclude = x->mask.n_exclude;
   for (int i = 0; i < PA_MAX_TERMS; ++i) {
     pa_term t = x->mask.terms[i];
     // (no distance reaches the clamp)
     t.p0 = imin(t.p0, kMaxPosition);
     t.p1 = imin(t.p1, kMaxPosition);
     t.p2 = imin(t.p2, kMaxPosition);
-    a.mask.terms[i] = t;
+    a.terms[i] = t;
   }
   a.o = static_cast<char*>(x->o);
   a.o_st = x->o_st * esz;
@@ -113,11 +130,21 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
   a.lse_st = x->lse_st;
   a.lse_sh = x->lse_sh;
   a.part_o = static_cast<float*>(x->workspace);
-  a.part_ml = reinterpret_cast<float*>(static_cast<char*>(x->workspace) + p.part_bytes);
-  a.slots = (int32_t)p.slots;
   a.target = kTarget;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  auto with = [&](const Part& part) {
+    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(x->workspace) + part.o_bytes);
+    a.slots = (int32_t)part.slots;
+  };
+  with(p.rows);
   a.least = 8;
   a.row_min = 0;
+  a.row_max = p.tile ? kFewRows : INT_MAX;
+  if (int rc = launch_paged_rows(a, x->dtype, x->D, p.rows.max_tiles, s)) return rc;
+  if (!p.tile) return PA_OK;
+  with(p.tiles);
+  a.least = 4;
+  a.row_min = kFewRows;
   a.row_max = INT_MAX;
-  return launch_paged_rows(a, x->dtype, x->D, p.max_tiles, static_cast<hipStream_t>(stream));
+  return launch_paged_tile(a, x->dtype, x->D, p.tiles.max_tiles, s);
 }

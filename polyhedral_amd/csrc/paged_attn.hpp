@@ -10,6 +10,8 @@
 // A request whose tiles are split has a slot of the workspace per unit, numbered in unit order.
 #pragma once
 
+#include <stddef.h>
+
 #include "lds_rows.hpp"
 #include "page_math.hpp"
 
@@ -29,18 +31,28 @@ struct PagedK {
   const int32_t* q_start;
   int32_t R, T, Hkv, G;
   float c;  // scale * log2(e)
-  PageMask mask;
+  int32_t n_include, n_exclude;
+  pa_term terms[PA_MAX_TERMS];
   char* o;
   int64_t o_st, o_sh;
   float* lse;
   int64_t lse_st, lse_sh;  // elements
   float* part_o;   // [slots][BM][D]: unnormalised
-  float* part_ml;  // [slots][BM][2]: maximum (unscaled) and sum
+  float* part_ml;  // [slots][BM][2]: maximum (tiles of 128 rows: times c) and sum
   int32_t slots;
   int32_t target;     // units a split aims for
   int32_t least;      // least blocks of a share
   int32_t row_min, row_max;  // requests with row_min < rows <= row_max are this kernel's
 };
+
+// The mask of a kernel whose first argument is a PagedK.
+typedef const __attribute__((address_space(4))) pa_term cterm;
+typedef PageMask<cterm*> KernelMask;
+__device__ __forceinline__ KernelMask kernel_mask(const PagedK& a) {
+  typedef const __attribute__((address_space(4))) char cchar;
+  cchar* args = (cchar*)__builtin_amdgcn_kernarg_segment_ptr();
+  return {a.n_include, a.n_exclude, (cterm*)(args + offsetof(PagedK, terms))};
+}
 
 struct Work {
   int32_t tiles, blocks;
@@ -63,7 +75,7 @@ __device__ __forceinline__ Work work_of(const PagedK& a, const Request& q) {
   const int32_t rows = q.n * a.G;
   if (rows <= a.row_min || rows > a.row_max) return {0, 0};
   const int32_t span = imin(q.n, (BM + a.G - 1) / a.G + 1);
-  return {(rows + BM - 1) / BM, key_list(a.mask, q.len - span, q.len - 1, q.len, LG).count()};
+  return {(rows + BM - 1) / BM, key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG).count()};
 }
 
 __device__ __forceinline__ int32_t wave_scan(int32_t x, int lane) {
@@ -159,6 +171,16 @@ __device__ __forceinline__ void share_of(int32_t n, int32_t split, int32_t split
 
 int check_pages(const char* who, int64_t n_pages, int32_t page_size, int* page_lg);
 
-int launch_paged_rows(PagedK a, int dtype, int D, int64_t max_tiles, hipStream_t s);
+// The maximum m of a row's scores so far as the base of its exponentials: 0 for -inf (no live key
+// so far; every score is -inf then).
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+constexpr int kRows = 16;       // query rows of a tile of paged_rows_kernel
+constexpr int kTileRows = 128;  // and of paged_tile_kernel
+constexpr int kTileLg = 6;      // log2 keys of a step of paged_tile_kernel
+
+int launch_paged_rows(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s);
+int launch_paged_tile(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s);
+int launch_paged_tile_merge(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s);
 
 }  // namespace pa

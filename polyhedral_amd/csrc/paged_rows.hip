@@ -14,7 +14,8 @@
 // multiple of 16 rows), so a segment is one 64-bit offset.
 //
 // Scores, maxima, sums and O are float32; P is rounded to 16 bits as an MFMA operand only, its
-// sum taken before.
+// sum taken before.  Maxima are kept unscaled and p = exp2((x - m) c): a maximum that is rounded
+// after its scaling would leave its own p at any power of two where scores are huge.
 //
 // A dead key contributes nothing whatever its K and V hold: its score is replaced by -inf, and
 // where a step is masked for some row and its V rows hold an infinity or NaN, the products are
@@ -50,13 +51,7 @@ __device__ __forceinline__ float quad_sum(float x) {
   return row_sum(__builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]));
 }
 
-constexpr int kRows = 16;   // query rows of a tile
 constexpr int kWaves = 4;
-
-// The maximum m of a row's scores so far as the base of its exponentials: 0 for -inf (no live key
-// so far; every score is -inf then).  Maxima are kept unscaled and p = exp2((x - m) c): a maximum
-// that is rounded after its scaling would leave its own p at any power of two where scores are huge.
-__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
 // Bits of the words that hold an infinity or NaN in some half (f16 / bf16): the largest magnitude
 // of each half against the type's first one that is not finite.
@@ -123,7 +118,8 @@ void paged_rows_kernel(const PagedK a) {
   }
 
   // ---- the keys of this share ------------------------------------------------------
-  const KeyList kl = key_list(a.mask, q_lo, q_hi, len, S::LG);
+  const KernelMask mask = kernel_mask(a);
+  const KeyList kl = key_list(mask, q_lo, q_hi, len, S::LG);
   int32_t j0, j1;
   share_of(kl.count(), u.split, u.splits, &j0, &j1);
   const int n_steps = j1 - j0 > w ? (j1 - j0 - w + kWaves - 1) / kWaves : 0;
@@ -150,7 +146,7 @@ void paged_rows_kernel(const PagedK a) {
     const int32_t page = checked_page(r_page, a.n_pages);
     int v = kDead;
     if (key < len && page >= 0) {
-      v = mask_verdict(a.mask, q_lo, q_hi, key, key + 15);
+      v = mask_verdict(mask, q_lo, q_hi, key, key + 15);
       if (v == kFull && key + 15 >= len) v = kPartial;
     }
     c_live = __ballot(v != kDead);
@@ -257,7 +253,7 @@ void paged_rows_kernel(const PagedK a) {
     }
     uint32_t word = 0xffffffffu;  // the step's keys live for this lane's row
     if (s.full != ALL) {
-      word = mask_word(a.mask, q_pos, s.key, len);
+      word = mask_word(mask, q_pos, s.key, len);
       if (!(s.live & 1u)) word &= 0xffff0000u;
       if (NS == 1 || !(s.live & 2u)) word &= 0x0000ffffu;
 #pragma unroll
@@ -456,20 +452,22 @@ void paged_rows_kernel(const PagedK a) {
 // The shares of a split tile become its rows: a wave per row, a share's maximum and sum per lane
 // for the weights, then the shares' rows, lanes along the columns.  The order of the sums is that of
 // the shares.
-template <typename T, int D, int LG>
+// C: maxima are unscaled.
+template <typename T, int D, int BM, int LG, bool C>
 __global__ __launch_bounds__(64 * kRows) void paged_merge_kernel(const PagedK a) {
   constexpr int CPL = D / 64;
   const int lane = threadIdx.x & 63;
-  const int row = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Unit u = find_unit<kRows, LG, true>(a, (int32_t)blockIdx.x, lane);
+  const int row = (int)blockIdx.y * kRows + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float c = C ? a.c : 1.f;
+  const Unit u = find_unit<BM, LG, true>(a, (int32_t)blockIdx.x, lane);
   if (!u.found || u.slot + u.splits > a.slots) return;
-  const int ir = u.tile * kRows + row;
+  const int ir = u.tile * BM + row;
   if (ir >= u.rq.n * a.G) return;
   typedef float fv __attribute__((ext_vector_type(CPL)));
-  const float* ml = a.part_ml + 2 * ((int64_t)u.slot * kRows + row);
-  const float* po = a.part_o + ((int64_t)u.slot * kRows + row) * D + CPL * lane;
+  const float* ml = a.part_ml + 2 * ((int64_t)u.slot * BM + row);
+  const float* po = a.part_o + ((int64_t)u.slot * BM + row) * D + CPL * lane;
   float M = -INFINITY, L = 0.f;
-  for (int s = lane; s < u.splits; s += 64) M = nan_max(M, ml[(int64_t)s * 2 * kRows]);
+  for (int s = lane; s < u.splits; s += 64) M = nan_max(M, ml[(int64_t)s * 2 * BM]);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) M = nan_max(M, __shfl_xor(M, o));
   fv out = {};
@@ -477,15 +475,15 @@ __global__ __launch_bounds__(64 * kRows) void paged_merge_kernel(const PagedK a)
     const int s = s0 + lane;
     float f = 0.f;
     if (s < u.splits) {
-      f = __builtin_amdgcn_exp2f((ml[(int64_t)s * 2 * kRows] - base_of(M)) * a.c);
-      L += f * ml[(int64_t)s * 2 * kRows + 1];
+      f = __builtin_amdgcn_exp2f((ml[(int64_t)s * 2 * BM] - base_of(M)) * c);
+      L += f * ml[(int64_t)s * 2 * BM + 1];
     }
     const int n = imin(u.splits - s0, 64);
     for (int b = 0; b < n; b += 16) {
       fv x[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        x[e] = b + e < n ? *reinterpret_cast<const fv*>(po + (int64_t)(s0 + b + e) * kRows * D) : fv{};
+        x[e] = b + e < n ? *reinterpret_cast<const fv*>(po + (int64_t)(s0 + b + e) * BM * D) : fv{};
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         out += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), (b + e) & 63)) * x[e];
@@ -499,7 +497,7 @@ __global__ __launch_bounds__(64 * kRows) void paged_merge_kernel(const PagedK a)
 #pragma unroll
   for (int e = 0; e < CPL; ++e) orow[e] = (T)out[e];
   if (a.lse && lane == 0)
-    a.lse[(int64_t)(u.rq.start + tok) * a.lse_st + (int64_t)head * a.lse_sh] = L == 0.f ? -INFINITY : (M * a.c + log2f(L)) * kLn2;
+    a.lse[(int64_t)(u.rq.start + tok) * a.lse_st + (int64_t)head * a.lse_sh] = L == 0.f ? -INFINITY : (M * c + log2f(L)) * kLn2;
 }
 
 template <typename T, int D>
@@ -511,19 +509,35 @@ int launch_rows_t(const PagedK& a, int64_t max_tiles, hipStream_t s) {
   PA_LAUNCH_CHECK("paged_rows_kernel");
   // (a split tile has two shares at least)
   const int64_t groups = max_tiles * a.Hkv < a.target ? max_tiles * a.Hkv : a.target;
-  hipLaunchKernelGGL((paged_merge_kernel<T, D, RowsShape<T, D>::LG>), dim3((unsigned)groups), dim3(64 * kRows), 0, s, a);
+  hipLaunchKernelGGL((paged_merge_kernel<T, D, kRows, RowsShape<T, D>::LG, true>), dim3((unsigned)groups), dim3(64 * kRows),
+                     0, s, a);
+  PA_LAUNCH_CHECK("paged_merge_kernel");
+  return PA_OK;
+}
+
+template <typename T, int D>
+int launch_tile_merge_t(const PagedK& a, int64_t max_tiles, hipStream_t s) {
+  const int64_t groups = max_tiles * a.Hkv < a.target ? max_tiles * a.Hkv : a.target;
+  hipLaunchKernelGGL((paged_merge_kernel<T, D, kTileRows, kTileLg, false>), dim3((unsigned)groups, kTileRows / kRows),
+                     dim3(64 * kRows), 0, s, a);
   PA_LAUNCH_CHECK("paged_merge_kernel");
   return PA_OK;
 }
 
 }  // namespace
 
-int launch_paged_rows(PagedK a, int dtype, int D, int64_t max_tiles, hipStream_t s) {
+int launch_paged_rows(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s) {
   if (dtype == PA_BF16)
     return D == 64 ? launch_rows_t<__bf16, 64>(a, max_tiles, s) : launch_rows_t<__bf16, 128>(a, max_tiles, s);
   if (dtype == PA_F16)
     return D == 64 ? launch_rows_t<_Float16, 64>(a, max_tiles, s) : launch_rows_t<_Float16, 128>(a, max_tiles, s);
   return D == 64 ? launch_rows_t<float, 64>(a, max_tiles, s) : launch_rows_t<float, 128>(a, max_tiles, s);
+}
+
+int launch_paged_tile_merge(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s) {
+  if (dtype == PA_BF16)
+    return D == 64 ? launch_tile_merge_t<__bf16, 64>(a, max_tiles, s) : launch_tile_merge_t<__bf16, 128>(a, max_tiles, s);
+  return D == 64 ? launch_tile_merge_t<_Float16, 64>(a, max_tiles, s) : launch_tile_merge_t<_Float16, 128>(a, max_tiles, s);
 }
 
 }  // namespace pa

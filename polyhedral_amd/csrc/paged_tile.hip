@@ -1,0 +1,418 @@
+// Attention of chunks of new tokens over a paged cache, f16 / bf16: tiles of 128 query rows (new
+// tokens times the heads that share a KV head), 64 keys a step.
+//
+// A work-group is four waves of 32 rows.  Scores are taken transposed (S^T = K Q^T) on 32x32x16
+// MFMAs, so a lane owns a query row, a maximum is in its registers but for one exchange, and P^T is
+// already the B operand of O^T += V^T P^T.  K and V rows come by LDS DMA into a ring of two slots
+// each (layout in lds_rows.hpp), wave w moving segment w (16 rows, inside one page) of a step.  The
+// scores of step j + 1 are computed beside the exponentials of step j, whose products follow: one
+// straight line of MFMA, LDS and VALU work in an order that is spelled out, behind one wait and one
+// barrier per step.
+//
+// The blocks of keys that may be live for the tile are a list of two ranges (page_math.hpp); its
+// entries are held 16 steps at a time, a segment per lane, with each wave's verdicts on its own
+// rows.  Steps that are all live for a wave take the straight line.  The others mask by words of 32
+// keys computed from the mask's terms, leave blocks out that are dead for the wave, and, where a
+// masked block's V rows hold an infinity or NaN, take the products key by key, added only to the rows
+// that the key is live for: a dead key contributes nothing whatever it holds.
+//
+// Scores, maxima, sums and O are float32; P is rounded to 16 bits as an MFMA operand only, its sum
+// taken before.
+#include <math.h>
+
+#include <type_traits>
+
+#include "paged_attn.hpp"
+
+namespace pa {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ bool not_finite16(uint32_t lo, uint32_t hi) {
+  constexpr uint32_t inf = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+  return lo >= inf || hi >= (inf << 16);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+void paged_tile_kernel(const PagedK a) {
+  using Frag = typename Mma<T>::frag;
+  using R = Rows<D>;
+  constexpr int ESZ = 2, NQF = D / 16, NDB = D / 32;
+  constexpr int SLOT = 64 * R::ROW;          // a step's K or V
+  constexpr int VRING = 0, KRING = 2 * SLOT;
+  __shared__ __attribute__((aligned(2 * SLOT))) char smem[4 * SLOT];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char_t*)smem;
+
+  const int tid = threadIdx.x, lane = tid & 63, G = lane >> 5, m = lane & 31;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  const Unit u = find_unit<kTileRows, kTileLg, false>(a, (int32_t)blockIdx.x, lane);
+  if (!u.found) return;
+
+  // ---- rows ------------------------------------------------------------------------
+  const int rows = u.rq.n * a.G, len = u.rq.len, pos0 = len - u.rq.n;
+  const int i0 = u.tile * kTileRows;
+  const int n_rows = imin(rows - i0, kTileRows);
+  const int w0 = imin(i0 + 32 * w, rows - 1), w1 = imin(i0 + 32 * w + 31, rows - 1);  // this wave's rows
+  int q_pos;  // position of this lane's row (a lane past the rows repeats the last)
+  const int q_lo = pos0 + w0 / a.G, q_hi = pos0 + w1 / a.G;
+
+  Frag qf[NQF];
+  {
+    const int i = imin(i0 + 32 * w + m, rows - 1), tok = i / a.G, head = u.h * a.G + (i - tok * a.G);
+    q_pos = pos0 + tok;
+    const char* qrow = a.q + (int64_t)(u.rq.start + tok) * a.q_st + (int64_t)head * a.q_sh;
+#pragma unroll
+    for (int kc = 0; kc < NQF; ++kc)
+      qf[kc] = __builtin_bit_cast(Frag, *reinterpret_cast<const uint4*>(qrow + (16 * kc + 8 * G) * ESZ));
+  }
+
+  // ---- the keys of this share ---------------------------------------------------------
+  const KernelMask mask = kernel_mask(a);
+  const KeyList kl = key_list(mask, pos0 + i0 / a.G, pos0 + (i0 + n_rows - 1) / a.G, len, kTileLg);
+  int32_t j0, j1;
+  share_of(kl.count(), u.split, u.splits, &j0, &j1);
+  const int n_steps = j1 - j0;
+  const int32_t* table = a.tables + (int64_t)u.r * a.pitch;
+  const char* kbase = a.k + u.h * a.c_sh;
+  const char* vbase = a.v + u.h * a.c_sh;
+  uint32_t doff[R::NI];
+  dma_offsets<D>(doff, a.c_sn, lane);
+#pragma unroll
+  for (int x = 1; x < R::NI; ++x) doff[x] += (uint32_t)(x * R::RPI * a.c_sn);
+
+  // 16 steps: lane 4 s + t holds segment t of step s, its offset in the cache; bit 4 s + t of live /
+  // full: some pair of it may be live for this wave / all are.  The next 16 steps' pages are loaded
+  // halfway through these.
+  int32_t r_page = -1;
+  int64_t c_off = 0;
+  uint64_t c_live = 0ull, c_full = 0ull;
+  auto key_of = [&](int c) __attribute__((always_inline)) -> int32_t {
+    const int s = 16 * c + (lane >> 2);
+    return s < n_steps ? (kl.block(j0 + s) << kTileLg) + 16 * (lane & 3) : len;
+  };
+  auto load_raw = [&](int c) __attribute__((always_inline)) {
+    const int32_t key = key_of(c);
+    r_page = key < len ? table[key >> a.page_lg] : -1;
+  };
+  auto take_raw = [&](int c) __attribute__((always_inline)) {
+    const int32_t key = key_of(c);
+    const int32_t page = checked_page(r_page, a.n_pages);
+    int v = kDead;
+    if (key < len && page >= 0) {
+      v = mask_verdict(mask, q_lo, q_hi, key, key + 15);
+      if (v == kFull && key + 15 >= len) v = kPartial;
+    }
+    c_live = __ballot(v != kDead);
+    c_full = __ballot(v == kFull);
+    // (keys without a page read the cache's first one, and are dead)
+    c_off = (int64_t)imax(page, 0) * a.c_sp + (int64_t)(key & ((1 << a.page_lg) - 1)) * a.c_sn;
+  };
+  struct Step {
+    int64_t off;          // of the segment that this wave moves
+    uint32_t live, full;  // 4 bits: the step's segments
+  };
+  auto step_of = [&](int j) __attribute__((always_inline)) -> Step {
+    if ((j & 15) == 0) take_raw(j >> 4);
+    if ((j & 15) == 8) load_raw((j >> 4) + 1);
+    const int l0 = 4 * (j & 15);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)c_off, l0 + w);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(c_off >> 32), l0 + w);
+    return Step{(int64_t)((uint64_t)lo | ((uint64_t)hi << 32)), (uint32_t)(c_live >> l0) & 15u, (uint32_t)(c_full >> l0) & 15u};
+  };
+  auto dma = [&](uint32_t ring, const char* base) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < R::NI; ++x) dma_x4(lds0 + ring + (uint32_t)(w * 16 * R::ROW) + x * 1024, base, doff[x]);
+  };
+
+  // (K reads are on the slot of the step ahead, V reads on that of the current one; a slot is one bit
+  // of an address, as the rings are aligned to two slots)
+  TileReads<D> rd = tile_reads<D>((lds_cptr)smem, lane);
+
+  f32x16 acc[NDB];
+#pragma unroll
+  for (int x = 0; x < NDB; ++x) acc[x] = f32x16{0};
+  float m_run = -INFINITY, l_part = 0.f;  // (log2 units)
+  f32x16 sc0 = {}, sc1 = {};
+  uint32_t wd0 = 0u, wd1 = 0u;            // the current step's words of this lane's row, where it is masked
+
+  // Scores of both blocks of the step in the K slot that the row reads are on.
+  auto qk = [&](f32x16& x0, f32x16& x1) __attribute__((always_inline)) {
+    u32x4 ka[NQF], kb[NQF];
+#pragma unroll
+    for (int kc = 0; kc < NQF; ++kc) ka[kc] = *(lds_u4*)(rd.row(kc) + KRING);
+#pragma unroll
+    for (int kc = 0; kc < NQF; ++kc) kb[kc] = *(lds_u4*)(rd.row(kc) + KRING + 32 * R::ROW);
+    x0 = Mma<T>::mma(__builtin_bit_cast(Frag, ka[0]), qf[0], f32x16{0});
+#pragma unroll
+    for (int kc = 1; kc < NQF; ++kc) x0 = Mma<T>::mma(__builtin_bit_cast(Frag, ka[kc]), qf[kc], x0);
+    x1 = Mma<T>::mma(__builtin_bit_cast(Frag, kb[0]), qf[0], f32x16{0});
+#pragma unroll
+    for (int kc = 1; kc < NQF; ++kc) x1 = Mma<T>::mma(__builtin_bit_cast(Frag, kb[kc]), qf[kc], x1);
+  };
+  // -inf for the keys of a block that are dead for this lane's row
+  auto mask_block = [&](f32x16& x, uint32_t word) __attribute__((always_inline)) {
+    word >>= 4 * G;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float xv = x[e];  // (a scalar copy: bit-casting the vector element reads element 0)
+      const int32_t keep = __builtin_amdgcn_sbfe((int32_t)word, 8 * (e >> 2) + (e & 3), 1);
+      x[e] = __builtin_bit_cast(float, (__builtin_bit_cast(int32_t, xv) & keep) | (int32_t)(0xff800000u & ~(uint32_t)keep));
+    }
+  };
+  auto shape = [&](const Step& s, int j, f32x16& x0, f32x16& x1) __attribute__((always_inline)) {
+    if (s.full == 15u) return;
+    const int key = kl.block(j0 + j) << kTileLg;
+    wd0 = s.live & 3u ? mask_word(mask, q_pos, key, len) : 0u;
+    wd1 = s.live & 12u ? mask_word(mask, q_pos, key + 32, len) : 0u;
+    if (!(s.live & 1u)) wd0 &= 0xffff0000u;
+    if (!(s.live & 2u)) wd0 &= 0x0000ffffu;
+    if (!(s.live & 4u)) wd1 &= 0xffff0000u;
+    if (!(s.live & 8u)) wd1 &= 0x0000ffffu;
+    mask_block(x0, wd0);
+    mask_block(x1, wd1);
+  };
+  auto block_max = [&](const f32x16& x, float mx) __attribute__((always_inline)) -> float {
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) mx = nan_max(mx, nan_max(x[e], x[e + 1]));
+    return mx;
+  };
+  auto raise = [&](float mx) __attribute__((always_inline)) {
+    const float m_new = nan_max(m_run, row_nan_max(mx) * a.c);
+    if (__ballot(m_new > m_run + kLazy) != 0ull) {
+      const float alpha = __builtin_amdgcn_exp2f(m_run - base_of(m_new));
+      m_run = m_new;
+      l_part *= alpha;
+#pragma unroll
+      for (int x = 0; x < NDB; ++x) acc[x] *= alpha;
+    }
+  };
+  auto exps = [&](const f32x16& x, int c, float neg_m) __attribute__((always_inline)) -> Frag {
+    f32x8 pv;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * c + e], a.c, neg_m));
+      l_part += pv[e];
+    }
+    return Mma<T>::cvt(pv);
+  };
+  // Products with chunk x (keys 16 x .. 16 x + 15) of the step in the V slot that the transposed
+  // reads are on.
+  auto pv = [&](Frag pf, int x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) acc[db] = Mma<T>::mma(tr_frag<T, D>(rd, db, VRING + 16 * x * R::ROW), pf, acc[db]);
+  };
+  // Softmax and products of the current step where it is not all live for this wave.
+  auto masked_step = [&](const Step& s) __attribute__((always_inline)) {
+    if (s.live == 0u) return;
+    const float neg_m = -base_of(m_run);
+    Frag pf[4];
+    uint32_t odd = 0u;  // chunks with dead pairs whose V rows hold what is not finite
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      pf[x] = exps(x < 2 ? sc0 : sc1, x & 1, neg_m);
+      if (((s.live & ~s.full) >> x) & 1u) {
+        uint32_t lo = 0u, hi = 0u;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const u32x4 v = __builtin_bit_cast(u32x4, tr_frag<T, D>(rd, db, VRING + 16 * x * R::ROW));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t y = v[e];
+            lo = max(lo, y & 0x7fffu);
+            hi = max(hi, y & 0x7fff0000u);
+          }
+        }
+        if (__ballot(not_finite16<T>(lo, hi)) != 0ull) odd |= 1u << x;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (((s.live & ~odd) >> x) & 1u) pv(pf[x], x);
+    if (odd == 0u) return;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (!((odd >> x) & 1u)) continue;
+      const u32x4 pw = __builtin_bit_cast(u32x4, pf[x]);
+      // element e of lane half h is key 8 (e / 4) + 4 h + e % 4 of the chunk
+#pragma unroll 1
+      for (int y = 0; y < 16; ++y) {
+        const int h = y & 1, e = y >> 1;
+        const uint32_t half = G == h ? ((e & 1) ? 0xffff0000u : 0x0000ffffu) : 0u;
+        u32x4 keep;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) keep[z] = z == (e >> 1) ? half : 0u;
+        const bool on = ((x < 2 ? wd0 : wd1) >> (16 * (x & 1) + 8 * (e >> 2) + 4 * h + (e & 3))) & 1u;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const u32x4 v = __builtin_bit_cast(u32x4, tr_frag<T, D>(rd, db, VRING + 16 * x * R::ROW)) & keep;
+          const f32x16 p = Mma<T>::mma(__builtin_bit_cast(Frag, v), __builtin_bit_cast(Frag, pw & keep), f32x16{0});
+#pragma unroll
+          for (int z = 0; z < 16; ++z) acc[db][z] = on ? acc[db][z] + p[z] : acc[db][z];
+        }
+      }
+    }
+  };
+  auto full_step = [&]() __attribute__((always_inline)) {
+    const float neg_m = -base_of(m_run);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) pv(exps(x < 2 ? sc0 : sc1, x & 1, neg_m), x);
+  };
+
+  Step s_cur{}, s_next{}, s_after{};
+  if (n_steps > 0) {
+    load_raw(0);
+    s_cur = step_of(0);
+    dma(KRING, kbase + s_cur.off);
+    dma(VRING, vbase + s_cur.off);
+    if (n_steps > 1) s_next = step_of(1);
+    dma_wait_all();
+#pragma unroll
+    for (int kc = 0; kc < NQF; ++kc) asm volatile("" ::"v"(qf[kc]));
+    __syncthreads();
+    if (n_steps > 1) dma(KRING + SLOT, kbase + s_next.off);
+    if (s_cur.live != 0u) {
+      qk(sc0, sc1);
+      shape(s_cur, 0, sc0, sc1);
+      raise(block_max(sc1, block_max(sc0, -INFINITY)));
+    }
+    rd.template turn_rows<SLOT>();
+    // Iteration j, with a step after it: behind the wait and the barrier, K of step j + 1 and V of step
+    // j are in LDS, and the slots that the new DMA writes were last read before the barrier.
+    uint32_t p = 0u;  // j & 1, times a slot
+#pragma unroll 1
+    for (int j = 0; j + 1 < n_steps; ++j) {
+      dma_wait_all();
+      // (a use that makes the compiler's own wait for the page loads fall here)
+      asm volatile("" ::"v"(r_page));
+      __syncthreads();
+      if (j + 2 < n_steps) {
+        s_after = step_of(j + 2);
+        dma(KRING + p, kbase + s_after.off);
+      }
+      dma(VRING + (SLOT - p), vbase + s_next.off);
+      f32x16 sn0, sn1;
+      if (s_cur.full == 15u && s_next.live != 0u) {
+        const float neg_m = -base_of(m_run);
+        const Frag p00 = exps(sc0, 0, neg_m), p01 = exps(sc0, 1, neg_m), p10 = exps(sc1, 0, neg_m), p11 = exps(sc1, 1, neg_m);
+        qk(sn0, sn1);
+        pv(p00, 0);
+        pv(p01, 1);
+        pv(p10, 2);
+        pv(p11, 3);
+        // 4 K reads ahead; then MFMAs of the scores, each beside a read and exponentials; then those of
+        // the products, V reads running 4 MFMAs ahead
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+        for (int x = 0; x < 2 * NQF; ++x) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+          __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 6 : 10, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+        for (int x = 0; x < 4 * NDB; ++x) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+          __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 1 : 4, 1);
+        }
+      } else {
+        if (s_cur.full == 15u)
+          full_step();
+        else
+          masked_step(s_cur);
+        if (s_next.live != 0u) qk(sn0, sn1);
+      }
+      if (s_next.live != 0u) {
+        shape(s_next, j + 1, sn0, sn1);
+        raise(block_max(sn1, block_max(sn0, -INFINITY)));
+        sc0 = sn0;
+        sc1 = sn1;
+      }
+      s_cur = s_next;
+      s_next = s_after;
+      rd.template turn_rows<SLOT>();
+      rd.template turn_tr<SLOT>();
+      p = SLOT - p;
+    }
+    dma_wait_all();
+    __syncthreads();
+    if (s_cur.full == 15u)
+      full_step();
+    else
+      masked_step(s_cur);
+  }
+
+  // ---- the rows leave -------------------------------------------------------------------
+  const float l_tot = row_sum(l_part);
+  int lane_e = lane;  // (opaque: what follows is worked out again instead of held through the loop)
+  asm volatile("" : "+v"(lane_e));
+  const int m_e = lane_e & 31, G_e = lane_e >> 5;
+  const bool mine = 32 * w + m_e < n_rows;
+  if (u.splits > 1) {
+    if (u.slot >= a.slots) return;  // (not reached by starts in order; the same for the work-group)
+    if (mine) {
+      const int64_t row = (int64_t)u.slot * kTileRows + 32 * w + m_e;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<f32x4*>(a.part_o + row * D + 32 * db + 8 * e + 4 * G_e) =
+              f32x4{acc[db][4 * e], acc[db][4 * e + 1], acc[db][4 * e + 2], acc[db][4 * e + 3]};
+      if (G_e == 0) {
+        a.part_ml[2 * row] = m_run;
+        a.part_ml[2 * row + 1] = l_tot;
+      }
+    }
+    return;
+  }
+  const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
+  if (a.lse && G_e == 0 && mine) {
+    const int ir = i0 + 32 * w + m_e, tok = ir / a.G, head = u.h * a.G + (ir - tok * a.G);
+    a.lse[(int64_t)(u.rq.start + tok) * a.lse_st + (int64_t)head * a.lse_sh] =
+        l_tot == 0.f ? -INFINITY : (m_run + log2f(l_tot)) * kLn2;
+  }
+  // Through LDS (32 rows a wave, 16-byte units swizzled), so that they are stored as whole rows.
+  __syncthreads();  // every wave is past its last read of the rings
+  lds_char_t* stage = (lds_char_t*)smem + w * 32 * R::ROW;
+  typedef __attribute__((address_space(3))) u32x2 lds_w2;
+  constexpr int UM = R::UPR - 1;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const f32x4 x = f32x4{acc[db][4 * e], acc[db][4 * e + 1], acc[db][4 * e + 2], acc[db][4 * e + 3]} * inv;
+      *(lds_w2*)(stage + m_e * R::ROW + 16 * ((4 * db + e) ^ (m_e & UM)) + 8 * G_e) = __builtin_bit_cast(u32x2, Mma<T>::cvt4(x));
+    }
+  // (each wave reads back only the rows it wrote: LDS keeps a wave's accesses in order)
+#pragma unroll
+  for (int x = 0; x < 32 / R::RPI; ++x) {
+    const int rr = R::RPI * x + lane_e / R::UPR, un = lane_e % R::UPR;
+    const u32x4 v = *(lds_u4*)(stage + rr * R::ROW + 16 * (un ^ (rr & UM)));
+    const int row = 32 * w + rr;
+    if (row < n_rows) {
+      const int ir = i0 + row, t = ir / a.G, h = u.h * a.G + (ir - t * a.G);
+      *reinterpret_cast<u32x4*>(a.o + (int64_t)(u.rq.start + t) * a.o_st + (int64_t)h * a.o_sh + 16 * un) = v;
+    }
+  }
+}
+
+template <typename T, int D>
+int launch_tile_t(const PagedK& a, int64_t max_tiles, hipStream_t s) {
+  const int64_t grid = a.target + max_tiles * a.Hkv;
+  PA_CHECK_ARG(grid <= 0x7fffffffll, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)grid);
+  hipLaunchKernelGGL((paged_tile_kernel<T, D>), dim3((unsigned)grid), dim3(256), 0, s, a);
+  PA_LAUNCH_CHECK("paged_tile_kernel");
+  return launch_paged_tile_merge(a, __is_same(T, __bf16) ? PA_BF16 : PA_F16, D, max_tiles, s);
+}
+
+}  // namespace
+
+int launch_paged_tile(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s) {
+  if (dtype == PA_BF16)
+    return D == 64 ? launch_tile_t<__bf16, 64>(a, max_tiles, s) : launch_tile_t<__bf16, 128>(a, max_tiles, s);
+  return D == 64 ? launch_tile_t<_Float16, 64>(a, max_tiles, s) : launch_tile_t<_Float16, 128>(a, max_tiles, s);
+}
+
+}  // namespace pa

@@ -19,13 +19,7 @@ MAX = (1 << 30) - 1
 HARNESS = r"""
 #include "page_math.hpp"
 using namespace pa;
-static PageMask of(const pa_mask* m) {
-  PageMask p;
-  p.n_include = m->n_include;
-  p.n_exclude = m->n_exclude;
-  for (int i = 0; i < PA_MAX_TERMS; ++i) p.terms[i] = m->terms[i];
-  return p;
-}
+static PageMask<const pa_term*> of(const pa_mask* m) { return {m->n_include, m->n_exclude, m->terms}; }
 extern "C" {
 int verdict(const pa_mask* m, int q0, int q1, int k0, int k1) { return mask_verdict(of(m), q0, q1, k0, k1); }
 unsigned word(const pa_mask* m, int q, int k0, int len) { return mask_word(of(m), q, k0, len); }
