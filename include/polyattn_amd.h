@@ -516,8 +516,9 @@ int pa_attn_bwd(const pa_attn_bwd_args* args, void* stream);
  * counts as dead.  Rows of no request are left as they are.  lse may be NULL (natural log,
  * [T, Hq] at lse_st, lse_sh).  max_fresh: the most new tokens of a request (a hint: it selects
  * kernels and moves no result beyond rounding).  D = 64 or 128, f32 / f16 / bf16, scale > 0.
- * workspace: the bytes pa_paged_workspace gives for the same sizes, 256-byte aligned, not
- * shared by calls that overlap. */
+ * workspace: the bytes pa_paged_workspace gives for the same sizes, 256-byte aligned, the first
+ * zero_bytes of them zero before the first call with it and left zero by every call (of the same
+ * sizes); not shared by calls that overlap. */
 typedef struct pa_tables_args {
   const int32_t* before;
   const int32_t* fresh;
@@ -575,7 +576,7 @@ typedef struct pa_paged_args {
   int64_t workspace_bytes;
 } pa_paged_args;
 
-int pa_paged_workspace(const pa_paged_args* args, int64_t* bytes);
+int pa_paged_workspace(const pa_paged_args* args, int64_t* bytes, int64_t* zero_bytes);
 int pa_paged_attn(const pa_paged_args* args, void* stream);
 
 #ifdef __cplusplus

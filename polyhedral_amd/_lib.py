@@ -127,7 +127,7 @@ SIGNATURES = {
     "pa_page_release": (ctypes.c_int, [c_vp, c_vp, c_i32, c_vp, c_i64, c_i32, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp]),
     "pa_paged_append": (ctypes.c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64,
                                        c_i32, c_i32, c_i32, c_i32, c_vp]),
-    "pa_paged_workspace": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), ctypes.POINTER(c_i64)]),
+    "pa_paged_workspace": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), ctypes.POINTER(c_i64), ctypes.POINTER(c_i64)]),
     "pa_paged_attn": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), c_vp]),
 }
 

@@ -7,32 +7,28 @@
 namespace pa {
 namespace {
 
-constexpr int kTarget = 512;   // units that the splits of a call aim for
-constexpr int kFewRows = 32;   // rows of a request (new tokens times heads of a group) up to which
-                               // the 16-row kernel takes it
+constexpr int kTarget = 512;   // units that the splits of a kernel's part aim for
+constexpr int kFewRows = 16;   // rows of a request (new tokens times heads of a group) up to which
+                               // it is a tile of few rows
 
-struct Part {           // one kernel's share of a call
-  int64_t max_tiles;    // tiles of all requests, at most
-  int64_t slots, o_bytes, bytes;
-};
-
+// Workspace: the counts of both parts, then their slots.
 struct PagedPlan {
   int page_lg;
-  bool tile;            // some request may have more than kFewRows rows, for paged_tile_kernel
-  Part rows, tiles;
+  bool tile;            // some request may have more than kFewRows rows
+  PagedPart rows, tiles;
+  int64_t zero, bytes;
 };
 
-Part part_of(const pa_paged_args* x, int BM) {
-  Part p;
-  const int64_t some = x->T < x->R ? x->T : x->R;  // requests with rows, at most
-  p.max_tiles = x->T * (x->Hq / x->Hkv) / BM + some;
-  const int64_t units = kTarget + p.max_tiles * x->Hkv;
-  // (a tile is split into two shares at least, and then has less than twice the shares that its
-  // blocks fill)
-  p.slots = 2 * kTarget < units ? 2 * kTarget : units;
-  p.o_bytes = p.slots * BM * x->D * 4;
-  p.bytes = p.o_bytes + p.slots * BM * 2 * 4;
-  return p;
+// A part whose requests have at most max_tiles tiles: its grid and slots.  (The shares of all tiles are
+// at most kTarget and one more for each tile and KV head; a tile that is split has two shares at
+// least, and then less than twice those that its blocks fill.)
+int part_of(const pa_paged_args* x, int64_t max_tiles, PagedPart* p) {
+  const int64_t grid = kTarget + max_tiles * x->Hkv;
+  PA_CHECK_ARG(grid <= 0x3fffffffll, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)grid);
+  p->grid = (int32_t)grid;
+  p->slots = (int32_t)(2 * kTarget < grid ? 2 * kTarget : grid);
+  p->target = kTarget;
+  return PA_OK;
 }
 
 int plan_of(const pa_paged_args* x, PagedPlan* p) {
@@ -48,23 +44,35 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   PA_CHECK_ARG(x->cols >= 0 && ((int64_t)x->cols << p->page_lg) <= kMaxPosition && x->pitch >= x->cols,
                "pa_paged_attn: %d columns of %d, pitch %lld", x->cols, x->page_size, (long long)x->pitch);
   PA_CHECK_ARG(x->scale > 0.f && x->scale < INFINITY, "pa_paged_attn: scale=%g must be positive", (double)x->scale);
-  p->tile = x->dtype != PA_F32 && x->n_pages > 0 && x->max_fresh * (x->Hq / x->Hkv) > kFewRows;
-  p->rows = part_of(x, kRows);
-  p->tiles = part_of(x, kTileRows);
+  const int64_t G = x->Hq / x->Hkv, some = x->T < x->R ? x->T : x->R;  // some: requests with rows, at most
+  p->tile = x->dtype != PA_F32 && x->n_pages > 0 && x->max_fresh * G > kFewRows;
+  int64_t few = x->T * G / kRows + some;
+  if (p->tile && few > some * (kFewRows / kRows)) few = some * (kFewRows / kRows);
+  if (int rc = part_of(x, few, &p->rows)) return rc;
+  p->rows.least = 8;
+  p->rows.row_min = 0;
+  p->rows.row_max = p->tile ? kFewRows : INT_MAX;
+  p->tiles = PagedPart{};
+  if (p->tile) {
+    if (int rc = part_of(x, x->T * G / kTileRows + some, &p->tiles)) return rc;
+    p->tiles.least = 4;
+    p->tiles.row_min = kFewRows;
+    p->tiles.row_max = INT_MAX;
+  }
+  p->zero = (4 * ((int64_t)p->rows.slots + p->tiles.slots) + 255) / 256 * 256;
+  p->bytes = p->zero + 4ll * p->rows.slots * slot_floats(kRows, x->D) + 4ll * p->tiles.slots * slot_floats(kTileRows, x->D);
   return PA_OK;
 }
-
-// (the kernels of a call run one after the other and share the workspace)
-int64_t bytes_of(const PagedPlan& p) { return p.tile && p.tiles.bytes > p.rows.bytes ? p.tiles.bytes : p.rows.bytes; }
 
 }  // namespace
 }  // namespace pa
 
-extern "C" int pa_paged_workspace(const pa_paged_args* x, int64_t* bytes) {
+extern "C" int pa_paged_workspace(const pa_paged_args* x, int64_t* bytes, int64_t* zero) {
   pa::PagedPlan p;
   if (int rc = pa::plan_of(x, &p)) return rc;
-  PA_CHECK_ARG(bytes, "pa_paged_workspace: null output");
-  *bytes = pa::bytes_of(p);
+  PA_CHECK_ARG(bytes && zero, "pa_paged_workspace: null output");
+  *bytes = p.bytes;
+  *zero = p.zero;
   return PA_OK;
 }
 
@@ -90,8 +98,8 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
   PA_CHECK_ARG(x->q_st >= 0 && x->q_sh >= 0 && x->o_st >= 0 && x->o_sh >= 0 && x->c_sp >= 0 && x->c_sh >= 0 &&
                    x->c_sn >= x->D && x->c_sn <= (1 << 21),
                "pa_paged_attn: negative strides, or cache rows closer than D or further than 2^21");
-  PA_CHECK_ARG(x->workspace && reinterpret_cast<uintptr_t>(x->workspace) % 256 == 0 && x->workspace_bytes >= bytes_of(p),
-               "pa_paged_attn: needs a 256-byte aligned workspace of %lld bytes", (long long)bytes_of(p));
+  PA_CHECK_ARG(x->workspace && reinterpret_cast<uintptr_t>(x->workspace) % 256 == 0 && x->workspace_bytes >= p.bytes,
+               "pa_paged_attn: needs a 256-byte aligned workspace of %lld bytes", (long long)p.bytes);
   PagedK a;
   a.q = static_cast<const char*>(x->q);
   a.q_st = x->q_st * esz;
@@ -129,22 +137,14 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
   a.lse = x->lse;
   a.lse_st = x->lse_st;
   a.lse_sh = x->lse_sh;
-  a.part_o = static_cast<float*>(x->workspace);
-  a.target = kTarget;
+  a.tiles = p.tiles;
+  a.rows = p.rows;
+  char* ws = static_cast<char*>(x->workspace);
+  a.rows.count = reinterpret_cast<int32_t*>(ws);
+  a.tiles.count = a.rows.count + p.rows.slots;
+  a.rows.part = ws + p.zero;
+  a.tiles.part = a.rows.part + 4ll * p.rows.slots * slot_floats(kRows, x->D);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  auto with = [&](const Part& part) {
-    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(x->workspace) + part.o_bytes);
-    a.slots = (int32_t)part.slots;
-  };
-  with(p.rows);
-  a.least = 8;
-  a.row_min = 0;
-  a.row_max = p.tile ? kFewRows : INT_MAX;
-  if (int rc = launch_paged_rows(a, x->dtype, x->D, p.rows.max_tiles, s)) return rc;
-  if (!p.tile) return PA_OK;
-  with(p.tiles);
-  a.least = 4;
-  a.row_min = kFewRows;
-  a.row_max = INT_MAX;
-  return launch_paged_tile(a, x->dtype, x->D, p.tiles.max_tiles, s);
+  if (x->dtype == PA_F32) return launch_paged_f32(a, x->D, s);
+  return x->dtype == PA_BF16 ? launch_paged_bf16(a, x->D, s) : launch_paged_f16(a, x->D, s);
 }

@@ -1,5 +1,5 @@
-// Attention over a paged cache: the arguments its kernels share, and how their work-groups find
-// their work.
+// Attention over a paged cache: the arguments its kernels share, how their work-groups find their
+// work, and how the shares of a split tile become one.
 //
 // Query rows of a request are its new tokens times the G = Hq / Hkv heads that share a KV head
 // (row i: token i / G, head i % G), cut into tiles of BM rows.  A unit of work is one tile, one
@@ -7,7 +7,10 @@
 // it.  Lengths are on the device, so every wave works out the split itself: a first pass over
 // the requests sums tiles x blocks, which gives the blocks of a share, and a second one finds
 // the unit's request (both are one load and a few scans for up to 64 requests).
-// A request whose tiles are split has a slot of the workspace per unit, numbered in unit order.
+//
+// The units of a split tile write their states to slots of the workspace, count themselves, and the
+// last one merges them all, in the order of the shares whichever it is.  (A second launch that
+// merges took 5 us where nothing was split, and 30 to 70 behind large grids of chunks.)
 #pragma once
 
 #include <stddef.h>
@@ -16,6 +19,17 @@
 #include "page_math.hpp"
 
 namespace pa {
+
+// What one of the two kernels' bodies does in a call.
+struct PagedPart {
+  char* part;           // [slots] states of split tiles' units
+  int32_t* count;       // [slots] units done, at a tile's first slot; zero between calls
+  int32_t slots;
+  int32_t target;       // units that the splits aim for
+  int32_t least;        // least blocks of a share
+  int32_t row_min, row_max;  // requests with row_min < rows <= row_max
+  int32_t grid;
+};
 
 struct PagedK {
   const char* q;
@@ -37,12 +51,7 @@ struct PagedK {
   int64_t o_st, o_sh;
   float* lse;
   int64_t lse_st, lse_sh;  // elements
-  float* part_o;   // [slots][BM][D]: unnormalised
-  float* part_ml;  // [slots][BM][2]: maximum (tiles of 128 rows: times c) and sum
-  int32_t slots;
-  int32_t target;     // units a split aims for
-  int32_t least;      // least blocks of a share
-  int32_t row_min, row_max;  // requests with row_min < rows <= row_max are this kernel's
+  PagedPart tiles, rows;
 };
 
 // The mask of a kernel whose first argument is a PagedK.
@@ -61,99 +70,115 @@ struct Work {
 struct Unit {
   bool found;
   Request rq;
-  int32_t r, tile, tiles, h, split, splits;
-  int32_t slot;   // of this unit (merge: of the group's first unit)
+  int32_t r, tile, h, split, splits;
+  int32_t slot;  // of the tile's first share
 };
-
-__device__ __forceinline__ Request load_request(const PagedK& a, int r) {
-  return request_of(a.q_start[r], a.q_start[r + 1], a.lengths[r], a.T, a.cols << a.page_lg);
-}
 
 // Tiles of a request and blocks of 1 << LG keys of its last whole one (a causal mask's longest).
 template <int BM, int LG>
-__device__ __forceinline__ Work work_of(const PagedK& a, const Request& q) {
+__device__ __forceinline__ Work work_of(const PagedK& a, const PagedPart& p, const Request& q) {
   const int32_t rows = q.n * a.G;
-  if (rows <= a.row_min || rows > a.row_max) return {0, 0};
+  if (rows <= p.row_min || rows > p.row_max) return {0, 0};
   const int32_t span = imin(q.n, (BM + a.G - 1) / a.G + 1);
   return {(rows + BM - 1) / BM, key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG).count()};
 }
 
-__device__ __forceinline__ int32_t wave_scan(int32_t x, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int32_t y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
+// Sum over lanes 0 .. l, by DPP moves inside rows of 16 lanes and broadcasts of their last ones.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int32_t dpp_move(int32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int32_t wave_scan(int32_t x) {
+  x += dpp_move<0x111, 0xf>(x);
+  x += dpp_move<0x112, 0xf>(x);
+  x += dpp_move<0x114, 0xf>(x);
+  x += dpp_move<0x118, 0xf>(x);
+  x += dpp_move<0x142, 0xa>(x);
+  x += dpp_move<0x143, 0xc>(x);
   return x;
 }
+__device__ __forceinline__ float wave_total(float x) {
+  auto add = [&](int32_t y) __attribute__((always_inline)) { x += __builtin_bit_cast(float, y); };
+  add(dpp_move<0x111, 0xf>(__builtin_bit_cast(int32_t, x)));
+  add(dpp_move<0x112, 0xf>(__builtin_bit_cast(int32_t, x)));
+  add(dpp_move<0x114, 0xf>(__builtin_bit_cast(int32_t, x)));
+  add(dpp_move<0x118, 0xf>(__builtin_bit_cast(int32_t, x)));
+  add(dpp_move<0x142, 0xa>(__builtin_bit_cast(int32_t, x)));
+  add(dpp_move<0x143, 0xc>(__builtin_bit_cast(int32_t, x)));
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int32_t, x), 63));
+}
 
-// Unit (GROUP: the group of all splits of a tile and head, of tiles with more than one) `id`.
-template <int BM, int LG, bool GROUP>
-__device__ __forceinline__ Unit find_unit(const PagedK& a, int32_t id, int lane) {
+// Request r0 + lane (past R: none).  `end`: the largest start so far.  Starts that fall back are
+// taken as that, so whatever q_start holds the requests' rows are disjoint, and the units and slots
+// stay within what the host sized for T rows.
+__device__ __forceinline__ Request load_request(const PagedK& a, int r0, int lane, int32_t& end) {
+  const int r = r0 + lane;
+  int32_t s0 = 0, s1 = 0, len = 0;
+  if (r < a.R) {
+    s0 = a.q_start[r];
+    s1 = a.q_start[r + 1];
+    len = a.lengths[r];
+  }
+  s0 = imin(imax(s0, 0), a.T);
+  s1 = imin(imax(s1, 0), a.T);
+  if (__ballot(r < a.R && (s1 < s0 || s0 < end)) != 0ull) {
+    s0 = imax(s0, end);
+#pragma unroll 1
+    for (int o = 1; o < 64; o <<= 1) {
+      const int32_t y = __shfl_up(s0, o);
+      if (lane >= o) s0 = imax(s0, y);
+    }
+    s1 = imax(s1, s0);
+  }
+  end = __builtin_amdgcn_readlane(s1, imin(a.R - 1 - r0, 63));
+  return request_of(s0, s1, len, a.T, a.cols << a.page_lg);
+}
+
+template <int BM, int LG>
+__device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, int32_t id, int lane) {
   Unit u;
   u.found = false;
   Request q{0, 0, 0};
   Work w{0, 0};
   float total = 0.f;  // (a share needs no exact total)
+  int32_t end = 0;
   for (int r0 = 0; r0 < a.R; r0 += 64) {
-    const int r = r0 + lane;
-    w = {0, 0};
-    if (r < a.R) {
-      q = load_request(a, r);
-      w = work_of<BM, LG>(a, q);
-    }
-    total += (float)w.tiles * (float)w.blocks;
+    q = load_request(a, r0, lane, end);
+    w = work_of<BM, LG>(a, p, q);
+    total += wave_total((float)w.tiles * (float)w.blocks);
   }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o);
   // (rounded up, so the units stay within target + tiles Hkv, which the grid is sized for)
-  const float share = total * (float)a.Hkv / (float)a.target * 1.0001f;
-  const int32_t chunk = imax(a.least, share < 1e9f ? (int32_t)share + 1 : (1 << 30));
+  const float share = total * (float)a.Hkv / (float)p.target * 1.0001f;
+  const int32_t chunk = imax(p.least, share < 1e9f ? (int32_t)share + 1 : (1 << 30));
 
-  int32_t before = 0, slot = 0;  // units (groups) and slots of earlier requests
+  int32_t before = 0, slot = 0;  // units and slots of earlier requests
+  end = 0;
   for (int r0 = 0; r0 < a.R; r0 += 64) {
-    const int r = r0 + lane;
     if (a.R > 64) {
-      w = {0, 0};
-      if (r < a.R) {
-        q = load_request(a, r);
-        w = work_of<BM, LG>(a, q);
-      }
+      q = load_request(a, r0, lane, end);
+      w = work_of<BM, LG>(a, p, q);
     }
     const int32_t splits = imax((w.blocks + chunk - 1) / chunk, 1);
     const int32_t units = w.tiles * a.Hkv * splits, mine = splits > 1 ? units : 0;
-    const int32_t n = GROUP ? (splits > 1 ? w.tiles * a.Hkv : 0) : units;
-    const int32_t n_in = wave_scan(n, lane), s_in = wave_scan(mine, lane);
-    const int32_t at = before + n_in - n;
-    const uint64_t hit = __ballot(at <= id && id < at + n);
+    const int32_t n_in = wave_scan(units), s_in = wave_scan(mine);
+    const int32_t at = before + n_in - units;
+    const uint64_t hit = __ballot(at <= id && id < at + units);
     if (hit) {
       const int l = (int)__builtin_ctzll(hit);
       auto get = [&](int32_t x) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(x, l); };
       u.found = true;
       u.r = r0 + l;
       u.rq = {get(q.start), get(q.n), get(q.len)};
-      u.tiles = get(w.tiles);
       u.splits = get(splits);
-      int32_t x = id - get(at);
-      const int32_t s0 = slot + get(s_in - mine);
-      if (GROUP) {
-        u.tile = x / a.Hkv;
-        u.h = x - u.tile * a.Hkv;
-        u.split = 0;
-        u.slot = s0 + x * u.splits;
-      } else {
-        // a KV head's shares side by side, its tiles a multiple of Hkv units apart: with 8 KV heads
-        // the tiles of one fall on one XCD (work-groups are dealt to the XCDs in turn) and share
-        // its L2
-        const int32_t per = a.Hkv * u.splits;
-        u.tile = x / per;
-        u.slot = s0 + x;
-        x -= u.tile * per;
-        u.h = x / u.splits;
-        u.split = x - u.h * u.splits;
-      }
+      // a KV head's shares side by side, its tiles a multiple of Hkv units apart: with 8 KV heads
+      // the tiles of one fall on one XCD (work-groups are dealt to the XCDs in turn) and share
+      // its L2
+      const int32_t x = id - get(at), per = a.Hkv * u.splits, tile = x / per, y = x - tile * per;
+      u.h = y / u.splits;
+      u.split = y - u.h * u.splits;
+      u.slot = slot + get(s_in - mine) + x - u.split;
       // (a causal mask's longest tile first)
-      u.tile = u.tiles - 1 - u.tile;
+      u.tile = get(w.tiles) - 1 - tile;
       return u;
     }
     before += __builtin_amdgcn_readlane(n_in, 63);
@@ -169,18 +194,54 @@ __device__ __forceinline__ void share_of(int32_t n, int32_t split, int32_t split
   *j1 = *j0 + per + (split < more ? 1 : 0);
 }
 
-int check_pages(const char* who, int64_t n_pages, int32_t page_size, int* page_lg);
+// The states of a tile's shares pass from one work-group to another, maybe on another XCD, whose L2
+// does not see this one's: agent-scope stores and loads go past it, and a store is complete (the
+// wait below) before the tile's count says so.
+__device__ __forceinline__ void share_store(float* p, float x) {
+  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float share_load(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x4 share_load4(const char* p) {
+  const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const uint64_t y = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p) + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return f32x4{__builtin_bit_cast(float, (uint32_t)x), __builtin_bit_cast(float, (uint32_t)(x >> 32)),
+               __builtin_bit_cast(float, (uint32_t)y), __builtin_bit_cast(float, (uint32_t)(y >> 32))};
+}
+__device__ __forceinline__ void share_store4(char* p, f32x4 x) {
+  const u32x4 y = __builtin_bit_cast(u32x4, x);
+  store_x4_sc1(p, y.x, y.y, y.z, y.w);
+}
+// After its stores by the whole work-group: whether this is the tile's last share (told through
+// `flag` in LDS).  The last one clears the count for the next call.
+__device__ __forceinline__ bool last_share(const PagedPart& p, const Unit& u, int tid, int32_t* flag) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    const int32_t n = __hip_atomic_fetch_add(p.count + u.slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = n == u.splits - 1;
+    if (n == u.splits - 1) __hip_atomic_store(p.count + u.slot, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return *flag != 0;
+}
 
 // The maximum m of a row's scores so far as the base of its exponentials: 0 for -inf (no live key
 // so far; every score is -inf then).
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-constexpr int kRows = 16;       // query rows of a tile of paged_rows_kernel
-constexpr int kTileRows = 128;  // and of paged_tile_kernel
-constexpr int kTileLg = 6;      // log2 keys of a step of paged_tile_kernel
+constexpr int kRows = 16;       // query rows of a tile of few rows
+constexpr int kTileRows = 128;  // and of a chunk's tile
+constexpr int kTileLg = 6;      // log2 keys of a step of a chunk's tile
+// floats of a slot: O of every row, then maximum and sum
+constexpr int slot_floats(int BM, int D) { return BM * (D + 2); }
 
-int launch_paged_rows(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s);
-int launch_paged_tile(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s);
-int launch_paged_tile_merge(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s);
+int check_pages(const char* who, int64_t n_pages, int32_t page_size, int* page_lg);
+
+// Launches the parts whose grid is not 0.
+int launch_paged_bf16(const PagedK& a, int D, hipStream_t s);
+int launch_paged_f16(const PagedK& a, int D, hipStream_t s);
+int launch_paged_f32(const PagedK& a, int D, hipStream_t s);
 
 }  // namespace pa

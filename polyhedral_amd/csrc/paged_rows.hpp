@@ -21,6 +21,8 @@
 // where a step is masked for some row and its V rows hold an infinity or NaN, the products are
 // taken key by key and added to the rows that the key is live for (a product with a zero would be
 // NaN).
+#pragma once
+
 #include <math.h>
 
 #include <type_traits>
@@ -82,21 +84,19 @@ struct RowsShape {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2)))
-void paged_rows_kernel(const PagedK a) {
+__device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* smem, int32_t* flag) {
   using S = RowsShape<T, D>;
   constexpr bool F32 = S::F32;
   constexpr int NS = S::NS, PER = S::PER, ROW = S::ROW, ESZ = sizeof(T);
   constexpr int NB = D / 16;                       // blocks of 16 output columns
   constexpr int NK = F32 ? D / 16 : D / 32;        // 16-byte units of a K or Q row that a lane holds
   constexpr int SEG = 16 * ROW, STAGE = 2 * SEG;
-
-  __shared__ __attribute__((aligned(256))) char smem[S::SMEM];
+  const PagedPart& part = a.rows;
 
   const int tid = threadIdx.x, lane = tid & 63, q16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const Unit u = find_unit<kRows, S::LG, false>(a, (int32_t)blockIdx.x, lane);
+  const Unit u = find_unit<kRows, S::LG>(a, part, id, lane);
   if (!u.found) return;
 
   // ---- the tile's rows -----------------------------------------------------------
@@ -394,7 +394,7 @@ void paged_rows_kernel(const PagedK a) {
     compute(0, s0, d0);
   }
 
-  // ---- the waves' states become one ------------------------------------------------
+  // ---- the waves' states become one, and those of the tile's shares ---------------------
   const float l_own = quad_sum(l_part);
   __syncthreads();  // every wave is past its ring
   float* red_o = reinterpret_cast<float*>(smem);                 // [wave][row][OP]
@@ -406,39 +406,74 @@ void paged_rows_kernel(const PagedK a) {
     red_ml[2 * (w * kRows + q16)] = m_run;
     red_ml[2 * (w * kRows + q16) + 1] = l_own;
   }
-  __syncthreads();
   // thread: a row and D / 16 of its columns
   constexpr int CPT = D / 16;
   const int row = tid >> 4, c0 = (tid & 15) * CPT;
-  if (row >= n_rows) return;
-  float mw[kWaves], M = -INFINITY, L = 0.f;
+  float M, L, out[CPT];
+  auto gather = [&]() __attribute__((always_inline)) {
+    __syncthreads();
+    float mw[kWaves];
+    M = -INFINITY;
+    L = 0.f;
 #pragma unroll
-  for (int x = 0; x < kWaves; ++x) {
-    mw[x] = red_ml[2 * (x * kRows + row)];
-    M = nan_max(M, mw[x]);
-  }
-  float out[CPT];
-#pragma unroll
-  for (int e = 0; e < CPT; ++e) out[e] = 0.f;
-#pragma unroll
-  for (int x = 0; x < kWaves; ++x) {
-    const float f = __builtin_amdgcn_exp2f((mw[x] - base_of(M)) * a.c);
-    L += f * red_ml[2 * (x * kRows + row) + 1];
-#pragma unroll
-    for (int e = 0; e < CPT; ++e) out[e] += f * red_o[(x * kRows + row) * S::OP + c0 + e];
-  }
-  if (u.splits > 1) {
-    if (u.slot >= a.slots) return;  // (not reached by starts in order)
-    float* po = a.part_o + ((int64_t)u.slot * kRows + row) * D + c0;
-#pragma unroll
-    for (int e = 0; e < CPT; e += 4) *reinterpret_cast<f32x4*>(po + e) = f32x4{out[e], out[e + 1], out[e + 2], out[e + 3]};
-    if (c0 == 0) {
-      float* ml = a.part_ml + 2 * ((int64_t)u.slot * kRows + row);
-      ml[0] = M;
-      ml[1] = L;
+    for (int x = 0; x < kWaves; ++x) {
+      mw[x] = red_ml[2 * (x * kRows + row)];
+      M = nan_max(M, mw[x]);
     }
-    return;
+#pragma unroll
+    for (int e = 0; e < CPT; ++e) out[e] = 0.f;
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) {
+      const float f = __builtin_amdgcn_exp2f((mw[x] - base_of(M)) * a.c);
+      L += f * red_ml[2 * (x * kRows + row) + 1];
+#pragma unroll
+      for (int e = 0; e < CPT; ++e) out[e] += f * red_o[(x * kRows + row) * S::OP + c0 + e];
+    }
+  };
+  gather();
+  if (u.splits > 1) {
+    constexpr int SLOT_B = slot_floats(kRows, D) * 4, ML = kRows * D * 4;
+    char* first = part.part + (int64_t)u.slot * SLOT_B;  // of the tile's shares
+    if (row < n_rows) {
+      char* own = first + (int64_t)u.split * SLOT_B;
+#pragma unroll
+      for (int e = 0; e < CPT; e += 4)
+        share_store4(own + (row * D + c0 + e) * 4, f32x4{out[e], out[e + 1], out[e + 2], out[e + 3]});
+      if (c0 == 0) {
+        share_store(reinterpret_cast<float*>(own + ML) + 2 * row, M);
+        share_store(reinterpret_cast<float*>(own + ML) + 2 * row + 1, L);
+      }
+    }
+    if (!last_share(part, u, tid, flag)) return;
+    // every fourth share to a wave, four rows at a time; then as the waves' states above
+    const int col = (lane & 15) * CPT;
+    for (int r = lane >> 4; r - (lane >> 4) < n_rows; r += 4) {
+      const char* ml = first + ML + 8 * r;
+      const char* po = first + (r * D + col) * 4;
+      float m = -INFINITY, l = 0.f;
+#pragma unroll 4
+      for (int s = w; s < u.splits; s += kWaves) m = nan_max(m, share_load(reinterpret_cast<const float*>(ml + (int64_t)s * SLOT_B)));
+      f32x4 x[CPT / 4];
+#pragma unroll
+      for (int e = 0; e < CPT / 4; ++e) x[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int s = w; s < u.splits; s += kWaves) {
+        const float* at = reinterpret_cast<const float*>(ml + (int64_t)s * SLOT_B);
+        const float f = __builtin_amdgcn_exp2f((share_load(at) - base_of(m)) * a.c);
+        l += f * share_load(at + 1);
+#pragma unroll
+        for (int e = 0; e < CPT / 4; ++e) x[e] += f * share_load4(po + (int64_t)s * SLOT_B + 16 * e);
+      }
+#pragma unroll
+      for (int e = 0; e < CPT / 4; ++e) *reinterpret_cast<f32x4*>(red_o + (w * kRows + r) * S::OP + col + 4 * e) = x[e];
+      if (col == 0) {
+        red_ml[2 * (w * kRows + r)] = m;
+        red_ml[2 * (w * kRows + r) + 1] = l;
+      }
+    }
+    gather();
   }
+  if (row >= n_rows) return;
   const int ir = i0 + row, t_r = ir / a.G, h_r = u.h * a.G + (ir - t_r * a.G);
   const float inv = L == 0.f ? 0.f : 1.f / L;
   char* orow = a.o + (int64_t)(u.rq.start + t_r) * a.o_st + (int64_t)h_r * a.o_sh;
@@ -449,95 +484,5 @@ void paged_rows_kernel(const PagedK a) {
     a.lse[(int64_t)(u.rq.start + t_r) * a.lse_st + (int64_t)h_r * a.lse_sh] = L == 0.f ? -INFINITY : (M * a.c + log2f(L)) * kLn2;
 }
 
-// The shares of a split tile become its rows: a wave per row, a share's maximum and sum per lane
-// for the weights, then the shares' rows, lanes along the columns.  The order of the sums is that of
-// the shares.
-// C: maxima are unscaled.
-template <typename T, int D, int BM, int LG, bool C>
-__global__ __launch_bounds__(64 * kRows) void paged_merge_kernel(const PagedK a) {
-  constexpr int CPL = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int row = (int)blockIdx.y * kRows + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const float c = C ? a.c : 1.f;
-  const Unit u = find_unit<BM, LG, true>(a, (int32_t)blockIdx.x, lane);
-  if (!u.found || u.slot + u.splits > a.slots) return;
-  const int ir = u.tile * BM + row;
-  if (ir >= u.rq.n * a.G) return;
-  typedef float fv __attribute__((ext_vector_type(CPL)));
-  const float* ml = a.part_ml + 2 * ((int64_t)u.slot * BM + row);
-  const float* po = a.part_o + ((int64_t)u.slot * BM + row) * D + CPL * lane;
-  float M = -INFINITY, L = 0.f;
-  for (int s = lane; s < u.splits; s += 64) M = nan_max(M, ml[(int64_t)s * 2 * BM]);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) M = nan_max(M, __shfl_xor(M, o));
-  fv out = {};
-  for (int s0 = 0; s0 < u.splits; s0 += 64) {
-    const int s = s0 + lane;
-    float f = 0.f;
-    if (s < u.splits) {
-      f = __builtin_amdgcn_exp2f((ml[(int64_t)s * 2 * BM] - base_of(M)) * c);
-      L += f * ml[(int64_t)s * 2 * BM + 1];
-    }
-    const int n = imin(u.splits - s0, 64);
-    for (int b = 0; b < n; b += 16) {
-      fv x[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        x[e] = b + e < n ? *reinterpret_cast<const fv*>(po + (int64_t)(s0 + b + e) * BM * D) : fv{};
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        out += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), (b + e) & 63)) * x[e];
-    }
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) L += __shfl_xor(L, o);
-  const int tok = ir / a.G, head = u.h * a.G + (ir - tok * a.G);
-  out *= L == 0.f ? 0.f : 1.f / L;
-  T* orow = reinterpret_cast<T*>(a.o + (int64_t)(u.rq.start + tok) * a.o_st + (int64_t)head * a.o_sh) + CPL * lane;
-#pragma unroll
-  for (int e = 0; e < CPL; ++e) orow[e] = (T)out[e];
-  if (a.lse && lane == 0)
-    a.lse[(int64_t)(u.rq.start + tok) * a.lse_st + (int64_t)head * a.lse_sh] = L == 0.f ? -INFINITY : (M * c + log2f(L)) * kLn2;
-}
-
-template <typename T, int D>
-int launch_rows_t(const PagedK& a, int64_t max_tiles, hipStream_t s) {
-  // (units: at most target, and one more for every tile and KV head)
-  const int64_t grid = a.target + max_tiles * a.Hkv;
-  PA_CHECK_ARG(grid <= 0x7fffffffll, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)grid);
-  hipLaunchKernelGGL((paged_rows_kernel<T, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
-  PA_LAUNCH_CHECK("paged_rows_kernel");
-  // (a split tile has two shares at least)
-  const int64_t groups = max_tiles * a.Hkv < a.target ? max_tiles * a.Hkv : a.target;
-  hipLaunchKernelGGL((paged_merge_kernel<T, D, kRows, RowsShape<T, D>::LG, true>), dim3((unsigned)groups), dim3(64 * kRows),
-                     0, s, a);
-  PA_LAUNCH_CHECK("paged_merge_kernel");
-  return PA_OK;
-}
-
-template <typename T, int D>
-int launch_tile_merge_t(const PagedK& a, int64_t max_tiles, hipStream_t s) {
-  const int64_t groups = max_tiles * a.Hkv < a.target ? max_tiles * a.Hkv : a.target;
-  hipLaunchKernelGGL((paged_merge_kernel<T, D, kTileRows, kTileLg, false>), dim3((unsigned)groups, kTileRows / kRows),
-                     dim3(64 * kRows), 0, s, a);
-  PA_LAUNCH_CHECK("paged_merge_kernel");
-  return PA_OK;
-}
-
 }  // namespace
-
-int launch_paged_rows(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s) {
-  if (dtype == PA_BF16)
-    return D == 64 ? launch_rows_t<__bf16, 64>(a, max_tiles, s) : launch_rows_t<__bf16, 128>(a, max_tiles, s);
-  if (dtype == PA_F16)
-    return D == 64 ? launch_rows_t<_Float16, 64>(a, max_tiles, s) : launch_rows_t<_Float16, 128>(a, max_tiles, s);
-  return D == 64 ? launch_rows_t<float, 64>(a, max_tiles, s) : launch_rows_t<float, 128>(a, max_tiles, s);
-}
-
-int launch_paged_tile_merge(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s) {
-  if (dtype == PA_BF16)
-    return D == 64 ? launch_tile_merge_t<__bf16, 64>(a, max_tiles, s) : launch_tile_merge_t<__bf16, 128>(a, max_tiles, s);
-  return D == 64 ? launch_tile_merge_t<_Float16, 64>(a, max_tiles, s) : launch_tile_merge_t<_Float16, 128>(a, max_tiles, s);
-}
-
 }  // namespace pa

@@ -11,13 +11,18 @@
 //
 // The blocks of keys that may be live for the tile are a list of two ranges (page_math.hpp); its
 // entries are held 16 steps at a time, a segment per lane, with each wave's verdicts on its own
-// rows.  Steps that are all live for a wave take the straight line.  The others mask by words of 32
-// keys computed from the mask's terms, leave blocks out that are dead for the wave, and, where a
-// masked block's V rows hold an infinity or NaN, take the products key by key, added only to the rows
-// that the key is live for: a dead key contributes nothing whatever it holds.
+// rows; a step that is not all live for a wave is masked by words of 32 keys computed from the mask's
+// terms, and its dead pairs have P = 0.
+//
+// A dead key contributes nothing whatever it holds, but 0 times an infinity or NaN in its V row is
+// NaN.  That shows in the sums, so a work-group whose sums are not finite takes its list again, step
+// by step, and where a masked chunk of 16 keys has V rows that are not finite it takes the products
+// key by key, added only to the rows that the key is live for.
 //
 // Scores, maxima, sums and O are float32; P is rounded to 16 bits as an MFMA operand only, its sum
 // taken before.
+#pragma once
+
 #include <math.h>
 
 #include <type_traits>
@@ -34,20 +39,25 @@ __device__ __forceinline__ bool not_finite16(uint32_t lo, uint32_t hi) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
-void paged_tile_kernel(const PagedK a) {
+struct TileShape {
+  static constexpr int SLOT = 64 * Rows<D>::ROW;   // a step's K or V
+  static constexpr int SMEM = 4 * SLOT;            // aligned to two slots
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* smem, int32_t* flag) {
   using Frag = typename Mma<T>::frag;
   using R = Rows<D>;
   constexpr int ESZ = 2, NQF = D / 16, NDB = D / 32;
-  constexpr int SLOT = 64 * R::ROW;          // a step's K or V
+  constexpr int SLOT = TileShape<T, D>::SLOT;
   constexpr int VRING = 0, KRING = 2 * SLOT;
-  __shared__ __attribute__((aligned(2 * SLOT))) char smem[4 * SLOT];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char_t*)smem;
+  const PagedPart& part = a.tiles;
 
   const int tid = threadIdx.x, lane = tid & 63, G = lane >> 5, m = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const Unit u = find_unit<kTileRows, kTileLg, false>(a, (int32_t)blockIdx.x, lane);
+  const Unit u = find_unit<kTileRows, kTileLg>(a, part, id, lane);
   if (!u.found) return;
 
   // ---- rows ------------------------------------------------------------------------
@@ -134,8 +144,11 @@ void paged_tile_kernel(const PagedK a) {
 #pragma unroll
   for (int x = 0; x < NDB; ++x) acc[x] = f32x16{0};
   float m_run = -INFINITY, l_part = 0.f;  // (log2 units)
-  f32x16 sc0 = {}, sc1 = {};
-  uint32_t wd0 = 0u, wd1 = 0u;            // the current step's words of this lane's row, where it is masked
+  f32x16 sa0 = {}, sa1 = {}, sb0 = {}, sb1 = {};  // scores of the current step and the next, in turn
+  // (held in a register: a scalar load of an argument inside the loop would wait for the LDS reads
+  // in flight)
+  float c_exp = a.c;
+  asm volatile("" : "+s"(c_exp));
 
   // Scores of both blocks of the step in the K slot that the row reads are on.
   auto qk = [&](f32x16& x0, f32x16& x1) __attribute__((always_inline)) {
@@ -161,17 +174,22 @@ void paged_tile_kernel(const PagedK a) {
       x[e] = __builtin_bit_cast(float, (__builtin_bit_cast(int32_t, xv) & keep) | (int32_t)(0xff800000u & ~(uint32_t)keep));
     }
   };
+  // The words of this lane's row for both blocks of step j.
+  auto words = [&](const Step& s, int j, uint32_t& w0, uint32_t& w1) __attribute__((always_inline)) {
+    const int key = kl.block(j0 + j) << kTileLg;
+    w0 = s.live & 3u ? mask_word(mask, q_pos, key, len) : 0u;
+    w1 = s.live & 12u ? mask_word(mask, q_pos, key + 32, len) : 0u;
+    if (!(s.live & 1u)) w0 &= 0xffff0000u;
+    if (!(s.live & 2u)) w0 &= 0x0000ffffu;
+    if (!(s.live & 4u)) w1 &= 0xffff0000u;
+    if (!(s.live & 8u)) w1 &= 0x0000ffffu;
+  };
   auto shape = [&](const Step& s, int j, f32x16& x0, f32x16& x1) __attribute__((always_inline)) {
     if (s.full == 15u) return;
-    const int key = kl.block(j0 + j) << kTileLg;
-    wd0 = s.live & 3u ? mask_word(mask, q_pos, key, len) : 0u;
-    wd1 = s.live & 12u ? mask_word(mask, q_pos, key + 32, len) : 0u;
-    if (!(s.live & 1u)) wd0 &= 0xffff0000u;
-    if (!(s.live & 2u)) wd0 &= 0x0000ffffu;
-    if (!(s.live & 4u)) wd1 &= 0xffff0000u;
-    if (!(s.live & 8u)) wd1 &= 0x0000ffffu;
-    mask_block(x0, wd0);
-    mask_block(x1, wd1);
+    uint32_t w0, w1;
+    words(s, j, w0, w1);
+    mask_block(x0, w0);
+    mask_block(x1, w1);
   };
   auto block_max = [&](const f32x16& x, float mx) __attribute__((always_inline)) -> float {
 #pragma unroll
@@ -179,7 +197,7 @@ void paged_tile_kernel(const PagedK a) {
     return mx;
   };
   auto raise = [&](float mx) __attribute__((always_inline)) {
-    const float m_new = nan_max(m_run, row_nan_max(mx) * a.c);
+    const float m_new = nan_max(m_run, row_nan_max(mx) * c_exp);
     if (__ballot(m_new > m_run + kLazy) != 0ull) {
       const float alpha = __builtin_amdgcn_exp2f(m_run - base_of(m_new));
       m_run = m_new;
@@ -188,14 +206,19 @@ void paged_tile_kernel(const PagedK a) {
       for (int x = 0; x < NDB; ++x) acc[x] *= alpha;
     }
   };
+  // P of chunk c of a block, summed into l_part.  (The empty asm makes the products wait for the sum:
+  // left to itself the scheduler sums at the step's end and holds 32 values until then, and the
+  // fragments of Q go to scratch memory.)
   auto exps = [&](const f32x16& x, int c, float neg_m) __attribute__((always_inline)) -> Frag {
-    f32x8 pv;
+    f32x8 e8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * c + e], a.c, neg_m));
-      l_part += pv[e];
-    }
-    return Mma<T>::cvt(pv);
+    for (int e = 0; e < 8; ++e) e8[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * c + e], c_exp, neg_m));
+    l_part += ((e8[0] + e8[1]) + (e8[2] + e8[3])) + ((e8[4] + e8[5]) + (e8[6] + e8[7]));
+    u32x4 pw = __builtin_bit_cast(u32x4, Mma<T>::cvt(e8));
+    uint32_t p0 = pw[0];
+    asm("" : "+v"(l_part), "+v"(p0));
+    pw[0] = p0;
+    return __builtin_bit_cast(Frag, pw);
   };
   // Products with chunk x (keys 16 x .. 16 x + 15) of the step in the V slot that the transposed
   // reads are on.
@@ -203,64 +226,60 @@ void paged_tile_kernel(const PagedK a) {
 #pragma unroll
     for (int db = 0; db < NDB; ++db) acc[db] = Mma<T>::mma(tr_frag<T, D>(rd, db, VRING + 16 * x * R::ROW), pf, acc[db]);
   };
-  // Softmax and products of the current step where it is not all live for this wave.
-  auto masked_step = [&](const Step& s) __attribute__((always_inline)) {
-    if (s.live == 0u) return;
-    const float neg_m = -base_of(m_run);
-    Frag pf[4];
-    uint32_t odd = 0u;  // chunks with dead pairs whose V rows hold what is not finite
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      pf[x] = exps(x < 2 ? sc0 : sc1, x & 1, neg_m);
-      if (((s.live & ~s.full) >> x) & 1u) {
-        uint32_t lo = 0u, hi = 0u;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          const u32x4 v = __builtin_bit_cast(u32x4, tr_frag<T, D>(rd, db, VRING + 16 * x * R::ROW));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t y = v[e];
-            lo = max(lo, y & 0x7fffu);
-            hi = max(hi, y & 0x7fff0000u);
-          }
-        }
-        if (__ballot(not_finite16<T>(lo, hi)) != 0ull) odd |= 1u << x;
-      }
-    }
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (((s.live & ~odd) >> x) & 1u) pv(pf[x], x);
-    if (odd == 0u) return;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      if (!((odd >> x) & 1u)) continue;
-      const u32x4 pw = __builtin_bit_cast(u32x4, pf[x]);
-      // element e of lane half h is key 8 (e / 4) + 4 h + e % 4 of the chunk
-#pragma unroll 1
-      for (int y = 0; y < 16; ++y) {
-        const int h = y & 1, e = y >> 1;
-        const uint32_t half = G == h ? ((e & 1) ? 0xffff0000u : 0x0000ffffu) : 0u;
-        u32x4 keep;
-#pragma unroll
-        for (int z = 0; z < 4; ++z) keep[z] = z == (e >> 1) ? half : 0u;
-        const bool on = ((x < 2 ? wd0 : wd1) >> (16 * (x & 1) + 8 * (e >> 2) + 4 * h + (e & 3))) & 1u;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          const u32x4 v = __builtin_bit_cast(u32x4, tr_frag<T, D>(rd, db, VRING + 16 * x * R::ROW)) & keep;
-          const f32x16 p = Mma<T>::mma(__builtin_bit_cast(Frag, v), __builtin_bit_cast(Frag, pw & keep), f32x16{0});
-#pragma unroll
-          for (int z = 0; z < 16; ++z) acc[db][z] = on ? acc[db][z] + p[z] : acc[db][z];
-        }
-      }
-    }
-  };
-  auto full_step = [&]() __attribute__((always_inline)) {
+  auto sums_step = [&](const f32x16& x0, const f32x16& x1) __attribute__((always_inline)) {
     const float neg_m = -base_of(m_run);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) pv(exps(x < 2 ? sc0 : sc1, x & 1, neg_m), x);
+    for (int x = 0; x < 4; ++x) pv(exps(x < 2 ? x0 : x1, x & 1, neg_m), x);
   };
 
   Step s_cur{}, s_next{}, s_after{};
+  uint32_t p = 0u;  // j & 1, times a slot
+  // Iteration j, with a step after it: behind the wait and the barrier, K of step j + 1 and V of step
+  // j are in LDS, and the slots that the new DMA writes were last read before the barrier.
+  // x0, x1: the step's scores; y0, y1: those of the next.
+  auto iterate = [&](int j, const f32x16& x0, const f32x16& x1, f32x16& y0, f32x16& y1) __attribute__((always_inline)) {
+    dma_wait_all();
+    // (a use that makes the compiler's own wait for the page loads fall here)
+    asm volatile("" ::"v"(r_page));
+    __syncthreads();
+    if (j + 2 < n_steps) {
+      s_after = step_of(j + 2);
+      dma(KRING + p, kbase + s_after.off);
+    }
+    dma(VRING + (SLOT - p), vbase + s_next.off);
+    if ((s_cur.live | s_next.live) != 0u) {
+      const float neg_m = -base_of(m_run);
+      const Frag p00 = exps(x0, 0, neg_m), p01 = exps(x0, 1, neg_m), p10 = exps(x1, 0, neg_m), p11 = exps(x1, 1, neg_m);
+      qk(y0, y1);
+      pv(p00, 0);
+      pv(p01, 1);
+      pv(p10, 2);
+      pv(p11, 3);
+      // 4 K reads ahead; then MFMAs of the scores, each beside a read and exponentials; then those of
+      // the products, V reads running 4 MFMAs ahead
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+      for (int x = 0; x < 2 * NQF; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 6 : 10, 1);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+      for (int x = 0; x < 4 * NDB; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 1 : 4, 1);
+      }
+      shape(s_next, j + 1, y0, y1);
+      raise(block_max(y1, block_max(y0, -INFINITY)));
+    }
+    s_cur = s_next;
+    s_next = s_after;
+    rd.template turn_rows<SLOT>();
+    rd.template turn_tr<SLOT>();
+    p = SLOT - p;
+  };
   if (n_steps > 0) {
     load_raw(0);
     s_cur = step_of(0);
@@ -272,100 +291,143 @@ void paged_tile_kernel(const PagedK a) {
     for (int kc = 0; kc < NQF; ++kc) asm volatile("" ::"v"(qf[kc]));
     __syncthreads();
     if (n_steps > 1) dma(KRING + SLOT, kbase + s_next.off);
-    if (s_cur.live != 0u) {
-      qk(sc0, sc1);
-      shape(s_cur, 0, sc0, sc1);
-      raise(block_max(sc1, block_max(sc0, -INFINITY)));
-    }
+    qk(sa0, sa1);
+    shape(s_cur, 0, sa0, sa1);
+    raise(block_max(sa1, block_max(sa0, -INFINITY)));
     rd.template turn_rows<SLOT>();
-    // Iteration j, with a step after it: behind the wait and the barrier, K of step j + 1 and V of step
-    // j are in LDS, and the slots that the new DMA writes were last read before the barrier.
-    uint32_t p = 0u;  // j & 1, times a slot
+    int j = 0;
 #pragma unroll 1
-    for (int j = 0; j + 1 < n_steps; ++j) {
-      dma_wait_all();
-      // (a use that makes the compiler's own wait for the page loads fall here)
-      asm volatile("" ::"v"(r_page));
-      __syncthreads();
-      if (j + 2 < n_steps) {
-        s_after = step_of(j + 2);
-        dma(KRING + p, kbase + s_after.off);
-      }
-      dma(VRING + (SLOT - p), vbase + s_next.off);
-      f32x16 sn0, sn1;
-      if (s_cur.full == 15u && s_next.live != 0u) {
-        const float neg_m = -base_of(m_run);
-        const Frag p00 = exps(sc0, 0, neg_m), p01 = exps(sc0, 1, neg_m), p10 = exps(sc1, 0, neg_m), p11 = exps(sc1, 1, neg_m);
-        qk(sn0, sn1);
-        pv(p00, 0);
-        pv(p01, 1);
-        pv(p10, 2);
-        pv(p11, 3);
-        // 4 K reads ahead; then MFMAs of the scores, each beside a read and exponentials; then those of
-        // the products, V reads running 4 MFMAs ahead
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
-#pragma unroll
-        for (int x = 0; x < 2 * NQF; ++x) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
-          __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 6 : 10, 1);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
-#pragma unroll
-        for (int x = 0; x < 4 * NDB; ++x) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-          __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
-          __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 1 : 4, 1);
-        }
-      } else {
-        if (s_cur.full == 15u)
-          full_step();
-        else
-          masked_step(s_cur);
-        if (s_next.live != 0u) qk(sn0, sn1);
-      }
-      if (s_next.live != 0u) {
-        shape(s_next, j + 1, sn0, sn1);
-        raise(block_max(sn1, block_max(sn0, -INFINITY)));
-        sc0 = sn0;
-        sc1 = sn1;
-      }
-      s_cur = s_next;
-      s_next = s_after;
-      rd.template turn_rows<SLOT>();
-      rd.template turn_tr<SLOT>();
-      p = SLOT - p;
+    for (; j + 2 < n_steps; j += 2) {
+      iterate(j, sa0, sa1, sb0, sb1);
+      iterate(j + 1, sb0, sb1, sa0, sa1);
+    }
+    if (j + 1 < n_steps) {
+      iterate(j, sa0, sa1, sb0, sb1);
+      sa0 = sb0;
+      sa1 = sb1;
     }
     dma_wait_all();
     __syncthreads();
-    if (s_cur.full == 15u)
-      full_step();
-    else
-      masked_step(s_cur);
+    if (s_cur.live != 0u) sums_step(sa0, sa1);
+  }
+
+  // ---- sums that are not finite: the list again, step by step ------------------------------
+  float big = 0.f;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) big = nan_max(big, nan_max(__builtin_fabsf(acc[db][e]), __builtin_fabsf(acc[db][e + 1])));
+  if (__syncthreads_or(!(big < INFINITY))) {
+    rd = tile_reads<D>((lds_cptr)smem, lane);
+#pragma unroll
+    for (int x = 0; x < NDB; ++x) acc[x] = f32x16{0};
+    m_run = -INFINITY;
+    l_part = 0.f;
+    load_raw(0);
+#pragma unroll 1
+    for (int j = 0; j < n_steps; ++j) {
+      const Step s = step_of(j);
+      dma(KRING, kbase + s.off);
+      dma(VRING, vbase + s.off);
+      dma_wait_all();
+      __syncthreads();
+      qk(sa0, sa1);
+      uint32_t w0 = ~0u, w1 = ~0u;
+      if (s.full != 15u) {
+        words(s, j, w0, w1);
+        mask_block(sa0, w0);
+        mask_block(sa1, w1);
+      }
+      raise(block_max(sa1, block_max(sa0, -INFINITY)));
+      const float neg_m = -base_of(m_run);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const Frag pf = exps(x < 2 ? sa0 : sa1, x & 1, neg_m);
+        if (!((s.live >> x) & 1u)) continue;
+        uint32_t lo = 0u, hi = 0u;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const u32x4 v = __builtin_bit_cast(u32x4, tr_frag<T, D>(rd, db, VRING + 16 * x * R::ROW));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t y = v[e];
+            lo = max(lo, y & 0x7fffu);
+            hi = max(hi, y & 0x7fff0000u);
+          }
+        }
+        if (((s.full >> x) & 1u) || __ballot(not_finite16<T>(lo, hi)) == 0ull) {
+          pv(pf, x);
+          continue;
+        }
+        const u32x4 pw = __builtin_bit_cast(u32x4, pf);
+        // element e of lane half h is key 8 (e / 4) + 4 h + e % 4 of the chunk
+#pragma unroll 1
+        for (int y = 0; y < 16; ++y) {
+          const int h = y & 1, e = y >> 1;
+          const uint32_t half = G == h ? ((e & 1) ? 0xffff0000u : 0x0000ffffu) : 0u;
+          u32x4 keep;
+#pragma unroll
+          for (int z = 0; z < 4; ++z) keep[z] = z == (e >> 1) ? half : 0u;
+          const bool on = ((x < 2 ? w0 : w1) >> (16 * (x & 1) + 8 * (e >> 2) + 4 * h + (e & 3))) & 1u;
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) {
+            const u32x4 v = __builtin_bit_cast(u32x4, tr_frag<T, D>(rd, db, VRING + 16 * x * R::ROW)) & keep;
+            const f32x16 p = Mma<T>::mma(__builtin_bit_cast(Frag, v), __builtin_bit_cast(Frag, pw & keep), f32x16{0});
+#pragma unroll
+            for (int z = 0; z < 16; ++z) acc[db][z] = on ? acc[db][z] + p[z] : acc[db][z];
+          }
+        }
+      }
+      __syncthreads();  // every wave is past the slots
+    }
   }
 
   // ---- the rows leave -------------------------------------------------------------------
-  const float l_tot = row_sum(l_part);
+  float l_tot = row_sum(l_part);
   int lane_e = lane;  // (opaque: what follows is worked out again instead of held through the loop)
   asm volatile("" : "+v"(lane_e));
   const int m_e = lane_e & 31, G_e = lane_e >> 5;
   const bool mine = 32 * w + m_e < n_rows;
   if (u.splits > 1) {
-    if (u.slot >= a.slots) return;  // (not reached by starts in order; the same for the work-group)
-    if (mine) {
-      const int64_t row = (int64_t)u.slot * kTileRows + 32 * w + m_e;
+    // a slot is the waves' registers as they are: 16 bytes of O per lane, then maximum and sum
+    constexpr int SLOT_B = slot_floats(kTileRows, D) * 4, WB = SLOT_B / 4;
+    const char* first = part.part + (int64_t)u.slot * SLOT_B + w * WB + 16 * lane_e;
+    {
+      char* own = const_cast<char*>(first) + (int64_t)u.split * SLOT_B;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<f32x4*>(a.part_o + row * D + 32 * db + 8 * e + 4 * G_e) =
-              f32x4{acc[db][4 * e], acc[db][4 * e + 1], acc[db][4 * e + 2], acc[db][4 * e + 3]};
+          share_store4(own + (4 * db + e) * 1024, f32x4{acc[db][4 * e], acc[db][4 * e + 1], acc[db][4 * e + 2], acc[db][4 * e + 3]});
       if (G_e == 0) {
-        a.part_ml[2 * row] = m_run;
-        a.part_ml[2 * row + 1] = l_tot;
+        float* ml = reinterpret_cast<float*>(own + NDB * 4096 - 8 * lane_e);
+        share_store(ml, m_run);
+        share_store(ml + 1, l_tot);
       }
     }
-    return;
+    if (!last_share(part, u, tid, flag)) return;
+    m_run = -INFINITY;
+#pragma unroll 1
+    for (int s = 0; s < u.splits; ++s)
+      m_run = nan_max(m_run, share_load(reinterpret_cast<const float*>(first + (int64_t)s * SLOT_B + NDB * 4096 - 16 * lane_e + 8 * m_e)));
+    l_tot = 0.f;
+#pragma unroll
+    for (int x = 0; x < NDB; ++x) acc[x] = f32x16{0};
+#pragma unroll 1
+    for (int s = 0; s < u.splits; ++s) {
+      const char* at = first + (int64_t)s * SLOT_B;
+      const float* ml = reinterpret_cast<const float*>(at + NDB * 4096 - 16 * lane_e + 8 * m_e);
+      const float f = __builtin_amdgcn_exp2f(share_load(ml) - base_of(m_run));
+      l_tot += f * share_load(ml + 1);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f32x4 x = share_load4(at + (4 * db + e) * 1024);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) acc[db][4 * e + z] += f * x[z];
+        }
+    }
   }
   const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
   if (a.lse && G_e == 0 && mine) {
@@ -398,21 +460,5 @@ void paged_tile_kernel(const PagedK a) {
   }
 }
 
-template <typename T, int D>
-int launch_tile_t(const PagedK& a, int64_t max_tiles, hipStream_t s) {
-  const int64_t grid = a.target + max_tiles * a.Hkv;
-  PA_CHECK_ARG(grid <= 0x7fffffffll, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)grid);
-  hipLaunchKernelGGL((paged_tile_kernel<T, D>), dim3((unsigned)grid), dim3(256), 0, s, a);
-  PA_LAUNCH_CHECK("paged_tile_kernel");
-  return launch_paged_tile_merge(a, __is_same(T, __bf16) ? PA_BF16 : PA_F16, D, max_tiles, s);
-}
-
 }  // namespace
-
-int launch_paged_tile(const PagedK& a, int dtype, int D, int64_t max_tiles, hipStream_t s) {
-  if (dtype == PA_BF16)
-    return D == 64 ? launch_tile_t<__bf16, 64>(a, max_tiles, s) : launch_tile_t<__bf16, 128>(a, max_tiles, s);
-  return D == 64 ? launch_tile_t<_Float16, 64>(a, max_tiles, s) : launch_tile_t<_Float16, 128>(a, max_tiles, s);
-}
-
 }  // namespace pa

@@ -279,9 +279,11 @@ def prepare_attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_f
         if lse.dtype != torch.float32 or lse.shape != (T, Hq) or lse.device != dev:
             raise ValueError(f"lse must be float32 [{T}, {Hq}] on {dev}")
         a.lse, a.lse_st, a.lse_sh = ptr(lse), lse.stride(0), lse.stride(1)
-    nbytes = ctypes.c_int64(0)
-    _lib.check(_lib.lib().pa_paged_workspace(ctypes.byref(a), ctypes.byref(nbytes)), "pa_paged_workspace")
+    nbytes, zero = ctypes.c_int64(0), ctypes.c_int64(0)
+    _lib.check(_lib.lib().pa_paged_workspace(ctypes.byref(a), ctypes.byref(nbytes), ctypes.byref(zero)), "pa_paged_workspace")
     ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        ws[:zero.value].zero_()   # (every run leaves it zero)
     a.workspace, a.workspace_bytes = ptr(ws), nbytes.value
     return PagedLaunch("pa_paged_attn", (ctypes.byref(a),), [a, q, k, v, tables, lengths, q_start, dm, o, lse, ws], k, o)
 

@@ -210,7 +210,7 @@ def test_release_and_append_refusals():
 def test_attention_refusals():
     keep, p = _buf()
     lib = _lib.lib()
-    need = ctypes.c_int64(0)
+    need, zero = ctypes.c_int64(0), ctypes.c_int64(0)
 
     def args(**change):
         a = _lib.PaPagedArgs()
@@ -228,7 +228,9 @@ def test_attention_refusals():
     def call(**change):
         return lib.pa_paged_attn(ctypes.byref(args(**change)), None)
     assert lib.pa_paged_attn(None, None) == _lib.PA_E_INVALID
-    assert lib.pa_paged_workspace(ctypes.byref(args()), ctypes.byref(need)) == 0 and need.value > 0
+    assert lib.pa_paged_workspace(ctypes.byref(args()), ctypes.byref(need), ctypes.byref(zero)) == 0
+    assert 0 < zero.value < need.value
+    _refused(lib.pa_paged_workspace(ctypes.byref(args()), ctypes.byref(need), None), "null")
     assert call(R=0) == 0 and call(T=0) == 0
     _refused(call(workspace_bytes=need.value - 1), "workspace")
     _refused(call(workspace=p + 16), "workspace")
