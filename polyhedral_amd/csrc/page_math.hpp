@@ -20,14 +20,17 @@ namespace pa {
 
 constexpr int32_t kMaxPosition = (1 << 30) - 1;  // positions and lengths stay at or below it
 
-// The terms of a pa_mask without tables.  They are walked in rolled loops through a pointer (on the
-// device one into the kernel's arguments, read by scalar loads): one copy of each term's code, and
-// no registers held for terms that are not there.
+// The terms of a pa_mask without tables.  They are walked in rolled loops, so there is one copy of
+// each term's code: the first one, which most masks consist of, from registers, the others through
+// a pointer (on the device one into the kernel's arguments, read by scalar loads).
 template <typename Ptr>
 struct PageMask {
   int32_t n_include, n_exclude;
+  pa_term first;
   Ptr terms;
-  PA_HD pa_term term(int i) const { return pa_term{terms[i].kind, terms[i].p0, terms[i].p1, terms[i].p2}; }
+  PA_HD pa_term term(int i) const {
+    return i == 0 ? first : pa_term{terms[i].kind, terms[i].p0, terms[i].p1, terms[i].p2};
+  }
 };
 
 enum Verdict { kDead = 0, kPartial = 1, kFull = 2 };
@@ -203,6 +206,22 @@ PA_HD int32_t checked_page(int32_t page, int64_t n_pages) {
 PA_HD int32_t slot_of(int32_t page, int32_t position, int page_lg, int64_t n_pages) {
   const int32_t p = checked_page(page, n_pages);
   return p < 0 ? -1 : (p << page_lg) + (position & ((1 << page_lg) - 1));
+}
+
+// Division of numbers below 2^30 by d in 1 .. 65535 as a product: with l = ceil(log2 d), k = max(32,
+// 30 + l) and m = ceil(2^k / d), m d - 2^k < d <= 2^(k - 30), so x m / 2^k is above x / d by less
+// than 1 / d.
+struct Divisor {
+  uint32_t d, m, shift;  // shift: k - 32
+};
+inline Divisor divisor_of(uint32_t d) {
+  int l = 0;
+  while ((1u << l) < d) ++l;
+  const int k = l > 2 ? 30 + l : 32;
+  return {d, (uint32_t)(((1ull << k) + d - 1) / d), (uint32_t)(k - 32)};  // (m is not used for d = 1)
+}
+PA_HD int32_t divide(int32_t x, const Divisor& v) {
+  return v.d == 1 ? x : (int32_t)((uint32_t)(((uint64_t)(uint32_t)x * v.m) >> 32) >> v.shift);
 }
 
 // Rows and length of a request, whatever its entries hold: rows start .. start + n - 1 of T

@@ -7,8 +7,9 @@
 namespace pa {
 namespace {
 
-constexpr int kTarget = 512;   // units that the splits of a kernel's part aim for
-constexpr int kFewRows = 16;   // rows of a request (new tokens times heads of a group) up to which
+constexpr int kTileTarget = 512;   // units that the splits of the chunks' tiles aim for, and of the
+constexpr int kRowsTarget = 1024;  // tiles of few rows (two work-groups run per CU)
+constexpr int kFewRows = 32;   // rows of a request (new tokens times heads of a group) up to which
                                // it is a tile of few rows
 
 // Workspace: the counts of both parts, then their slots.
@@ -20,14 +21,18 @@ struct PagedPlan {
 };
 
 // A part whose requests have at most max_tiles tiles: its grid and slots.  (The shares of all tiles are
-// at most kTarget and one more for each tile and KV head; a tile that is split has two shares at
-// least, and then less than twice those that its blocks fill.)
-int part_of(const pa_paged_args* x, int64_t max_tiles, PagedPart* p) {
-  const int64_t grid = kTarget + max_tiles * x->Hkv;
-  PA_CHECK_ARG(grid <= 0x3fffffffll, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)grid);
-  p->grid = (int32_t)grid;
-  p->slots = (int32_t)(2 * kTarget < grid ? 2 * kTarget : grid);
-  p->target = kTarget;
+// at most the target and one more for each tile and KV head; a tile that is split has two shares at
+// least, and then less than twice those that its blocks fill.  The work-groups without a unit each
+// hold a place on a CU for 1.5 us; a grid without them, whose groups loop over units, costs more: 276
+// -> 296 us of sinks in chunks, 15 -> 17 us of one token over 8000, by registers that the loop holds.)
+int part_of(const pa_paged_args* x, int BM, int target, int64_t max_tiles, PagedPart* p) {
+  const int64_t most = target + max_tiles * x->Hkv;
+  PA_CHECK_ARG(most <= 0x3fffffffll, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)most);
+  p->grid = (int32_t)most;
+  p->slots = (int32_t)(2 * target < most ? 2 * target : most);
+  p->target = target;
+  const int G = x->Hq / x->Hkv;
+  p->span = (BM + G - 1) / G + 1;
   return PA_OK;
 }
 
@@ -48,14 +53,18 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   p->tile = x->dtype != PA_F32 && x->n_pages > 0 && x->max_fresh * G > kFewRows;
   int64_t few = x->T * G / kRows + some;
   if (p->tile && few > some * (kFewRows / kRows)) few = some * (kFewRows / kRows);
-  if (int rc = part_of(x, few, &p->rows)) return rc;
-  p->rows.least = 8;
+  if (int rc = part_of(x, kRows, kRowsTarget, few, &p->rows)) return rc;
+  p->rows.long_share = 32;
+  p->rows.least = 4;
+  p->rows.root_over = 0.7f;
   p->rows.row_min = 0;
   p->rows.row_max = p->tile ? kFewRows : INT_MAX;
   p->tiles = PagedPart{};
   if (p->tile) {
-    if (int rc = part_of(x, x->T * G / kTileRows + some, &p->tiles)) return rc;
-    p->tiles.least = 4;
+    if (int rc = part_of(x, kTileRows, kTileTarget, x->T * G / kTileRows + some, &p->tiles)) return rc;
+    p->tiles.long_share = 0;
+    p->tiles.least = 8;
+    p->tiles.root_over = 1.f;
     p->tiles.row_min = kFewRows;
     p->tiles.row_max = INT_MAX;
   }
@@ -120,6 +129,7 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
   a.T = (int32_t)x->T;
   a.Hkv = x->Hkv;
   a.G = x->Hq / x->Hkv;
+  a.by_G = divisor_of((uint32_t)a.G);
   a.c = x->scale * 1.4426950408889634f;
   a.n_include = x->mask.n_include;
   a.n_exclude = x->mask.n_exclude;

@@ -25,8 +25,12 @@ struct PagedPart {
   char* part;           // [slots] states of split tiles' units
   int32_t* count;       // [slots] units done, at a tile's first slot; zero between calls
   int32_t slots;
-  int32_t target;       // units that the splits aim for
-  int32_t least;        // least blocks of a share
+  // Blocks of a share: total / target, or where that is less than `long_share` blocks the smaller of
+  // long_share and 2 total / target; but at least `least`, and the root of the tile's blocks over
+  // root_over (the time of a share against that of merging them all).
+  int32_t target, long_share, least;
+  float root_over;
+  int32_t span;         // new tokens that a tile can hold rows of
   int32_t row_min, row_max;  // requests with row_min < rows <= row_max
   int32_t grid;
 };
@@ -44,6 +48,7 @@ struct PagedK {
   const int32_t* lengths;
   const int32_t* q_start;
   int32_t R, T, Hkv, G;
+  Divisor by_G;
   float c;  // scale * log2(e)
   int32_t n_include, n_exclude;
   pa_term terms[PA_MAX_TERMS];
@@ -60,7 +65,7 @@ typedef PageMask<cterm*> KernelMask;
 __device__ __forceinline__ KernelMask kernel_mask(const PagedK& a) {
   typedef const __attribute__((address_space(4))) char cchar;
   cchar* args = (cchar*)__builtin_amdgcn_kernarg_segment_ptr();
-  return {a.n_include, a.n_exclude, (cterm*)(args + offsetof(PagedK, terms))};
+  return {a.n_include, a.n_exclude, a.terms[0], (cterm*)(args + offsetof(PagedK, terms))};
 }
 
 struct Work {
@@ -79,7 +84,7 @@ template <int BM, int LG>
 __device__ __forceinline__ Work work_of(const PagedK& a, const PagedPart& p, const Request& q) {
   const int32_t rows = q.n * a.G;
   if (rows <= p.row_min || rows > p.row_max) return {0, 0};
-  const int32_t span = imin(q.n, (BM + a.G - 1) / a.G + 1);
+  const int32_t span = imin(q.n, p.span);
   return {(rows + BM - 1) / BM, key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG).count()};
 }
 
@@ -148,7 +153,8 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, i
     total += wave_total((float)w.tiles * (float)w.blocks);
   }
   // (rounded up, so the units stay within target + tiles Hkv, which the grid is sized for)
-  const float share = total * (float)a.Hkv / (float)p.target * 1.0001f;
+  float share = total * (float)a.Hkv / (float)p.target * 1.0001f;
+  share = fmaxf(share, fminf(2.f * share, (float)p.long_share));
   const int32_t chunk = imax(p.least, share < 1e9f ? (int32_t)share + 1 : (1 << 30));
 
   int32_t before = 0, slot = 0;  // units and slots of earlier requests
@@ -158,7 +164,9 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, i
       q = load_request(a, r0, lane, end);
       w = work_of<BM, LG>(a, p, q);
     }
-    const int32_t splits = imax((w.blocks + chunk - 1) / chunk, 1);
+    // (to the nearest: a tile little longer than a share stays whole)
+    const uint32_t mine_chunk = (uint32_t)imax(chunk, (int32_t)(__builtin_amdgcn_sqrtf((float)w.blocks) * p.root_over) + 1);
+    const int32_t splits = imax((int32_t)(((uint32_t)w.blocks + mine_chunk / 2u) / mine_chunk), 1);
     const int32_t units = w.tiles * a.Hkv * splits, mine = splits > 1 ? units : 0;
     const int32_t n_in = wave_scan(units), s_in = wave_scan(mine);
     const int32_t at = before + n_in - units;
@@ -173,8 +181,9 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, i
       // a KV head's shares side by side, its tiles a multiple of Hkv units apart: with 8 KV heads
       // the tiles of one fall on one XCD (work-groups are dealt to the XCDs in turn) and share
       // its L2
-      const int32_t x = id - get(at), per = a.Hkv * u.splits, tile = x / per, y = x - tile * per;
-      u.h = y / u.splits;
+      const int32_t x = id - get(at), per = a.Hkv * u.splits;
+      const int32_t tile = (int32_t)((uint32_t)x / (uint32_t)per), y = x - tile * per;
+      u.h = (int32_t)((uint32_t)y / (uint32_t)u.splits);
       u.split = y - u.h * u.splits;
       u.slot = slot + get(s_in - mine) + x - u.split;
       // (a causal mask's longest tile first)
@@ -187,9 +196,12 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, i
   return u;
 }
 
+// Token of a request's row i (its head of the group: i - token G).
+__device__ __forceinline__ int32_t token_of(const PagedK& a, int32_t i) { return divide(i, a.by_G); }
+
 // Blocks j0 .. j1 - 1 of a list of n are share `split` of `splits`.
 __device__ __forceinline__ void share_of(int32_t n, int32_t split, int32_t splits, int32_t* j0, int32_t* j1) {
-  const int32_t per = n / splits, more = n - per * splits;
+  const int32_t per = (int32_t)((uint32_t)n / (uint32_t)splits), more = n - per * splits;
   *j0 = split * per + imin(split, more);
   *j1 = *j0 + per + (split < more ? 1 : 0);
 }

@@ -104,10 +104,10 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
   const int i0 = u.tile * kRows;
   const int n_rows = imin(rows - i0, kRows);
   const int i = imin(i0 + q16, rows - 1);          // (a lane past the rows repeats the last)
-  const int tok = i / a.G, head = u.h * a.G + (i - tok * a.G);
+  const int tok = token_of(a, i), head = u.h * a.G + (i - tok * a.G);
   const int pos0 = u.rq.len - u.rq.n;
   const int q_pos = pos0 + tok;
-  const int q_lo = pos0 + i0 / a.G, q_hi = pos0 + (i0 + n_rows - 1) / a.G;
+  const int q_lo = pos0 + token_of(a, i0), q_hi = pos0 + token_of(a, i0 + n_rows - 1);
   const int len = u.rq.len;
 
   u32x4 qf[NK];
@@ -474,7 +474,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
     gather();
   }
   if (row >= n_rows) return;
-  const int ir = i0 + row, t_r = ir / a.G, h_r = u.h * a.G + (ir - t_r * a.G);
+  const int ir = i0 + row, t_r = token_of(a, ir), h_r = u.h * a.G + (ir - t_r * a.G);
   const float inv = L == 0.f ? 0.f : 1.f / L;
   char* orow = a.o + (int64_t)(u.rq.start + t_r) * a.o_st + (int64_t)h_r * a.o_sh;
 #pragma unroll

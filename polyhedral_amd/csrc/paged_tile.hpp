@@ -65,22 +65,11 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   const int i0 = u.tile * kTileRows;
   const int n_rows = imin(rows - i0, kTileRows);
   const int w0 = imin(i0 + 32 * w, rows - 1), w1 = imin(i0 + 32 * w + 31, rows - 1);  // this wave's rows
-  int q_pos;  // position of this lane's row (a lane past the rows repeats the last)
-  const int q_lo = pos0 + w0 / a.G, q_hi = pos0 + w1 / a.G;
-
-  Frag qf[NQF];
-  {
-    const int i = imin(i0 + 32 * w + m, rows - 1), tok = i / a.G, head = u.h * a.G + (i - tok * a.G);
-    q_pos = pos0 + tok;
-    const char* qrow = a.q + (int64_t)(u.rq.start + tok) * a.q_st + (int64_t)head * a.q_sh;
-#pragma unroll
-    for (int kc = 0; kc < NQF; ++kc)
-      qf[kc] = __builtin_bit_cast(Frag, *reinterpret_cast<const uint4*>(qrow + (16 * kc + 8 * G) * ESZ));
-  }
+  const int q_lo = pos0 + token_of(a, w0), q_hi = pos0 + token_of(a, w1);
 
   // ---- the keys of this share ---------------------------------------------------------
   const KernelMask mask = kernel_mask(a);
-  const KeyList kl = key_list(mask, pos0 + i0 / a.G, pos0 + (i0 + n_rows - 1) / a.G, len, kTileLg);
+  const KeyList kl = key_list(mask, pos0 + token_of(a, i0), pos0 + token_of(a, i0 + n_rows - 1), len, kTileLg);
   int32_t j0, j1;
   share_of(kl.count(), u.split, u.splits, &j0, &j1);
   const int n_steps = j1 - j0;
@@ -119,6 +108,20 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
     // (keys without a page read the cache's first one, and are dead)
     c_off = (int64_t)imax(page, 0) * a.c_sp + (int64_t)(key & ((1 << a.page_lg) - 1)) * a.c_sn;
   };
+  load_raw(0);  // (in flight beside the loads of Q)
+
+  // ---- Q ----------------------------------------------------------------------------------
+  int q_pos;  // position of this lane's row (a lane past the rows repeats the last)
+  Frag qf[NQF];
+  {
+    const int i = imin(i0 + 32 * w + m, rows - 1), tok = token_of(a, i), head = u.h * a.G + (i - tok * a.G);
+    q_pos = pos0 + tok;
+    const char* qrow = a.q + (int64_t)(u.rq.start + tok) * a.q_st + (int64_t)head * a.q_sh;
+#pragma unroll
+    for (int kc = 0; kc < NQF; ++kc)
+      qf[kc] = __builtin_bit_cast(Frag, *reinterpret_cast<const uint4*>(qrow + (16 * kc + 8 * G) * ESZ));
+  }
+
   struct Step {
     int64_t off;          // of the segment that this wave moves
     uint32_t live, full;  // 4 bits: the step's segments
@@ -281,7 +284,6 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
     p = SLOT - p;
   };
   if (n_steps > 0) {
-    load_raw(0);
     s_cur = step_of(0);
     dma(KRING, kbase + s_cur.off);
     dma(VRING, vbase + s_cur.off);
@@ -392,7 +394,8 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
     // a slot is the waves' registers as they are: 16 bytes of O per lane, then maximum and sum
     constexpr int SLOT_B = slot_floats(kTileRows, D) * 4, WB = SLOT_B / 4;
     const char* first = part.part + (int64_t)u.slot * SLOT_B + w * WB + 16 * lane_e;
-    {
+    const bool has = 32 * w < n_rows;  // (a wave without rows stores and merges nothing)
+    if (has) {
       char* own = const_cast<char*>(first) + (int64_t)u.split * SLOT_B;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
@@ -405,38 +408,41 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
         share_store(ml + 1, l_tot);
       }
     }
-    if (!last_share(part, u, tid, flag)) return;
+    if (!last_share(part, u, tid, flag) || !has) return;
+    const char* ml0 = first + NDB * 4096 - 16 * lane_e + 8 * m_e;
     m_run = -INFINITY;
-#pragma unroll 1
-    for (int s = 0; s < u.splits; ++s)
-      m_run = nan_max(m_run, share_load(reinterpret_cast<const float*>(first + (int64_t)s * SLOT_B + NDB * 4096 - 16 * lane_e + 8 * m_e)));
+#pragma unroll 8
+    for (int s = 0; s < u.splits; ++s) m_run = nan_max(m_run, share_load(reinterpret_cast<const float*>(ml0 + (int64_t)s * SLOT_B)));
     l_tot = 0.f;
 #pragma unroll
     for (int x = 0; x < NDB; ++x) acc[x] = f32x16{0};
-#pragma unroll 1
+#pragma unroll 2
     for (int s = 0; s < u.splits; ++s) {
       const char* at = first + (int64_t)s * SLOT_B;
-      const float* ml = reinterpret_cast<const float*>(at + NDB * 4096 - 16 * lane_e + 8 * m_e);
+      f32x4 x[NDB][4];
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[db][e] = share_load4(at + (4 * db + e) * 1024);
+      const float* ml = reinterpret_cast<const float*>(ml0 + (int64_t)s * SLOT_B);
       const float f = __builtin_amdgcn_exp2f(share_load(ml) - base_of(m_run));
       l_tot += f * share_load(ml + 1);
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const f32x4 x = share_load4(at + (4 * db + e) * 1024);
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int z = 0; z < 4; ++z) acc[db][4 * e + z] += f * x[z];
-        }
+          for (int z = 0; z < 4; ++z) acc[db][4 * e + z] += f * x[db][e][z];
     }
   }
   const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
   if (a.lse && G_e == 0 && mine) {
-    const int ir = i0 + 32 * w + m_e, tok = ir / a.G, head = u.h * a.G + (ir - tok * a.G);
+    const int ir = i0 + 32 * w + m_e, tok = token_of(a, ir), head = u.h * a.G + (ir - tok * a.G);
     a.lse[(int64_t)(u.rq.start + tok) * a.lse_st + (int64_t)head * a.lse_sh] =
         l_tot == 0.f ? -INFINITY : (m_run + log2f(l_tot)) * kLn2;
   }
   // Through LDS (32 rows a wave, 16-byte units swizzled), so that they are stored as whole rows.
-  __syncthreads();  // every wave is past its last read of the rings
+  // (every wave is past its last read of the rings: the sums' check was a barrier)
   lds_char_t* stage = (lds_char_t*)smem + w * 32 * R::ROW;
   typedef __attribute__((address_space(3))) u32x2 lds_w2;
   constexpr int UM = R::UPR - 1;
@@ -447,16 +453,21 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
       const f32x4 x = f32x4{acc[db][4 * e], acc[db][4 * e + 1], acc[db][4 * e + 2], acc[db][4 * e + 3]} * inv;
       *(lds_w2*)(stage + m_e * R::ROW + 16 * ((4 * db + e) ^ (m_e & UM)) + 8 * G_e) = __builtin_bit_cast(u32x2, Mma<T>::cvt4(x));
     }
-  // (each wave reads back only the rows it wrote: LDS keeps a wave's accesses in order)
+  // (each wave reads back only the rows it wrote: LDS keeps a wave's accesses in order; a row's
+  // place in the output is worked out by its own lane)
+  int64_t o_off;
+  {
+    const int ir = i0 + 32 * w + m_e, t = token_of(a, ir), h = u.h * a.G + (ir - t * a.G);
+    o_off = (int64_t)(u.rq.start + t) * a.o_st + (int64_t)h * a.o_sh;
+  }
 #pragma unroll
   for (int x = 0; x < 32 / R::RPI; ++x) {
     const int rr = R::RPI * x + lane_e / R::UPR, un = lane_e % R::UPR;
     const u32x4 v = *(lds_u4*)(stage + rr * R::ROW + 16 * (un ^ (rr & UM)));
-    const int row = 32 * w + rr;
-    if (row < n_rows) {
-      const int ir = i0 + row, t = ir / a.G, h = u.h * a.G + (ir - t * a.G);
-      *reinterpret_cast<u32x4*>(a.o + (int64_t)(u.rq.start + t) * a.o_st + (int64_t)h * a.o_sh + 16 * un) = v;
-    }
+    const uint32_t lo = (uint32_t)__shfl((int32_t)(uint32_t)o_off, rr);
+    const int32_t hi = __shfl((int32_t)(o_off >> 32), rr);
+    if (32 * w + rr < n_rows)
+      *reinterpret_cast<u32x4*>(a.o + (int64_t)((uint64_t)lo | ((uint64_t)(uint32_t)hi << 32)) + 16 * un) = v;
   }
 }
 

@@ -19,7 +19,7 @@ MAX = (1 << 30) - 1
 HARNESS = r"""
 #include "page_math.hpp"
 using namespace pa;
-static PageMask<const pa_term*> of(const pa_mask* m) { return {m->n_include, m->n_exclude, m->terms}; }
+static PageMask<const pa_term*> of(const pa_mask* m) { return {m->n_include, m->n_exclude, m->terms[0], m->terms}; }
 extern "C" {
 int verdict(const pa_mask* m, int q0, int q1, int k0, int k1) { return mask_verdict(of(m), q0, q1, k0, k1); }
 unsigned word(const pa_mask* m, int q, int k0, int len) { return mask_word(of(m), q, k0, len); }
@@ -27,6 +27,7 @@ void list(const pa_mask* m, int q0, int q1, int len, int lg, int* out) {
   const KeyList l = key_list(of(m), q0, q1, len, lg);
   out[0] = l.low; out[1] = l.first; out[2] = l.high;
 }
+int divided(int x, unsigned d) { return divide(x, divisor_of(d)); }
 int slot(int page, int pos, int lg, long long n) { return slot_of(page, pos, lg, n); }
 void request(int s0, int s1, int len, int T, int max_len, int* out) {
   const Request r = request_of(s0, s1, len, T, max_len);
@@ -118,6 +119,17 @@ def test_the_largest_positions_and_parameters(host, kind, p):
             host.verdict(m, q, q, k0, k0 + 31)
         host.list(m, q, q, MAX, 5, out)
         assert out[0] >= 0 and out[2] >= 0
+
+
+def test_division_by_a_product(host):
+    rng = np.random.default_rng(1)
+    for d in [*range(1, 70), 127, 128, 129, 255, 1000, 4095, 4097, 32768, 32769, 65534, 65535]:
+        top = (1 << 30) - 1
+        xs = [0, 1, d - 1, d, d + 1, top, top // d * d, top // d * d - 1, *(int(x) for x in rng.integers(0, 1 << 30, 60))]
+        xs += [int(q) * d + e for q in rng.integers(0, top // d, 40) for e in (-1, 0, 1)]
+        for x in xs:
+            if 0 <= x <= top:
+                assert host.divided(x, d) == x // d, (x, d)
 
 
 def test_bad_pages_and_starts(host):
