@@ -220,6 +220,10 @@ __device__ __forceinline__ void dma_x1(uint32_t m0, const char* gbase, uint32_t 
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(m0), "v"(voff), "s"(gbase)
                : "m0");
 }
+// The same from a 64-bit address per lane.
+__device__ __forceinline__ void dma_x4_va(uint32_t m0, const char* p) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(p) : "m0");
+}
 __device__ __forceinline__ void dma_wait_all() { asm volatile("s_waitcnt vmcnt(0)"); }
 // The same DMA with agent-scope coherence (sc1): reads data another work-group published
 // with agent-scope stores, whichever XCD's L2 it went through.

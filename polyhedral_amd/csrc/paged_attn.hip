@@ -12,6 +12,19 @@ constexpr int kRowsTarget = 1024;  // tiles of few rows (two work-groups run per
 constexpr int kFewRows = 32;   // rows of a request (new tokens times heads of a group) up to which
                                // it is a tile of few rows
 
+// One in how many keys a mask leaves live for a token far from it: the stride of a mask's one lattice
+// when its other terms are bands (windows, sinks); 0 for any other mask.
+int stride_of(const pa_mask& m) {
+  int stride = 0;
+  for (int i = 0; i < m.n_include; ++i) {
+    const pa_term& t = m.terms[i];
+    if (t.kind == PA_WINDOW || t.kind == PA_SINKS || t.kind == PA_TWOBAND) continue;
+    if ((t.kind != PA_DILATED && t.kind != PA_LOCAL_STRIDED) || stride) return 0;
+    stride = t.kind == PA_DILATED ? t.p0 : t.p1;
+  }
+  return stride;
+}
+
 // Workspace: the counts of both parts, then their slots.
 struct PagedPlan {
   int page_lg;
@@ -141,6 +154,7 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
     t.p2 = imin(t.p2, kMaxPosition);
     a.terms[i] = t;
   }
+  a.stride = stride_of(x->mask);
   a.o = static_cast<char*>(x->o);
   a.o_st = x->o_st * esz;
   a.o_sh = x->o_sh * esz;

@@ -20,6 +20,10 @@
 
 namespace pa {
 
+constexpr int kRows = 16;       // query rows of a tile of few rows
+constexpr int kTileRows = 128;  // and of a chunk's tile
+constexpr int kTileLg = 6;      // log2 keys of a step of a chunk's tile
+
 // What one of the two kernels' bodies does in a call.
 struct PagedPart {
   char* part;           // [slots] states of split tiles' units
@@ -52,6 +56,7 @@ struct PagedK {
   float c;  // scale * log2(e)
   int32_t n_include, n_exclude;
   pa_term terms[PA_MAX_TERMS];
+  int32_t stride;  // of a mask that is a lattice beyond a band: 1 in `stride` keys is live for a token; else 0
   char* o;
   int64_t o_st, o_sh;
   float* lse;
@@ -69,7 +74,7 @@ __device__ __forceinline__ KernelMask kernel_mask(const PagedK& a) {
 }
 
 struct Work {
-  int32_t tiles, blocks;
+  int32_t tiles, blocks, least;  // least: blocks of a share
 };
 
 struct Unit {
@@ -83,9 +88,11 @@ struct Unit {
 template <int BM, int LG>
 __device__ __forceinline__ Work work_of(const PagedK& a, const PagedPart& p, const Request& q) {
   const int32_t rows = q.n * a.G;
-  if (rows <= p.row_min || rows > p.row_max) return {0, 0};
+  if (rows <= p.row_min || rows > p.row_max) return {0, 0, 1};
   const int32_t span = imin(q.n, p.span);
-  return {(rows + BM - 1) / BM, key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG).count()};
+  // (a share that is taken by lists: one list of 512 keys for each wave)
+  const int32_t least = BM == kRows && 2 * span <= a.stride ? 2048 >> LG : p.least;
+  return {(rows + BM - 1) / BM, key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG).count(), least};
 }
 
 // Sum over lanes 0 .. l, by DPP moves inside rows of 16 lanes and broadcasts of their last ones.
@@ -144,7 +151,7 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, i
   Unit u;
   u.found = false;
   Request q{0, 0, 0};
-  Work w{0, 0};
+  Work w{0, 0, 1};
   float total = 0.f;  // (a share needs no exact total)
   int32_t end = 0;
   for (int r0 = 0; r0 < a.R; r0 += 64) {
@@ -155,7 +162,7 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, i
   // (rounded up, so the units stay within target + tiles Hkv, which the grid is sized for)
   float share = total * (float)a.Hkv / (float)p.target * 1.0001f;
   share = fmaxf(share, fminf(2.f * share, (float)p.long_share));
-  const int32_t chunk = imax(p.least, share < 1e9f ? (int32_t)share + 1 : (1 << 30));
+  const int32_t chunk = share < 1e9f ? (int32_t)share + 1 : (1 << 30);
 
   int32_t before = 0, slot = 0;  // units and slots of earlier requests
   end = 0;
@@ -165,7 +172,7 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, i
       w = work_of<BM, LG>(a, p, q);
     }
     // (to the nearest: a tile little longer than a share stays whole)
-    const uint32_t mine_chunk = (uint32_t)imax(chunk, (int32_t)(__builtin_amdgcn_sqrtf((float)w.blocks) * p.root_over) + 1);
+    const uint32_t mine_chunk = (uint32_t)imax(imax(chunk, w.least), (int32_t)(__builtin_amdgcn_sqrtf((float)w.blocks) * p.root_over) + 1);
     const int32_t splits = imax((int32_t)(((uint32_t)w.blocks + mine_chunk / 2u) / mine_chunk), 1);
     const int32_t units = w.tiles * a.Hkv * splits, mine = splits > 1 ? units : 0;
     const int32_t n_in = wave_scan(units), s_in = wave_scan(mine);
@@ -243,9 +250,6 @@ __device__ __forceinline__ bool last_share(const PagedPart& p, const Unit& u, in
 // so far; every score is -inf then).
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-constexpr int kRows = 16;       // query rows of a tile of few rows
-constexpr int kTileRows = 128;  // and of a chunk's tile
-constexpr int kTileLg = 6;      // log2 keys of a step of a chunk's tile
 // floats of a slot: O of every row, then maximum and sum
 constexpr int slot_floats(int BM, int D) { return BM * (D + 2); }
 

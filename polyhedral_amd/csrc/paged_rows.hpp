@@ -17,6 +17,9 @@
 // sum taken before.  Maxima are kept unscaled and p = exp2((x - m) c): a maximum that is rounded
 // after its scaling would leave its own p at any power of two where scores are huge.
 //
+// A lattice leaves few keys of a block live for a few tokens.  Where its stride is at least twice the
+// tile's tokens, a wave lists the live keys of 512 at a time and reads their rows alone.
+//
 // A dead key contributes nothing whatever its K and V hold: its score is replaced by -inf, and
 // where a step is masked for some row and its V rows hold an infinity or NaN, the products are
 // taken key by key and added to the rows that the key is live for (a product with a zero would be
@@ -80,7 +83,9 @@ struct RowsShape {
   static constexpr int RING = F32 ? 0 : kWaves * 2 * 2 * 16 * ROW;
   static constexpr int OP = D + 4;                 // floats of a row of a wave's O at the end
   static constexpr int ENDS = kWaves * kRows * (OP + 2) * 4;
-  static constexpr int SMEM = RING > ENDS ? RING : ENDS;
+  static constexpr int LIST = 512;                 // keys of a wave's list of live ones
+  static constexpr int LIST_AT = RING > ENDS ? RING : ENDS;
+  static constexpr int SMEM = LIST_AT + kWaves * LIST * 4;
 };
 
 template <typename T, int D>
@@ -133,10 +138,11 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
   int32_t c_key = 0, r_page = -1;
   int64_t c_off = 0;
   uint64_t c_live = 0ull, c_full = 0ull;
-  auto key_of = [&](int c) __attribute__((always_inline)) -> int32_t {
-    const int st = c * PER + lane / NS;
+  // (the lane's segment of step st)
+  auto key_at = [&](int st) __attribute__((always_inline)) -> int32_t {
     return st < n_steps ? (kl.block(j0 + w + kWaves * st) << S::LG) + (NS == 2 ? 16 * (lane & 1) : 0) : len;
   };
+  auto key_of = [&](int c) __attribute__((always_inline)) -> int32_t { return key_at(c * PER + lane / NS); };
   auto load_raw = [&](int c) __attribute__((always_inline)) {
     const int32_t key = key_of(c);
     r_page = key < len ? table[key >> a.page_lg] : -1;
@@ -230,9 +236,9 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
   for (int db = 0; db < NB; ++db) acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = -INFINITY, l_part = 0.f;
 
-  auto compute = [&](int SB, const Step& s, const Data& d) __attribute__((always_inline)) {
-    if (s.live == 0u) return;
-    constexpr uint32_t ALL = (1u << NS) - 1u;
+  // One step's keys; all: every one is live for every row, else bit i of word: key i is live for this
+  // lane's row.
+  auto compute = [&](int SB, bool all, uint32_t word, const Data& d) __attribute__((always_inline)) {
     f32x4 x[NS];
 #pragma unroll
     for (int t = 0; t < NS; ++t) {
@@ -251,11 +257,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
         }
       }
     }
-    uint32_t word = 0xffffffffu;  // the step's keys live for this lane's row
-    if (s.full != ALL) {
-      word = mask_word(mask, q_pos, s.key, len);
-      if (!(s.live & 1u)) word &= 0xffff0000u;
-      if (NS == 1 || !(s.live & 2u)) word &= 0x0000ffffu;
+    if (!all) {
 #pragma unroll
       for (int t = 0; t < NS; ++t)
 #pragma unroll
@@ -282,7 +284,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
     }
     if constexpr (F32) {
       bool fin = true;
-      if (s.full != ALL) {
+      if (!all) {
         float big = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -321,7 +323,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
                      __builtin_bit_cast(uint2, x2).y};
       };
       bool fin = true;
-      if (s.full != ALL) {
+      if (!all) {
         Finite16<T> f;
 #pragma unroll
         for (int db = 0; db < NB; ++db) {
@@ -356,7 +358,18 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
     }
   };
 
-  Step s0{}, s1{};
+  auto compute_block = [&](int SB, const Step& s, const Data& d) __attribute__((always_inline)) {
+    if (s.live == 0u) return;
+    const bool all = s.full == (1u << NS) - 1u;
+    uint32_t word = 0xffffffffu;
+    if (!all) {
+      word = mask_word(mask, q_pos, s.key, len);
+      if (!(s.live & 1u)) word &= 0xffff0000u;
+      if (NS == 1 || !(s.live & 2u)) word &= 0x0000ffffu;
+    }
+    compute(SB, all, word, d);
+  };
+
   Data d0{}, d1{};
   // The step's V rows are in LDS and its K rows in registers once everything issued is done.
   // The memory clobber keeps the ring's reads on their side of the wait (no barrier does),
@@ -376,22 +389,126 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
     }
     asm volatile("" ::"v"(r_page));
   };
-  if (n_steps > 0) {
-    load_raw(0);
-    prefetch(0, 0, s0, d0);
-  }
-  int st = 0;
-  for (; st + 1 < n_steps; st += 2) {
-    arrive(d0);
-    prefetch(st + 1, 1, s1, d1);
-    compute(0, s0, d0);
-    arrive(d1);
-    if (st + 2 < n_steps) prefetch(st + 2, 0, s0, d0);
-    compute(1, s1, d1);
-  }
-  if (st < n_steps) {
-    arrive(d0);
-    compute(0, s0, d0);
+  const int n_tok = q_hi - q_lo + 1;
+  if (n_steps > 0) load_raw(0);
+  if (2 * n_tok > a.stride) {
+    // ---- block by block -------------------------------------------------------------
+    Step s0{}, s1{};
+    if (n_steps > 0) prefetch(0, 0, s0, d0);
+    int st = 0;
+    for (; st + 1 < n_steps; st += 2) {
+      arrive(d0);
+      prefetch(st + 1, 1, s1, d1);
+      compute_block(0, s0, d0);
+      arrive(d1);
+      if (st + 2 < n_steps) prefetch(st + 2, 0, s0, d0);
+      compute_block(1, s1, d1);
+    }
+    if (st < n_steps) {
+      arrive(d0);
+      compute_block(0, s0, d0);
+    }
+  } else {
+    // ---- by lists of live keys -------------------------------------------------------
+    // 32 segments at a time: lane l (below 32) finds which of segment l's keys are live for which
+    // tokens of the tile, and the wave lists the keys that are for some: segment and key in it, and
+    // a bit per token above.  Steps then take 32 (f32: 16) listed keys each, row by row.
+    constexpr int PL = S::LIST / 16;            // segments of a list
+    uint32_t* list = reinterpret_cast<uint32_t*>(smem + S::LIST_AT) + w * S::LIST;
+    const int tq = q_pos - q_lo;                // this lane's token among the tile's
+    for (int c = 0; c * (PL / NS) < n_steps; ++c) {
+      const int st0 = c * (PL / NS);            // first step (block) of this list
+      const int32_t key = lane < PL ? key_at(st0 + lane / NS) : len;
+      const int32_t page = checked_page(r_page, a.n_pages);
+      const bool some = key < len && page >= 0 && mask_verdict(mask, q_lo, q_hi, key, key + 15) != kDead;
+      c_off = (int64_t)imax(page, 0) * a.c_sp + (int64_t)(key & ((1 << a.page_lg) - 1)) * a.c_sn;
+      if ((c + 1) * (PL / NS) < n_steps) {
+        const int32_t next = lane < PL ? key_at(st0 + PL / NS + lane / NS) : len;
+        r_page = next < len ? table[next >> a.page_lg] : -1;
+      }
+      uint32_t any = 0u, of[8] = {};            // of[p]: tokens of keys 2 p (low half) and 2 p + 1
+#pragma unroll 1
+      for (int t = 0; t < n_tok; ++t) {
+        const uint32_t x = some ? mask_word(mask, q_lo + t, key, len) & 0xffffu : 0u;
+        any |= x;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) of[p] |= ((x >> (2 * p)) & 1u) << t | ((x >> (2 * p + 1)) & 1u) << (16 + t);
+      }
+      const int n_mine = __builtin_popcount(any), n_in = wave_scan(n_mine);
+      const int total = __builtin_amdgcn_readlane(n_in, 63);
+      int at = n_in - n_mine;
+#pragma unroll
+      for (int b = 0; b < 16; ++b)
+        if ((any >> b) & 1u)
+          list[at++] = (uint32_t)(16 * lane + b) | ((b & 1) ? of[b >> 1] & 0xffff0000u : of[b >> 1] << 16);
+      asm volatile("" ::: "memory");  // (a wave's LDS accesses stay in order)
+      // offset in the cache of listed key i (past the list: the last one's)
+      auto row_off = [&](int i) __attribute__((always_inline)) -> int64_t {
+        const uint32_t e = list[imin(i, total - 1)];
+        const int l = (e >> 4) & (PL - 1);
+        const uint32_t lo = (uint32_t)__shfl((int32_t)(uint32_t)c_off, l);
+        const int32_t hi = __shfl((int32_t)(c_off >> 32), l);
+        return (int64_t)((uint64_t)lo | ((uint64_t)(uint32_t)hi << 32)) + (int64_t)(e & 15u) * a.c_sn;
+      };
+      auto fetch = [&](int i0, int SB, Data& d) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < NS; ++t) {
+          const char* kp = kbase + row_off(i0 + 16 * t + q16) + 16 * g;
+#pragma unroll
+          for (int kc = 0; kc < NK; ++kc) d.k[t][kc] = *reinterpret_cast<const u32x4*>(kp + 64 * kc);
+          if constexpr (F32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const char* vp = vbase + row_off(i0 + 4 * g + j) + 4 * q16;
+#pragma unroll
+              for (int db = 0; db < NB; ++db) d.v[j][db] = *reinterpret_cast<const float*>(vp + 64 * db);
+            }
+          } else {
+            using R = Rows<D>;
+#pragma unroll
+            for (int j = 0; j < R::NI; ++j) {
+              const int r = R::RPI * j + lane / R::UPR;
+              const int sw = D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
+              dma_x4_va(ring0 + SB * STAGE + t * SEG + j * 1024,
+                        vbase + row_off(i0 + 16 * t + r) + 16 * ((lane % R::UPR) ^ sw));
+            }
+          }
+        }
+      };
+      auto take = [&](int i0, int SB, const Data& d) __attribute__((always_inline)) {
+        uint32_t word = 0u;
+        const int n = imin(total - i0, 16 * NS);
+        if (n_tok == 1) {
+          word = n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4 * NS; ++x) {
+            const u32x4 e = *reinterpret_cast<const u32x4*>(list + i0 + 4 * x);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) word |= ((e[z] >> (16 + tq)) & 1u) << (4 * x + z);
+          }
+          if (n < 32) word &= (1u << n) - 1u;  // (entries past the list are of an earlier one)
+        }
+        compute(SB, n_tok == 1 && n == 16 * NS, word, d);
+      };
+      constexpr int ST = 16 * NS;
+      if (total > 0) fetch(0, 0, d0);
+      int i = 0;
+      for (; i + ST < total; i += 2 * ST) {
+        arrive(d0);
+        fetch(i + ST, 1, d1);
+        take(i, 0, d0);
+        arrive(d1);
+        if (i + 2 * ST < total) fetch(i + 2 * ST, 0, d0);
+        take(i + ST, 1, d1);
+      }
+      if (i < total) {
+        arrive(d0);
+        take(i, 0, d0);
+      }
+      // (the last step's reads of its stage are done before the next list's DMA into it)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
   }
 
   // ---- the waves' states become one, and those of the tile's shares ---------------------

@@ -298,6 +298,23 @@ def test_chunks(gpu, dtype, D, Hq, Hkv):
     b.check(pm.LocalStrided(60, 16))
 
 
+LATTICES = [pm.Dilated(2), pm.Dilated(16), pm.Dilated(33), pm.Dilated(5000), pm.LocalStrided(40, 16), pm.LocalStrided(0, 64),
+            MaskSpec(((2, 16, 0, 0),), ((1, 40, 0, 0),)), MaskSpec(((2, 32, 0, 0), (5, 10, 3, 0))),
+            MaskSpec(((2, 8, 0, 0), (2, 12, 0, 0))), MaskSpec(((3, 30, 24, 0),), ((2, 48, 0, 0), (1, 2, 0, 0)))]
+
+
+@pytest.mark.parametrize("mask", LATTICES, ids=lambda m: getattr(m, "name", str(getattr(m, "include", m))))
+@pytest.mark.parametrize("dtype,D,Hq,Hkv", [(torch.bfloat16, 128, 8, 1), (torch.float16, 64, 4, 4), (torch.float32, 64, 4, 2),
+                                            (torch.float32, 128, 2, 2)])
+def test_lattices_of_few_tokens(gpu, dtype, D, Hq, Hkv, mask):
+    """Lists of live keys: none, one, exactly a step's and one more, a band inside the lattice, pages that
+    end inside, more keys than a list, several shares, tokens of one tile with lists of their own."""
+    sizes = [(1, 1), (1, 16), (1, 17), (2, 40), (3, 512), (1, 513), (5, 700), (1, 2049), (8, 2500), (16, 900), (0, 7), (1, 6000)]
+    b = Batch(gpu, dtype, D, 16, Hq, Hkv, sizes, seed=D + Hq)
+    b.tables[7, 40:44] = -1
+    b.check(mask)
+
+
 @pytest.mark.parametrize("mask", [pm.Causal(), pm.SinksWindow(64, 1024), pm.LocalStrided(256, 16)], ids=lambda m: m.name)
 @pytest.mark.parametrize("dtype,D,sizes", [
     (torch.bfloat16, 128, [(1, 20001)]), (torch.float16, 64, [(1, 9000), (3, 16384), (1, 31), (2, 5000)]),
@@ -354,7 +371,7 @@ def test_masked_places_may_hold_anything(gpu, dtype, D, n, what):
     1) round by 2^-24 of it each, in either order; then both round to the type, half a step each."""
     L, w = 200, 50
     for t in (L - 1, L - n // 2 - 1, L - n - 3, L - w - n // 2, 3):
-        for mask in (pm.SlidingWindow(w), pm.SinksWindow(2, w)):
+        for mask in (pm.SlidingWindow(w), pm.SinksWindow(2, w), pm.LocalStrided(10, 24)):
             b = Batch(gpu, dtype, D, 32, 8, 4, [(n, L), (2, 33)], seed=n)
             clean, lse0 = b.run(mask)
             page, off = int(b.tables[0, t // 32]), t % 32
