@@ -28,7 +28,8 @@ int stride_of(const pa_mask& m) {
 // Workspace: the counts of both parts, then their slots.
 struct PagedPlan {
   int page_lg;
-  bool tile;            // some request may have more than kFewRows rows
+  bool tile;            // some request may have more rows than a tile of few rows takes
+  int stride;
   PagedPart rows, tiles;
   int64_t zero, bytes;
 };
@@ -61,24 +62,32 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   PA_CHECK_ARG(x->max_fresh >= 0, "pa_paged_attn: max_fresh=%lld", (long long)x->max_fresh);
   PA_CHECK_ARG(x->cols >= 0 && ((int64_t)x->cols << p->page_lg) <= kMaxPosition && x->pitch >= x->cols,
                "pa_paged_attn: %d columns of %d, pitch %lld", x->cols, x->page_size, (long long)x->pitch);
+  PA_CHECK_ARG(!x->mask.perm_q && !x->mask.perm_kv, "pa_paged_attn: the mask takes no permutation tables");
+  for (int i = 0; i < x->mask.n_include + x->mask.n_exclude && i < PA_MAX_TERMS; ++i)
+    PA_CHECK_ARG(x->mask.terms[i].kind != PA_DENSE, "pa_paged_attn: PA_DENSE has no meaning here");
+  if (int rc = check_mask(&x->mask, 0)) return rc;
   PA_CHECK_ARG(x->scale > 0.f && x->scale < INFINITY, "pa_paged_attn: scale=%g must be positive", (double)x->scale);
+  p->stride = stride_of(x->mask);
   const int64_t G = x->Hq / x->Hkv, some = x->T < x->R ? x->T : x->R;  // some: requests with rows, at most
-  p->tile = x->dtype != PA_F32 && x->n_pages > 0 && x->max_fresh * G > kFewRows;
+  // (tiles of few rows that take lists read 1 / stride of the keys for each token, a chunk's tile all)
+  const int span = (int)((kRows + G - 1) / G) + 1;
+  const int64_t few_rows = 2 * span <= p->stride && G * p->stride / 2 > kFewRows ? (G * p->stride / 2 < kTileRows ? G * p->stride / 2 : kTileRows) : kFewRows;
+  p->tile = x->dtype != PA_F32 && x->n_pages > 0 && x->max_fresh * G > few_rows;
   int64_t few = x->T * G / kRows + some;
-  if (p->tile && few > some * (kFewRows / kRows)) few = some * (kFewRows / kRows);
+  if (p->tile && few > some * ((few_rows + kRows - 1) / kRows)) few = some * ((few_rows + kRows - 1) / kRows);
   if (int rc = part_of(x, kRows, kRowsTarget, few, &p->rows)) return rc;
   p->rows.long_share = 32;
   p->rows.least = 4;
   p->rows.root_over = 0.7f;
   p->rows.row_min = 0;
-  p->rows.row_max = p->tile ? kFewRows : INT_MAX;
+  p->rows.row_max = p->tile ? (int32_t)few_rows : INT_MAX;
   p->tiles = PagedPart{};
   if (p->tile) {
     if (int rc = part_of(x, kTileRows, kTileTarget, x->T * G / kTileRows + some, &p->tiles)) return rc;
     p->tiles.long_share = 0;
     p->tiles.least = 8;
     p->tiles.root_over = 1.f;
-    p->tiles.row_min = kFewRows;
+    p->tiles.row_min = (int32_t)few_rows;
     p->tiles.row_max = INT_MAX;
   }
   p->zero = (4 * ((int64_t)p->rows.slots + p->tiles.slots) + 255) / 256 * 256;
@@ -102,10 +111,6 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
   using namespace pa;
   PagedPlan p;
   if (int rc = plan_of(x, &p)) return rc;
-  PA_CHECK_ARG(!x->mask.perm_q && !x->mask.perm_kv, "pa_paged_attn: the mask takes no permutation tables");
-  for (int i = 0; i < x->mask.n_include + x->mask.n_exclude && i < PA_MAX_TERMS; ++i)
-    PA_CHECK_ARG(x->mask.terms[i].kind != PA_DENSE, "pa_paged_attn: PA_DENSE has no meaning here");
-  if (int rc = check_mask(&x->mask, 0)) return rc;
   if (x->R == 0 || x->T == 0) return PA_OK;
   PA_CHECK_ARG(x->q && x->o && x->lengths && x->q_start, "pa_paged_attn: null q / o / lengths / q_start");
   PA_CHECK_ARG(x->cols == 0 || x->tables, "pa_paged_attn: null tables");
@@ -154,7 +159,7 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
     t.p2 = imin(t.p2, kMaxPosition);
     a.terms[i] = t;
   }
-  a.stride = stride_of(x->mask);
+  a.stride = p.stride;
   a.o = static_cast<char*>(x->o);
   a.o_st = x->o_st * esz;
   a.o_sh = x->o_sh * esz;

@@ -90,8 +90,8 @@ __device__ __forceinline__ Work work_of(const PagedK& a, const PagedPart& p, con
   const int32_t rows = q.n * a.G;
   if (rows <= p.row_min || rows > p.row_max) return {0, 0, 1};
   const int32_t span = imin(q.n, p.span);
-  // (a share that is taken by lists: one list of 512 keys for each wave)
-  const int32_t least = BM == kRows && 2 * span <= a.stride ? 2048 >> LG : p.least;
+  // (a share that is taken by lists: for one token a list of 512 keys for each wave, for more fewer)
+  const int32_t least = BM == kRows && 2 * span <= a.stride ? imax((int32_t)((2048u >> LG) / (uint32_t)imax(span, 1)), p.least) : p.least;
   return {(rows + BM - 1) / BM, key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG).count(), least};
 }
 

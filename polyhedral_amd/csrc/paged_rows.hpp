@@ -420,7 +420,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
       const int st0 = c * (PL / NS);            // first step (block) of this list
       const int32_t key = lane < PL ? key_at(st0 + lane / NS) : len;
       const int32_t page = checked_page(r_page, a.n_pages);
-      const bool some = key < len && page >= 0 && mask_verdict(mask, q_lo, q_hi, key, key + 15) != kDead;
+      const bool some = key < len && page >= 0;
       c_off = (int64_t)imax(page, 0) * a.c_sp + (int64_t)(key & ((1 << a.page_lg) - 1)) * a.c_sn;
       if ((c + 1) * (PL / NS) < n_steps) {
         const int32_t next = lane < PL ? key_at(st0 + PL / NS + lane / NS) : len;
@@ -562,30 +562,59 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
       }
     }
     if (!last_share(part, u, tid, flag)) return;
-    // every fourth share to a wave, four rows at a time; then as the waves' states above
-    const int col = (lane & 15) * CPT;
-    for (int r = lane >> 4; r - (lane >> 4) < n_rows; r += 4) {
-      const char* ml = first + ML + 8 * r;
-      const char* po = first + (r * D + col) * 4;
-      float m = -INFINITY, l = 0.f;
-#pragma unroll 4
-      for (int s = w; s < u.splits; s += kWaves) m = nan_max(m, share_load(reinterpret_cast<const float*>(ml + (int64_t)s * SLOT_B)));
-      f32x4 x[CPT / 4];
+    // every fourth share to a wave, two of them at once: lane (row 4 i + l / 16, the columns of l % 16)
+    // for all i, every load of a pair on its way before the first is used; then as the waves' states
+    // above
+    const int r0 = lane >> 4, col = (lane & 15) * CPT;
+    float m[4], l[4];
+    f32x4 x[4][CPT / 4];
 #pragma unroll
-      for (int e = 0; e < CPT / 4; ++e) x[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int s = w; s < u.splits; s += kWaves) {
-        const float* at = reinterpret_cast<const float*>(ml + (int64_t)s * SLOT_B);
-        const float f = __builtin_amdgcn_exp2f((share_load(at) - base_of(m)) * a.c);
-        l += f * share_load(at + 1);
+    for (int i = 0; i < 4; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
 #pragma unroll
-        for (int e = 0; e < CPT / 4; ++e) x[e] += f * share_load4(po + (int64_t)s * SLOT_B + 16 * e);
+      for (int e = 0; e < CPT / 4; ++e) x[i][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll 1
+    for (int s = w; s < u.splits; s += 2 * kWaves) {
+      float ms[2][4], ls[2][4];
+      f32x4 os[2][4][CPT / 4];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const char* at = first + (int64_t)imin(s + y * kWaves, u.splits - 1) * SLOT_B;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (4 * i >= n_rows) break;
+          const float* ml = reinterpret_cast<const float*>(at + ML + 8 * (4 * i + r0));
+          ms[y][i] = share_load(ml);
+          ls[y][i] = share_load(ml + 1);
+#pragma unroll
+          for (int e = 0; e < CPT / 4; ++e) os[y][i][e] = share_load4(at + ((4 * i + r0) * D + col + 4 * e) * 4);
+        }
       }
 #pragma unroll
-      for (int e = 0; e < CPT / 4; ++e) *reinterpret_cast<f32x4*>(red_o + (w * kRows + r) * S::OP + col + 4 * e) = x[e];
+      for (int y = 0; y < 2; ++y) {
+        if (s + y * kWaves >= u.splits) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (4 * i >= n_rows) break;
+          const float mn = nan_max(m[i], ms[y][i]);
+          const float f0 = __builtin_amdgcn_exp2f((m[i] - base_of(mn)) * a.c), f1 = __builtin_amdgcn_exp2f((ms[y][i] - base_of(mn)) * a.c);
+          m[i] = mn;
+          l[i] = f0 * l[i] + f1 * ls[y][i];
+#pragma unroll
+          for (int e = 0; e < CPT / 4; ++e) x[i][e] = f0 * x[i][e] + f1 * os[y][i][e];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * i + r0;
+#pragma unroll
+      for (int e = 0; e < CPT / 4; ++e) *reinterpret_cast<f32x4*>(red_o + (w * kRows + r) * S::OP + col + 4 * e) = x[i][e];
       if (col == 0) {
-        red_ml[2 * (w * kRows + r)] = m;
-        red_ml[2 * (w * kRows + r) + 1] = l;
+        red_ml[2 * (w * kRows + r)] = m[i];
+        red_ml[2 * (w * kRows + r) + 1] = l[i];
       }
     }
     gather();
