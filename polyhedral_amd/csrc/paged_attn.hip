@@ -148,6 +148,7 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
   a.Hkv = x->Hkv;
   a.G = x->Hq / x->Hkv;
   a.by_G = divisor_of((uint32_t)a.G);
+  a.by_Hkv = divisor_of((uint32_t)a.Hkv);
   a.c = x->scale * 1.4426950408889634f;
   a.n_include = x->mask.n_include;
   a.n_exclude = x->mask.n_exclude;

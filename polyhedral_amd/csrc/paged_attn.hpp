@@ -52,7 +52,7 @@ struct PagedK {
   const int32_t* lengths;
   const int32_t* q_start;
   int32_t R, T, Hkv, G;
-  Divisor by_G;
+  Divisor by_G, by_Hkv;
   float c;  // scale * log2(e)
   int32_t n_include, n_exclude;
   pa_term terms[PA_MAX_TERMS];
@@ -91,7 +91,7 @@ __device__ __forceinline__ Work work_of(const PagedK& a, const PagedPart& p, con
   if (rows <= p.row_min || rows > p.row_max) return {0, 0, 1};
   const int32_t span = imin(q.n, p.span);
   // (a share that is taken by lists: for one token a list of 512 keys for each wave, for more fewer)
-  const int32_t least = BM == kRows && 2 * span <= a.stride ? imax((int32_t)((2048u >> LG) / (uint32_t)imax(span, 1)), p.least) : p.least;
+  const int32_t least = BM == kRows && 2 * span <= a.stride ? imax((2048 >> LG) >> (31 - __builtin_clz((uint32_t)imax(span, 1))), p.least) : p.least;
   return {(rows + BM - 1) / BM, key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG).count(), least};
 }
 
@@ -162,7 +162,7 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, i
   // (rounded up, so the units stay within target + tiles Hkv, which the grid is sized for)
   float share = total * (float)a.Hkv / (float)p.target * 1.0001f;
   share = fmaxf(share, fminf(2.f * share, (float)p.long_share));
-  const int32_t chunk = share < 1e9f ? (int32_t)share + 1 : (1 << 30);
+  const float chunk = share;
 
   int32_t before = 0, slot = 0;  // units and slots of earlier requests
   end = 0;
@@ -172,10 +172,10 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, i
       w = work_of<BM, LG>(a, p, q);
     }
     // (to the nearest: a tile little longer than a share stays whole)
-    const uint32_t mine_chunk = (uint32_t)imax(imax(chunk, w.least), (int32_t)(__builtin_amdgcn_sqrtf((float)w.blocks) * p.root_over) + 1);
-    const int32_t splits = imax((int32_t)(((uint32_t)w.blocks + mine_chunk / 2u) / mine_chunk), 1);
-    const int32_t units = w.tiles * a.Hkv * splits, mine = splits > 1 ? units : 0;
-    const int32_t n_in = wave_scan(units), s_in = wave_scan(mine);
+    const float b = (float)w.blocks, mine = fmaxf(fmaxf(chunk, (float)w.least), __builtin_amdgcn_sqrtf(b) * p.root_over);
+    const int32_t splits = imax((int32_t)(b * __builtin_amdgcn_rcpf(mine) + 0.5f), 1);
+    const int32_t units = w.tiles * a.Hkv * splits, slotted = splits > 1 ? units : 0;
+    const int32_t n_in = wave_scan(units), s_in = wave_scan(slotted);
     const int32_t at = before + n_in - units;
     const uint64_t hit = __ballot(at <= id && id < at + units);
     if (hit) {
@@ -185,14 +185,13 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, i
       u.r = r0 + l;
       u.rq = {get(q.start), get(q.n), get(q.len)};
       u.splits = get(splits);
-      // a KV head's shares side by side, its tiles a multiple of Hkv units apart: with 8 KV heads
-      // the tiles of one fall on one XCD (work-groups are dealt to the XCDs in turn) and share
-      // its L2
-      const int32_t x = id - get(at), per = a.Hkv * u.splits;
-      const int32_t tile = (int32_t)((uint32_t)x / (uint32_t)per), y = x - tile * per;
-      u.h = (int32_t)((uint32_t)y / (uint32_t)u.splits);
-      u.split = y - u.h * u.splits;
-      u.slot = slot + get(s_in - mine) + x - u.split;
+      // KV heads side by side, so that those of one head are Hkv units apart: with 8 of them a head's
+      // work falls on one XCD (work-groups are dealt to the XCDs in turn) and shares its L2
+      const int32_t x = id - get(at), y = divide(x, a.by_Hkv);
+      u.h = x - y * a.Hkv;
+      const int32_t tile = u.splits == 1 ? y : (int32_t)((uint32_t)y / (uint32_t)u.splits);
+      u.split = y - tile * u.splits;
+      u.slot = slot + get(s_in - slotted) + (tile * a.Hkv + u.h) * u.splits;
       // (a causal mask's longest tile first)
       u.tile = get(w.tiles) - 1 - tile;
       return u;
