@@ -44,7 +44,7 @@ int part_of(const pa_paged_args* x, int BM, int target, int64_t max_tiles, Paged
   PA_CHECK_ARG(most <= 0x3fffffffll, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)most);
   p->grid = (int32_t)most;
   p->slots = (int32_t)(2 * target < most ? 2 * target : most);
-  p->target = target;
+  p->by_target = 1.0001f / (float)target;
   const int G = x->Hq / x->Hkv;
   p->span = (BM + G - 1) / G + 1;
   return PA_OK;
@@ -76,7 +76,7 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   int64_t few = x->T * G / kRows + some;
   if (p->tile && few > some * ((few_rows + kRows - 1) / kRows)) few = some * ((few_rows + kRows - 1) / kRows);
   if (int rc = part_of(x, kRows, kRowsTarget, few, &p->rows)) return rc;
-  p->rows.long_share = 32;
+  p->rows.long_share = 32.f;
   p->rows.least = 4;
   p->rows.root_over = 0.7f;
   p->rows.row_min = 0;
@@ -84,7 +84,7 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   p->tiles = PagedPart{};
   if (p->tile) {
     if (int rc = part_of(x, kTileRows, kTileTarget, x->T * G / kTileRows + some, &p->tiles)) return rc;
-    p->tiles.long_share = 0;
+    p->tiles.long_share = 0.f;
     p->tiles.least = 8;
     p->tiles.root_over = 1.f;
     p->tiles.row_min = (int32_t)few_rows;

@@ -30,10 +30,10 @@ struct PagedPart {
   int32_t* count;       // [slots] units done, at a tile's first slot; zero between calls
   int32_t slots;
   // Blocks of a share: total / target, or where that is less than `long_share` blocks the smaller of
-  // long_share and 2 total / target; but at least `least`, and the root of the tile's blocks over
+  // long_share and 2 total / target; but at least `least`, and the root of the tile's blocks times
   // root_over (the time of a share against that of merging them all).
-  int32_t target, long_share, least;
-  float root_over;
+  float by_target, long_share, root_over;  // by_target: 1.0001 / target
+  int32_t least;
   int32_t span;         // new tokens that a tile can hold rows of
   int32_t row_min, row_max;  // requests with row_min < rows <= row_max
   int32_t grid;
@@ -120,19 +120,26 @@ __device__ __forceinline__ float wave_total(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int32_t, x), 63));
 }
 
+// What q_start and lengths hold for request r0 + lane (past R: zeros).
+struct RawRequest {
+  int32_t s0, s1, len;
+};
+__device__ __forceinline__ RawRequest raw_request(const PagedK& a, int r0, int lane) {
+  RawRequest x{0, 0, 0};
+  if (r0 + lane < a.R) {
+    x.s0 = a.q_start[r0 + lane];
+    x.s1 = a.q_start[r0 + lane + 1];
+    x.len = a.lengths[r0 + lane];
+  }
+  return x;
+}
+
 // Request r0 + lane (past R: none).  `end`: the largest start so far.  Starts that fall back are
 // taken as that, so whatever q_start holds the requests' rows are disjoint, and the units and slots
 // stay within what the host sized for T rows.
-__device__ __forceinline__ Request load_request(const PagedK& a, int r0, int lane, int32_t& end) {
+__device__ __forceinline__ Request load_request(const PagedK& a, const RawRequest& x, int r0, int lane, int32_t& end) {
   const int r = r0 + lane;
-  int32_t s0 = 0, s1 = 0, len = 0;
-  if (r < a.R) {
-    s0 = a.q_start[r];
-    s1 = a.q_start[r + 1];
-    len = a.lengths[r];
-  }
-  s0 = imin(imax(s0, 0), a.T);
-  s1 = imin(imax(s1, 0), a.T);
+  int32_t s0 = imin(imax(x.s0, 0), a.T), s1 = imin(imax(x.s1, 0), a.T);
   if (__ballot(r < a.R && (s1 < s0 || s0 < end)) != 0ull) {
     s0 = imax(s0, end);
 #pragma unroll 1
@@ -143,11 +150,11 @@ __device__ __forceinline__ Request load_request(const PagedK& a, int r0, int lan
     s1 = imax(s1, s0);
   }
   end = __builtin_amdgcn_readlane(s1, imin(a.R - 1 - r0, 63));
-  return request_of(s0, s1, len, a.T, a.cols << a.page_lg);
+  return request_of(s0, s1, x.len, a.T, a.cols << a.page_lg);
 }
 
 template <int BM, int LG>
-__device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, int32_t id, int lane) {
+__device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, const RawRequest& raw, int32_t id, int lane) {
   Unit u;
   u.found = false;
   Request q{0, 0, 0};
@@ -155,24 +162,23 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, i
   float total = 0.f;  // (a share needs no exact total)
   int32_t end = 0;
   for (int r0 = 0; r0 < a.R; r0 += 64) {
-    q = load_request(a, r0, lane, end);
+    q = load_request(a, r0 == 0 ? raw : raw_request(a, r0, lane), r0, lane, end);
     w = work_of<BM, LG>(a, p, q);
     total += wave_total((float)w.tiles * (float)w.blocks);
   }
   // (rounded up, so the units stay within target + tiles Hkv, which the grid is sized for)
-  float share = total * (float)a.Hkv / (float)p.target * 1.0001f;
-  share = fmaxf(share, fminf(2.f * share, (float)p.long_share));
-  const float chunk = share;
+  float share = total * (float)a.Hkv * p.by_target;
+  share = fmaxf(share, fminf(2.f * share, p.long_share));
 
   int32_t before = 0, slot = 0;  // units and slots of earlier requests
   end = 0;
   for (int r0 = 0; r0 < a.R; r0 += 64) {
     if (a.R > 64) {
-      q = load_request(a, r0, lane, end);
+      q = load_request(a, r0 == 0 ? raw : raw_request(a, r0, lane), r0, lane, end);
       w = work_of<BM, LG>(a, p, q);
     }
     // (to the nearest: a tile little longer than a share stays whole)
-    const float b = (float)w.blocks, mine = fmaxf(fmaxf(chunk, (float)w.least), __builtin_amdgcn_sqrtf(b) * p.root_over);
+    const float b = (float)w.blocks, mine = fmaxf(fmaxf(share, (float)w.least), __builtin_amdgcn_sqrtf(b) * p.root_over);
     const int32_t splits = imax((int32_t)(b * __builtin_amdgcn_rcpf(mine) + 0.5f), 1);
     const int32_t units = w.tiles * a.Hkv * splits, slotted = splits > 1 ? units : 0;
     const int32_t n_in = wave_scan(units), s_in = wave_scan(slotted);

@@ -101,7 +101,36 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
   const int tid = threadIdx.x, lane = tid & 63, q16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const Unit u = find_unit<kRows, S::LG>(a, part, id, lane);
+  const RawRequest raw = raw_request(a, 0, lane);
+  // (what depends on the lane alone, while these are on their way)
+  const uint32_t koff = (uint32_t)(q16 * (int32_t)a.c_sn) + 16u * (uint32_t)g;
+  uint32_t voff[F32 ? 4 : Rows<D>::NI];
+  if constexpr (F32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) voff[j] = (uint32_t)((4 * g + j) * (int32_t)a.c_sn) + 4u * (uint32_t)q16;
+  } else {
+    using R = Rows<D>;
+#pragma unroll
+    for (int j = 0; j < R::NI; ++j) {
+      const int r = R::RPI * j + lane / R::UPR;
+      const int sw = D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
+      voff[j] = (uint32_t)(r * (int32_t)a.c_sn) + 16u * (uint32_t)((lane % R::UPR) ^ sw);
+    }
+  }
+  const uint32_t ring0 = (uint32_t)(uintptr_t)(lds_char_t*)smem + (uint32_t)(w * 2 * STAGE);
+  lds_cptr vptr[F32 ? 1 : NB];
+  if constexpr (!F32) {
+    // transposed reads of 16 columns (block db) of rows 4 g + q16 / 4 of a segment
+#pragma unroll
+    for (int db = 0; db < NB; ++db) {
+      const int r = 4 * g + (q16 >> 2);
+      const int sw = D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
+      vptr[db] = (lds_cptr)smem + w * 2 * STAGE + r * ROW + 16 * ((2 * db + ((q16 & 3) >> 1)) ^ sw) + 8 * (q16 & 1);
+      asm volatile("" : "+v"(vptr[db]));
+    }
+  }
+
+  const Unit u = find_unit<kRows, S::LG>(a, part, raw, id, lane);
   if (!u.found) return;
 
   // ---- the tile's rows -----------------------------------------------------------
@@ -150,11 +179,9 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
   auto take_raw = [&](int c) __attribute__((always_inline)) {
     const int32_t key = key_of(c);
     const int32_t page = checked_page(r_page, a.n_pages);
-    int v = kDead;
-    if (key < len && page >= 0) {
-      v = mask_verdict(mask, q_lo, q_hi, key, key + 15);
-      if (v == kFull && key + 15 >= len) v = kPartial;
-    }
+    int v = mask_verdict(mask, q_lo, q_hi, key, key + 15);  // (does not wait for the pages)
+    if (v == kFull && key + 15 >= len) v = kPartial;
+    if (key >= len || page < 0) v = kDead;
     c_live = __ballot(v != kDead);
     c_full = __ballot(v == kFull);
     c_key = key;
@@ -166,33 +193,6 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
       if (dead) c_off = (int64_t)((uint64_t)(uint32_t)lo | ((uint64_t)(uint32_t)hi << 32));
     }
   };
-
-  const uint32_t koff = (uint32_t)(q16 * (int32_t)a.c_sn) + 16u * (uint32_t)g;
-  uint32_t voff[F32 ? 4 : Rows<D>::NI];
-  if constexpr (F32) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) voff[j] = (uint32_t)((4 * g + j) * (int32_t)a.c_sn) + 4u * (uint32_t)q16;
-  } else {
-    using R = Rows<D>;
-#pragma unroll
-    for (int j = 0; j < R::NI; ++j) {
-      const int r = R::RPI * j + lane / R::UPR;
-      const int sw = D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
-      voff[j] = (uint32_t)(r * (int32_t)a.c_sn) + 16u * (uint32_t)((lane % R::UPR) ^ sw);
-    }
-  }
-  const uint32_t ring0 = (uint32_t)(uintptr_t)(lds_char_t*)smem + (uint32_t)(w * 2 * STAGE);
-  lds_cptr vptr[F32 ? 1 : NB];
-  if constexpr (!F32) {
-    // transposed reads of 16 columns (block db) of rows 4 g + q16 / 4 of a segment
-#pragma unroll
-    for (int db = 0; db < NB; ++db) {
-      const int r = 4 * g + (q16 >> 2);
-      const int sw = D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
-      vptr[db] = (lds_cptr)smem + w * 2 * STAGE + r * ROW + 16 * ((2 * db + ((q16 & 3) >> 1)) ^ sw) + 8 * (q16 & 1);
-      asm volatile("" : "+v"(vptr[db]));
-    }
-  }
 
   struct Step {
     int key;

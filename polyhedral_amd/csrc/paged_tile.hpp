@@ -57,7 +57,16 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   const int tid = threadIdx.x, lane = tid & 63, G = lane >> 5, m = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const Unit u = find_unit<kTileRows, kTileLg>(a, part, id, lane);
+  const RawRequest raw = raw_request(a, 0, lane);
+  // (what depends on the lane alone, while these are on their way)
+  uint32_t doff[R::NI];
+  dma_offsets<D>(doff, a.c_sn, lane);
+#pragma unroll
+  for (int x = 1; x < R::NI; ++x) doff[x] += (uint32_t)(x * R::RPI * a.c_sn);
+  // (K reads are on the slot of the step ahead, V reads on that of the current one; a slot is one bit
+  // of an address, as the rings are aligned to two slots)
+  TileReads<D> rd = tile_reads<D>((lds_cptr)smem, lane);
+  const Unit u = find_unit<kTileRows, kTileLg>(a, part, raw, id, lane);
   if (!u.found) return;
 
   // ---- rows ------------------------------------------------------------------------
@@ -76,11 +85,6 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   const int32_t* table = a.tables + (int64_t)u.r * a.pitch;
   const char* kbase = a.k + u.h * a.c_sh;
   const char* vbase = a.v + u.h * a.c_sh;
-  uint32_t doff[R::NI];
-  dma_offsets<D>(doff, a.c_sn, lane);
-#pragma unroll
-  for (int x = 1; x < R::NI; ++x) doff[x] += (uint32_t)(x * R::RPI * a.c_sn);
-
   // 16 steps: lane 4 s + t holds segment t of step s, its offset in the cache; bit 4 s + t of live /
   // full: some pair of it may be live for this wave / all are.  The next 16 steps' pages are loaded
   // halfway through these.
@@ -98,11 +102,9 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   auto take_raw = [&](int c) __attribute__((always_inline)) {
     const int32_t key = key_of(c);
     const int32_t page = checked_page(r_page, a.n_pages);
-    int v = kDead;
-    if (key < len && page >= 0) {
-      v = mask_verdict(mask, q_lo, q_hi, key, key + 15);
-      if (v == kFull && key + 15 >= len) v = kPartial;
-    }
+    int v = mask_verdict(mask, q_lo, q_hi, key, key + 15);  // (does not wait for the pages)
+    if (v == kFull && key + 15 >= len) v = kPartial;
+    if (key >= len || page < 0) v = kDead;
     c_live = __ballot(v != kDead);
     c_full = __ballot(v == kFull);
     // (keys without a page read the cache's first one, and are dead)
@@ -138,10 +140,6 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
 #pragma unroll
     for (int x = 0; x < R::NI; ++x) dma_x4(lds0 + ring + (uint32_t)(w * 16 * R::ROW) + x * 1024, base, doff[x]);
   };
-
-  // (K reads are on the slot of the step ahead, V reads on that of the current one; a slot is one bit
-  // of an address, as the rings are aligned to two slots)
-  TileReads<D> rd = tile_reads<D>((lds_cptr)smem, lane);
 
   f32x16 acc[NDB];
 #pragma unroll
