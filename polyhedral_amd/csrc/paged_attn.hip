@@ -7,8 +7,6 @@
 namespace pa {
 namespace {
 
-constexpr int kTileTarget = 512;   // units that the splits of the chunks' tiles aim for, and of the
-constexpr int kRowsTarget = 1024;  // tiles of few rows (two work-groups run per CU)
 constexpr int kFewRows = 32;   // rows of a request (new tokens times heads of a group) up to which
                                // it is a tile of few rows
 
@@ -35,16 +33,16 @@ struct PagedPlan {
 };
 
 // A part whose requests have at most max_tiles tiles: its grid and slots.  (The shares of all tiles are
-// at most the target and one more for each tile and KV head; a tile that is split has two shares at
+// at most `shares` and one more for each tile and KV head; a tile that is split has two shares at
 // least, and then less than twice those that its blocks fill.  The work-groups without a unit each
 // hold a place on a CU for 1.5 us; a grid without them, whose groups loop over units, costs more: 276
 // -> 296 us of sinks in chunks, 15 -> 17 us of one token over 8000, by registers that the loop holds.)
-int part_of(const pa_paged_args* x, int BM, int target, int64_t max_tiles, PagedPart* p) {
-  const int64_t most = target + max_tiles * x->Hkv;
+int part_of(const pa_paged_args* x, int BM, int shares, int64_t max_tiles, PagedPart* p) {
+  const int64_t most = shares + max_tiles * x->Hkv;
   PA_CHECK_ARG(most <= 0x3fffffffll, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)most);
   p->grid = (int32_t)most;
-  p->slots = (int32_t)(2 * target < most ? 2 * target : most);
-  p->by_target = 1.0001f / (float)target;
+  p->slots = (int32_t)(2 * shares < most ? 2 * shares : most);
+  p->by_shares = 1.0001f / (float)shares;
   const int G = x->Hq / x->Hkv;
   p->span = (BM + G - 1) / G + 1;
   return PA_OK;
@@ -75,16 +73,14 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   p->tile = x->dtype != PA_F32 && x->n_pages > 0 && x->max_fresh * G > few_rows;
   int64_t few = x->T * G / kRows + some;
   if (p->tile && few > some * ((few_rows + kRows - 1) / kRows)) few = some * ((few_rows + kRows - 1) / kRows);
-  if (int rc = part_of(x, kRows, kRowsTarget, few, &p->rows)) return rc;
-  p->rows.long_share = 32.f;
+  if (int rc = part_of(x, kRows, p->tile ? 256 : 1024, few, &p->rows)) return rc;
   p->rows.least = 4;
   p->rows.root_over = 0.7f;
   p->rows.row_min = 0;
   p->rows.row_max = p->tile ? (int32_t)few_rows : INT_MAX;
   p->tiles = PagedPart{};
   if (p->tile) {
-    if (int rc = part_of(x, kTileRows, kTileTarget, x->T * G / kTileRows + some, &p->tiles)) return rc;
-    p->tiles.long_share = 0.f;
+    if (int rc = part_of(x, kTileRows, 512, x->T * G / kTileRows + some, &p->tiles)) return rc;
     p->tiles.least = 8;
     p->tiles.root_over = 1.f;
     p->tiles.row_min = (int32_t)few_rows;

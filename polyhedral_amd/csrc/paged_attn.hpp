@@ -29,11 +29,11 @@ struct PagedPart {
   char* part;           // [slots] states of split tiles' units
   int32_t* count;       // [slots] units done, at a tile's first slot; zero between calls
   int32_t slots;
-  // Blocks of a share: total / target, or where that is less than `long_share` blocks the smaller of
-  // long_share and 2 total / target; but at least `least`, and the root of the tile's blocks times
-  // root_over (the time of a share against that of merging them all).
-  float by_target, long_share, root_over;  // by_target: 1.0001 / target
+  // A share is at least `least` blocks, and the root of its tile's blocks times root_over (the time of
+  // a share against that of merging them all).
   int32_t least;
+  float root_over;
+  float by_shares;      // 1.0001 / the most shares that all the work is cut into, beyond one a tile
   int32_t span;         // new tokens that a tile can hold rows of
   int32_t row_min, row_max;  // requests with row_min < rows <= row_max
   int32_t grid;
@@ -166,9 +166,12 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, c
     w = work_of<BM, LG>(a, p, q);
     total += wave_total((float)w.tiles * (float)w.blocks);
   }
-  // (rounded up, so the units stay within target + tiles Hkv, which the grid is sized for)
-  float share = total * (float)a.Hkv * p.by_target;
-  share = fmaxf(share, fminf(2.f * share, p.long_share));
+  // Blocks of a share: all of the part's work over `shares`; few rows: that over half as many where it
+  // is less than 32 blocks (two work-groups run per CU, so 1024 shares are two rounds: 64 requests of
+  // 300 to 8000 tokens 157 -> 147 us against one round, 8 of 4000, whose shares are short, 27 -> 34).
+  // (Rounded up, so the units stay within shares + tiles Hkv, which the grid is sized for.)
+  float share = total * (float)a.Hkv * p.by_shares;
+  if (BM == kRows) share = fmaxf(share, fminf(2.f * share, 32.f));
 
   int32_t before = 0, slot = 0;  // units and slots of earlier requests
   end = 0;
