@@ -495,7 +495,7 @@ int pa_attn_bwd(const pa_attn_bwd_args* args, void* stream);
  *   4  more new tokens than rows (`tokens`)
  * and then nothing is taken: tables stay, lengths = before, q_start is all 0, the slots and
  * positions -1, *free_left = free_count.  lengths may be `before` and free_left may be
- * free_count.  A token whose page is none of the cache gets slot -1.  workspace: int32 [3 R +
+ * free_count; no other output overlaps an input.  A token whose page is none of the cache gets slot -1.  workspace: int32 [3 R +
  * 2].
  *
  * pa_page_release: pages first[r] .. last[r] - 1 of request r's table (clamped to the table;

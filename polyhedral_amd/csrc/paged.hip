@@ -2,11 +2,13 @@
 //
 // pa_page_tables: with first[r] = ceil(before[r] / ps) and need[r] = ceil((before[r] +
 // fresh[r]) / ps) - first[r], the exclusive sums of fresh give the rows of each request, those
-// of need its place in the run of free pages that is taken, and then every token's slot and
-// every new table entry follow from one binary search each.  One work-group takes the sums
-// (tables_scan_kernel); when the tokens are few it writes the rest too, from sums that it holds
-// in LDS, and the step is one launch.  Otherwise a second kernel writes it with a thread per
-// token and per new page.  What bounds it: latency.
+// of need its place in the run of free pages that is taken, and then every token's slot and every
+// new table entry follow from one binary search each.  A work-group takes all the sums and holds
+// them in LDS; where there are many tokens, many work-groups do, and each writes its part of the
+// tokens and pages (the sums of 96 requests again cost less than a second launch).  Where the state
+// advances in place, which the other work-groups may still read, or the sums pass the LDS, one
+// work-group writes sums and state, and a second kernel the tokens and pages.
+// What bounds it: latency (three trips to memory one after the other, and the launch).
 #include "common.hpp"
 #include "page_math.hpp"
 
@@ -85,7 +87,8 @@ __device__ __forceinline__ int64_t shfl_up64(int64_t x, int o) {
   return (int64_t)((uint64_t)(uint32_t)lo | ((uint64_t)(uint32_t)hi << 32));
 }
 
-// The sums; FUSED: the tokens and pages too (R <= kScanRequests).
+// The sums; FUSED: the tokens and pages too (R <= kScanRequests; one work-group alone where the state
+// advances in place).
 template <bool FUSED>
 __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(const TablesK a) {
   constexpr int NW = kScanThreads / 64;
@@ -94,6 +97,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(const TablesK
   __shared__ int32_t sums[FUSED ? 3 * kScanRequests + 2 : 1];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int one = (1 << a.page_lg) - 1;
+  const int32_t top = *a.free_count;  // (first, beside the other loads)
   const int64_t max_len = (int64_t)a.cols << a.page_lg;
   int32_t* row0 = FUSED ? sums : a.row0;
   int32_t* page0 = FUSED ? sums + a.R + 1 : a.page0;
@@ -150,7 +154,6 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(const TablesK
     }
     __syncthreads();
   }
-  const int32_t top = *a.free_count;
   if (t_sum > a.tokens) bad |= 4;
   if (top < 0 || top > a.n_pages || p_sum > top) bad |= 1;
   if (bad) atomicOr(&bad_s, bad);
@@ -158,20 +161,24 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(const TablesK
   bad = bad_s;
   if (bad) t_sum = p_sum = 0;
   if (tid == 0) {
-    *a.status = bad;
-    *a.free_left = top - (int32_t)p_sum;
     row0[a.R] = (int32_t)t_sum;
     page0[a.R] = (int32_t)p_sum;
-    a.q_start[a.R] = (int32_t)t_sum;
+    if (blockIdx.x == 0) {
+      *a.status = bad;
+      *a.free_left = top - (int32_t)p_sum;
+      a.q_start[a.R] = (int32_t)t_sum;
+    }
   }
-  for (int r = tid; r < a.R; r += kScanThreads) {
-    a.lengths[r] = bad ? a.before[r] : a.before[r] + a.fresh[r];
-    a.q_start[r] = bad ? 0 : row0[r];
-  }
+  if (blockIdx.x == 0)
+    for (int r = tid; r < a.R; r += kScanThreads) {
+      a.lengths[r] = bad ? a.before[r] : a.before[r] + a.fresh[r];
+      a.q_start[r] = bad ? 0 : row0[r];
+    }
   if constexpr (FUSED) {
     __syncthreads();  // the last entries
     const TablesView v{row0, page0, held};
-    for (int64_t i = tid; i < a.tokens + p_sum; i += kScanThreads) write_item(a, v, i, p_sum, top);
+    for (int64_t i = (int64_t)blockIdx.x * kScanThreads + tid; i < a.tokens + p_sum; i += (int64_t)gridDim.x * kScanThreads)
+      write_item(a, v, i, p_sum, top);
   }
 }
 
@@ -307,6 +314,9 @@ extern "C" int pa_page_tables(const pa_tables_args* x, void* stream) {
   PA_CHECK_ARG(x->R == 0 || x->cols == 0 || x->tables, "pa_page_tables: null tables");
   PA_CHECK_ARG(x->n_pages == 0 || x->free_list, "pa_page_tables: null free_list");
   PA_CHECK_ARG(x->tokens == 0 || x->slots, "pa_page_tables: null slots");
+  // (lengths are written beside reads of before)
+  PA_CHECK_ARG(x->lengths == x->before || x->lengths >= x->before + x->R || x->before >= x->lengths + x->R,
+               "pa_page_tables: lengths and before overlap in part");
   TablesK a;
   a.before = x->before;
   a.fresh = x->fresh;
@@ -329,15 +339,18 @@ extern "C" int pa_page_tables(const pa_tables_args* x, void* stream) {
   a.page0 = x->workspace + x->R + 1;
   a.held = x->workspace + 2 * (int64_t)x->R + 2;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (x->R <= kScanRequests && x->tokens <= 4 * kScanThreads) {
-    hipLaunchKernelGGL(tables_scan_kernel<true>, dim3(1), dim3(kScanThreads), 0, s, a);
+  // (new pages: at most one per page_size tokens and one per request)
+  const int64_t items = x->tokens + (x->tokens >> lg) + x->R;
+  const bool few = x->tokens <= 4 * kScanThreads;
+  if (x->R <= kScanRequests && (few || (x->lengths != x->before && x->free_left != x->free_count))) {
+    const int64_t groups = few ? 1 : (items + kScanThreads - 1) / kScanThreads;
+    hipLaunchKernelGGL(tables_scan_kernel<true>, dim3((unsigned)(groups < 512 ? groups : 512)), dim3(kScanThreads), 0, s, a);
     PA_LAUNCH_CHECK("tables_scan_kernel");
     return PA_OK;
   }
   hipLaunchKernelGGL(tables_scan_kernel<false>, dim3(1), dim3(kScanThreads), 0, s, a);
   PA_LAUNCH_CHECK("tables_scan_kernel");
-  // (new pages: at most one per page_size tokens and one per request)
-  const int64_t items = x->tokens + (x->tokens >> lg) + x->R, blocks = (items + 255) / 256;
+  const int64_t blocks = (items + 255) / 256;
   hipLaunchKernelGGL(tables_fill_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, a);
   PA_LAUNCH_CHECK("tables_fill_kernel");
   return PA_OK;

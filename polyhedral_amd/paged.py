@@ -300,7 +300,7 @@ class PagedKVCache:
     A step: ``step = cache.begin(fresh)``, then for each layer ``cache.append(k_new, v_new, step,
     layer)`` and ``cache.attend(q, mask, step, layer)``.  ``trim`` gives back what a window has
     left behind, ``finish`` all of some requests' pages (their rows then start anew).  All state
-    is on the device and advances there; only ``check`` waits for it."""
+    is on the device; only ``check`` waits for it."""
 
     def __init__(self, requests, max_length, pages, heads, D, dtype=torch.bfloat16, page_size=64, layers=1, device=None):
         _page_size(page_size)
@@ -336,13 +336,11 @@ class PagedKVCache:
         if tokens is None:
             raise ValueError("tokens (the rows of the packed step) is needed with counts on the device")
         _ints(fresh, "fresh", (self.requests,), self.device)
-        new = lambda n: torch.empty(n, dtype=torch.int32, device=self.device)  # noqa: E731
-        # (lengths and the free count advance in place: the step's lengths are its own copy)
-        step = build_tables(self.lengths, fresh, self.tables, self.free_list, self.free_count, self.page_size, tokens,
-                            TableStep(self.lengths, new(self.requests + 1), new(tokens), new(tokens), self.free_count, new(1)))
+        step = build_tables(self.lengths, fresh, self.tables, self.free_list, self.free_count, self.page_size, tokens)
         with torch.cuda.device(self.device):
             self.failed |= step.status
-        return step._replace(lengths=self.lengths.clone(), free_count=self.free_count.clone())
+        self.lengths, self.free_count = step.lengths, step.free_count
+        return step
 
     def append(self, k_new, v_new, step, layer=0):
         """k_new, v_new [tokens, heads, D] of a step into a layer's pages."""
@@ -354,8 +352,7 @@ class PagedKVCache:
                          out, lse)
 
     def _release(self, first, last):
-        status = release(first, last, self.tables, self.free_list, self.free_count,
-                         (self.free_count, torch.empty(1, dtype=torch.int32, device=self.device)))[1]
+        self.free_count, status = release(first, last, self.tables, self.free_list, self.free_count)
         with torch.cuda.device(self.device):
             self.failed |= status * LIST_FULL
 
@@ -368,7 +365,7 @@ class PagedKVCache:
         with torch.cuda.device(self.device):
             last = done.to(torch.int32) * self.tables.shape[1]
             self._release(torch.zeros_like(last), last)
-            self.lengths.masked_fill_(done, 0)
+            self.lengths = self.lengths.masked_fill(done, 0)   # (a step's own lengths stay)
 
     def trim(self, window, sinks=0):
         """Gives back the pages that neither the next token's window nor the first ``sinks`` tokens

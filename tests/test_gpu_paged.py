@@ -117,12 +117,12 @@ def test_pages_that_are_none_of_the_cache_give_no_slot(gpu):
 
 def test_tables_advance_in_place(gpu):
     """lengths = before and free_left = free_count: every run is a step; against numpy, both kernels."""
-    for R, tokens in ((7, 40), (2500, 3000)):
+    for R, tokens in ((7, 40), (2500, 3000), (9, 9000)):
         rng = np.random.default_rng(R)
         P, cols = 16, 12
         lengths, free = np.zeros(R, dtype=np.int64), np.arange(R * 4)
         tables, count = np.full((R, cols), -1, dtype=np.int64), R * 4
-        fresh = rng.integers(0, 2, R)
+        fresh = rng.integers(0, 2, R)   # (rows past the few tokens of a step are padding)
         t, ln, fl, fc = dev(tables, gpu), dev(lengths, gpu), dev(free, gpu), dev([count], gpu)
         new = lambda n: torch.empty(n, dtype=I32, device=gpu)  # noqa: E731
         out = paged.TableStep(ln, new(R + 1), new(tokens), new(tokens), fc, new(1))

@@ -185,6 +185,7 @@ def test_tables_refusals():
     _refused(call(cols=1 << 26, pitch=1 << 26), "columns")
     _refused(call(pitch=3), "pitch")
     _refused(call(tokens=-1), "tokens")
+    _refused(call(lengths=p + 4), "overlap")
     for f in ("before", "fresh", "free_list", "free_count", "tables", "lengths", "q_start", "slots", "free_left", "status",
               "workspace"):
         _refused(call(**{f: None}), "null")
