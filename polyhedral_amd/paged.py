@@ -42,19 +42,28 @@ nothing was taken then, and no row has a slot)."""
 
 class PagedLaunch:
     """A validated call of the library with the tensors its pointers refer to; __call__ launches
-    it on the current stream of its device and returns its result."""
+    it on the current stream of its device and returns its result.  Runs of one launch share its
+    outputs and its workspace: they must not overlap (runs in one stream do not)."""
 
-    def __init__(self, entry, call_args, keep, anchor, result):
+    def __init__(self, entry, call_args, keep, anchor, result, zero=None):
         self.entry, self.keep, self.anchor, self.result = entry, keep, anchor, result
         self._fn, self._args = getattr(_lib.lib(), entry), call_args
+        self._zero = zero   # memory that is zero before the first run, and left zero by each
 
     def __call__(self):
         t = self.anchor
         if t.device.index == torch.cuda.current_device():
-            _lib.check(self._fn(*self._args, _lib.stream_of(t)), self.entry)
-        else:
-            with torch.cuda.device(t.device):
-                _lib.check(self._fn(*self._args, _lib.stream_of(t)), self.entry)
+            return self._run(t)
+        with torch.cuda.device(t.device):
+            return self._run(t)
+
+    def _run(self, t):
+        if self._zero is not None:
+            # (in the stream of the first run; a run that is only captured has not cleared it)
+            self._zero.zero_()
+            if not torch.cuda.is_current_stream_capturing():
+                self._zero = None
+        _lib.check(self._fn(*self._args, _lib.stream_of(t)), self.entry)
         return self.result
 
 
@@ -282,10 +291,9 @@ def prepare_attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_f
     nbytes, zero = ctypes.c_int64(0), ctypes.c_int64(0)
     _lib.check(_lib.lib().pa_paged_workspace(ctypes.byref(a), ctypes.byref(nbytes), ctypes.byref(zero)), "pa_paged_workspace")
     ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        ws[:zero.value].zero_()   # (every run leaves it zero)
     a.workspace, a.workspace_bytes = ptr(ws), nbytes.value
-    return PagedLaunch("pa_paged_attn", (ctypes.byref(a),), [a, q, k, v, tables, lengths, q_start, dm, o, lse, ws], k, o)
+    return PagedLaunch("pa_paged_attn", (ctypes.byref(a),), [a, q, k, v, tables, lengths, q_start, dm, o, lse, ws], k, o,
+                       zero=ws[:zero.value])
 
 
 def attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_fresh=None, out=None, lse=None):
@@ -322,6 +330,7 @@ class PagedKVCache:
         self.free_list = torch.arange(pages - 1, -1, -1, **i32)   # page 0 is taken first
         self.free_count = torch.full((1,), pages, **i32)
         self.failed = torch.zeros(1, **i32)    # the status bits of all steps so far
+        self._last = (None, None)              # the newest step and its most new tokens of a request
 
     def begin(self, fresh, tokens=None):
         """Room for fresh[r] more tokens of every request (int32 [requests] on the device, or a list
@@ -329,8 +338,10 @@ class PagedKVCache:
         padding).  Returns the TableStep; lengths count the new tokens from here on.  A step that
         does not fit (pages, max_length, rows) takes nothing, gives no row a slot, and shows in
         step.status and ``check``."""
+        most = None
         if not isinstance(fresh, torch.Tensor):
             fresh = [int(f) for f in fresh]
+            most = max(fresh, default=0)
             tokens = sum(fresh) if tokens is None else tokens
             fresh = torch.tensor(fresh, dtype=torch.int32, device=self.device)
         if tokens is None:
@@ -340,6 +351,7 @@ class PagedKVCache:
         with torch.cuda.device(self.device):
             self.failed |= step.status
         self.lengths, self.free_count = step.lengths, step.free_count
+        self._last = (step, most)
         return step
 
     def append(self, k_new, v_new, step, layer=0):
@@ -347,7 +359,10 @@ class PagedKVCache:
         append(k_new, v_new, step.slots, self.k[layer], self.v[layer])
 
     def attend(self, q, mask, step, layer=0, scale=None, max_fresh=None, out=None, lse=None):
-        """o [tokens, Hq, D] of a step's tokens against a layer's pages (see prepare_attention)."""
+        """o [tokens, Hq, D] of a step's tokens against a layer's pages (see prepare_attention; of the
+        newest step max_fresh is known where its counts were a list)."""
+        if max_fresh is None and step is self._last[0]:
+            max_fresh = self._last[1]
         return attention(q, self.k[layer], self.v[layer], self.tables, step.lengths, step.q_start, mask, scale, max_fresh,
                          out, lse)
 

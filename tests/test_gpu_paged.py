@@ -497,6 +497,59 @@ def test_a_captured_step_replays_for_other_lengths(gpu):
     e.check()
 
 
+def test_a_launch_captured_before_its_first_run(gpu):
+    """The workspace is cleared by the first run that happens, whether a replay or an eager one; two
+    graphs with launches of their own run on two streams at once."""
+    b = Batch(gpu, torch.bfloat16, 128, 32, 8, 2, [(1, 6000), (70, 900), (1, 40)])
+    want, wl = b.run(pm.Causal())
+    outs, graphs, launches = [], [], []
+    for _ in range(2):
+        o, lse = torch.full_like(want, 7.0), torch.full_like(wl, 7.0)
+        junk = torch.full((1 << 26,), 0x5a, dtype=torch.uint8, device=gpu)   # memory that the workspace may get
+        del junk
+        launch = paged.prepare_attention(b.q, b.k, b.v, *b.dev(), pm.Causal(), out=o, lse=lse)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            launch()
+        outs.append((o, lse))
+        graphs.append(graph)
+        launches.append(launch)
+    launches[0]()                                  # eager before any replay
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for i in range(6):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, lse in outs:
+            assert torch.equal(o, want) and torch.equal(lse, wl), i
+            o.fill_(7.0)
+            lse.fill_(7.0)
+        torch.cuda.synchronize()
+
+
+def test_two_calls_at_once(gpu):
+    """Calls of different batches on two streams, each with its own workspace."""
+    a = Batch(gpu, torch.bfloat16, 128, 16, 8, 2, [(1, 9000), (1, 3000)], seed=1)
+    c = Batch(gpu, torch.float16, 64, 64, 4, 4, [(300, 2000), (2, 5000)], seed=2)
+    want = [x.run(pm.Causal()) for x in (a, c)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for s, x in zip(streams, (a, c)):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                o = torch.full((x.T, x.Hq, x.D), 7.0, dtype=x.dtype, device=gpu)
+                args = x.dev()
+                for _ in range(4):
+                    paged.attention(x.q, x.k, x.v, *args, pm.Causal(), out=o)
+                got.append(o)
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w[0]) for g, w in zip(got, want))
+
+
 # ---- all of it together ----------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,D,P,G", [(torch.bfloat16, 128, 16, 4), (torch.float32, 64, 32, 1), (torch.float16, 64, 64, 3)])
 @pytest.mark.parametrize("sinks", [False, True])
@@ -524,7 +577,7 @@ def test_serving_a_batch(gpu, dtype, D, P, G, sinks):
         for layer in range(layers):
             kn, vn, q = (torch.randn(T, n, D, generator=g).to(dtype).to(gpu) for n in (H, H, H * G))
             cache.append(kn, vn, step, layer)
-            o = cache.attend(q, mask, step, layer)
+            o = cache.attend(q, mask, step, layer, out=torch.zeros_like(q))
             f = lambda t: t.float().cpu().numpy().astype(np.float64)  # noqa: E731
             for r in range(R):
                 new = np.stack([f(kn), f(vn)])[:, starts[r]:starts[r + 1]]
