@@ -17,7 +17,11 @@
 // A dead key contributes nothing whatever it holds, but 0 times an infinity or NaN in its V row is
 // NaN.  That shows in the sums, so a work-group whose sums are not finite takes its list again, step
 // by step, and where a masked chunk of 16 keys has V rows that are not finite it takes the products
-// key by key, added only to the rows that the key is live for.
+// key by key, added only to the rows that the key is live for.  So does one with maxima past 2^24 in
+// log2 units: p = exp2(fma(x, c, -m)) has the rounding of m = max(x c) in its exponent, the same for
+// all keys of the row, so it falls out of the result while it is small (below 2^24 half a unit at
+// most) but empties or overflows the row where m is large; that row's second pass has m in units of
+// the scores and p = exp2((x - m) c).
 //
 // Scores, maxima, sums and O are float32; P is rounded to 16 bits as an MFMA operand only, its sum
 // taken before.
@@ -197,10 +201,12 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
     for (int e = 0; e < 16; e += 2) mx = nan_max(mx, nan_max(x[e], x[e + 1]));
     return mx;
   };
-  auto raise = [&](float mx) __attribute__((always_inline)) {
-    const float m_new = nan_max(m_run, row_nan_max(mx) * c_exp);
-    if (__ballot(m_new > m_run + kLazy) != 0ull) {
-      const float alpha = __builtin_amdgcn_exp2f(m_run - base_of(m_new));
+  // (huge: this row's m_run is in units of the scores)
+  auto raise = [&](float mx, bool huge) __attribute__((always_inline)) {
+    const float m_new = nan_max(m_run, huge ? row_nan_max(mx) : row_nan_max(mx) * c_exp);
+    if (__ballot(huge ? (m_new - m_run) * c_exp > kLazy : m_new > m_run + kLazy) != 0ull) {
+      const float up = m_run - base_of(m_new);
+      const float alpha = __builtin_amdgcn_exp2f(huge ? up * c_exp : up);
       m_run = m_new;
       l_part *= alpha;
 #pragma unroll
@@ -210,10 +216,11 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   // P of chunk c of a block, summed into l_part.  (The empty asm makes the products wait for the sum:
   // left to itself the scheduler sums at the step's end and holds 32 values until then, and the
   // fragments of Q go to scratch memory.)
-  auto exps = [&](const f32x16& x, int c, float neg_m) __attribute__((always_inline)) -> Frag {
+  auto exps = [&](const f32x16& x, int c, float neg_m, bool huge) __attribute__((always_inline)) -> Frag {
     f32x8 e8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) e8[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * c + e], c_exp, neg_m));
+    for (int e = 0; e < 8; ++e)
+      e8[e] = __builtin_amdgcn_exp2f(huge ? (x[8 * c + e] + neg_m) * c_exp : __builtin_fmaf(x[8 * c + e], c_exp, neg_m));
     l_part += ((e8[0] + e8[1]) + (e8[2] + e8[3])) + ((e8[4] + e8[5]) + (e8[6] + e8[7]));
     u32x4 pw = __builtin_bit_cast(u32x4, Mma<T>::cvt(e8));
     uint32_t p0 = pw[0];
@@ -230,7 +237,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   auto sums_step = [&](const f32x16& x0, const f32x16& x1) __attribute__((always_inline)) {
     const float neg_m = -base_of(m_run);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) pv(exps(x < 2 ? x0 : x1, x & 1, neg_m), x);
+    for (int x = 0; x < 4; ++x) pv(exps(x < 2 ? x0 : x1, x & 1, neg_m, false), x);
   };
 
   Step s_cur{}, s_next{}, s_after{};
@@ -253,7 +260,8 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
       // CU: sinks in chunks 279 -> 269 us, 16 prompts of 512 92 -> 84, nothing on long lists)
       __builtin_amdgcn_s_setprio(1);
       const float neg_m = -base_of(m_run);
-      const Frag p00 = exps(x0, 0, neg_m), p01 = exps(x0, 1, neg_m), p10 = exps(x1, 0, neg_m), p11 = exps(x1, 1, neg_m);
+      const Frag p00 = exps(x0, 0, neg_m, false), p01 = exps(x0, 1, neg_m, false), p10 = exps(x1, 0, neg_m, false),
+                 p11 = exps(x1, 1, neg_m, false);
       qk(y0, y1);
       pv(p00, 0);
       pv(p01, 1);
@@ -277,7 +285,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
       }
       __builtin_amdgcn_s_setprio(0);
       shape(s_next, j + 1, y0, y1);
-      raise(block_max(y1, block_max(y0, -INFINITY)));
+      raise(block_max(y1, block_max(y0, -INFINITY)), false);
     }
     s_cur = s_next;
     s_next = s_after;
@@ -297,7 +305,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
     if (n_steps > 1) dma(KRING + SLOT, kbase + s_next.off);
     qk(sa0, sa1);
     shape(s_cur, 0, sa0, sa1);
-    raise(block_max(sa1, block_max(sa0, -INFINITY)));
+    raise(block_max(sa1, block_max(sa0, -INFINITY)), false);
     rd.template turn_rows<SLOT>();
     int j = 0;
 #pragma unroll 1
@@ -315,13 +323,16 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
     if (s_cur.live != 0u) sums_step(sa0, sa1);
   }
 
-  // ---- sums that are not finite: the list again, step by step ------------------------------
+  // ---- sums that are not finite, scores that are huge: the list again, step by step --------
   float big = 0.f;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
     for (int e = 0; e < 16; e += 2) big = nan_max(big, nan_max(__builtin_fabsf(acc[db][e]), __builtin_fabsf(acc[db][e + 1])));
-  if (__syncthreads_or(!(big < INFINITY))) {
+  // (a row's maximum may have been huge before it had one near 0: its sum is not finite then; -inf: a
+  // row without a live key)
+  const bool huge = (__builtin_fabsf(m_run) > 0x1p24f && m_run != -INFINITY) || !(row_sum(l_part) < INFINITY);
+  if (__syncthreads_or(huge || !(big < INFINITY))) {
     rd = tile_reads<D>((lds_cptr)smem, lane);
 #pragma unroll
     for (int x = 0; x < NDB; ++x) acc[x] = f32x16{0};
@@ -342,11 +353,11 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
         mask_block(sa0, w0);
         mask_block(sa1, w1);
       }
-      raise(block_max(sa1, block_max(sa0, -INFINITY)));
+      raise(block_max(sa1, block_max(sa0, -INFINITY)), huge);
       const float neg_m = -base_of(m_run);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const Frag pf = exps(x < 2 ? sa0 : sa1, x & 1, neg_m);
+        const Frag pf = exps(x < 2 ? sa0 : sa1, x & 1, neg_m, huge);
         if (!((s.live >> x) & 1u)) continue;
         uint32_t lo = 0u, hi = 0u;
 #pragma unroll
@@ -384,6 +395,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
       }
       __syncthreads();  // every wave is past the slots
     }
+    if (huge) m_run *= c_exp;
   }
 
   // ---- the rows leave -------------------------------------------------------------------

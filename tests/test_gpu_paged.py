@@ -361,6 +361,36 @@ def test_scores_far_below_zero_still_sum_to_one(gpu):
             assert (got - want).abs().max() < 1e-5
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 64), (torch.float32, 128)])
+@pytest.mark.parametrize("n", [2, 150])
+def test_huge_scores(gpu, dtype, D, n):
+    """Scores at 1e9 (f16) or 1e31, of either sign, the same for all keys of a row, or far apart: equal
+    ones share the row (their mean, each term rounded to the type at most), and a lower one by an ulp
+    is nothing; rows that see such keys first and others later are as if they had not."""
+    big = (6e4, 1.6e4) if dtype == torch.float16 else (2.0 ** 60, 2.0 ** 44)
+    L, P = 700, 16
+    for sign, some in ((-1, False), (1, False), (1, True), (-1, True)):
+        b = Batch(gpu, dtype, D, P, 4, 2, [(n, L), (n, n)], poison=0.0)
+        b.q.zero_()
+        b.q[..., 0] = big[0]
+        t = np.arange(L)
+        page, off = (torch.as_tensor(x, device=gpu) for x in (b.tables[0, t // P], t % P))
+        b.k.zero_()
+        b.k[page[:333] if some else page, :, off[:333] if some else off, 0] = sign * big[1]
+        o, lse = b.run(pm.Causal())
+        assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+        v = b.v[page, :, off].double().repeat_interleave(2, dim=1)          # [L, Hq, D]
+        top = sign * big[0] * float(b.k.abs().max()) * D ** -0.5 if not some or sign > 0 else 0.0
+        for i in (0, n // 2, n - 1):
+            m = L - n + i + 1
+            keys = v[:m] if not some else (v[:333] if sign > 0 else v[333:m])
+            want, mass = keys.mean(0), keys.abs().mean(0)
+            u = po.HALF_STEP[dtype]
+            assert ((o[i].double() - want).abs() <= 1.01 * u * (want.abs() + mass) + 2.0 ** -18 * mass).all()
+            wl = top + np.log(len(keys))
+            assert (lse[i].double() - wl).abs().max() <= 2.0 ** -18 + 2.0 ** -22 * abs(wl)
+
+
 # ---- what is dead contributes nothing -----------------------------------------------------------
 @pytest.mark.parametrize("what", [NAN, INF, -INF])
 @pytest.mark.parametrize("dtype,D", TYPES)
