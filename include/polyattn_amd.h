@@ -495,13 +495,15 @@ int pa_attn_bwd(const pa_attn_bwd_args* args, void* stream);
  *   4  more new tokens than rows (`tokens`)
  * and then nothing is taken: tables stay, lengths = before, q_start is all 0, the slots and
  * positions -1, *free_left = free_count.  lengths may be `before` and free_left may be
- * free_count; no other output overlaps an input.  A token whose page is none of the cache gets slot -1.  workspace: int32 [3 R +
- * 2].
+ * free_count; no other output overlaps an input.  A token whose page is none of the cache gets
+ * slot -1.  Pages are not shared: a page is in one request's table or in the free list.
+ * workspace: int32 [3 R + 2], not shared by calls that overlap.
  *
  * pa_page_release: pages first[r] .. last[r] - 1 of request r's table (clamped to the table;
  * entries that are none of the cache are skipped) go back to the end of the free list in order
  * of (request, page), and their entries become -1.  *status 0, or 1 when the list would pass
- * n_pages (nothing is done then).  free_left may be free_count.  workspace: int32 [R].
+ * n_pages (nothing is done then).  free_left may be free_count.  workspace: int32 [R], not
+ * shared by calls that overlap.
  *
  * pa_paged_append: row i of k_new / v_new [T, Hkv, D] (n_st, n_sh: token and head strides in
  * elements) is written to slot slots[i]; a slot outside the cache (-1) is skipped.  Slots are
@@ -516,9 +518,9 @@ int pa_attn_bwd(const pa_attn_bwd_args* args, void* stream);
  * counts as dead.  Rows of no request are left as they are.  lse may be NULL (natural log,
  * [T, Hq] at lse_st, lse_sh).  max_fresh: the most new tokens of a request (a hint: it selects
  * kernels and moves no result beyond rounding).  D = 64 or 128, f32 / f16 / bf16, scale > 0.
- * workspace: the bytes pa_paged_workspace gives for the same sizes, 256-byte aligned, the first
- * zero_bytes of them zero before the first call with it and left zero by every call (of the same
- * sizes); not shared by calls that overlap. */
+ * o overlaps no input.  workspace: the bytes pa_paged_workspace gives for the same sizes, hint,
+ * type and mask (no pointer is read), 256-byte aligned, the first zero_bytes of them zero before
+ * the first call with it and left zero by every call of these; not shared by calls that overlap. */
 typedef struct pa_tables_args {
   const int32_t* before;
   const int32_t* fresh;

@@ -314,9 +314,25 @@ extern "C" int pa_page_tables(const pa_tables_args* x, void* stream) {
   PA_CHECK_ARG(x->R == 0 || x->cols == 0 || x->tables, "pa_page_tables: null tables");
   PA_CHECK_ARG(x->n_pages == 0 || x->free_list, "pa_page_tables: null free_list");
   PA_CHECK_ARG(x->tokens == 0 || x->slots, "pa_page_tables: null slots");
-  // (lengths are written beside reads of before)
-  PA_CHECK_ARG(x->lengths == x->before || x->lengths >= x->before + x->R || x->before >= x->lengths + x->R,
-               "pa_page_tables: lengths and before overlap in part");
+  // (outputs are written beside reads of the inputs, by other work-groups too)
+  struct Span {
+    const char* name;
+    const int32_t* p;
+    int64_t n;
+  };
+  const int64_t R = x->R;
+  const Span in[] = {{"before", x->before, R}, {"fresh", x->fresh, R}, {"free_list", x->free_list, x->n_pages},
+                     {"free_count", x->free_count, 1}, {"tables", x->tables, R ? (int64_t)((uint64_t)(R - 1) * (uint64_t)x->pitch) + x->cols : 0}};
+  const Span out[] = {{"lengths", x->lengths, R}, {"q_start", x->q_start, R + 1}, {"slots", x->slots, x->tokens},
+                      {"positions", x->positions, x->positions ? x->tokens : 0}, {"free_left", x->free_left, 1},
+                      {"status", x->status, 1}, {"workspace", x->workspace, 3 * R + 2}};
+  for (const Span& o : out)
+    for (const Span& i : in) {
+      if (o.p == i.p && ((o.p == x->lengths && i.p == x->before) || (o.p == x->free_left && i.p == x->free_count)) && o.n == i.n)
+        continue;
+      const uintptr_t a = reinterpret_cast<uintptr_t>(o.p), b = reinterpret_cast<uintptr_t>(i.p);
+      PA_CHECK_ARG(o.n == 0 || i.n == 0 || a + 4 * o.n <= b || b + 4 * i.n <= a, "pa_page_tables: %s and %s overlap", o.name, i.name);
+    }
   TablesK a;
   a.before = x->before;
   a.fresh = x->fresh;
@@ -391,6 +407,7 @@ extern "C" int pa_paged_append(const void* k_new, const void* v_new, int64_t n_s
   PA_CHECK_ARG(al(k_new, n_st, n_sh, 0) && al(v_new, n_st, n_sh, 0) && al(k, c_sp, c_sh, c_sn) && al(v, c_sp, c_sh, c_sn),
                "pa_paged_append: rows must be 16-byte aligned");
   PA_CHECK_ARG(n_st >= 0 && n_sh >= 0 && c_sp >= 0 && c_sh >= 0 && c_sn >= D, "pa_paged_append: negative strides, or rows closer than D");
+  PA_CHECK_ARG((n_pages == 1 || c_sp >= D) && (Hkv == 1 || c_sh >= D), "pa_paged_append: pages or heads closer than D");
   const int upr_lg = (D * esz == 128) ? 3 : (D * esz == 256) ? 4 : 5;
   const int64_t units = (T * Hkv) << upr_lg, blocks = (units + 255) / 256;
   const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384), 2);

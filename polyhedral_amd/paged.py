@@ -43,7 +43,9 @@ nothing was taken then, and no row has a slot)."""
 class PagedLaunch:
     """A validated call of the library with the tensors its pointers refer to; __call__ launches
     it on the current stream of its device and returns its result.  Runs of one launch share its
-    outputs and its workspace: they must not overlap (runs in one stream do not)."""
+    outputs and its workspace: they must not overlap (runs in one stream do not), and a run on another
+    stream than the one the launch was prepared on comes after that one's earlier work.  Keep it until
+    its runs, or the graphs that hold them, are done."""
 
     def __init__(self, entry, call_args, keep, anchor, result, zero=None):
         self.entry, self.keep, self.anchor, self.result = entry, keep, anchor, result

@@ -191,6 +191,50 @@ def test_tables_refusals():
         _refused(call(**{f: None}), "null")
 
 
+def test_tables_outputs_may_not_overlap_inputs():
+    keep, p = _buf()
+    inputs = {"before": 2, "fresh": 2, "free_list": 8, "free_count": 1, "tables": 8}
+    outputs = {"lengths": 2, "q_start": 3, "slots": 10, "positions": 10, "free_left": 1, "status": 1, "workspace": 8}
+    for o, n in outputs.items():
+        for i, m in inputs.items():
+            for shift in (0, 4 * (m - 1), -4 * (n - 1)):
+                if shift == 0 and (o, i) in (("lengths", "before"), ("free_left", "free_count")):
+                    continue   # (the state that advances in place)
+                a = _lib.PaTablesArgs()
+                for x, f in enumerate(list(inputs) + list(outputs)):
+                    setattr(a, f, p + 256 * (x + 1))
+                a.R, a.n_pages, a.page_size, a.pitch, a.cols, a.tokens = 2, 8, 16, 4, 4, 10
+                setattr(a, o, getattr(a, i) + shift)
+                _refused(_lib.lib().pa_page_tables(ctypes.byref(a), None), f"{o} and {i} overlap")
+
+
+def test_append_refuses_pages_that_overlap():
+    keep, p = _buf()
+    for sp, sh, pages, H in ((0, 2048, 4, 2), (4096, 0, 4, 2), (120, 2048, 2, 1), (4096, 64, 1, 2)):
+        _refused(_lib.lib().pa_paged_append(p, p, 256, 128, p, 3, p, p, sp, sh, 128, pages, 16, H, 128, _lib.PA_BF16, None),
+                 "pages or heads closer than D")
+
+
+def test_struct_layouts(tmp_path):
+    """gcc's offsets of every field against the ctypes structures."""
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    lines, want = [], []
+    for cname, cls in (("pa_tables_args", _lib.PaTablesArgs), ("pa_paged_args", _lib.PaPagedArgs)):
+        for fname, _ in cls._fields_:
+            lines.append(f'  printf("%zu %zu\\n", offsetof({cname}, {fname}), sizeof((({cname}*)0)->{fname}));')
+            want.append((getattr(cls, fname).offset, getattr(cls, fname).size))
+        lines.append(f'  printf("%zu 0\\n", sizeof({cname}));')
+        want.append((ctypes.sizeof(cls), 0))
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "polyattn_amd.h"\nint main(void) {\n' + "\n".join(lines) +
+                   "\n  return 0;\n}\n")
+    subprocess.run([cc, "-I", str(ROOT / "include"), str(src), "-o", str(tmp_path / "layout")], check=True)
+    out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout
+    assert [tuple(map(int, line.split())) for line in out.splitlines()] == want
+
+
 def test_release_and_append_refusals():
     keep, p = _buf()
     lib = _lib.lib()
