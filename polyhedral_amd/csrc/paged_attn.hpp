@@ -73,6 +73,11 @@ __device__ __forceinline__ KernelMask kernel_mask(const PagedK& a) {
   return {a.n_include, a.n_exclude, a.terms[0], (cterm*)(args + offsetof(PagedK, terms))};
 }
 
+// Whether a tile of few rows with that many tokens is taken by lists of live keys (paged_rows.hpp; one
+// in `stride` keys of a lattice is live for each: beyond, most of a block is listed.  16 requests of
+// 4000, stride 16, 8 heads: 8 tokens 48 us block by block, 37 by lists; 10 50 and 43; 14 51 and 55).
+__device__ __forceinline__ bool by_lists(int32_t tokens, int32_t stride) { return tokens <= stride - stride / 4; }
+
 struct Work {
   int32_t tiles, blocks, least;  // least: blocks of a share
 };
@@ -91,7 +96,7 @@ __device__ __forceinline__ Work work_of(const PagedK& a, const PagedPart& p, con
   if (rows <= p.row_min || rows > p.row_max) return {0, 0, 1};
   const int32_t span = imin(q.n, p.span);
   // (a share that is taken by lists: for one token a list of 512 keys for each wave, for more fewer)
-  const int32_t least = BM == kRows && 2 * span <= a.stride ? imax((2048 >> LG) >> (31 - __builtin_clz((uint32_t)imax(span, 1))), p.least) : p.least;
+  const int32_t least = BM == kRows && by_lists(span, a.stride) ? imax((2048 >> LG) >> (31 - __builtin_clz((uint32_t)imax(span, 1))), p.least) : p.least;
   return {(rows + BM - 1) / BM, key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG).count(), least};
 }
 
@@ -166,12 +171,14 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, c
     w = work_of<BM, LG>(a, p, q);
     total += wave_total((float)w.tiles * (float)w.blocks);
   }
-  // Blocks of a share: all of the part's work over `shares`; few rows: that over half as many where it
-  // is less than 32 blocks (two work-groups run per CU, so 1024 shares are two rounds: 64 requests of
-  // 300 to 8000 tokens 157 -> 147 us against one round, 8 of 4000, whose shares are short, 27 -> 34).
-  // (Rounded up, so the units stay within shares + tiles Hkv, which the grid is sized for.)
+  // Blocks of a share: all of the part's work over `shares` (rounded up, so the units stay within shares
+  // + tiles Hkv, which the grid is sized for).  Two work-groups run per CU, so 1024 shares of few rows are
+  // two rounds, which suits long lists of uneven lengths (64 requests of 300 to 8192 in one round of
+  // 512: 160 us, in two 148); short ones are cut for one round.  A little fewer than the round holds, as
+  // shares are rounded to whole blocks and tiles, and a few units more cost a round of their own: 8
+  // requests of 300 to 8192 30 -> 24 us, 16 49 -> 44, 5 of 6000 32 -> 27, the 64 148 -> 144.
   float share = total * (float)a.Hkv * p.by_shares;
-  if (BM == kRows) share = fmaxf(share, fminf(2.f * share, 32.f));
+  if (BM == kRows) share *= share < 24.f ? 2.4f : 1.08f;
 
   int32_t before = 0, slot = 0;  // units and slots of earlier requests
   end = 0;
