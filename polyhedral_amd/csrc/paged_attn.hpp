@@ -234,14 +234,19 @@ __device__ __forceinline__ void share_of(int32_t n, int32_t split, int32_t split
 __device__ __forceinline__ void share_store(float* p, float x) {
   __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float share_load(const float* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// The states of a tile's shares as a buffer: loads of 16 bytes at agent scope, which no atomic load has.
+// (As pairs of 8-byte ones every line is asked for twice.)
+typedef __amdgpu_buffer_rsrc_t Shares;
+__device__ __forceinline__ Shares shares_at(char* first, int32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(first, 0, bytes, 0x00027000);  // (raw 32-bit data)
 }
-__device__ __forceinline__ f32x4 share_load4(const char* p) {
-  const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  const uint64_t y = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p) + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return f32x4{__builtin_bit_cast(float, (uint32_t)x), __builtin_bit_cast(float, (uint32_t)(x >> 32)),
-               __builtin_bit_cast(float, (uint32_t)y), __builtin_bit_cast(float, (uint32_t)(y >> 32))};
+constexpr int kSc1 = 16;  // agent scope
+__device__ __forceinline__ f32x4 share_load4(Shares s, int32_t lane_off, int32_t off) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(s, lane_off, off, kSc1));
+}
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ f32x2 share_load2(Shares s, int32_t lane_off, int32_t off) {
+  return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(s, lane_off, off, kSc1));
 }
 __device__ __forceinline__ void share_store4(char* p, f32x4 x) {
   const u32x4 y = __builtin_bit_cast(u32x4, x);

@@ -571,6 +571,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
     // for all i, every load of a pair on its way before the first is used; then as the waves' states
     // above
     const int r0 = lane >> 4, col = (lane & 15) * CPT;
+    const Shares all = shares_at(first, u.splits * SLOT_B);
     float m[4], l[4];
     f32x4 x[4][CPT / 4];
 #pragma unroll
@@ -586,15 +587,15 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
       f32x4 os[2][4][CPT / 4];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const char* at = first + (int64_t)imin(s + y * kWaves, u.splits - 1) * SLOT_B;
+        const int32_t at = imin(s + y * kWaves, u.splits - 1) * SLOT_B;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (4 * i >= n_rows) break;
-          const float* ml = reinterpret_cast<const float*>(at + ML + 8 * (4 * i + r0));
-          ms[y][i] = share_load(ml);
-          ls[y][i] = share_load(ml + 1);
+          const f32x2 ml = share_load2(all, 8 * (4 * i + r0), at + ML);
+          ms[y][i] = ml[0];
+          ls[y][i] = ml[1];
 #pragma unroll
-          for (int e = 0; e < CPT / 4; ++e) os[y][i][e] = share_load4(at + ((4 * i + r0) * D + col + 4 * e) * 4);
+          for (int e = 0; e < CPT / 4; ++e) os[y][i][e] = share_load4(all, ((4 * i + r0) * D + col + 4 * e) * 4, at);
         }
       }
 #pragma unroll

@@ -414,10 +414,10 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   if (u.splits > 1) {
     // a slot is the waves' registers as they are: 16 bytes of O per lane, then maximum and sum
     constexpr int SLOT_B = slot_floats(kTileRows, D) * 4, WB = SLOT_B / 4;
-    const char* first = part.part + (int64_t)u.slot * SLOT_B + w * WB + 16 * lane_e;
+    char* first = part.part + (int64_t)u.slot * SLOT_B;
     const bool has = 32 * w < n_rows;  // (a wave without rows stores and merges nothing)
     if (has) {
-      char* own = const_cast<char*>(first) + (int64_t)u.split * SLOT_B;
+      char* own = first + (int64_t)u.split * SLOT_B + w * WB + 16 * lane_e;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -430,24 +430,24 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
       }
     }
     if (!last_share(part, u, tid, flag) || !has) return;
-    const char* ml0 = first + NDB * 4096 - 16 * lane_e + 8 * m_e;
+    const Shares all = shares_at(first, u.splits * SLOT_B);
     m_run = -INFINITY;
 #pragma unroll 8
-    for (int s = 0; s < u.splits; ++s) m_run = nan_max(m_run, share_load(reinterpret_cast<const float*>(ml0 + (int64_t)s * SLOT_B)));
+    for (int s = 0; s < u.splits; ++s) m_run = nan_max(m_run, share_load2(all, 8 * m_e, s * SLOT_B + w * WB + NDB * 4096)[0]);
     l_tot = 0.f;
 #pragma unroll
     for (int x = 0; x < NDB; ++x) acc[x] = f32x16{0};
 #pragma unroll 2
     for (int s = 0; s < u.splits; ++s) {
-      const char* at = first + (int64_t)s * SLOT_B;
+      const int32_t at = s * SLOT_B + w * WB;
       f32x4 x[NDB][4];
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[db][e] = share_load4(at + (4 * db + e) * 1024);
-      const float* ml = reinterpret_cast<const float*>(ml0 + (int64_t)s * SLOT_B);
-      const float f = __builtin_amdgcn_exp2f(share_load(ml) - base_of(m_run));
-      l_tot += f * share_load(ml + 1);
+        for (int e = 0; e < 4; ++e) x[db][e] = share_load4(all, 16 * lane_e, at + (4 * db + e) * 1024);
+      const f32x2 ml = share_load2(all, 8 * m_e, at + NDB * 4096);
+      const float f = __builtin_amdgcn_exp2f(ml[0] - base_of(m_run));
+      l_tot += f * ml[1];
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
