@@ -10,5 +10,6 @@ Subpackages and modules:
   polyhedral_amd.perm       GPU class-A permutation
   polyhedral_amd.attention  GPU attention forward
   polyhedral_amd.split      disjoint split + log-sum-exp merge
+  polyhedral_amd.paged      serving a batch of requests from a paged key / value cache
 """
-__all__ = ["attention", "index", "perm", "spec", "split"]
+__all__ = ["attention", "index", "paged", "perm", "spec", "split"]

@@ -8,8 +8,8 @@ namespace pa {
 namespace {
 
 // Rows of a request (new tokens times heads of a group) up to which it is a tile of few rows.  Over
-// 4000 keys of 8 heads of 128, 48 rows as one tile of 128 rather than three of 16: 4 requests 68 -> 35
-// us, 64 requests 203 -> 273; 24 rows: rows are as fast or faster for both.
+// 4000 keys of 8 heads of 128, as tiles of 16 and as one of 128: 24 rows 23 and 28 us of 4 requests (204
+// and 200 of 64), 48 rows 28 and 31 (273 and 203), 64 rows 32 and 31 (330 and 210).
 constexpr int kFewRows = 32;
 
 // One in how many keys a mask leaves live for a token far from it: the stride of a mask's one lattice
@@ -69,12 +69,15 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   PA_CHECK_ARG(x->scale > 0.f && x->scale < INFINITY, "pa_paged_attn: scale=%g must be positive", (double)x->scale);
   p->stride = stride_of(x->mask);
   const int64_t G = x->Hq / x->Hkv, some = x->T < x->R ? x->T : x->R;  // some: requests with rows, at most
-  // (tiles of few rows that take lists read 1 / stride of the keys for each token, a chunk's tile all)
+  // (Tiles of few rows that take lists read 1 / stride of the keys for each token, a chunk's tile all: 64
+  // rows of 16 requests, stride 16, over 8000 keys 74 us and 141, 96 rows 146 both.)
   const int span = (int)((kRows + G - 1) / G) + 1;
   const int64_t few_rows = 2 * span <= p->stride && G * p->stride / 2 > kFewRows ? (G * p->stride / 2 < kTileRows ? G * p->stride / 2 : kTileRows) : kFewRows;
   p->tile = x->dtype != PA_F32 && x->n_pages > 0 && x->max_fresh * G > few_rows;
   int64_t few = x->T * G / kRows + some;
   if (p->tile && few > some * ((few_rows + kRows - 1) / kRows)) few = some * ((few_rows + kRows - 1) / kRows);
+  // (256 beside chunks, whose units are most of the grid: 36 requests of 1 or 20 to 1000 new tokens 54
+  // -> 52 us)
   if (int rc = part_of(x, kRows, p->tile ? 256 : 1024, few, &p->rows)) return rc;
   p->rows.least = 4;
   p->rows.root_over = 0.7f;

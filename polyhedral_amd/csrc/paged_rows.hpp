@@ -21,9 +21,9 @@
 // quarters of its stride, a wave lists the live keys of 512 at a time and reads their rows alone.
 //
 // What bounds it: HBM for long lists (64 requests of 300 to 8192 tokens, 32 heads on 8 of 128, bf16:
-// 739 MB in 147 us, 5.0 TB/s, the rate of a copy; two waves a SIMD at 250 registers hold 128 KB a CU
-// in flight), and for short ones the chain of trips to memory: requests, pages, rows, states, merge
-// (one token over 1001 keys of 4 heads, f32, 9.0 us; drafts under a lattice of 16, 17 MB, 18 us).
+// 739 MB in 143 us, 5.2 TB/s, where a copy reaches 5.0; two waves a SIMD at 245 registers hold 128 KB a
+// CU in flight), and for short ones the chain of trips to memory: requests, pages, rows, states, merge
+// (one token over 1001 keys of 4 heads, f32, 8.9 us; drafts under a lattice of 16, 17 MB, 17 us).
 //
 // A dead key contributes nothing whatever its K and V hold: its score is replaced by -inf, and
 // where a step is masked for some row and its V rows hold an infinity or NaN, the products are

@@ -26,11 +26,11 @@
 // Scores, maxima, sums and O are float32; P is rounded to 16 bits as an MFMA operand only, its sum
 // taken before.
 //
-// What bounds it: for long lists at D = 128 power (2000 new tokens of 30001, 32 heads on 8, bf16: 877
-// to 943 us, 1.01 to 1.08 PFLOP/s of the 1.12 of a large library product; the clock falls to 1.6 to 1.8
+// What bounds it: for long lists at D = 128 power (2000 new tokens of 30001, 32 heads on 8, bf16: 873
+// to 943 us, 1.01 to 1.09 PFLOP/s of the 1.12 of a large library product; the clock falls to 1.6 to 1.8
 // GHz with the matrix cores busy 54% of it), at D = 64 the exponentials' issue (4096 of 4096, 32 heads:
 // 104 us, 660 TFLOP/s), and for lists of a few steps what is outside them: 5 to 9 us a unit, two units
-// a CU (chunks of 1000 to 4096 under a window of 1024 and 64 sinks, 18 steps a unit: 270 us, 785
+// a CU (chunks of 1000 to 4096 under a window of 1024 and 64 sinks, 18 steps a unit: 267 us, 795
 // TFLOP/s).
 #pragma once
 
