@@ -308,9 +308,11 @@ class PagedKVCache:
     their tables: k, v [layers, pages, heads, page_size, D].
 
     A step: ``step = cache.begin(fresh)``, then for each layer ``cache.append(k_new, v_new, step,
-    layer)`` and ``cache.attend(q, mask, step, layer)``.  ``trim`` gives back what a window has
-    left behind, ``finish`` all of some requests' pages (their rows then start anew).  All state
-    is on the device; only ``check`` waits for it."""
+    layer)`` and ``cache.attend(q, mask, step, layer)``, before the next begin, trim or finish.
+    ``trim`` gives back what a window has left behind, ``finish`` all of some requests' pages (their
+    rows then start anew).  All state is in tensors on the device that stay where they are, so a
+    whole step with counts on the device can be captured in a graph, and every replay is a step;
+    only ``check`` waits for the device."""
 
     def __init__(self, requests, max_length, pages, heads, D, dtype=torch.bfloat16, page_size=64, layers=1, device=None):
         _page_size(page_size)
@@ -349,10 +351,11 @@ class PagedKVCache:
         if tokens is None:
             raise ValueError("tokens (the rows of the packed step) is needed with counts on the device")
         _ints(fresh, "fresh", (self.requests,), self.device)
-        step = build_tables(self.lengths, fresh, self.tables, self.free_list, self.free_count, self.page_size, tokens)
+        new = lambda n: torch.empty(n, dtype=torch.int32, device=self.device)  # noqa: E731
+        out = TableStep(self.lengths, new(self.requests + 1), new(tokens), new(tokens), self.free_count, new(1))
+        step = build_tables(self.lengths, fresh, self.tables, self.free_list, self.free_count, self.page_size, tokens, out)
         with torch.cuda.device(self.device):
             self.failed |= step.status
-        self.lengths, self.free_count = step.lengths, step.free_count
         self._last = (step, most)
         return step
 
@@ -369,7 +372,8 @@ class PagedKVCache:
                          out, lse)
 
     def _release(self, first, last):
-        self.free_count, status = release(first, last, self.tables, self.free_list, self.free_count)
+        status = torch.empty(1, dtype=torch.int32, device=self.device)
+        release(first, last, self.tables, self.free_list, self.free_count, (self.free_count, status))
         with torch.cuda.device(self.device):
             self.failed |= status * LIST_FULL
 
@@ -382,7 +386,7 @@ class PagedKVCache:
         with torch.cuda.device(self.device):
             last = done.to(torch.int32) * self.tables.shape[1]
             self._release(torch.zeros_like(last), last)
-            self.lengths = self.lengths.masked_fill(done, 0)   # (a step's own lengths stay)
+            self.lengths.masked_fill_(done, 0)
 
     def trim(self, window, sinks=0):
         """Gives back the pages that neither the next token's window nor the first ``sinks`` tokens

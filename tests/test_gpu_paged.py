@@ -634,6 +634,50 @@ def test_serving_a_batch(gpu, dtype, D, P, G, sinks):
     cache.check()
 
 
+@pytest.mark.parametrize("T", [40, 5000])
+def test_a_captured_step_of_a_cache(gpu, T):
+    """begin, append and attend of a cache in a graph, replayed for other counts, with requests that
+    finish and a window's pages given back eagerly in between: as a second cache without a graph."""
+    R, H, G, D, P, layers = 6, 2, 2, 64, 16, 2
+    mask = pm.SinksWindow(5, 60)
+    a, e = (paged.PagedKVCache(R, 600, 200, H, D, torch.float16, P, layers, gpu) for _ in range(2))
+    gen = torch.Generator().manual_seed(T)
+    rng = np.random.default_rng(T)
+    fresh = torch.zeros(R, dtype=I32, device=gpu)
+    kn, vn, q = (torch.zeros(T, n, D, dtype=torch.float16, device=gpu) for n in (H, H, H * G))
+
+    def a_step(cache, out):
+        step = cache.begin(fresh, T)
+        for layer in range(layers):
+            cache.append(kn, vn, step, layer)
+            cache.attend(q, mask, step, layer, out=out[layer])
+    oa, oe = (torch.zeros(layers, T, H * G, D, dtype=torch.float16, device=gpu) for _ in range(2))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a_step(a, oa)
+    for i in range(12):
+        n = rng.integers(0, 6, R)
+        if i % 4 == 0:
+            n[int(rng.integers(R))] = 12
+        fresh.copy_(torch.as_tensor(n, dtype=I32))
+        for x in (kn, vn, q):
+            x.copy_(torch.randn(x.shape, generator=gen))
+        graph.replay()
+        a_step(e, oe)
+        for x, y in ((a.tables, e.tables), (a.lengths, e.lengths), (a.free_count, e.free_count), (oa, oe)):
+            assert torch.equal(x, y), i
+        done = rng.random(R) < 0.1
+        for c in (a, e):
+            c.finish(done.tolist())
+            if i % 3 == 2:
+                c.trim(60, 5)
+    a.check()
+    fresh.fill_(T)   # (does not fit)
+    graph.replay()
+    with pytest.raises(RuntimeError, match="did not fit"):
+        a.check()
+
+
 def test_a_cache_that_is_full_says_so(gpu):
     cache = paged.PagedKVCache(2, 100, 3, 1, 64, torch.float16, 16, device=gpu)
     cache.begin([20, 10])
