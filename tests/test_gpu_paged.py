@@ -430,6 +430,47 @@ def test_masked_places_may_hold_anything(gpu, dtype, D, n, what):
                     assert (hit[..., keep] - clean[~d][..., keep].float()).abs().max() <= 0.05 if hit.numel() else True
 
 
+@pytest.mark.parametrize("dtype,D,Hq,Hkv,sizes", [
+    (torch.bfloat16, 128, 128, 1, [(1, 300), (3, 77), (0, 5)]), (torch.float32, 64, 96, 1, [(1, 200), (2, 40)]),
+    (torch.float16, 64, 40, 40, [(1, 60), (9, 130)]), (torch.bfloat16, 64, 37 * 3, 37, [(2, 50), (50, 90)]),
+    (torch.bfloat16, 128, 48, 2, [(1, 3000), (40, 41)])])
+def test_many_heads(gpu, dtype, D, Hq, Hkv, sizes):
+    b = Batch(gpu, dtype, D, 16, Hq, Hkv, sizes, seed=Hq)
+    b.check(pm.Causal())
+    b.check(pm.Dilated(16))
+
+
+def test_nothing_to_attend_to(gpu):
+    """No pages, no columns, no requests, no rows."""
+    q = torch.ones(3, 4, 64, dtype=torch.float16, device=gpu)
+    k = torch.zeros(0, 2, 16, 64, dtype=torch.float16, device=gpu)
+    i32 = lambda *x: torch.tensor(x, dtype=I32, device=gpu)  # noqa: E731
+    one = torch.zeros(5, 2, 16, 64, dtype=torch.float16, device=gpu)
+    for kv, tables in ((k, torch.zeros(1, 4, dtype=I32, device=gpu)), (one, torch.zeros(1, 0, dtype=I32, device=gpu)),
+                       (one, torch.full((1, 4), -1, dtype=I32, device=gpu))):
+        for most in (0, 100):
+            o, lse = torch.full_like(q, 7.0), torch.full((3, 4), 7.0, device=gpu)
+            paged.attention(q, kv, kv, tables, i32(50), i32(0, 2), pm.Causal(), max_fresh=most, out=o, lse=lse)
+            assert (o[:2] == 0).all() and (lse[:2] == -INF).all() and (o[2] == 7).all() and (lse[2] == 7).all()
+    o = torch.full_like(q, 7.0)
+    paged.attention(q, one, one, torch.zeros(0, 4, dtype=I32, device=gpu), i32(), i32(0), pm.Causal(), out=o)
+    assert (o == 7).all()
+    assert paged.attention(q[:0], one, one, torch.zeros(1, 4, dtype=I32, device=gpu), i32(50), i32(0, 0), pm.Causal()).shape == (0, 4, 64)
+    paged.append(one[:0, :, 0], one[:0, :, 0], i32(), one, one)
+    paged.append(one[:2, :, 0], one[:2, :, 0], i32(0, 5), k, k)
+
+
+def test_thousands_of_requests_and_pages_in_two_tables(gpu):
+    """More requests than a work-group has lanes many times over, some of which read the same pages (a
+    prompt that they share)."""
+    rng = np.random.default_rng(3)
+    sizes = [(int(rng.integers(0, 2)), int(rng.integers(1, 40))) for _ in range(3000)]
+    b = Batch(gpu, torch.float16, 64, 16, 2, 1, sizes, seed=3)
+    shared = np.flatnonzero(b.lengths > 16)
+    b.tables[shared[1:], 0] = b.tables[shared[0], 0]
+    b.check(pm.Causal())
+
+
 def test_entries_that_name_no_page_are_dead(gpu):
     """Table entries out of the cache's range hide their keys, wherever they are; so does a table
     that ends before the length."""
