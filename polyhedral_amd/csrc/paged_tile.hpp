@@ -186,22 +186,17 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
       x[e] = __builtin_bit_cast(float, (__builtin_bit_cast(int32_t, xv) & keep) | (int32_t)(0xff800000u & ~(uint32_t)keep));
     }
   };
-  // The words of this lane's row for both blocks of step j.
-  auto words = [&](const Step& s, int j, uint32_t& w0, uint32_t& w1) __attribute__((always_inline)) {
-    const int key = kl.block(j0 + j) << kTileLg;
-    w0 = s.live & 3u ? mask_word(mask, q_pos, key, len) : 0u;
-    w1 = s.live & 12u ? mask_word(mask, q_pos, key + 32, len) : 0u;
-    if (!(s.live & 1u)) w0 &= 0xffff0000u;
-    if (!(s.live & 2u)) w0 &= 0x0000ffffu;
-    if (!(s.live & 4u)) w1 &= 0xffff0000u;
-    if (!(s.live & 8u)) w1 &= 0x0000ffffu;
+  // The word of this lane's row for block b of step j.
+  auto word = [&](const Step& s, int j, int b) __attribute__((always_inline)) -> uint32_t {
+    const uint32_t live = (s.live >> (2 * b)) & 3u;
+    uint32_t x = live ? mask_word(mask, q_pos, (kl.block(j0 + j) << kTileLg) + 32 * b, len) : 0u;
+    if (!(live & 1u)) x &= 0xffff0000u;
+    if (!(live & 2u)) x &= 0x0000ffffu;
+    return x;
   };
   auto shape = [&](const Step& s, int j, f32x16& x0, f32x16& x1) __attribute__((always_inline)) {
-    if (s.full == 15u) return;
-    uint32_t w0, w1;
-    words(s, j, w0, w1);
-    mask_block(x0, w0);
-    mask_block(x1, w1);
+    if ((s.full & 3u) != 3u) mask_block(x0, word(s, j, 0));
+    if ((s.full & 12u) != 12u) mask_block(x1, word(s, j, 1));
   };
   auto block_max = [&](const f32x16& x, float mx) __attribute__((always_inline)) -> float {
 #pragma unroll
@@ -356,7 +351,8 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
       qk(sa0, sa1);
       uint32_t w0 = ~0u, w1 = ~0u;
       if (s.full != 15u) {
-        words(s, j, w0, w1);
+        w0 = word(s, j, 0);
+        w1 = word(s, j, 1);
         mask_block(sa0, w0);
         mask_block(sa1, w1);
       }
