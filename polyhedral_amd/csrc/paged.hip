@@ -106,7 +106,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(const TablesK
   if (tid == 0) bad_s = 0;
   __syncthreads();
 
-  int64_t t_sum = 0, p_sum = 0;  // of the requests before this round's (the same in every thread)
+  int64_t t_sum = 0, p_sum = 0;  // of the requests before this pass's (the same in every thread)
   int32_t bad = 0;
   for (int r0 = 0; r0 < a.R; r0 += kScanThreads) {
     const int r = r0 + tid;
