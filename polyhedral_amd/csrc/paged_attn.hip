@@ -76,9 +76,9 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   p->tile = x->dtype != PA_F32 && x->n_pages > 0 && x->max_fresh * G > few_rows;
   int64_t few = x->T * G / kRows + some;
   if (p->tile && few > some * ((few_rows + kRows - 1) / kRows)) few = some * ((few_rows + kRows - 1) / kRows);
-  // (256 beside chunks, whose units are most of the grid: 36 requests of 1 or 20 to 1000 new tokens 54
-  // -> 52 us)
-  if (int rc = part_of(x, kRows, p->tile ? 256 : 1024, few, &p->rows)) return rc;
+  // (beside chunks too: 61 requests of a token and 3 chunks with 256 shares 232 us, with 512 177, with 1024
+  // 166; 36 requests of which most are chunks 53 with any)
+  if (int rc = part_of(x, kRows, 1024, few, &p->rows)) return rc;
   p->rows.least = 4;
   p->rows.root_over = 0.7f;
   p->rows.row_min = 0;
