@@ -161,6 +161,8 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
     t.p2 = imin(t.p2, kMaxPosition);
     a.terms[i] = t;
   }
+  // (rows of 64 keys at 5 TB/s against a step's 1.9 us on 512 places, less a tenth)
+  a.few_weight = x->D == 128 ? 1.6f : 0.8f;
   a.stride = p.stride;
   a.o = static_cast<char*>(x->o);
   a.o_st = x->o_st * esz;

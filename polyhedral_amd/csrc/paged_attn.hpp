@@ -56,6 +56,7 @@ struct PagedK {
   float c;  // scale * log2(e)
   int32_t n_include, n_exclude;
   pa_term terms[PA_MAX_TERMS];
+  float few_weight;  // time of a block of few rows' keys, of that of a chunk's step (see find_unit)
   int32_t stride;  // of a mask that is a lattice beyond a band: 1 in `stride` keys is live for a token; else 0
   char* o;
   int64_t o_st, o_sh;
@@ -80,6 +81,7 @@ __device__ __forceinline__ bool by_lists(int32_t tokens, int32_t stride) { retur
 
 struct Work {
   int32_t tiles, blocks, least;  // least: blocks of a share
+  int32_t few;                   // blocks of a request with fewer rows than the part takes
 };
 
 struct Unit {
@@ -93,11 +95,13 @@ struct Unit {
 template <int BM, int LG>
 __device__ __forceinline__ Work work_of(const PagedK& a, const PagedPart& p, const Request& q) {
   const int32_t rows = q.n * a.G;
-  if (rows <= p.row_min || rows > p.row_max) return {0, 0, 1};
+  if (rows == 0 || rows > p.row_max || (BM == kRows && rows <= p.row_min)) return {0, 0, 1, 0};
   const int32_t span = imin(q.n, p.span);
   // (a share that is taken by lists: for one token a list of 512 keys for each wave, for more fewer)
   const int32_t least = BM == kRows && by_lists(span, a.stride) ? imax((2048 >> LG) >> (31 - __builtin_clz((uint32_t)imax(span, 1))), p.least) : p.least;
-  return {(rows + BM - 1) / BM, key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG).count(), least};
+  const int32_t blocks = key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG).count();
+  if (BM == kTileRows && rows <= p.row_min) return {0, 0, 1, blocks};
+  return {(rows + BM - 1) / BM, blocks, least, 0};
 }
 
 // Sum over lanes 0 .. l, by DPP moves inside rows of 16 lanes and broadcasts of their last ones.
@@ -163,13 +167,14 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, c
   Unit u;
   u.found = false;
   Request q{0, 0, 0};
-  Work w{0, 0, 1};
-  float total = 0.f;  // (a share needs no exact total)
+  Work w{0, 0, 1, 0};
+  float total = 0.f, few = 0.f;  // (a share needs no exact total)
   int32_t end = 0;
   for (int r0 = 0; r0 < a.R; r0 += 64) {
     q = load_request(a, r0 == 0 ? raw : raw_request(a, r0, lane), r0, lane, end);
     w = work_of<BM, LG>(a, p, q);
     total += wave_total((float)w.tiles * (float)w.blocks);
+    if (BM == kTileRows) few += wave_total((float)w.few);
   }
   // Blocks of a share: all of the part's work over `shares` (rounded up, so the units stay within shares
   // + tiles Hkv, which the grid is sized for).  Two work-groups run per CU, so 1024 shares of few rows are
@@ -179,6 +184,11 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, c
   // requests of 300 to 8192 30 -> 24 us, 16 49 -> 44, 5 of 6000 32 -> 27, the 64 148 -> 144.
   float share = total * (float)a.Hkv * p.by_shares;
   if (BM == kRows) share *= share < 24.f ? 2.4f : 1.08f;
+  // Where the requests with few rows take longer than the chunks, those get one place of a CU's two, and
+  // their MFMAs run beside the loads of the others instead of before them: 61 requests of a token and 3
+  // chunks 166 -> 150 us, 29 and 3 307 -> 284.  (36 requests of which the chunks take longer: 52 -> 70,
+  // units as long as the whole launch.)
+  if (BM == kTileRows && few * a.few_weight >= total) share *= 2.f;
 
   int32_t before = 0, slot = 0;  // units and slots of earlier requests
   end = 0;

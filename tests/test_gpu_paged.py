@@ -323,6 +323,15 @@ def test_long_axis_is_split(gpu, dtype, D, sizes, mask):
     Batch(gpu, dtype, D, 64, 4, 2, sizes, seed=len(sizes)).check(mask)
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("tokens", [5, 70])
+def test_tokens_beside_a_chunk(gpu, dtype, D, tokens):
+    """Few and many long requests of a token beside chunks, whose shares depend on that."""
+    sizes = [(1, 2500 + 7 * i) for i in range(tokens)]
+    sizes[tokens // 2:tokens // 2] = [(60, 1200), (41, 41)]
+    Batch(gpu, dtype, D, 64, 4, 2, sizes, seed=tokens).check(pm.Causal())
+
+
 @pytest.mark.parametrize("R", [63, 64, 65, 200])
 def test_many_requests(gpu, R):
     rng = np.random.default_rng(R)
