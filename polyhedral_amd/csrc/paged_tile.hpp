@@ -38,6 +38,7 @@
 
 #include <type_traits>
 
+#include "page_steps.hpp"
 #include "paged_attn.hpp"
 
 namespace pa {
@@ -48,6 +49,11 @@ __device__ __forceinline__ bool not_finite16(uint32_t lo, uint32_t hi) {
   constexpr uint32_t inf = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
   return lo >= inf || hi >= (inf << 16);
 }
+
+// Scores of a step's two blocks of 32 keys.
+struct StepScores {
+  f32x16 x0 = {}, x1 = {};
+};
 
 template <typename T, int D>
 struct TileShape {
@@ -156,7 +162,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
 #pragma unroll
   for (int x = 0; x < NDB; ++x) acc[x] = f32x16{0};
   float m_run = -INFINITY, l_part = 0.f;  // (log2 units)
-  f32x16 sa0 = {}, sa1 = {}, sb0 = {}, sb1 = {};  // scores of the current step and the next, in turn
+  StepScores sa, sb;  // of the current step and the next, in turn
   // (held in a register: a scalar load of an argument inside the loop would wait for the LDS reads
   // in flight)
   float c_exp = a.c;
@@ -246,8 +252,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   uint32_t p = 0u;  // j & 1, times a slot
   // Iteration j, with a step after it: behind the wait and the barrier, K of step j + 1 and V of step
   // j are in LDS, and the slots that the new DMA writes were last read before the barrier.
-  // x0, x1: the step's scores; y0, y1: those of the next.
-  auto iterate = [&](int j, const f32x16& x0, const f32x16& x1, f32x16& y0, f32x16& y1) __attribute__((always_inline)) {
+  auto next = [&](int j) __attribute__((always_inline)) -> LiveSteps {
     dma_wait_all();
     // (a use that makes the compiler's own wait for the page loads fall here)
     asm volatile("" ::"v"(r_page));
@@ -257,38 +262,43 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
       dma(KRING + p, kbase + s_after.off);
     }
     dma(VRING + (SLOT - p), vbase + s_next.off);
-    if ((s_cur.live | s_next.live) != 0u) {
-      // (MFMAs go before the masking, maxima, prologues and epilogues of the other work-group on the
-      // CU: sinks in chunks 279 -> 269 us, 16 prompts of 512 92 -> 84, nothing on long lists)
-      __builtin_amdgcn_s_setprio(1);
-      const float neg_m = -base_of(m_run);
-      const Frag p00 = exps(x0, 0, neg_m, false), p01 = exps(x0, 1, neg_m, false), p10 = exps(x1, 0, neg_m, false),
-                 p11 = exps(x1, 1, neg_m, false);
-      qk(y0, y1);
-      pv(p00, 0);
-      pv(p01, 1);
-      pv(p10, 2);
-      pv(p11, 3);
-      // 4 K reads ahead; then MFMAs of the scores, each beside a read and exponentials; then those of
-      // the products, V reads running 4 MFMAs ahead
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+    return {s_cur.live != 0u, s_next.live != 0u};
+  };
+  auto body = [&](int j, bool live, const StepScores& x, StepScores& y) __attribute__((always_inline)) {
+    // (MFMAs go before the masking, maxima, prologues and epilogues of the other work-group on the
+    // CU: sinks in chunks 279 -> 269 us, 16 prompts of 512 92 -> 84, nothing on long lists)
+    __builtin_amdgcn_s_setprio(1);
+    // (x of a dead step may be an earlier one's scores: every exponential is 0 then, or NaN where that
+    // step's sums already were)
+    const float neg_m = live ? -base_of(m_run) : -INFINITY;
+    const Frag p00 = exps(x.x0, 0, neg_m, false), p01 = exps(x.x0, 1, neg_m, false), p10 = exps(x.x1, 0, neg_m, false),
+               p11 = exps(x.x1, 1, neg_m, false);
+    qk(y.x0, y.x1);
+    pv(p00, 0);
+    pv(p01, 1);
+    pv(p10, 2);
+    pv(p11, 3);
+    // 4 K reads ahead; then MFMAs of the scores, each beside a read and exponentials; then those of
+    // the products, V reads running 4 MFMAs ahead
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
 #pragma unroll
-      for (int x = 0; x < 2 * NQF; ++x) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
-        __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 6 : 10, 1);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
-#pragma unroll
-      for (int x = 0; x < 4 * NDB; ++x) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
-        __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 1 : 4, 1);
-      }
-      __builtin_amdgcn_s_setprio(0);
-      shape(s_next, j + 1, y0, y1);
-      raise(block_max(y1, block_max(y0, -INFINITY)), false);
+    for (int z = 0; z < 2 * NQF; ++z) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 6 : 10, 1);
     }
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+    for (int z = 0; z < 4 * NDB; ++z) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+      __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 1 : 4, 1);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    shape(s_next, j + 1, y.x0, y.x1);
+    raise(block_max(y.x1, block_max(y.x0, -INFINITY)), false);
+  };
+  auto turn = [&]() __attribute__((always_inline)) {
     s_cur = s_next;
     s_next = s_after;
     rd.template turn_rows<SLOT>();
@@ -305,24 +315,14 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
     for (int kc = 0; kc < NQF; ++kc) asm volatile("" ::"v"(qf[kc]));
     __syncthreads();
     if (n_steps > 1) dma(KRING + SLOT, kbase + s_next.off);
-    qk(sa0, sa1);
-    shape(s_cur, 0, sa0, sa1);
-    raise(block_max(sa1, block_max(sa0, -INFINITY)), false);
+    qk(sa.x0, sa.x1);
+    shape(s_cur, 0, sa.x0, sa.x1);
+    raise(block_max(sa.x1, block_max(sa.x0, -INFINITY)), false);
     rd.template turn_rows<SLOT>();
-    int j = 0;
-#pragma unroll 1
-    for (; j + 2 < n_steps; j += 2) {
-      iterate(j, sa0, sa1, sb0, sb1);
-      iterate(j + 1, sb0, sb1, sa0, sa1);
-    }
-    if (j + 1 < n_steps) {
-      iterate(j, sa0, sa1, sb0, sb1);
-      sa0 = sb0;
-      sa1 = sb1;
-    }
+    walk_steps(n_steps, sa, sb, next, body, turn);
     dma_wait_all();
     __syncthreads();
-    if (s_cur.live != 0u) sums_step(sa0, sa1);
+    if (s_cur.live != 0u) sums_step(sa.x0, sa.x1);
   }
 
   // ---- sums that are not finite, scores that are huge: the list again, step by step --------
@@ -348,19 +348,19 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
       dma(VRING, vbase + s.off);
       dma_wait_all();
       __syncthreads();
-      qk(sa0, sa1);
+      qk(sa.x0, sa.x1);
       uint32_t w0 = ~0u, w1 = ~0u;
       if (s.full != 15u) {
         w0 = word(s, j, 0);
         w1 = word(s, j, 1);
-        mask_block(sa0, w0);
-        mask_block(sa1, w1);
+        mask_block(sa.x0, w0);
+        mask_block(sa.x1, w1);
       }
-      raise(block_max(sa1, block_max(sa0, -INFINITY)), huge);
+      raise(block_max(sa.x1, block_max(sa.x0, -INFINITY)), huge);
       const float neg_m = -base_of(m_run);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const Frag pf = exps(x < 2 ? sa0 : sa1, x & 1, neg_m, huge);
+        const Frag pf = exps(x < 2 ? sa.x0 : sa.x1, x & 1, neg_m, huge);
         if (!((s.live >> x) & 1u)) continue;
         uint32_t lo = 0u, hi = 0u;
 #pragma unroll
