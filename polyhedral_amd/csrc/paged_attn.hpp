@@ -258,6 +258,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2 share_load2(Shares s, int32_t lane_off, int32_t off) {
   return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(s, lane_off, off, kSc1));
 }
+__device__ __forceinline__ float share_load1(Shares s, int32_t lane_off, int32_t off) {
+  return __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(s, lane_off, off, kSc1));
+}
 __device__ __forceinline__ void share_store4(char* p, f32x4 x) {
   const u32x4 y = __builtin_bit_cast(u32x4, x);
   store_x4_sc1(p, y.x, y.y, y.z, y.w);
@@ -280,8 +283,8 @@ __device__ __forceinline__ bool last_share(const PagedPart& p, const Unit& u, in
 // so far; every score is -inf then).
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-// floats of a slot: O of every row, then maximum and sum
-constexpr int slot_floats(int BM, int D) { return BM * (D + 2); }
+// floats of a slot: O of every row, then maximum and sum (and of a chunk's tile what the maximum lacks)
+constexpr int slot_floats(int BM, int D) { return BM * (D + (BM == kTileRows ? 3 : 2)); }
 
 int check_pages(const char* who, int64_t n_pages, int32_t page_size, int* page_lg);
 

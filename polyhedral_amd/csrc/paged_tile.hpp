@@ -21,7 +21,8 @@
 // log2 units: p = exp2(fma(x, c, -m)) has the rounding of m = max(x c) in its exponent, the same for
 // all keys of the row, so it falls out of the result while it is small (below 2^24 half a unit at
 // most) but empties or overflows the row where m is large; that row's second pass has m in units of
-// the scores and p = exp2((x - m) c).
+// the scores and p = exp2((x - m) c), and what the rounding of m c leaves out goes with it to the
+// merge of its shares.
 //
 // Scores, maxima, sums and O are float32; P is rounded to 16 bits as an MFMA operand only, its sum
 // taken before.
@@ -334,6 +335,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   // (a row's maximum may have been huge before it had one near 0: its sum is not finite then; -inf: a
   // row without a live key)
   const bool huge = (__builtin_fabsf(m_run) > 0x1p24f && m_run != -INFINITY) || !(row_sum(l_part) < INFINITY);
+  float m_rest = 0.f;  // what the rounding of a huge row's maximum to log2 units left out of m_run
   if (__syncthreads_or(huge || !(big < INFINITY))) {
     rd = tile_reads<D>((lds_cptr)smem, lane);
 #pragma unroll
@@ -398,7 +400,11 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
       }
       __syncthreads();  // every wave is past the slots
     }
-    if (huge) m_run *= c_exp;
+    if (huge) {
+      const float m_x = m_run;
+      m_run = m_x * c_exp;
+      if (__builtin_fabsf(m_run) < INFINITY) m_rest = __builtin_fmaf(m_x, c_exp, -m_run);
+    }
   }
 
   // ---- the rows leave -------------------------------------------------------------------
@@ -408,7 +414,9 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   const int m_e = lane_e & 31, G_e = lane_e >> 5;
   const bool mine = 32 * w + m_e < n_rows;
   if (u.splits > 1) {
-    // a slot is the waves' registers as they are: 16 bytes of O per lane, then maximum and sum
+    // a slot is the waves' registers as they are: 16 bytes of O per lane, then maximum and sum, then
+    // what the maximum lacks (which is as large as the difference of two shares' maxima, where these are
+    // huge)
     constexpr int SLOT_B = slot_floats(kTileRows, D) * 4, WB = SLOT_B / 4;
     char* first = part.part + (int64_t)u.slot * SLOT_B;
     const bool has = 32 * w < n_rows;  // (a wave without rows stores and merges nothing)
@@ -423,13 +431,20 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
         float* ml = reinterpret_cast<float*>(own + NDB * 4096 - 8 * lane_e);
         share_store(ml, m_run);
         share_store(ml + 1, l_tot);
+        share_store(reinterpret_cast<float*>(own + NDB * 4096 + 256 - 12 * lane_e), m_rest);
       }
     }
     if (!last_share(part, u, tid, flag) || !has) return;
     const Shares all = shares_at(first, u.splits * SLOT_B);
     m_run = -INFINITY;
+    m_rest = 0.f;
 #pragma unroll 8
-    for (int s = 0; s < u.splits; ++s) m_run = nan_max(m_run, share_load2(all, 8 * m_e, s * SLOT_B + w * WB + NDB * 4096)[0]);
+    for (int s = 0; s < u.splits; ++s) {
+      const int32_t at = s * SLOT_B + w * WB + NDB * 4096;
+      const float ms = share_load2(all, 8 * m_e, at)[0], rs = share_load1(all, 4 * m_e, at + 256);
+      m_rest = ms > m_run ? rs : ms == m_run ? nan_max(m_rest, rs) : m_rest;
+      m_run = nan_max(m_run, ms);
+    }
     l_tot = 0.f;
 #pragma unroll
     for (int x = 0; x < NDB; ++x) acc[x] = f32x16{0};
@@ -442,7 +457,8 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[db][e] = share_load4(all, 16 * lane_e, at + (4 * db + e) * 1024);
       const f32x2 ml = share_load2(all, 8 * m_e, at + NDB * 4096);
-      const float f = __builtin_amdgcn_exp2f(ml[0] - base_of(m_run));
+      const float rest = share_load1(all, 4 * m_e, at + NDB * 4096 + 256);
+      const float f = __builtin_amdgcn_exp2f((ml[0] - base_of(m_run)) + (rest - m_rest));
       l_tot += f * ml[1];
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
