@@ -322,7 +322,9 @@ class PagedKVCache:
             raise ValueError(f"{pages} pages of {page_size} rows: slots stay below 2^31")
         if max_length > MAX_POSITION - page_size:
             raise ValueError(f"max_length={max_length} passes {MAX_POSITION - page_size}")
-        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        dev = torch.device("cuda" if device is None else device)
+        if dev.type == "cuda" and dev.index is None:   # (tensors name their device by its index)
+            dev = torch.device("cuda", torch.cuda.current_device())
         i32 = dict(dtype=torch.int32, device=dev)
         self.k = torch.zeros(layers, pages, heads, page_size, D, dtype=dtype, device=dev)
         self.v = torch.zeros_like(self.k)
