@@ -518,8 +518,9 @@ int pa_attn_bwd(const pa_attn_bwd_args* args, void* stream);
  * counts as dead.  Rows of no request are left as they are.  lse may be NULL (natural log,
  * [T, Hq] at lse_st, lse_sh).  max_fresh: the most new tokens of a request (a hint: it selects
  * kernels and moves no result beyond rounding).  D = 64 or 128, f32 / f16 / bf16, scale > 0.
- * o overlaps no input.  workspace: the bytes pa_paged_workspace gives for the same sizes, hint,
- * type and mask (no pointer is read), 256-byte aligned, the first zero_bytes of them zero before
+ * o, lse and the workspace share no byte with an input or with each other, and no two rows of o or
+ * of lse do (parts of one buffer's rows may be q and o in turn, or o and lse).  workspace: the bytes
+ * pa_paged_workspace gives for the same sizes, hint, type and mask (no pointer is read), 256-byte aligned, the first zero_bytes of them zero before
  * the first call with it and left zero by every call of these; not shared by calls that overlap. */
 typedef struct pa_tables_args {
   const int32_t* before;

@@ -251,8 +251,10 @@ def prepare_attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_f
     past a request's length are never live, and neither are keys whose table entry names no page.
     scale: positive, 1/sqrt(D) by default.  max_fresh: the most new tokens of a request, where the
     program knows it (it selects kernels; any value gives right results).  out: [tokens, Hq, D];
-    lse: None or float32 [tokens, Hq], the natural-log sum-exp.  A row with no live key gives 0
-    and -inf; rows of no request are left as they are.  The result is out."""
+    lse: None or float32 [tokens, Hq], the natural-log sum-exp; neither shares memory with an
+    input, the other or itself (a call that does is refused when it is launched).  A row with no
+    live key gives 0 and -inf; rows of no request are left as they are (in a new ``out``: as its
+    memory was).  The result is out."""
     pages, Hkv, P, D = _cache(k, v)
     if q.dim() != 3:
         raise ValueError("q must be [tokens, heads, D]")

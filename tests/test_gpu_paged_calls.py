@@ -1,11 +1,11 @@
 """Calls that the paged cache's documentation allows (polyhedral_amd.paged), beside those of
 tests/test_gpu_paged.py."""
-import numpy as np
 import pytest
 import torch
 
-from polyhedral_amd import paged
+from polyhedral_amd import _lib, paged
 from polyhedral_amd.polyattn import masks as pm
+from tests.test_gpu_paged import Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +25,48 @@ def test_a_cache_on_any_name_of_its_device(gpu, device):
     cache.finish([True, False])
     assert cache.lengths.tolist() == [0, 3]
     cache.check()
+
+
+# ---- tensors that are parts of one buffer -------------------------------------------------------
+@pytest.mark.parametrize("dtype,D,sizes", [(torch.float32, 64, [(1, 300), (3, 40)]), (torch.bfloat16, 128, [(1, 3000), (150, 400)]),
+                                           (torch.float16, 64, [(40, 90)])])
+def test_outputs_beside_inputs_in_one_buffer(gpu, dtype, D, sizes):
+    """q and out are heads of one buffer in turn, or halves of its rows; out and lse are packed; K and V
+    of a page lie side by side."""
+    b = Batch(gpu, dtype, D, 16, 4, 2, sizes)
+    want, wl = b.run(pm.Causal())
+    kv = torch.stack([b.k, b.v], dim=1)
+    k, v = kv[:, 0], kv[:, 1]
+    heads = torch.full((b.T, 4, 2, D), 7.0, dtype=dtype, device=gpu)
+    heads[:, :, 0] = b.q
+    halves = torch.full((b.T, 8, D), 7.0, dtype=dtype, device=gpu)
+    halves[:, 4:] = b.q
+    lse = torch.full((b.T, 4), 7.0, device=gpu)
+    for q, o in ((heads[:, :, 0], heads[:, :, 1]), (halves[:, 4:], halves[:, :4])):
+        paged.attention(q, k, v, *b.dev(), pm.Causal(), out=o, lse=lse)
+        assert torch.equal(o, want) and torch.equal(lse, wl) and torch.equal(q, b.q)
+    if dtype == torch.float32:
+        packed = torch.full((b.T, 4, D + 4), 7.0, device=gpu)
+        paged.attention(b.q, k, v, *b.dev(), pm.Causal(), out=packed[..., :D], lse=packed[..., D])
+        assert torch.equal(packed[..., :D], want) and torch.equal(packed[..., D], wl) and (packed[..., D + 1:] == 7).all()
+
+
+def test_outputs_that_share_memory_are_refused(gpu):
+    b = Batch(gpu, torch.float16, 64, 16, 4, 2, [(1, 20), (2, 30)])
+    shape = (b.T, 4, 64)
+    lse = torch.zeros(b.T, 4, device=gpu)
+
+    def refused(match, **change):
+        before = {n: t.clone() for n, t in (("q", b.q), ("k", b.k), ("v", b.v))}
+        with pytest.raises(_lib.PolyattnError, match=match):
+            paged.attention(b.q, b.k, b.v, *b.dev(), pm.Causal(), **change)
+        assert all(torch.equal(t.nan_to_num(), getattr(b, n).nan_to_num()) for n, t in before.items())
+    refused("rows of o overlap", out=torch.zeros(1, 4, 64, dtype=b.dtype, device=gpu).expand(shape))
+    refused("rows of o overlap", out=torch.zeros(b.T, 1, 64, dtype=b.dtype, device=gpu).expand(shape))
+    refused("rows of lse overlap", lse=torch.zeros(1, 4, device=gpu).expand(b.T, 4))
+    refused("rows of lse overlap", lse=torch.zeros(b.T, 1, device=gpu).expand(b.T, 4))
+    refused("o and q", out=b.q)
+    refused("o and k", out=b.k.view(-1, 4, 64)[:b.T])
+    both = torch.zeros(b.T, 4, 64, dtype=torch.float32, device=gpu)
+    refused("o and lse", out=both.view(torch.float16)[..., :64], lse=both[..., 0])
+    paged.attention(b.q, b.k, b.v, *b.dev(), pm.Causal(), lse=lse)

@@ -1,0 +1,162 @@
+"""Which tensors of a call share memory (csrc/page_spans.hpp), compiled for the host, against sets of
+bytes; and the C entry points' refusals of outputs that share it, which come before any device work."""
+import ctypes
+import itertools
+import pathlib
+import shutil
+import subprocess
+
+import numpy as np
+import pytest
+
+from polyhedral_amd import _lib
+
+ROOT = pathlib.Path(__file__).resolve().parents[1]
+
+HARNESS = r"""
+#include "page_spans.hpp"
+using namespace pa;
+static Strided<2> of(const long long* x) {
+  return strided<2>(reinterpret_cast<const void*>(x[0]), x[1], {x[2], x[3]}, {x[4], x[5]});
+}
+extern "C" {
+int self2(const long long* x) { return overlaps_itself(of(x)); }
+int both2(const long long* x, const long long* y) { return overlap(of(x), of(y)); }
+int nested3(long long w, const long long* n, const long long* s) {
+  return nested(strided<3>(nullptr, w, {n[0], n[1], n[2]}, {s[0], s[1], s[2]}));
+}
+int flat_rows(long long at, long long bytes, const long long* x) {
+  return overlap(flat(reinterpret_cast<const void*>(at), bytes), of(x));
+}
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    if shutil.which("g++") is None:
+        pytest.skip("g++ not available")
+    d = tmp_path_factory.mktemp("page_spans")
+    (d / "h.cpp").write_text(HARNESS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-fsanitize=undefined", "-fno-sanitize-recover",
+                    f"-I{ROOT / 'polyhedral_amd' / 'csrc'}", "-o", str(d / "h.so"), str(d / "h.cpp")], check=True,
+                   capture_output=True)
+    lib = ctypes.CDLL(str(d / "h.so"))
+    lib.nested3.argtypes = [ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p]
+    lib.flat_rows.argtypes = [ctypes.c_longlong, ctypes.c_longlong, ctypes.c_void_p]
+    return lib
+
+
+def _ll(*x):
+    return (ctypes.c_longlong * len(x))(*x)
+
+
+def _bytes(at, w, n, m, s, t):
+    """The bytes of each row."""
+    return [set(range(at + i * s + j * t, at + i * s + j * t + w)) for i in range(n) for j in range(m)]
+
+
+def test_rows_on_top_of_each_other(host):
+    for w, n, m in itertools.product((1, 3, 4), (0, 1, 2, 3), (0, 1, 2, 4)):
+        for s, t in itertools.product((-7, -4, 0, 1, 2, 3, 4, 5, 6, 8, 9, 12, 13), repeat=2):
+            rows = _bytes(1000, w, n, m, s, t)
+            want = sum(map(len, rows)) > len(set().union(*rows))
+            assert host.self2(_ll(1000, w, n, m, s, t)) == want, (w, n, m, s, t)
+
+
+def test_parts_of_one_buffer(host):
+    """The same sizes and strides: exact."""
+    rng = np.random.default_rng(0)
+    for _ in range(6000):
+        n, m = (int(x) for x in rng.integers(1, 5, 2))
+        w, u = (int(x) for x in rng.integers(1, 6, 2))
+        s, t = (int(x) for x in rng.integers(-14, 15, 2))
+        d = int(rng.integers(-60, 61))
+        a, b = set().union(*_bytes(1000, w, n, m, s, t)), set().union(*_bytes(1000 + d, u, n, m, s, t))
+        assert host.both2(_ll(1000, w, n, m, s, t), _ll(1000 + d, u, n, m, s, t)) == bool(a & b), (n, m, w, u, s, t, d)
+
+
+def test_other_tensors_by_their_spans(host):
+    rng = np.random.default_rng(1)
+    for _ in range(3000):
+        x, y = ([1000 + int(rng.integers(-80, 81)), int(rng.integers(1, 6)), *(int(v) for v in rng.integers(0, 4, 2)),
+                 *(int(v) for v in rng.integers(-9, 20, 2))] for _ in range(2))
+        a, b = (set().union(*_bytes(*v)) for v in (x, y))
+        meet = bool(a and b and min(a) <= max(b) and min(b) <= max(a))
+        got = host.both2(_ll(*x), _ll(*y))
+        assert got <= meet and (got or not a & b), (x, y)
+        assert host.flat_rows(x[0], x[1], _ll(*y)) == bool(b and x[0] <= max(b) and min(b) < x[0] + x[1])
+
+
+def test_nested_strides_are_apart(host):
+    rng = np.random.default_rng(2)
+    some = 0
+    for _ in range(4000):
+        w, n, s = int(rng.integers(1, 4)), [int(x) for x in rng.integers(1, 4, 3)], [int(x) for x in rng.integers(0, 30, 3)]
+        cells = [sum(i * t for i, t in zip(at, s)) + b for at in np.ndindex(*n) for b in range(w)]
+        if host.nested3(w, _ll(*n), _ll(*s)):
+            some += 1
+            assert len(set(cells)) == len(cells), (w, n, s)
+    assert some > 100
+    # the layouts of a dense cache in any order of its dimensions are nested
+    for order in itertools.permutations(range(3)):
+        n, s, size = [5, 3, 16], [0, 0, 0], 256
+        for i in order:
+            s[i], size = size, size * n[i]
+        assert host.nested3(256, _ll(*n), _ll(*s))
+
+
+def test_the_largest_sizes_and_strides(host):
+    big = (1 << 63) - 1
+    assert host.self2(_ll(1 << 40, big, 1 << 30, 65535, big, big)) == 1
+    assert host.self2(_ll(1 << 40, 256, 1 << 30, 4, 1024, 256)) == 0
+    assert host.self2(_ll(1 << 40, 256, 1 << 30, 4, 1023, 256)) == 1
+    assert host.both2(_ll(1 << 40, 256, 1 << 30, 32, big, 256), _ll((1 << 40) + 32 * 256, 256, 1 << 30, 32, big, 256)) == 0
+
+
+# ---- refusals of the C entry points ---------------------------------------------------------
+def _refused(rc, text):
+    assert rc == _lib.PA_E_INVALID
+    assert text in _lib.lib().pa_last_error().decode(), _lib.lib().pa_last_error()
+
+
+ATTENTION = ("q", "k", "v", "tables", "lengths", "q_start", "o", "lse", "workspace")
+
+
+def _attention(at, **change):
+    """T = 3 rows of 4 heads of 128 bf16, 2 KV heads, 4 pages of 16, each tensor 64 KiB from the next."""
+    a = _lib.PaPagedArgs()
+    for i, f in enumerate(ATTENTION):
+        setattr(a, f, at + i * 65536)
+    a.q_st, a.q_sh, a.o_st, a.o_sh, a.c_sp, a.c_sh, a.c_sn, a.lse_st, a.lse_sh = 512, 128, 512, 128, 4096, 2048, 128, 4, 1
+    a.n_pages, a.page_size, a.pitch, a.cols, a.R, a.T, a.max_fresh = 4, 16, 4, 4, 2, 3, 2
+    a.Hq, a.Hkv, a.D, a.dtype, a.scale = 4, 2, 128, _lib.PA_BF16, 0.1
+    a.mask.n_include = 1
+    a.workspace_bytes = 1 << 40
+    for f, x in change.items():
+        setattr(a, f, x)
+    return _lib.lib().pa_paged_attn(ctypes.byref(a), None)
+
+
+def test_attention_refuses_outputs_whose_rows_overlap():
+    at = 1 << 40   # (no address is read)
+    for change in (dict(o_st=0), dict(o_sh=0), dict(o_sh=64), dict(o_st=256), dict(o_st=504), dict(o_st=128)):
+        _refused(_attention(at, **change), "rows of o overlap")
+    for change in (dict(lse_st=0), dict(lse_sh=0), dict(lse_st=1), dict(lse_st=3), dict(lse_st=-1)):
+        _refused(_attention(at, **change), "rows of lse overlap")
+
+
+@pytest.mark.parametrize("out", ["o", "lse", "workspace"])
+def test_attention_refuses_outputs_that_overlap_others(out):
+    at = 1 << 40
+    size = {"q": 3072, "k": 32768, "v": 32768, "tables": 32, "lengths": 8, "q_start": 12, "o": 3072, "lse": 48}
+    for f, n in size.items():
+        if f == out:
+            continue
+        base = at + ATTENTION.index(f) * 65536
+        if out == "workspace":
+            places = [base - 256, base]
+        else:
+            places = [base, base + (n - 1) // 16 * 16, base - (size[out] - 1) // 16 * 16]
+        for p in places:
+            _refused(_attention(at, **{out: p}), "overlap")
