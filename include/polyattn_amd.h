@@ -502,8 +502,9 @@ int pa_attn_bwd(const pa_attn_bwd_args* args, void* stream);
  * pa_page_release: pages first[r] .. last[r] - 1 of request r's table (clamped to the table;
  * entries that are none of the cache are skipped) go back to the end of the free list in order
  * of (request, page), and their entries become -1.  *status 0, or 1 when the list would pass
- * n_pages (nothing is done then).  free_left may be free_count.  workspace: int32 [R], not
- * shared by calls that overlap.
+ * n_pages (nothing is done then).  free_left may be free_count; else tables, free_list and the
+ * outputs share no memory with each other or with an input.  workspace: int32 [R], not shared by
+ * calls that overlap.
  *
  * pa_paged_append: row i of k_new / v_new [T, Hkv, D] (n_st, n_sh: token and head strides in
  * elements) is written to slot slots[i]; a slot outside the cache (-1) is skipped.  Slots are

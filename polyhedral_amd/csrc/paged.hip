@@ -10,8 +10,13 @@
 // work-group writes sums and state, and a second kernel the tokens and pages.
 // What bounds it: latency (three trips to memory one after the other, and the launch): 256 requests of
 // a token each 5.0 us, 96 with 78000 tokens 5.3 (in two launches 8.4).
+#include <string.h>
+
+#include <initializer_list>
+
 #include "common.hpp"
 #include "page_math.hpp"
+#include "page_spans.hpp"
 
 namespace pa {
 namespace {
@@ -289,6 +294,25 @@ int page_lg_of(int32_t ps) {
   return -1;
 }
 
+struct Named {
+  const char* name;
+  Strided<1> at;
+  const char* same = "";  // an input that this output may be
+};
+Strided<1> tables_span(const int32_t* tables, int32_t R, int64_t pitch, int32_t cols) {
+  return strided<1>(tables, 4ll * cols, {cols ? R : 0}, {4 * pitch});
+}
+int check_apart(const char* who, std::initializer_list<Named> in, std::initializer_list<Named> out) {
+  for (const Named& o : out) {
+    for (const Named& i : in)
+      PA_CHECK_ARG(!overlap(o.at, i.at) || (!strcmp(o.same, i.name) && o.at.at == i.at.at && span(o.at) == span(i.at)),
+                   "%s: %s and %s overlap", who, o.name, i.name);
+    for (const Named& i : out)
+      PA_CHECK_ARG(&i == &o || !overlap(o.at, i.at), "%s: %s and %s overlap", who, o.name, i.name);
+  }
+  return PA_OK;
+}
+
 }  // namespace
 
 // The cache's shape as every entry point checks it; page_lg is set.
@@ -385,6 +409,14 @@ extern "C" int pa_page_release(const int32_t* first, const int32_t* last, int32_
   PA_CHECK_ARG(R == 0 || (first && last && workspace && (cols == 0 || tables)),
                "pa_page_release: null first / last / tables / workspace");
   PA_CHECK_ARG(n_pages == 0 || free_list, "pa_page_release: null free_list");
+  // (what is written shares no memory with anything else, but for the count that advances in place)
+  const int64_t n = R;
+  if (int rc = check_apart("pa_page_release", {{"first", flat(first, 4 * n)}, {"last", flat(last, 4 * n)},
+                                               {"free_count", flat(free_count, 4)}},
+                           {{"tables", tables_span(tables, R, pitch, cols)}, {"free_list", flat(free_list, 4 * n_pages)},
+                            {"free_left", flat(free_left, 4), "free_count"}, {"status", flat(status, 4)},
+                            {"workspace", flat(workspace, 4 * n)}}))
+    return rc;
   hipLaunchKernelGGL(release_kernel, dim3(1), dim3(kScanThreads), 0, static_cast<hipStream_t>(stream), first, last, R,
                      tables, pitch, cols, free_list, free_count, n_pages, free_left, status, workspace);
   PA_LAUNCH_CHECK("release_kernel");

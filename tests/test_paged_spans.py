@@ -160,3 +160,22 @@ def test_attention_refuses_outputs_that_overlap_others(out):
             places = [base, base + (n - 1) // 16 * 16, base - (size[out] - 1) // 16 * 16]
         for p in places:
             _refused(_attention(at, **{out: p}), "overlap")
+
+
+RELEASE_IN, RELEASE_OUT = {"first": 8, "last": 8, "free_count": 4}, {"tables": 32, "free_list": 32, "free_left": 4, "status": 4,
+                                                                     "workspace": 8}
+
+
+def test_release_refuses_tensors_that_overlap():
+    at = 1 << 40   # (no address is read)
+    size = {**RELEASE_IN, **RELEASE_OUT}
+    place = {f: at + 4096 * i for i, f in enumerate(size)}
+    for o in RELEASE_OUT:
+        for i, n in size.items():
+            for p in {place[i], place[i] + n - 4, place[i] - size[o] + 4}:
+                if i == o or (p == place[i] and {o, i} == {"free_left", "free_count"}):
+                    continue
+                w = {**place, o: p}
+                rc = _lib.lib().pa_page_release(w["first"], w["last"], 2, w["tables"], 4, 4, w["free_list"], w["free_count"], 8,
+                                                w["free_left"], w["status"], w["workspace"], None)
+                _refused(rc, "overlap")
