@@ -495,9 +495,10 @@ int pa_attn_bwd(const pa_attn_bwd_args* args, void* stream);
  *   4  more new tokens than rows (`tokens`)
  * and then nothing is taken: tables stay, lengths = before, q_start is all 0, the slots and
  * positions -1, *free_left = free_count.  lengths may be `before` and free_left may be
- * free_count; no other output overlaps an input.  A token whose page is none of the cache gets
- * slot -1.  Pages are not shared: a page is in one request's table or in the free list.
- * workspace: int32 [3 R + 2], not shared by calls that overlap.
+ * free_count; else tables and the outputs share no memory with each other or with an input.  A
+ * token whose page is none of the cache gets slot -1.  Pages are not shared: a page is in one
+ * request's table or in the free list.  workspace: int32 [3 R + 2], not shared by calls that
+ * overlap.
  *
  * pa_page_release: pages first[r] .. last[r] - 1 of request r's table (clamped to the table;
  * entries that are none of the cache are skipped) go back to the end of the free list in order

@@ -342,24 +342,16 @@ extern "C" int pa_page_tables(const pa_tables_args* x, void* stream) {
   PA_CHECK_ARG(x->n_pages == 0 || x->free_list, "pa_page_tables: null free_list");
   PA_CHECK_ARG(x->tokens == 0 || x->slots, "pa_page_tables: null slots");
   // (outputs are written beside reads of the inputs, by other work-groups too)
-  struct Span {
-    const char* name;
-    const int32_t* p;
-    int64_t n;
-  };
   const int64_t R = x->R;
-  const Span in[] = {{"before", x->before, R}, {"fresh", x->fresh, R}, {"free_list", x->free_list, x->n_pages},
-                     {"free_count", x->free_count, 1}, {"tables", x->tables, R ? (int64_t)((uint64_t)(R - 1) * (uint64_t)x->pitch) + x->cols : 0}};
-  const Span out[] = {{"lengths", x->lengths, R}, {"q_start", x->q_start, R + 1}, {"slots", x->slots, x->tokens},
-                      {"positions", x->positions, x->positions ? x->tokens : 0}, {"free_left", x->free_left, 1},
-                      {"status", x->status, 1}, {"workspace", x->workspace, 3 * R + 2}};
-  for (const Span& o : out)
-    for (const Span& i : in) {
-      if (o.p == i.p && ((o.p == x->lengths && i.p == x->before) || (o.p == x->free_left && i.p == x->free_count)) && o.n == i.n)
-        continue;
-      const uintptr_t a = reinterpret_cast<uintptr_t>(o.p), b = reinterpret_cast<uintptr_t>(i.p);
-      PA_CHECK_ARG(o.n == 0 || i.n == 0 || a + 4 * o.n <= b || b + 4 * i.n <= a, "pa_page_tables: %s and %s overlap", o.name, i.name);
-    }
+  if (int rc = check_apart("pa_page_tables", {{"before", flat(x->before, 4 * R)}, {"fresh", flat(x->fresh, 4 * R)},
+                                              {"free_list", flat(x->free_list, 4 * x->n_pages)}, {"free_count", flat(x->free_count, 4)}},
+                           {{"lengths", flat(x->lengths, 4 * R), "before"}, {"q_start", flat(x->q_start, 4 * (R + 1))},
+                            {"slots", flat(x->slots, 4 * x->tokens)},
+                            {"positions", flat(x->positions, x->positions ? 4 * x->tokens : 0)},
+                            {"free_left", flat(x->free_left, 4), "free_count"}, {"status", flat(x->status, 4)},
+                            {"workspace", flat(x->workspace, 4 * (3 * R + 2))},
+                            {"tables", tables_span(x->tables, x->R, x->pitch, x->cols)}}))
+    return rc;
   TablesK a;
   a.before = x->before;
   a.fresh = x->fresh;

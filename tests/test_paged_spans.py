@@ -179,3 +179,24 @@ def test_release_refuses_tensors_that_overlap():
                 rc = _lib.lib().pa_page_release(w["first"], w["last"], 2, w["tables"], 4, 4, w["free_list"], w["free_count"], 8,
                                                 w["free_left"], w["status"], w["workspace"], None)
                 _refused(rc, "overlap")
+
+
+TABLES_IN = {"before": 8, "fresh": 8, "free_list": 32, "free_count": 4}
+TABLES_OUT = {"lengths": 8, "q_start": 12, "slots": 40, "positions": 40, "free_left": 4, "status": 4, "workspace": 32, "tables": 32}
+
+
+def test_tables_refuse_tensors_that_overlap():
+    """Outputs and the tables, against each other and against the inputs."""
+    at = 1 << 40   # (no address is read)
+    size = {**TABLES_IN, **TABLES_OUT}
+    for o in TABLES_OUT:
+        for i, n in size.items():
+            for shift in {0, n - 4, 4 - size[o]}:
+                if i == o or (shift == 0 and {o, i} in ({"free_left", "free_count"}, {"lengths", "before"})):
+                    continue
+                a = _lib.PaTablesArgs()
+                for x, f in enumerate(size):
+                    setattr(a, f, at + 4096 * x)
+                a.R, a.n_pages, a.page_size, a.pitch, a.cols, a.tokens = 2, 8, 16, 4, 4, 10
+                setattr(a, o, getattr(a, i) + shift)
+                _refused(_lib.lib().pa_page_tables(ctypes.byref(a), None), "overlap")
