@@ -509,7 +509,8 @@ int pa_attn_bwd(const pa_attn_bwd_args* args, void* stream);
  *
  * pa_paged_append: row i of k_new / v_new [T, Hkv, D] (n_st, n_sh: token and head strides in
  * elements) is written to slot slots[i]; a slot outside the cache (-1) is skipped.  Slots are
- * distinct.
+ * distinct, and k_new, v_new are no rows that slots name.  The strides of k and v nest (taken from
+ * the smallest, each passes all the rows within it), k and v beside each other in one buffer too.
  *
  * pa_paged_attn: rows q_start[r] .. q_start[r + 1] - 1 of q [T, Hq, D] are request r's newest
  * tokens, at positions lengths[r] - n .. lengths[r] - 1.  Query head h reads KV head h / (Hq /

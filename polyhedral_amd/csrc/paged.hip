@@ -435,6 +435,20 @@ extern "C" int pa_paged_append(const void* k_new, const void* v_new, int64_t n_s
                "pa_paged_append: rows must be 16-byte aligned");
   PA_CHECK_ARG(n_st >= 0 && n_sh >= 0 && c_sp >= 0 && c_sh >= 0 && c_sn >= D, "pa_paged_append: negative strides, or rows closer than D");
   PA_CHECK_ARG((n_pages == 1 || c_sp >= D) && (Hkv == 1 || c_sh >= D), "pa_paged_append: pages or heads closer than D");
+  // K and V are written by different work-groups, a row by one: no two rows share a byte, within K, within
+  // V or between the two (which nest as one more dimension where they lie in one buffer, by the places in
+  // a page's pitch where these are some pages apart; k may be v where k_new is v_new)
+  const int64_t n4[] = {n_pages, Hkv, page_size, 2}, s4[] = {c_sp * esz, c_sh * esz, c_sn * esz, 0};
+  Strided<4> kv = strided<4>(k, D * esz, n4, s4);
+  const wide apart = strided<1>(v, 0, {1}, {0}).at - kv.at;
+  kv.s[3] = apart < 0 ? -apart : apart;
+  if (apart == 0 && k_new == v_new) kv.n[3] = 1;
+  bool ok = nested(kv);
+  if (!ok && kv.s[0] > 0) {
+    kv.s[3] %= kv.s[0];
+    ok = nested(kv);
+  }
+  PA_CHECK_ARG(ok, "pa_paged_append: rows of k and v overlap");
   const int upr_lg = (D * esz == 128) ? 3 : (D * esz == 256) ? 4 : 5;
   const int64_t units = (T * Hkv) << upr_lg, blocks = (units + 255) / 256;
   const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384), 2);

@@ -70,3 +70,29 @@ def test_outputs_that_share_memory_are_refused(gpu):
     both = torch.zeros(b.T, 4, 64, dtype=torch.float32, device=gpu)
     refused("o and lse", out=both.view(torch.float16)[..., :64], lse=both[..., 0])
     paged.attention(b.q, b.k, b.v, *b.dev(), pm.Causal(), lse=lse)
+
+
+@pytest.mark.parametrize("layout", ["[pages, 2, H, P, D]", "[pages, H, P, 2, D]", "[2, pages, H, P, D]", "[pages, P, 2, H, D]",
+                                    "[2 pages, H, P, D]", "v before k", "v a page on", "v two pages on", "k is v"])
+def test_append_into_one_buffer_of_keys_and_values(gpu, layout):
+    pages, H, P, D = 5, 3, 16, 64
+    order = {"[pages, 2, H, P, D]": (0, 4, 1, 2, 3), "[pages, H, P, 2, D]": (0, 1, 2, 4, 3), "[pages, P, 2, H, D]": (0, 2, 4, 1, 3),
+             "[2 pages, H, P, D]": (0, 4, 1, 2, 3)}.get(layout, (4, 0, 1, 2, 3))
+    sizes = (pages, H, P, D, 2)
+    buf = torch.zeros([sizes[i] for i in order], dtype=torch.float16, device=gpu)
+    kv = buf.permute([order.index(i) for i in (4, 0, 1, 2, 3)])
+    if layout.endswith("on"):
+        on = 1 if layout == "v a page on" else 2
+        buf = torch.zeros(pages + on, 2, H, P, D, dtype=torch.float16, device=gpu)
+        kv = buf[:pages, 0], buf[on:, 1]
+    k, v = (kv[1], kv[0]) if layout == "v before k" else (kv[0], kv[0 if layout == "k is v" else 1])
+    new = torch.randn(2, 7, H, D, device=gpu).half()
+    kn, vn = new[0], new[0 if layout == "k is v" else 1]
+    slots = torch.tensor([0, 17, -1, 79, 33, 5, 80], dtype=I32, device=gpu)
+    want = [torch.zeros(pages, H, P, D, dtype=torch.float16, device=gpu) for _ in range(2)]
+    for w, n in zip(want, (kn, vn)):
+        for i, s in enumerate(slots.tolist()):
+            if 0 <= s < pages * P:
+                w[s // P, :, s % P] = n[i]
+    paged.append(kn, vn, slots, k, v)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])

@@ -200,3 +200,17 @@ def test_tables_refuse_tensors_that_overlap():
                 a.R, a.n_pages, a.page_size, a.pitch, a.cols, a.tokens = 2, 8, 16, 4, 4, 10
                 setattr(a, o, getattr(a, i) + shift)
                 _refused(_lib.lib().pa_page_tables(ctypes.byref(a), None), "overlap")
+
+
+def test_append_refuses_a_cache_whose_rows_overlap():
+    at = 1 << 40   # (no address is read)
+
+    def append(sp, sh, sn, v, pages=4, P=16, H=2, same=False):
+        return _lib.lib().pa_paged_append(at, at if same else at + 4096, 256, 128, at + 8192, 3, at + 65536, at + 65536 + v, sp, sh,
+                                          sn, pages, P, H, 128, _lib.PA_BF16, None)
+    for args in ((4096, 128, 128, 1 << 20), (2048, 2048, 128, 1 << 20), (4096, 2048, 136, 1 << 20), (4096, 2048, 256, 1 << 20),
+                 (512, 256, 128, 1 << 20)):                     # (rows of a head on top of the next head's, and so on)
+        _refused(append(*args), "rows of k and v overlap")
+    for v in (0, 128, 256, 4096, -4096, 8192, 3 * 8192):        # k and v in one place, or some pages apart
+        _refused(append(4096, 2048, 128, v), "rows of k and v overlap")
+    _refused(append(4096, 128, 128, 0, same=True), "rows of k and v overlap")
