@@ -319,7 +319,7 @@ int check_apart(const char* who, std::initializer_list<Named> in, std::initializ
 int check_pages(const char* who, int64_t n_pages, int32_t page_size, int* page_lg) {
   *page_lg = page_lg_of(page_size);
   PA_CHECK_ARG(*page_lg >= 0, "%s: page_size=%d (16, 32, 64, 128 or 256)", who, page_size);
-  PA_CHECK_ARG(n_pages >= 0 && n_pages * page_size < (1ll << 31), "%s: n_pages=%lld (slots stay below 2^31)", who,
+  PA_CHECK_ARG(n_pages >= 0 && n_pages < (1ll << 31) && n_pages * page_size < (1ll << 31), "%s: n_pages=%lld (slots stay below 2^31)", who,
                (long long)n_pages);
   return PA_OK;
 }

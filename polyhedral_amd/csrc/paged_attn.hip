@@ -58,7 +58,7 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   PA_CHECK_ARG(x->D == 64 || x->D == 128, "pa_paged_attn: D=%d (64 or 128)", x->D);
   PA_CHECK_ARG(x->Hkv >= 1 && x->Hq >= x->Hkv && x->Hq % x->Hkv == 0 && x->Hq <= 65535,
                "pa_paged_attn: %d query heads and %d KV heads (a multiple, at most 65535)", x->Hq, x->Hkv);
-  PA_CHECK_ARG(x->R >= 0 && x->T >= 0 && x->T * x->Hq <= kMaxPosition, "pa_paged_attn: R=%d T=%lld Hq=%d (T Hq < 2^30)",
+  PA_CHECK_ARG(x->R >= 0 && x->T >= 0 && x->T <= kMaxPosition && x->T * x->Hq <= kMaxPosition, "pa_paged_attn: R=%d T=%lld Hq=%d (T Hq < 2^30)",
                x->R, (long long)x->T, x->Hq);
   PA_CHECK_ARG(x->max_fresh >= 0, "pa_paged_attn: max_fresh=%lld", (long long)x->max_fresh);
   PA_CHECK_ARG(x->cols >= 0 && ((int64_t)x->cols << p->page_lg) <= kMaxPosition && x->pitch >= x->cols,
@@ -74,7 +74,8 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   // rows of 16 requests, stride 16, over 8000 keys 74 us and 141, 96 rows 146 both.)
   const int span = (int)((kRows + G - 1) / G) + 1;
   const int64_t few_rows = 2 * span <= p->stride && G * p->stride / 2 > kFewRows ? (G * p->stride / 2 < kTileRows ? G * p->stride / 2 : kTileRows) : kFewRows;
-  p->tile = x->dtype != PA_F32 && x->n_pages > 0 && x->max_fresh * G > few_rows;
+  const int64_t most = x->max_fresh < x->T ? x->max_fresh : x->T;  // new tokens of a request
+  p->tile = x->dtype != PA_F32 && x->n_pages > 0 && most * G > few_rows;
   int64_t few = x->T * G / kRows + some;
   if (p->tile && few > some * ((few_rows + kRows - 1) / kRows)) few = some * ((few_rows + kRows - 1) / kRows);
   // (beside chunks too: 61 requests of a token and 3 chunks with 256 shares 232 us, with 512 177, with 1024
