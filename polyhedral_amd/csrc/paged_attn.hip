@@ -13,6 +13,9 @@ namespace {
 // and 200 of 64), 48 rows 28 and 31 (273 and 203), 64 rows 32 and 31 (330 and 210).
 constexpr int kFewRows = 32;
 
+// Work-groups of a launch: a grid of 256 threads each has less than 2^32 of them.
+constexpr int64_t kMaxGroups = 0xffffffffll / 256;
+
 // One in how many keys a mask leaves live for a token far from it: the stride of a mask's one lattice
 // when its other terms are bands (windows, sinks); 0 for any other mask.
 int stride_of(const pa_mask& m) {
@@ -42,7 +45,7 @@ struct PagedPlan {
 // -> 296 us of sinks in chunks, 15 -> 17 us of one token over 8000, by registers that the loop holds.)
 int part_of(const pa_paged_args* x, int BM, int shares, int64_t max_tiles, PagedPart* p) {
   const int64_t most = shares + max_tiles * x->Hkv;
-  PA_CHECK_ARG(most <= 0x3fffffffll, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)most);
+  PA_CHECK_ARG(most <= kMaxGroups, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)most);
   p->grid = (int32_t)most;
   p->slots = (int32_t)(2 * shares < most ? 2 * shares : most);
   p->by_shares = 1.0001f / (float)shares;
@@ -93,6 +96,8 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
     p->tiles.row_min = (int32_t)few_rows;
     p->tiles.row_max = INT_MAX;
   }
+  PA_CHECK_ARG((int64_t)p->rows.grid + p->tiles.grid <= kMaxGroups, "pa_paged_attn: %lld work-groups exceed the grid limit",
+               (long long)p->rows.grid + p->tiles.grid);
   p->zero = (4 * ((int64_t)p->rows.slots + p->tiles.slots) + 255) / 256 * 256;
   p->bytes = p->zero + 4ll * p->rows.slots * slot_floats(kRows, x->D) + 4ll * p->tiles.slots * slot_floats(kTileRows, x->D);
   return PA_OK;

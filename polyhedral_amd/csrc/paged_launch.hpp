@@ -36,7 +36,6 @@ void paged_both_kernel(const PagedK a) {
 template <typename T, int D>
 int launch_paged_t(const PagedK& a, hipStream_t s) {
   const int64_t grid = (int64_t)a.tiles.grid + a.rows.grid;
-  PA_CHECK_ARG(grid <= 0x7fffffffll, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)grid);
   if constexpr (sizeof(T) == 2) {
     if (a.tiles.grid) {
       hipLaunchKernelGGL((paged_both_kernel<T, D>), dim3((unsigned)grid), dim3(256), 0, s, a);

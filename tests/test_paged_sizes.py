@@ -39,3 +39,15 @@ def test_sizes_whose_products_pass_64_bits_are_refused():
 def test_a_hint_past_the_rows_is_the_rows(most):
     assert _workspace(max_fresh=most) == _workspace(max_fresh=300)
     assert _workspace(max_fresh=300) != _workspace(max_fresh=1)
+
+
+def test_more_work_groups_than_a_grid_has_are_refused():
+    """A launch has less than 2^32 threads, 256 of them a work-group: tokens of 2^21 requests, 8 KV heads."""
+    for dtype in (_lib.PA_F32, _lib.PA_BF16):
+        for most in (1, 1 << 20):
+            for n in (1 << 21, 1 << 24, (1 << 27) - 1):
+                _refused(_workspace(T=n, R=n, Hq=8, Hkv=8, max_fresh=most, dtype=dtype)[0], "grid limit")
+        assert _workspace(T=1 << 20, R=1 << 20, Hq=8, Hkv=8, max_fresh=1, dtype=dtype)[0] == 0
+    # each part within it, both together not
+    assert _workspace(T=1 << 20, R=1 << 20, Hq=11, Hkv=11, max_fresh=1)[0] == 0
+    _refused(_workspace(T=1 << 20, R=1 << 20, Hq=11, Hkv=11, max_fresh=100)[0], "grid limit")
