@@ -177,17 +177,22 @@ def release(first, last, tables, free_list, free_count, out=None):
     return prepare_release(first, last, tables, free_list, free_count, out)()
 
 
+def _strides(t):
+    """The strides of all dimensions but the last; 0 where there is one entry, which no step leaves."""
+    return tuple(s if n > 1 else 0 for n, s in zip(t.shape, t.stride()[:-1]))
+
+
 def _cache(k, v):
     """The checked shape (pages, heads, page_size, D) of a cache's tensors."""
     _lib.require_device(k, v)
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride() or k.device != v.device:
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or _strides(k) != _strides(v) or k.device != v.device:
         raise ValueError("k and v must be [pages, heads, page_size, D] of one shape, dtype, strides and device")
     _lib.dtype_code(k)
     pages, H, P, D = k.shape
     _page_size(P)
     if D not in (64, 128):
         raise ValueError(f"D={D} (64 or 128)")
-    if k.numel() and k.stride(3) != 1:
+    if k.numel() and (k.stride(3) != 1 or v.stride(3) != 1):
         raise ValueError("the cache needs a unit stride in its last dimension")
     return pages, H, P, D
 
@@ -202,19 +207,18 @@ def _rows(t, name, shape, like):
 
 
 def prepare_append(k_new, v_new, slots, k, v):
-    """A PagedLaunch that writes k_new, v_new [tokens, heads, D] to their slots (int32 [tokens],
-    distinct; a slot outside the cache, as -1, is skipped) of k, v [pages, heads, page_size, D];
-    its result is (k, v)."""
+    """A PagedLaunch that writes k_new, v_new [tokens, heads, D] (of the same strides, and no rows that
+    slots name) to their slots (int32 [tokens], distinct; a slot outside the cache, as -1, is skipped)
+    of k, v [pages, heads, page_size, D], whose rows do not overlap; its result is (k, v)."""
     pages, H, P, D = _cache(k, v)
     T = k_new.shape[0]
     _rows(k_new, "k_new", (T, H, D), k)
     _rows(v_new, "v_new", (T, H, D), k)
-    if k_new.stride() != v_new.stride():
+    if _strides(k_new) != _strides(v_new):
         raise ValueError("k_new and v_new must share strides")
     _ints(slots, "slots", (T,), k.device)
     p = _lib.ptr
-    args = (p(k_new), p(v_new), k_new.stride(0), k_new.stride(1), p(slots), T, p(k), p(v), *k.stride()[:3], pages, P, H, D,
-            _lib.dtype_code(k))
+    args = (p(k_new), p(v_new), *_strides(k_new), p(slots), T, p(k), p(v), *_strides(k), pages, P, H, D, _lib.dtype_code(k))
     return PagedLaunch("pa_paged_append", args, [k_new, v_new, slots, k, v], k, (k, v))
 
 
@@ -278,15 +282,15 @@ def prepare_attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_f
     _rows(o, "out", (T, Hq, D), k)
     a = _lib.PaPagedArgs()
     ptr = _lib.address
-    a.q, a.q_st, a.q_sh = ptr(q), q.stride(0), q.stride(1)
+    a.q, (a.q_st, a.q_sh) = ptr(q), _strides(q)
     a.k, a.v = ptr(k), ptr(v)
-    a.c_sp, a.c_sh, a.c_sn = k.stride()[:3]
+    a.c_sp, a.c_sh, a.c_sn = _strides(k)
     a.n_pages, a.page_size = pages, P
     a.tables, a.pitch, a.cols = ptr(tables), pitch, tables.shape[1]
     a.lengths, a.q_start, a.R, a.T, a.max_fresh = ptr(lengths), ptr(q_start), R, T, min(max_fresh, T)
     a.Hq, a.Hkv, a.D, a.dtype, a.scale = Hq, Hkv, D, _lib.dtype_code(q), scale
     a.mask = dm.struct()
-    a.o, a.o_st, a.o_sh = ptr(o), o.stride(0), o.stride(1)
+    a.o, (a.o_st, a.o_sh) = ptr(o), _strides(o)
     if lse is not None:
         _lib.require_device(lse)
         if lse.dtype != torch.float32 or lse.shape != (T, Hq) or lse.device != dev:

@@ -96,3 +96,33 @@ def test_append_into_one_buffer_of_keys_and_values(gpu, layout):
                 w[s // P, :, s % P] = n[i]
     paged.append(kn, vn, slots, k, v)
     assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+def test_strides_of_one_entry_do_not_matter(gpu):
+    """One token, one head or one page: whatever stride its dimension has."""
+    H, P, D = 2, 16, 64
+    k, v = (torch.zeros(4, H, P, D, dtype=torch.float16, device=gpu) for _ in range(2))
+    fused = torch.randn(2, 3 * H * D + 5, device=gpu).half()
+    part = lambda i: fused.as_strided((1, H, D), (3 * H * D + 5, D, 1), i * H * D)  # noqa: E731
+    slot = torch.tensor([20], dtype=I32, device=gpu)
+    # k_new a part of a row whose pitch is no multiple of 16 bytes, v_new a tensor of its own
+    kn, vn = part(1), torch.randn(1, H, D, device=gpu).half()
+    assert kn.stride() != vn.stride()
+    paged.append(kn, vn, slot, k, v)
+    assert torch.equal(k[1, :, 4], kn[0]) and torch.equal(v[1, :, 4], vn[0]) and int((k != 0).any(-1).sum()) == H
+    # one head
+    two = torch.randn(3, 2, D, device=gpu).half()
+    k1, v1 = (torch.zeros(4, 1, P, D, dtype=torch.float16, device=gpu) for _ in range(2))
+    paged.append(two.as_strided((3, 1, D), (2 * D, 5, 1)), two[:, 1:], torch.tensor([1, 2, 3], dtype=I32, device=gpu), k1, v1)
+    assert torch.equal(k1[0, 0, 1:4], two[:, 0]) and torch.equal(v1[0, 0, 1:4], two[:, 1])
+    # one page and one token: its query heads in a row of the fused projection, of an odd pitch
+    q = part(0)
+    page_k = k.as_strided((1, H, P, D), (1, P * D, D, 1), H * P * D)
+    page_v = v[1:2]
+    i32 = lambda *x: torch.tensor(x, dtype=I32, device=gpu)  # noqa: E731
+    args = (torch.zeros(1, 1, dtype=I32, device=gpu), i32(5), i32(0, 1), pm.SlidingWindow(1))
+    out = torch.empty(H * D, dtype=torch.float16, device=gpu).as_strided((1, H, D), (H * D + 3, D, 1))
+    assert torch.equal(paged.attention(q, page_k, page_v, *args, out=out), vn) and out.stride() != vn.stride()
+    # strides that do count are still compared
+    with pytest.raises(ValueError, match="share strides"):
+        paged.append(two, two.transpose(0, 1).contiguous().transpose(0, 1), i32(1, 2, 3), k, v)
