@@ -1,5 +1,6 @@
 """Calls that the paged cache's documentation allows (polyhedral_amd.paged), beside those of
 tests/test_gpu_paged.py."""
+import numpy as np
 import pytest
 import torch
 
@@ -126,3 +127,24 @@ def test_strides_of_one_entry_do_not_matter(gpu):
     # strides that do count are still compared
     with pytest.raises(ValueError, match="share strides"):
         paged.append(two, two.transpose(0, 1).contiguous().transpose(0, 1), i32(1, 2, 3), k, v)
+
+
+# ---- what is out of range ---------------------------------------------------------------------------
+def test_lengths_and_starts_out_of_range_are_clamped(gpu):
+    """Lengths to what the table reaches, starts to the rows there are and to those before them."""
+    b = Batch(gpu, torch.bfloat16, 128, 16, 4, 2, [(2, 50), (1, 30), (40, 90)], pad=0)
+    cols = b.tables.shape[1]
+    for lengths, starts in (([1 << 30, -5, 90], [0, 2, 3, 43]), ([50, 30, 90], [0, 100, 3, 1 << 30]), ([1, 0, 1], [0, 2, 3, 43]),
+                            ([50, 30, 90], [-9, 2, 1, 43]), ([50, 30, 90], [5, 7, 8, 20])):
+        b.lengths = np.array(lengths)
+        b.q_start = np.array(starts)
+        o, lse = b.run(pm.Causal())
+        s = np.maximum.accumulate(np.clip(starts, 0, b.T))
+        c = Batch(gpu, torch.bfloat16, 128, 16, 4, 2, [(2, 50), (1, 30), (40, 90)], pad=0)
+        c.lengths, c.q_start = np.clip(lengths, 0, cols * 16), s
+        want, wl = c.run(pm.Causal())
+        assert torch.equal(torch.nan_to_num(o.float()), torch.nan_to_num(want.float())) and torch.equal(lse.isnan(), wl.isnan())
+        assert torch.equal(torch.nan_to_num(lse), torch.nan_to_num(wl))
+        outside = torch.ones(b.T, dtype=torch.bool, device=gpu)
+        outside[int(s[0]):int(s[-1])] = False
+        assert (o[outside] == 7).all() and (lse[outside] == 7).all()
