@@ -74,13 +74,22 @@ def _single(kind, p0, p1, p2):
     return MaskSpec(((kind, p0, p1, p2),))
 
 
+FAR = (1 << 30) - 1   # no distance of two positions passes it
+
+
+def _parameter(p):
+    """A term's parameter as the int32 of a pa_term, that would wrap round: what passes it is as far
+    as any distance, what is below 0 stays so (and is refused)."""
+    return FAR if p > 0x7fffffff else max(p, -(1 << 31))
+
+
 @lru_cache(maxsize=256)
 def _term_struct(include, exclude):
     """A pa_mask of these terms, without tables (copied by DeviceMask.struct)."""
     m = _lib.PaMask()
     m.n_include, m.n_exclude = len(include), len(exclude)
     for i, t in enumerate(include + exclude):
-        m.terms[i] = _lib.PaTerm(*t)
+        m.terms[i] = _lib.PaTerm(t[0], *map(_parameter, t[1:]))
     return m
 
 
