@@ -309,6 +309,15 @@ def attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_fresh=Non
     return prepare_attention(q, k, v, tables, lengths, q_start, mask, scale, max_fresh, out, lse)()
 
 
+def _on_device(values, dtype, device):
+    """A list's values on the device, through pinned memory that its allocator keeps until they have been
+    read: the host does not wait."""
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("values from the host have no place in a graph's capture: give a tensor on the device")
+        return torch.as_tensor(values, dtype=dtype).pin_memory().to(device, non_blocking=True)
+
+
 class PagedKVCache:
     """Keys and values of up to ``requests`` requests at once, for ``layers`` layers that share
     their tables: k, v [layers, pages, heads, page_size, D].
@@ -346,8 +355,8 @@ class PagedKVCache:
 
     def begin(self, fresh, tokens=None):
         """Room for fresh[r] more tokens of every request (int32 [requests] on the device, or a list
-        of counts), packed into ``tokens`` rows (default, for a list: their sum; rows beyond are
-        padding).  Returns the TableStep; lengths count the new tokens from here on.  A step that
+        of counts, which a graph's capture does not take), packed into ``tokens`` rows (default, for a
+        list: their sum; rows beyond are padding).  Returns the TableStep; lengths count the new tokens from here on.  A step that
         does not fit (pages, max_length, rows) takes nothing, gives no row a slot, and shows in
         step.status and ``check``."""
         most = None
@@ -355,7 +364,7 @@ class PagedKVCache:
             fresh = [int(f) for f in fresh]
             most = max(fresh, default=0)
             tokens = sum(fresh) if tokens is None else tokens
-            fresh = torch.tensor(fresh, dtype=torch.int32, device=self.device)
+            fresh = _on_device(fresh, torch.int32, self.device)
         if tokens is None:
             raise ValueError("tokens (the rows of the packed step) is needed with counts on the device")
         _ints(fresh, "fresh", (self.requests,), self.device)
@@ -386,9 +395,11 @@ class PagedKVCache:
             self.failed |= status * LIST_FULL
 
     def finish(self, done):
-        """Gives back the pages of the requests where done (bool [requests], on the device or a list)
-        is true and sets their lengths to 0."""
-        done = torch.as_tensor(done, dtype=torch.bool, device=self.device)
+        """Gives back the pages of the requests where done (bool [requests], on the device, or a list,
+        which a graph's capture does not take) is true and sets their lengths to 0."""
+        if not (isinstance(done, torch.Tensor) and done.is_cuda):
+            done = _on_device(done, torch.bool, self.device)
+        done = done.to(device=self.device, dtype=torch.bool)
         if done.shape != (self.requests,):
             raise ValueError(f"done must be [{self.requests}], got {list(done.shape)}")
         with torch.cuda.device(self.device):

@@ -148,3 +148,41 @@ def test_lengths_and_starts_out_of_range_are_clamped(gpu):
         outside = torch.ones(b.T, dtype=torch.bool, device=gpu)
         outside[int(s[0]):int(s[-1])] = False
         assert (o[outside] == 7).all() and (lse[outside] == 7).all()
+
+
+# ---- what waits for the device ----------------------------------------------------------------------
+def test_counts_in_a_list_do_not_wait_for_the_device(gpu):
+    """begin and finish return while the work before them still runs, and take the counts they were given
+    even where the same memory is given again before the device has read it."""
+    cache = paged.PagedKVCache(3, 256, 60, 1, 64, torch.float16, 16, device=gpu)
+    cache.begin([1, 0, 2])
+    cache.finish([False, True, False])
+    a = torch.randn(8192, 8192, device=gpu).bfloat16()
+    out = torch.empty_like(a)
+    torch.mm(a, a, out=out)
+    torch.cuda.synchronize()
+    for _ in range(40):
+        torch.mm(a, a, out=out)
+    done = torch.cuda.Event()
+    done.record()
+    steps = [cache.begin([i, 2 * i, 1]) for i in range(8)]
+    cache.finish([False, True, False])
+    cache.begin([0, 7, 0])
+    waited = done.query()
+    torch.cuda.synchronize()
+    assert not waited
+    assert cache.lengths.tolist() == [1 + 28, 7, 2 + 8]
+    assert [s.q_start.tolist() for s in steps] == [[0, i, 3 * i, 3 * i + 1] for i in range(8)]
+    cache.check()
+
+
+def test_counts_in_a_list_are_refused_in_a_capture(gpu):
+    """A graph would replay the copy of memory that has gone on to other uses."""
+    cache = paged.PagedKVCache(2, 64, 8, 1, 64, torch.float16, 16, device=gpu)
+    for call in (lambda: cache.begin([1, 1]), lambda: cache.finish([True, False])):
+        with pytest.raises(RuntimeError, match="capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        torch.cuda.synchronize()
+    cache.begin([1, 1])
+    assert cache.lengths.tolist() == [1, 1]
