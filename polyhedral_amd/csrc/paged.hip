@@ -441,14 +441,15 @@ extern "C" int pa_paged_append(const void* k_new, const void* v_new, int64_t n_s
   PA_CHECK_ARG((n_pages == 1 || c_sp >= D) && (Hkv == 1 || c_sh >= D), "pa_paged_append: pages or heads closer than D");
   // K and V are written by different work-groups, a row by one: no two rows share a byte, within K, within
   // V or between the two (which nest as one more dimension where they lie in one buffer, by the places in
-  // a page's pitch where these are some pages apart; k may be v where k_new is v_new)
+  // a page's pitch where pages lie outermost and these are some pages apart; k may be v where k_new is
+  // v_new)
   const int64_t n4[] = {n_pages, Hkv, page_size, 2}, s4[] = {c_sp * esz, c_sh * esz, c_sn * esz, 0};
   Strided<4> kv = strided<4>(k, D * esz, n4, s4);
   const wide apart = strided<1>(v, 0, {1}, {0}).at - kv.at;
   kv.s[3] = apart < 0 ? -apart : apart;
   if (apart == 0 && k_new == v_new) kv.n[3] = 1;
   bool ok = nested(kv);
-  if (!ok && kv.s[0] > 0) {
+  if (!ok && kv.s[0] > 0 && (Hkv == 1 || kv.s[0] >= kv.s[1]) && kv.s[0] >= kv.s[2]) {
     kv.s[3] %= kv.s[0];
     ok = nested(kv);
   }

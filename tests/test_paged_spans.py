@@ -214,3 +214,16 @@ def test_append_refuses_a_cache_whose_rows_overlap():
     for v in (0, 128, 256, 4096, -4096, 8192, 3 * 8192):        # k and v in one place, or some pages apart
         _refused(append(4096, 2048, 128, v), "rows of k and v overlap")
     _refused(append(4096, 128, 128, 0, same=True), "rows of k and v overlap")
+
+
+def test_append_refuses_values_on_the_next_heads_keys():
+    """Heads outermost, a page's pitch of two pages: v a page and a half on lies between the pages of its own
+    head, but on the keys of the next head, which start at an odd half."""
+    at, page = 1 << 40, 16 * 256
+    pages, sp = 5, 2 * page
+
+    def append(v, sh):
+        return _lib.lib().pa_paged_append(at, at + 4096, 256, 128, at + 8192, 3, at + (1 << 20), at + (1 << 20) + v, sp // 2, sh // 2,
+                                          128, pages, 16, 2, 128, _lib.PA_BF16, None)
+    _refused(append(page + pages * sp, pages * sp + page), "rows of k and v overlap")
+    _refused(append(-page - pages * sp, pages * sp + page), "rows of k and v overlap")
