@@ -518,14 +518,16 @@ int pa_attn_bwd(const pa_attn_bwd_args* args, void* stream);
  * at positions; any kind but PA_DENSE, perm_q / perm_kv NULL) of scale q . k_t, applied to
  * v_t; a row with no live key gives 0 and lse -inf.  Keys that are dead for a row contribute
  * nothing to it, whatever their K and V hold; a live key whose page is none of the cache
- * counts as dead.  A length below 0 or past cols * page_size counts as that, a start below 0 or past
- * T too, and one below an earlier start as the earlier one.  Rows of no request are left as they are.  lse may be NULL (natural log,
- * [T, Hq] at lse_st, lse_sh).  max_fresh: the most new tokens of a request (a hint: it selects
- * kernels and moves no result beyond rounding).  D = 64 or 128, f32 / f16 / bf16, scale > 0.
+ * counts as dead.  A length below 0 counts as 0 and one past cols * page_size as that; a start
+ * below 0 as 0, one past T as T, and one below an earlier start as the earlier one.  Rows of no
+ * request are left as they are.  lse may be NULL (natural log, [T, Hq] at lse_st, lse_sh).
+ * max_fresh: the most new tokens of a request (a hint: it selects kernels and moves no result
+ * beyond rounding).  D = 64 or 128, f32 / f16 / bf16, scale > 0.
  * o, lse and the workspace share no byte with an input or with each other, and no two rows of o or
  * of lse do (parts of one buffer's rows may be q and o in turn, or o and lse).  workspace: the bytes
- * pa_paged_workspace gives for the same sizes, hint, type and mask (no pointer is read), 256-byte aligned, the first zero_bytes of them zero before
- * the first call with it and left zero by every call of these; not shared by calls that overlap. */
+ * pa_paged_workspace gives for the same sizes, hint, type and mask (no pointer is read), 256-byte
+ * aligned, the first zero_bytes of them zero before the first call with it and left zero by every
+ * call of these; not shared by calls that overlap. */
 typedef struct pa_tables_args {
   const int32_t* before;
   const int32_t* fresh;

@@ -14,15 +14,15 @@ struct Strided {
   int64_t n[N];
   wide s[N];
 };
-// (strides of either sign: the same rows counted backwards)
+// (strides in units of `unit` bytes, of either sign: the same rows counted backwards)
 template <int N>
-inline Strided<N> strided(const void* p, int64_t w, const int64_t (&n)[N], const int64_t (&s)[N]) {
+inline Strided<N> strided(const void* p, int64_t w, const int64_t (&n)[N], const int64_t (&s)[N], int unit = 1) {
   Strided<N> x;
   x.at = (wide) reinterpret_cast<uintptr_t>(p);
   x.w = w;
   for (int i = 0; i < N; ++i) {
     x.n[i] = n[i];
-    x.s[i] = s[i] < 0 ? -(wide)s[i] : s[i];
+    x.s[i] = (s[i] < 0 ? -(wide)s[i] : s[i]) * unit;
     if (s[i] < 0 && n[i] > 0) x.at -= (n[i] - 1) * x.s[i];
   }
   return x;

@@ -304,7 +304,7 @@ struct Named {
   const char* same = "";  // an input that this output may be
 };
 Strided<1> tables_span(const int32_t* tables, int32_t R, int64_t pitch, int32_t cols) {
-  return strided<1>(tables, 4ll * cols, {cols ? R : 0}, {4 * pitch});
+  return strided<1>(tables, 4ll * cols, {cols ? R : 0}, {pitch}, 4);
 }
 int check_apart(const char* who, std::initializer_list<Named> in, std::initializer_list<Named> out) {
   for (const Named& o : out) {
@@ -443,8 +443,7 @@ extern "C" int pa_paged_append(const void* k_new, const void* v_new, int64_t n_s
   // V or between the two (which nest as one more dimension where they lie in one buffer, by the places in
   // a page's pitch where pages lie outermost and these are some pages apart; k may be v where k_new is
   // v_new)
-  const int64_t n4[] = {n_pages, Hkv, page_size, 2}, s4[] = {c_sp * esz, c_sh * esz, c_sn * esz, 0};
-  Strided<4> kv = strided<4>(k, D * esz, n4, s4);
+  Strided<4> kv = strided<4>(k, D * esz, {n_pages, Hkv, page_size, 2}, {c_sp, c_sh, c_sn, 0}, (int)esz);
   const wide apart = strided<1>(v, 0, {1}, {0}).at - kv.at;
   kv.s[3] = apart < 0 ? -apart : apart;
   if (apart == 0 && k_new == v_new) kv.n[3] = 1;

@@ -105,17 +105,18 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
 
 // Work-groups write o, lse and the workspace while others read the inputs: no two of them, and no two
 // rows of o or lse, share a byte.  (Heads of one buffer may be q and o in turn.)
-int check_overlaps(const pa_paged_args* x, int64_t esz, int64_t workspace) {
-  const int64_t P = x->page_size, es = esz;
-  const Strided<2> o = strided<2>(x->o, x->D * es, {x->T, x->Hq}, {x->o_st * es, x->o_sh * es});
-  const Strided<2> q = strided<2>(x->q, x->D * es, {x->T, x->Hq}, {x->q_st * es, x->q_sh * es});
-  const Strided<2> lse = strided<2>(x->lse, 4, {x->lse ? x->T : 0, x->Hq}, {4 * x->lse_st, 4 * x->lse_sh});
+int check_overlaps(const pa_paged_args* x, int esz, int64_t workspace) {
+  const int64_t row = x->D * esz;
+  const Strided<2> o = strided<2>(x->o, row, {x->T, x->Hq}, {x->o_st, x->o_sh}, esz);
+  const Strided<2> q = strided<2>(x->q, row, {x->T, x->Hq}, {x->q_st, x->q_sh}, esz);
+  const Strided<2> lse = strided<2>(x->lse, 4, {x->lse ? x->T : 0, x->Hq}, {x->lse_st, x->lse_sh}, 4);
   PA_CHECK_ARG(!overlaps_itself(o), "pa_paged_attn: rows of o overlap");
   PA_CHECK_ARG(!overlaps_itself(lse), "pa_paged_attn: rows of lse overlap");
-  const int64_t pages[] = {x->n_pages, x->Hkv, P}, steps[] = {x->c_sp * es, x->c_sh * es, x->c_sn * es};
-  const Strided<3> k = strided<3>(x->k, x->D * es, pages, steps), v = strided<3>(x->v, x->D * es, pages, steps);
-  const Strided<1> lengths = flat(x->lengths, 4ll * x->R), starts = flat(x->q_start, 4ll * (x->R + 1ll)), ws = flat(x->workspace, workspace);
-  const Strided<1> tables = strided<1>(x->tables, 4ll * x->cols, {x->cols ? x->R : 0}, {4 * x->pitch});
+  const int64_t pages[] = {x->n_pages, x->Hkv, x->page_size}, steps[] = {x->c_sp, x->c_sh, x->c_sn};
+  const Strided<3> k = strided<3>(x->k, row, pages, steps, esz), v = strided<3>(x->v, row, pages, steps, esz);
+  const Strided<1> tables = strided<1>(x->tables, 4ll * x->cols, {x->cols ? x->R : 0}, {x->pitch}, 4);
+  const Strided<1> lengths = flat(x->lengths, 4ll * x->R), starts = flat(x->q_start, 4ll * (x->R + 1ll));
+  const Strided<1> ws = flat(x->workspace, workspace);
   auto apart = [&](const char* name, const auto& out) {
     const char* other = overlap(out, q) ? "q" : overlap(out, k) ? "k" : overlap(out, v) ? "v" : overlap(out, tables) ? "tables"
                         : overlap(out, lengths) ? "lengths" : overlap(out, starts) ? "q_start" : nullptr;
@@ -163,7 +164,7 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
                "pa_paged_attn: negative strides, or cache rows closer than D or further than 2^21");
   PA_CHECK_ARG(x->workspace && reinterpret_cast<uintptr_t>(x->workspace) % 256 == 0 && x->workspace_bytes >= p.bytes,
                "pa_paged_attn: needs a 256-byte aligned workspace of %lld bytes", (long long)p.bytes);
-  if (int rc = check_overlaps(x, esz, p.bytes)) return rc;
+  if (int rc = check_overlaps(x, (int)esz, p.bytes)) return rc;
   PagedK a;
   a.q = static_cast<const char*>(x->q);
   a.q_st = x->q_st * esz;

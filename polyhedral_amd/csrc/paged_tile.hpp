@@ -29,10 +29,10 @@
 //
 // What bounds it: for long lists at D = 128 power (2000 new tokens of 30001, 32 heads on 8, bf16: 873
 // to 993 us from card to card, 0.96 to 1.09 PFLOP/s of the 1.07 to 1.12 of a large library product; the
-// clock falls to 1.6 to 1.8 GHz with the matrix cores busy 52 to 54% of it), at D = 64 the exponentials' issue (4096 of 4096, 32 heads:
-// 104 us, 660 TFLOP/s), and for lists of a few steps what is outside them: 5 to 9 us a unit, two units
-// a CU (chunks of 1000 to 4096 under a window of 1024 and 64 sinks, 18 steps a unit: 262 to 289 us, 735
-// to 810 TFLOP/s).
+// clock falls to 1.6 to 1.8 GHz with the matrix cores busy 52 to 54% of it), at D = 64 the exponentials'
+// issue (4096 of 4096, 32 heads: 104 us, 660 TFLOP/s), and for lists of a few steps what is outside them:
+// 5 to 9 us a unit, two units a CU (chunks of 1000 to 4096 under a window of 1024 and 64 sinks, 18 steps a
+// unit: 262 to 289 us, 735 to 810 TFLOP/s).
 #pragma once
 
 #include <math.h>

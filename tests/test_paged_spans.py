@@ -124,12 +124,12 @@ ATTENTION = ("q", "k", "v", "tables", "lengths", "q_start", "o", "lse", "workspa
 
 
 def _attention(at, **change):
-    """T = 3 rows of 4 heads of 128 bf16, 2 KV heads, 4 pages of 16, each tensor 64 KiB from the next."""
+    """T = 5 rows of 4 heads of 128 bf16, 2 KV heads, 4 pages of 16, each tensor 64 KiB from the next."""
     a = _lib.PaPagedArgs()
     for i, f in enumerate(ATTENTION):
         setattr(a, f, at + i * 65536)
     a.q_st, a.q_sh, a.o_st, a.o_sh, a.c_sp, a.c_sh, a.c_sn, a.lse_st, a.lse_sh = 512, 128, 512, 128, 4096, 2048, 128, 4, 1
-    a.n_pages, a.page_size, a.pitch, a.cols, a.R, a.T, a.max_fresh = 4, 16, 4, 4, 2, 3, 2
+    a.n_pages, a.page_size, a.pitch, a.cols, a.R, a.T, a.max_fresh = 4, 16, 4, 4, 2, 5, 2
     a.Hq, a.Hkv, a.D, a.dtype, a.scale = 4, 2, 128, _lib.PA_BF16, 0.1
     a.mask.n_include = 1
     a.workspace_bytes = 1 << 40
@@ -149,7 +149,7 @@ def test_attention_refuses_outputs_whose_rows_overlap():
 @pytest.mark.parametrize("out", ["o", "lse", "workspace"])
 def test_attention_refuses_outputs_that_overlap_others(out):
     at = 1 << 40
-    size = {"q": 3072, "k": 32768, "v": 32768, "tables": 32, "lengths": 8, "q_start": 12, "o": 3072, "lse": 48}
+    size = {"q": 5120, "k": 32768, "v": 32768, "tables": 32, "lengths": 8, "q_start": 12, "o": 5120, "lse": 80}
     for f, n in size.items():
         if f == out:
             continue
@@ -227,3 +227,15 @@ def test_append_refuses_values_on_the_next_heads_keys():
                                           128, pages, 16, 2, 128, _lib.PA_BF16, None)
     _refused(append(page + pages * sp, pages * sp + page), "rows of k and v overlap")
     _refused(append(-page - pages * sp, pages * sp + page), "rows of k and v overlap")
+
+
+def test_strides_past_64_bits_are_not_taken_for_short_ones():
+    """A pitch or stride whose bytes pass 64 bits: all above the first row is its span."""
+    at = 1 << 40
+    a = _lib.PaTablesArgs()
+    for x, f in enumerate(["tables", *TABLES_IN, *(f for f in TABLES_OUT if f != "tables")]):
+        setattr(a, f, at + 4096 * x)
+    a.R, a.n_pages, a.page_size, a.pitch, a.cols, a.tokens = 2, 8, 16, 1 << 62, 4, 10
+    _refused(_lib.lib().pa_page_tables(ctypes.byref(a), None), "and tables overlap")
+    for change in (dict(c_sp=1 << 61), dict(q_st=1 << 60), dict(pitch=1 << 62)):
+        _refused(_attention(at, **change), "overlap")
