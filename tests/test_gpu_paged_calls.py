@@ -186,3 +186,71 @@ def test_counts_in_a_list_are_refused_in_a_capture(gpu):
         torch.cuda.synchronize()
     cache.begin([1, 1])
     assert cache.lengths.tolist() == [1, 1]
+
+
+def test_captured_finish_and_trim(gpu):
+    """A whole round of a server in one graph, finish and trim with masks on the device among it, on a
+    stream of its own; replays against a second cache stepped eagerly."""
+    R, H, D, P = 5, 2, 64, 16
+    mask = pm.SinksWindow(3, 40)
+    a, e = (paged.PagedKVCache(R, 400, 100, H, D, torch.bfloat16, P, 1, gpu) for _ in range(2))
+    gen, rng = torch.Generator().manual_seed(3), np.random.default_rng(3)
+    T = 30
+    fresh, done = torch.zeros(R, dtype=I32, device=gpu), torch.zeros(R, dtype=torch.bool, device=gpu)
+    kn, vn, q = (torch.zeros(T, n, D, dtype=torch.bfloat16, device=gpu) for n in (H, H, 2 * H))
+    oa, oe = (torch.zeros(T, 2 * H, D, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+
+    def a_round(cache, out):
+        cache.finish(done)
+        step = cache.begin(fresh, T)
+        cache.append(kn, vn, step)
+        cache.attend(q, mask, step, out=out)
+        cache.trim(40, 3)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        a_round(a, oa)
+    for i in range(30):
+        n = rng.integers(0, 6, R)
+        fresh.copy_(torch.as_tensor(n, dtype=I32))
+        done.copy_(torch.as_tensor(rng.random(R) < 0.15))
+        for x in (kn, vn, q):
+            x.copy_(torch.randn(x.shape, generator=gen))
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            graph.replay()
+        a_round(e, oe)
+        torch.cuda.current_stream().wait_stream(stream)
+        for x, y in ((a.tables, e.tables), (a.lengths, e.lengths), (a.free_count, e.free_count), (oa, oe)):
+            assert torch.equal(x, y), i
+        used = a.tables.cpu().numpy()
+        used = used[used >= 0]
+        free = a.free_list.cpu().numpy()[:int(a.free_count)]
+        assert sorted(np.concatenate([used, free]).tolist()) == list(range(a.pages)), i
+    a.check()
+    e.check()
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float16, 1), (torch.bfloat16, 40), (torch.float32, 2)])
+def test_millions_of_tokens(gpu, dtype, n):
+    """One request of 3 million tokens whose keys are all alike: the mean of its values, row by row."""
+    L, P, D, G = 3_000_001, 256, 64, 4
+    pages = -(-L // P)
+    k = torch.ones(pages, 1, P, D, dtype=dtype, device=gpu)
+    v = torch.randn(pages, 1, P, D, device=gpu).add_(1.0).to(dtype)
+    perm = torch.randperm(pages, device=gpu)
+    q = torch.randn(n, G, D, device=gpu).to(dtype)
+    lse = torch.zeros(n, G, device=gpu)
+    o = paged.attention(q, k, v, perm[None].to(I32), torch.tensor([L], dtype=I32, device=gpu),
+                        torch.tensor([0, n], dtype=I32, device=gpu), pm.Causal(), lse=lse)
+    rows = v[perm].reshape(-1, D).double()
+    # every P is the same, 1 but for the rounding of its maximum in log2 units (2^-21 of it), which all sums
+    # share; O and the sum of P are two chains of at most 2^11 additions, in a share and over the shares, each
+    # off by 2^-24 of what is summed: 2^-12 in all; scores by (D + 2) 2^-24 of their terms
+    for i in range(n):
+        m = L - n + i + 1
+        want, mass = rows[:m].mean(0), rows[:m].abs().mean(0)
+        u = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+        assert ((o[i].double() - want).abs() <= 1.01 * u * want.abs() + 2.0 ** -11 * mass).all(), i   # (O and its divisor)
+        x = q[i].double().sum(-1) * D ** -0.5
+        terms = q[i].double().abs().sum(-1).max() * D ** -0.5
+        assert (lse[i].double() - x - np.log(m)).abs().max() <= 2.0 ** -12 + (D + 2) * 2.0 ** -24 * terms
