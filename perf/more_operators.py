@@ -334,8 +334,7 @@ def run(state):
     if own:
         for call in state["call"]:
             done = call()
-        return {"attn": (state["o"], state["lse"]), "weights": state["scores"], "choose": done,
-                "evict": tuple(state.get(x) for x in ("k", "v", "scores"))}[op]
+        return (state["o"], state["lse"]) if op == "attn" else done
     return {"attn": _plain_attention, "weights": _plain_weights, "choose": _plain_choose, "evict": _plain_evict}[op](state)
 
 
