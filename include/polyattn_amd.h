@@ -588,6 +588,143 @@ typedef struct pa_paged_args {
 int pa_paged_workspace(const pa_paged_args* args, int64_t* bytes, int64_t* zero_bytes);
 int pa_paged_attn(const pa_paged_args* args, void* stream);
 
+/* ---- a paged cache whose requests share a prefix, and that forgets (no counterpart in the
+ * reference) -------------------------------------------------------------------------------
+ * pa_share_rows: holders[r] is the request whose first shared[r] tokens request r shares (below 0 or
+ * from R on: none); r's table names the same pages there, in whole pages (shared[r] is taken down to
+ * them, and to lengths[r]).  Of the step's tokens (q_start, lengths as in pa_paged_attn) those of
+ * the requests with one holder g are put side by side, in order: rows start[g] .. start[g + 1] - 1
+ * of rows (their places in the packed step) and positions (lengths[r] - n + i); prefix[g] = the
+ * least that they share, low[g] / high[g] = their least and largest position, first[r] = prefix[g]
+ * for each of them.  A prefix that one request alone has tokens for is no group: start[g] = start[g +
+ * 1], prefix[g] = low[g] = high[g] = 0, and first[r] = 0.  Rows from start[R] on are -1.  start [R +
+ * 1]; prefix, low, high, first [R]; rows, positions [T]; workspace int32 [8 R].  The outputs and the
+ * workspace share no memory with each other or with an input.
+ *
+ * pa_shared_attn: pa_paged_attn of the same arguments, for requests that share prefixes as `sharing`
+ * says, computed once for all rows of a group: the keys t < prefix[g] of request g's table under
+ * the mask at the rows' positions, and the keys from first[r] on of each request's own table.  What
+ * rows and positions hold past [0, T) and below 0 is taken as the nearest; sharing of a step other
+ * than the call's gives other results, and nothing worse.  workspace as in pa_paged_attn, its sizes
+ * from pa_shared_workspace.
+ *
+ * pa_paged_weights: for every cached key t in first[r] .. lengths[r] - 1 of every request and KV head
+ *   scores = (t < lengths[r] - n ? scores : 0) + sum over r's n new tokens i and the G heads that read
+ *            the KV head, where t is live for i, of exp(scale q_i . k_t - lse_i)
+ * with lse [T, Hq] of their attention (-inf: the row has no weight).  Key t's score is row t %
+ * page_size of page tables[r][t / page_size]: float at scores + page * s_sp + head * s_sh + row.  Keys
+ * without a page and scores of no request's keys are left as they are; no key from first[r] on is
+ * in two requests' tables.  first may be NULL (0).  One token or many: every key's sum is taken by
+ * one wave in a fixed order.  scores shares no memory with an input or itself.
+ *
+ * pa_choose_keys: for each of `layers` layers, request and KV head the keys that stay.  With m =
+ * lengths[r] - first[r] (first may be NULL: 0; clamped to 0 .. lengths[r]): where m > limit, the `recent`
+ * newest and of the others the keep - recent with the largest scores (equal ones: the lowest places; NaN
+ * is above every number; a key without a page below every one), as places in ascending order,
+ * kept [layers, R, Hkv, keep]; after[r] = first[r] + keep.  Else kept is -1 and after[r] =
+ * lengths[r].  0 <= recent <= keep <= limit, keep >= 1.  scores as above, layers s_sl floats apart.  kept and
+ * after share no memory with an input or each other.
+ *
+ * pa_evict_rows: in each layer and KV head, row (K, V and score) kept[j] of request r goes to place
+ * first[r] + j, in place: kept as pa_choose_keys gives it, or any list with kept[j] >= first[r] + j;
+ * entries below that or past the table or without a page at either place move nothing.  K and V of
+ * layer l: l * c_sl elements on.  scores may be NULL.  Rows of k, v and scores share no memory with
+ * each other or with an input; no place from first[r] on is in two requests' tables. */
+typedef struct pa_share_args {
+  const int32_t* lengths;
+  const int32_t* q_start;
+  const int32_t* holders;
+  const int32_t* shared;
+  int32_t R, page_size;
+  int64_t T;
+  int32_t* start;
+  int32_t* rows;
+  int32_t* positions;
+  int32_t* prefix;
+  int32_t* low;
+  int32_t* high;
+  int32_t* first;
+  int32_t* workspace;
+} pa_share_args;
+
+int pa_share_rows(const pa_share_args* args, void* stream);
+
+typedef struct pa_sharing {
+  const int32_t* start;
+  const int32_t* rows;
+  const int32_t* positions;
+  const int32_t* prefix;
+  const int32_t* low;
+  const int32_t* high;
+  const int32_t* first;
+} pa_sharing;
+
+int pa_shared_workspace(const pa_paged_args* args, int64_t* bytes, int64_t* zero_bytes);
+int pa_shared_attn(const pa_paged_args* args, const pa_sharing* sharing, void* stream);
+
+typedef struct pa_weights_args {
+  const void* q;
+  int64_t q_st, q_sh;
+  const void* k;
+  int64_t c_sp, c_sh, c_sn;
+  int64_t n_pages;
+  int32_t page_size;
+  const int32_t* tables;
+  int64_t pitch;
+  int32_t cols;
+  const int32_t* lengths;
+  const int32_t* q_start;
+  const int32_t* first;
+  int32_t R;
+  int64_t T, max_fresh;
+  int32_t Hq, Hkv, D, dtype;
+  float scale;
+  pa_mask mask;
+  const float* lse;
+  int64_t lse_st, lse_sh;
+  float* scores;
+  int64_t s_sp, s_sh;
+} pa_weights_args;
+
+int pa_paged_weights(const pa_weights_args* args, void* stream);
+
+typedef struct pa_choose_args {
+  const float* scores;
+  int64_t s_sl, s_sp, s_sh;
+  int64_t n_pages;
+  int32_t page_size;
+  const int32_t* tables;
+  int64_t pitch;
+  int32_t cols;
+  const int32_t* lengths;
+  const int32_t* first;
+  int32_t layers, R, Hkv, keep, recent, limit;
+  int32_t* kept;
+  int32_t* after;
+} pa_choose_args;
+
+int pa_choose_keys(const pa_choose_args* args, void* stream);
+
+typedef struct pa_evict_args {
+  const int32_t* kept;
+  int32_t layers, R, Hkv, keep;
+  void* k;
+  void* v;
+  int64_t c_sl, c_sp, c_sh, c_sn;
+  float* scores;
+  int64_t s_sl, s_sp, s_sh;
+  int64_t n_pages;
+  int32_t page_size;
+  const int32_t* tables;
+  int64_t pitch;
+  int32_t cols;
+  const int32_t* lengths;
+  const int32_t* first;
+  int32_t D, dtype;
+} pa_evict_args;
+
+int pa_evict_rows(const pa_evict_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -90,6 +90,40 @@ class PaPagedArgs(ctypes.Structure):
                 ("lse_sh", c_i64), ("workspace", c_vp), ("workspace_bytes", c_i64)]
 
 
+class PaShareArgs(ctypes.Structure):
+    _fields_ = [("lengths", c_vp), ("q_start", c_vp), ("holders", c_vp), ("shared", c_vp), ("R", c_i32),
+                ("page_size", c_i32), ("T", c_i64), ("start", c_vp), ("rows", c_vp), ("positions", c_vp), ("prefix", c_vp),
+                ("low", c_vp), ("high", c_vp), ("first", c_vp), ("workspace", c_vp)]
+
+
+class PaSharing(ctypes.Structure):
+    _fields_ = [("start", c_vp), ("rows", c_vp), ("positions", c_vp), ("prefix", c_vp), ("low", c_vp), ("high", c_vp),
+                ("first", c_vp)]
+
+
+class PaWeightsArgs(ctypes.Structure):
+    _fields_ = [("q", c_vp), ("q_st", c_i64), ("q_sh", c_i64), ("k", c_vp), ("c_sp", c_i64), ("c_sh", c_i64),
+                ("c_sn", c_i64), ("n_pages", c_i64), ("page_size", c_i32), ("tables", c_vp), ("pitch", c_i64),
+                ("cols", c_i32), ("lengths", c_vp), ("q_start", c_vp), ("first", c_vp), ("R", c_i32), ("T", c_i64),
+                ("max_fresh", c_i64), ("Hq", c_i32), ("Hkv", c_i32), ("D", c_i32), ("dtype", c_i32), ("scale", c_f32),
+                ("mask", PaMask), ("lse", c_vp), ("lse_st", c_i64), ("lse_sh", c_i64), ("scores", c_vp), ("s_sp", c_i64),
+                ("s_sh", c_i64)]
+
+
+class PaChooseArgs(ctypes.Structure):
+    _fields_ = [("scores", c_vp), ("s_sl", c_i64), ("s_sp", c_i64), ("s_sh", c_i64), ("n_pages", c_i64),
+                ("page_size", c_i32), ("tables", c_vp), ("pitch", c_i64), ("cols", c_i32), ("lengths", c_vp),
+                ("first", c_vp), ("layers", c_i32), ("R", c_i32), ("Hkv", c_i32), ("keep", c_i32), ("recent", c_i32),
+                ("limit", c_i32), ("kept", c_vp), ("after", c_vp)]
+
+
+class PaEvictArgs(ctypes.Structure):
+    _fields_ = [("kept", c_vp), ("layers", c_i32), ("R", c_i32), ("Hkv", c_i32), ("keep", c_i32), ("k", c_vp), ("v", c_vp),
+                ("c_sl", c_i64), ("c_sp", c_i64), ("c_sh", c_i64), ("c_sn", c_i64), ("scores", c_vp), ("s_sl", c_i64),
+                ("s_sp", c_i64), ("s_sh", c_i64), ("n_pages", c_i64), ("page_size", c_i32), ("tables", c_vp),
+                ("pitch", c_i64), ("cols", c_i32), ("lengths", c_vp), ("first", c_vp), ("D", c_i32), ("dtype", c_i32)]
+
+
 # name -> (restype, argtypes); every symbol of include/polyattn_amd.h
 SIGNATURES = {
     "pa_last_error": (ctypes.c_char_p, []),
@@ -129,6 +163,12 @@ SIGNATURES = {
                                        c_i32, c_i32, c_i32, c_i32, c_vp]),
     "pa_paged_workspace": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), ctypes.POINTER(c_i64), ctypes.POINTER(c_i64)]),
     "pa_paged_attn": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), c_vp]),
+    "pa_share_rows": (ctypes.c_int, [ctypes.POINTER(PaShareArgs), c_vp]),
+    "pa_shared_workspace": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), ctypes.POINTER(c_i64), ctypes.POINTER(c_i64)]),
+    "pa_shared_attn": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), ctypes.POINTER(PaSharing), c_vp]),
+    "pa_paged_weights": (ctypes.c_int, [ctypes.POINTER(PaWeightsArgs), c_vp]),
+    "pa_choose_keys": (ctypes.c_int, [ctypes.POINTER(PaChooseArgs), c_vp]),
+    "pa_evict_rows": (ctypes.c_int, [ctypes.POINTER(PaEvictArgs), c_vp]),
 }
 
 _LIB = None

@@ -23,7 +23,8 @@ ARCH = "gfx950"
 SOURCES = ["common.hip", "index.hip", "permute.hip", "merge.hip", "attn_fwd.hip",
            "attn_bf16.hip", "attn_f16.hip", "attn_f32.hip", "attn_stream.hip", "attn_wsplit.hip",
            "attn_tile.hip", "attn_narrow.hip", "decode.hip", "bwd.hip", "paged.hip", "paged_attn.hip",
-           "paged_bf16.hip", "paged_f16.hip", "paged_f32.hip"]
+           "paged_bf16.hip", "paged_f16.hip", "paged_f32.hip", "paged_share.hip", "paged_shared_bf16.hip",
+           "paged_shared_f16.hip", "paged_shared_f32.hip", "paged_weights.hip", "paged_evict.hip"]
 
 # -packed-fp32-ops: keep the compiler from emitting v_pk_{add,mul,fma}_f32.
 HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-mcode-object-version=5",
@@ -51,7 +52,9 @@ def _torch_lib():
 EXTRA_FLAGS = {"attn_stream.hip": ["-fno-honor-nans", "-Wno-inline-asm"], "attn_tile.hip": ["-Wno-inline-asm"],
                "attn_narrow.hip": ["-Wno-inline-asm"], "bwd.hip": ["-Wno-inline-asm"],
                "decode.hip": ["-Wno-inline-asm"], "paged_bf16.hip": ["-Wno-inline-asm"],
-               "paged_f16.hip": ["-Wno-inline-asm"], "paged_f32.hip": ["-Wno-inline-asm"]}
+               "paged_f16.hip": ["-Wno-inline-asm"], "paged_f32.hip": ["-Wno-inline-asm"],
+               "paged_shared_bf16.hip": ["-Wno-inline-asm"], "paged_shared_f16.hip": ["-Wno-inline-asm"],
+               "paged_shared_f32.hip": ["-Wno-inline-asm"], "paged_weights.hip": ["-Wno-inline-asm"]}
 
 
 def _compile(src, hipcc):

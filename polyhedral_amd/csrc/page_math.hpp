@@ -151,6 +151,8 @@ struct KeyList {
   int32_t low, first, high;
   PA_HD int32_t count() const { return low + high; }
   PA_HD int32_t block(int32_t j) const { return j < low ? j : first + j - low; }
+  // Entries before block b.
+  PA_HD int32_t before(int32_t b) const { return imin(low, imax(b, 0)) + imin(imax(b - first, 0), high); }
 };
 
 template <typename Ptr>

@@ -10,13 +10,8 @@
 // work-group writes sums and state, and a second kernel the tokens and pages.
 // What bounds it: latency (three trips to memory one after the other, and the launch): 256 requests of
 // a token each 5.0 us, 96 with 78000 tokens 5.3 (in two launches 8.4).
-#include <string.h>
-
-#include <initializer_list>
-
 #include "common.hpp"
-#include "page_math.hpp"
-#include "page_spans.hpp"
+#include "page_checks.hpp"
 
 namespace pa {
 namespace {
@@ -296,25 +291,6 @@ int page_lg_of(int32_t ps) {
   for (int lg = 4; lg <= 8; ++lg)
     if (ps == 1 << lg) return lg;
   return -1;
-}
-
-struct Named {
-  const char* name;
-  Strided<1> at;
-  const char* same = "";  // an input that this output may be
-};
-Strided<1> tables_span(const int32_t* tables, int32_t R, int64_t pitch, int32_t cols) {
-  return strided<1>(tables, 4ll * cols, {cols ? R : 0}, {pitch}, 4);
-}
-int check_apart(const char* who, std::initializer_list<Named> in, std::initializer_list<Named> out) {
-  for (const Named& o : out) {
-    for (const Named& i : in)
-      PA_CHECK_ARG(!overlap(o.at, i.at) || (!strcmp(o.same, i.name) && o.at.at == i.at.at && span(o.at) == span(i.at)),
-                   "%s: %s and %s overlap", who, o.name, i.name);
-    for (const Named& i : out)
-      PA_CHECK_ARG(&i == &o || !overlap(o.at, i.at), "%s: %s and %s overlap", who, o.name, i.name);
-  }
-  return PA_OK;
 }
 
 }  // namespace

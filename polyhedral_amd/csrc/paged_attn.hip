@@ -2,7 +2,7 @@
 #include <limits.h>
 #include <math.h>
 
-#include "page_spans.hpp"
+#include "page_checks.hpp"
 #include "paged_attn.hpp"
 
 namespace pa {
@@ -35,7 +35,9 @@ struct PagedPlan {
   bool tile;            // some request may have more rows than a tile of few rows takes
   int stride;
   PagedPart rows, tiles;
+  PagedPart pre_rows, pre_tiles;  // of the prefixes that requests share
   int64_t zero, bytes;
+  int64_t pre_o, pre_ml;          // where their states begin
 };
 
 // A part whose requests have at most max_tiles tiles: its grid and slots.  (The shares of all tiles are
@@ -43,9 +45,9 @@ struct PagedPlan {
 // least, and then less than twice those that its blocks fill.  The work-groups without a unit each
 // hold a place on a CU for 1.5 us; a grid without them, whose groups loop over units, costs more: 276
 // -> 296 us of sinks in chunks, 15 -> 17 us of one token over 8000, by registers that the loop holds.)
-int part_of(const pa_paged_args* x, int BM, int shares, int64_t max_tiles, PagedPart* p) {
+int part_of(const char* who, const pa_paged_args* x, int BM, int shares, int64_t max_tiles, PagedPart* p) {
   const int64_t most = shares + max_tiles * x->Hkv;
-  PA_CHECK_ARG(most <= kMaxGroups, "pa_paged_attn: %lld work-groups exceed the grid limit", (long long)most);
+  PA_CHECK_ARG(most <= kMaxGroups, "%s: %lld work-groups exceed the grid limit", who, (long long)most);
   p->grid = (int32_t)most;
   p->slots = (int32_t)(2 * shares < most ? 2 * shares : most);
   p->by_shares = 1.0001f / (float)shares;
@@ -54,23 +56,23 @@ int part_of(const pa_paged_args* x, int BM, int shares, int64_t max_tiles, Paged
   return PA_OK;
 }
 
-int plan_of(const pa_paged_args* x, PagedPlan* p) {
-  PA_CHECK_ARG(x, "pa_paged_attn: null arguments");
-  if (int rc = check_pages("pa_paged_attn", x->n_pages, x->page_size, &p->page_lg)) return rc;
-  PA_CHECK_ARG(x->dtype == PA_BF16 || x->dtype == PA_F16 || x->dtype == PA_F32, "pa_paged_attn: dtype %d", x->dtype);
-  PA_CHECK_ARG(x->D == 64 || x->D == 128, "pa_paged_attn: D=%d (64 or 128)", x->D);
+int plan_of(const char* who, const pa_paged_args* x, bool sharing, PagedPlan* p) {
+  PA_CHECK_ARG(x, "%s: null arguments", who);
+  if (int rc = check_pages(who, x->n_pages, x->page_size, &p->page_lg)) return rc;
+  PA_CHECK_ARG(x->dtype == PA_BF16 || x->dtype == PA_F16 || x->dtype == PA_F32, "%s: dtype %d", who, x->dtype);
+  PA_CHECK_ARG(x->D == 64 || x->D == 128, "%s: D=%d (64 or 128)", who, x->D);
   PA_CHECK_ARG(x->Hkv >= 1 && x->Hq >= x->Hkv && x->Hq % x->Hkv == 0 && x->Hq <= 65535,
-               "pa_paged_attn: %d query heads and %d KV heads (a multiple, at most 65535)", x->Hq, x->Hkv);
-  PA_CHECK_ARG(x->R >= 0 && x->T >= 0 && x->T <= kMaxPosition && x->T * x->Hq <= kMaxPosition, "pa_paged_attn: R=%d T=%lld Hq=%d (T Hq < 2^30)",
+               "%s: %d query heads and %d KV heads (a multiple, at most 65535)", who, x->Hq, x->Hkv);
+  PA_CHECK_ARG(x->R >= 0 && x->T >= 0 && x->T <= kMaxPosition && x->T * x->Hq <= kMaxPosition, "%s: R=%d T=%lld Hq=%d (T Hq < 2^30)", who,
                x->R, (long long)x->T, x->Hq);
-  PA_CHECK_ARG(x->max_fresh >= 0, "pa_paged_attn: max_fresh=%lld", (long long)x->max_fresh);
+  PA_CHECK_ARG(x->max_fresh >= 0, "%s: max_fresh=%lld", who, (long long)x->max_fresh);
   PA_CHECK_ARG(x->cols >= 0 && ((int64_t)x->cols << p->page_lg) <= kMaxPosition && x->pitch >= x->cols,
-               "pa_paged_attn: %d columns of %d, pitch %lld", x->cols, x->page_size, (long long)x->pitch);
-  PA_CHECK_ARG(!x->mask.perm_q && !x->mask.perm_kv, "pa_paged_attn: the mask takes no permutation tables");
+               "%s: %d columns of %d, pitch %lld", who, x->cols, x->page_size, (long long)x->pitch);
+  PA_CHECK_ARG(!x->mask.perm_q && !x->mask.perm_kv, "%s: the mask takes no permutation tables", who);
   for (int i = 0; i < x->mask.n_include + x->mask.n_exclude && i < PA_MAX_TERMS; ++i)
-    PA_CHECK_ARG(x->mask.terms[i].kind != PA_DENSE, "pa_paged_attn: PA_DENSE has no meaning here");
+    PA_CHECK_ARG(x->mask.terms[i].kind != PA_DENSE, "%s: PA_DENSE has no meaning here", who);
   if (int rc = check_mask(&x->mask, 0)) return rc;
-  PA_CHECK_ARG(x->scale > 0.f && x->scale < INFINITY, "pa_paged_attn: scale=%g must be positive", (double)x->scale);
+  PA_CHECK_ARG(x->scale > 0.f && x->scale < INFINITY, "%s: scale=%g must be positive", who, (double)x->scale);
   p->stride = stride_of(x->mask);
   const int64_t G = x->Hq / x->Hkv, some = x->T < x->R ? x->T : x->R;  // some: requests with rows, at most
   // (Tiles of few rows that take lists read 1 / stride of the keys for each token, a chunk's tile all: 64
@@ -83,35 +85,60 @@ int plan_of(const pa_paged_args* x, PagedPlan* p) {
   if (p->tile && few > some * ((few_rows + kRows - 1) / kRows)) few = some * ((few_rows + kRows - 1) / kRows);
   // (beside chunks too: 61 requests of a token and 3 chunks with 256 shares 232 us, with 512 177, with 1024
   // 166; 36 requests of which most are chunks 53 with any)
-  if (int rc = part_of(x, kRows, 1024, few, &p->rows)) return rc;
+  if (int rc = part_of(who, x, kRows, 1024, few, &p->rows)) return rc;
   p->rows.least = 4;
   p->rows.root_over = 0.7f;
   p->rows.row_min = 0;
   p->rows.row_max = p->tile ? (int32_t)few_rows : INT_MAX;
   p->tiles = PagedPart{};
   if (p->tile) {
-    if (int rc = part_of(x, kTileRows, 512, x->T * G / kTileRows + some, &p->tiles)) return rc;
+    if (int rc = part_of(who, x, kTileRows, 512, x->T * G / kTileRows + some, &p->tiles)) return rc;
     p->tiles.least = 8;
     p->tiles.root_over = 1.f;
     p->tiles.row_min = (int32_t)few_rows;
     p->tiles.row_max = INT_MAX;
   }
-  PA_CHECK_ARG((int64_t)p->rows.grid + p->tiles.grid <= kMaxGroups, "pa_paged_attn: %lld work-groups exceed the grid limit",
+  PA_CHECK_ARG((int64_t)p->rows.grid + p->tiles.grid <= kMaxGroups, "%s: %lld work-groups exceed the grid limit", who,
                (long long)p->rows.grid + p->tiles.grid);
-  p->zero = (4 * ((int64_t)p->rows.slots + p->tiles.slots) + 255) / 256 * 256;
-  p->bytes = p->zero + 4ll * p->rows.slots * slot_floats(kRows, x->D) + 4ll * p->tiles.slots * slot_floats(kTileRows, x->D);
+  p->pre_rows = p->pre_tiles = PagedPart{};
+  if (sharing && some > 1) {
+    // (a group is two requests or more, so its rows may be many where each request's are few)
+    const bool tile = x->dtype != PA_F32 && x->n_pages > 0 && x->T * G > kFewRows;
+    const int64_t groups = some / 2;
+    few = x->T * G / kRows + groups;
+    if (tile && few > groups * (kFewRows / kRows)) few = groups * (kFewRows / kRows);
+    if (int rc = part_of(who, x, kRows, 1024, few, &p->pre_rows)) return rc;
+    p->pre_rows.least = 4;
+    p->pre_rows.root_over = 0.7f;
+    p->pre_rows.row_max = tile ? kFewRows : INT_MAX;
+    if (tile) {
+      if (int rc = part_of(who, x, kTileRows, 512, x->T * G / kTileRows + groups, &p->pre_tiles)) return rc;
+      p->pre_tiles.least = 8;
+      p->pre_tiles.root_over = 1.f;
+      p->pre_tiles.row_min = kFewRows;
+      p->pre_tiles.row_max = INT_MAX;
+    }
+    PA_CHECK_ARG((int64_t)p->pre_rows.grid + p->pre_tiles.grid <= kMaxGroups, "%s: %lld work-groups exceed the grid limit", who,
+                 (long long)p->pre_rows.grid + p->pre_tiles.grid);
+  }
+  const int64_t few_slots = (int64_t)p->rows.slots + p->pre_rows.slots, tile_slots = (int64_t)p->tiles.slots + p->pre_tiles.slots;
+  p->zero = (4 * (few_slots + tile_slots) + 255) / 256 * 256;
+  p->pre_o = p->zero + 4 * (few_slots * slot_floats(kRows, x->D) + tile_slots * slot_floats(kTileRows, x->D));
+  const int64_t rows = sharing ? x->T * x->Hq : 0;
+  p->pre_ml = p->pre_o + 4 * rows * x->D;
+  p->bytes = p->pre_ml + 16 * rows;
   return PA_OK;
 }
 
 // Work-groups write o, lse and the workspace while others read the inputs: no two of them, and no two
 // rows of o or lse, share a byte.  (Heads of one buffer may be q and o in turn.)
-int check_overlaps(const pa_paged_args* x, int esz, int64_t workspace) {
+int check_overlaps(const char* who, const pa_paged_args* x, const pa_sharing* share, int esz, int64_t workspace) {
   const int64_t row = x->D * esz;
   const Strided<2> o = strided<2>(x->o, row, {x->T, x->Hq}, {x->o_st, x->o_sh}, esz);
   const Strided<2> q = strided<2>(x->q, row, {x->T, x->Hq}, {x->q_st, x->q_sh}, esz);
   const Strided<2> lse = strided<2>(x->lse, 4, {x->lse ? x->T : 0, x->Hq}, {x->lse_st, x->lse_sh}, 4);
-  PA_CHECK_ARG(!overlaps_itself(o), "pa_paged_attn: rows of o overlap");
-  PA_CHECK_ARG(!overlaps_itself(lse), "pa_paged_attn: rows of lse overlap");
+  PA_CHECK_ARG(!overlaps_itself(o), "%s: rows of o overlap", who);
+  PA_CHECK_ARG(!overlaps_itself(lse), "%s: rows of lse overlap", who);
   const int64_t pages[] = {x->n_pages, x->Hkv, x->page_size}, steps[] = {x->c_sp, x->c_sh, x->c_sn};
   const Strided<3> k = strided<3>(x->k, row, pages, steps, esz), v = strided<3>(x->v, row, pages, steps, esz);
   const Strided<1> tables = strided<1>(x->tables, 4ll * x->cols, {x->cols ? x->R : 0}, {x->pitch}, 4);
@@ -120,51 +147,55 @@ int check_overlaps(const pa_paged_args* x, int esz, int64_t workspace) {
   auto apart = [&](const char* name, const auto& out) {
     const char* other = overlap(out, q) ? "q" : overlap(out, k) ? "k" : overlap(out, v) ? "v" : overlap(out, tables) ? "tables"
                         : overlap(out, lengths) ? "lengths" : overlap(out, starts) ? "q_start" : nullptr;
-    PA_CHECK_ARG(!other, "pa_paged_attn: %s and %s overlap", name, other);
+    if (share && !other) {
+      const int64_t R = x->R, n[] = {R + 1, x->T, x->T, R, R, R, R};
+      const int32_t* at[] = {share->start, share->rows, share->positions, share->prefix, share->low, share->high, share->first};
+      for (int i = 0; i < 7; ++i)
+        if (overlap(out, flat(at[i], 4 * n[i]))) other = "sharing";
+    }
+    PA_CHECK_ARG(!other, "%s: %s and %s overlap", who, name, other);
     return (int)PA_OK;
   };
   if (int rc = apart("o", o)) return rc;
   if (int rc = apart("lse", lse)) return rc;
   if (int rc = apart("workspace", ws)) return rc;
-  PA_CHECK_ARG(!overlap(o, lse), "pa_paged_attn: o and lse overlap");
-  PA_CHECK_ARG(!overlap(ws, o), "pa_paged_attn: workspace and o overlap");
-  PA_CHECK_ARG(!overlap(ws, lse), "pa_paged_attn: workspace and lse overlap");
+  PA_CHECK_ARG(!overlap(o, lse), "%s: o and lse overlap", who);
+  PA_CHECK_ARG(!overlap(ws, o), "%s: workspace and o overlap", who);
+  PA_CHECK_ARG(!overlap(ws, lse), "%s: workspace and lse overlap", who);
   return PA_OK;
 }
 
-}  // namespace
-}  // namespace pa
-
-extern "C" int pa_paged_workspace(const pa_paged_args* x, int64_t* bytes, int64_t* zero) {
-  pa::PagedPlan p;
-  if (int rc = pa::plan_of(x, &p)) return rc;
-  PA_CHECK_ARG(bytes && zero, "pa_paged_workspace: null output");
+int workspace_of(const char* who, const pa_paged_args* x, bool sharing, int64_t* bytes, int64_t* zero) {
+  PagedPlan p;
+  if (int rc = plan_of(who, x, sharing, &p)) return rc;
+  PA_CHECK_ARG(bytes && zero, "%s: null output", who);
   *bytes = p.bytes;
   *zero = p.zero;
   return PA_OK;
 }
 
-extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
-  using namespace pa;
+int run_paged(const char* who, const pa_paged_args* x, const pa_sharing* share, void* stream) {
   PagedPlan p;
-  if (int rc = plan_of(x, &p)) return rc;
+  if (int rc = plan_of(who, x, share != nullptr, &p)) return rc;
   if (x->R == 0 || x->T == 0) return PA_OK;
-  PA_CHECK_ARG(x->q && x->o && x->lengths && x->q_start, "pa_paged_attn: null q / o / lengths / q_start");
-  PA_CHECK_ARG(x->cols == 0 || x->tables, "pa_paged_attn: null tables");
-  PA_CHECK_ARG(x->n_pages == 0 || (x->k && x->v), "pa_paged_attn: null k / v");
+  PA_CHECK_ARG(x->q && x->o && x->lengths && x->q_start, "%s: null q / o / lengths / q_start", who);
+  PA_CHECK_ARG(!share || (share->start && share->rows && share->positions && share->prefix && share->low && share->high && share->first),
+               "%s: null sharing", who);
+  PA_CHECK_ARG(x->cols == 0 || x->tables, "%s: null tables", who);
+  PA_CHECK_ARG(x->n_pages == 0 || (x->k && x->v), "%s: null k / v", who);
   const int64_t esz = x->dtype == PA_F32 ? 4 : 2;
   auto al = [&](const void* q, int64_t s0, int64_t s1, int64_t s2) {
     return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (s0 * esz) % 16 == 0 && (s1 * esz) % 16 == 0 && (s2 * esz) % 16 == 0;
   };
   PA_CHECK_ARG(al(x->q, x->q_st, x->q_sh, 0) && al(x->o, x->o_st, x->o_sh, 0) && al(x->k, x->c_sp, x->c_sh, x->c_sn) &&
                    al(x->v, x->c_sp, x->c_sh, x->c_sn),
-               "pa_paged_attn: rows must be 16-byte aligned");
+               "%s: rows must be 16-byte aligned", who);
   PA_CHECK_ARG(x->q_st >= 0 && x->q_sh >= 0 && x->o_st >= 0 && x->o_sh >= 0 && x->c_sp >= 0 && x->c_sh >= 0 &&
                    x->c_sn >= x->D && x->c_sn <= (1 << 21),
-               "pa_paged_attn: negative strides, or cache rows closer than D or further than 2^21");
+               "%s: negative strides, or cache rows closer than D or further than 2^21", who);
   PA_CHECK_ARG(x->workspace && reinterpret_cast<uintptr_t>(x->workspace) % 256 == 0 && x->workspace_bytes >= p.bytes,
-               "pa_paged_attn: needs a 256-byte aligned workspace of %lld bytes", (long long)p.bytes);
-  if (int rc = check_overlaps(x, (int)esz, p.bytes)) return rc;
+               "%s: needs a 256-byte aligned workspace of %lld bytes", who, (long long)p.bytes);
+  if (int rc = check_overlaps(who, x, share, (int)esz, p.bytes)) return rc;
   PagedK a;
   a.q = static_cast<const char*>(x->q);
   a.q_st = x->q_st * esz;
@@ -214,7 +245,39 @@ extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) {
   a.tiles.count = a.rows.count + p.rows.slots;
   a.rows.part = ws + p.zero;
   a.tiles.part = a.rows.part + 4ll * p.rows.slots * slot_floats(kRows, x->D);
+  a.share = share ? *share : pa_sharing{};
+  a.pre_o = reinterpret_cast<float*>(ws + p.pre_o);
+  a.pre_ml = reinterpret_cast<float*>(ws + p.pre_ml);
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (share && p.pre_rows.grid) {
+    PagedK pre = a;
+    pre.rows = p.pre_rows;
+    pre.tiles = p.pre_tiles;
+    pre.rows.count = a.tiles.count + p.tiles.slots;
+    pre.tiles.count = pre.rows.count + p.pre_rows.slots;
+    pre.rows.part = a.tiles.part + 4ll * p.tiles.slots * slot_floats(kTileRows, x->D);
+    pre.tiles.part = pre.rows.part + 4ll * p.pre_rows.slots * slot_floats(kRows, x->D);
+    if (x->dtype == PA_F32) return launch_shared_f32(pre, a, x->D, s);
+    return x->dtype == PA_BF16 ? launch_shared_bf16(pre, a, x->D, s) : launch_shared_f16(pre, a, x->D, s);
+  }
   if (x->dtype == PA_F32) return launch_paged_f32(a, x->D, s);
   return x->dtype == PA_BF16 ? launch_paged_bf16(a, x->D, s) : launch_paged_f16(a, x->D, s);
+}
+
+}  // namespace
+}  // namespace pa
+
+extern "C" int pa_paged_workspace(const pa_paged_args* x, int64_t* bytes, int64_t* zero) {
+  return pa::workspace_of("pa_paged_attn", x, false, bytes, zero);
+}
+
+extern "C" int pa_paged_attn(const pa_paged_args* x, void* stream) { return pa::run_paged("pa_paged_attn", x, nullptr, stream); }
+
+extern "C" int pa_shared_workspace(const pa_paged_args* x, int64_t* bytes, int64_t* zero) {
+  return pa::workspace_of("pa_shared_attn", x, true, bytes, zero);
+}
+
+extern "C" int pa_shared_attn(const pa_paged_args* x, const pa_sharing* sharing, void* stream) {
+  PA_CHECK_ARG(sharing, "pa_shared_attn: null sharing");
+  return pa::run_paged("pa_shared_attn", x, sharing, stream);
 }

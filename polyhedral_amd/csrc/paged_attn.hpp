@@ -24,6 +24,12 @@ constexpr int kRows = 16;       // query rows of a tile of few rows
 constexpr int kTileRows = 128;  // and of a chunk's tile
 constexpr int kTileLg = 6;      // log2 keys of a step of a chunk's tile
 
+// Which rows and keys a body takes.  Requests that share a prefix are attended in two parts: the rows of
+// all of a group's requests against the prefix, whose states go to memory (kPrefix: "request" g is the
+// group of holder g, its rows found through a list, at positions of their own), and each request's rows
+// against its own keys, merged with those states (kOwn).
+enum Part { kWhole = 0, kPrefix = 1, kOwn = 2 };
+
 // What one of the two kernels' bodies does in a call.
 struct PagedPart {
   char* part;           // [slots] states of split tiles' units
@@ -63,6 +69,10 @@ struct PagedK {
   float* lse;
   int64_t lse_st, lse_sh;  // elements
   PagedPart tiles, rows;
+  // ---- requests that share prefixes (kPrefix, kOwn) ----
+  pa_sharing share;
+  float* pre_o;   // [T, Hq, D]: the rows' outputs over their prefix
+  float* pre_ml;  // [T, Hq, 4]: maximum (log2 units), what its rounding left out, sum
 };
 
 // The mask of a kernel whose first argument is a PagedK.
@@ -89,17 +99,19 @@ struct Unit {
   Request rq;
   int32_t r, tile, h, split, splits;
   int32_t slot;  // of the tile's first share
+  int32_t x0, x1;  // kPrefix: the group's positions; kOwn: the request's first own key
 };
 
 // Tiles of a request and blocks of 1 << LG keys of its last whole one (a causal mask's longest).
-template <int BM, int LG>
-__device__ __forceinline__ Work work_of(const PagedK& a, const PagedPart& p, const Request& q) {
+template <int BM, int LG, int PART>
+__device__ __forceinline__ Work work_of(const PagedK& a, const PagedPart& p, const Request& q, int32_t x0, int32_t x1) {
   const int32_t rows = q.n * a.G;
   if (rows == 0 || rows > p.row_max || (BM == kRows && rows <= p.row_min)) return {0, 0, 1, 0};
   const int32_t span = imin(q.n, p.span);
   // (a share that is taken by lists: for one token a list of 512 keys for each wave, for more fewer)
-  const int32_t least = BM == kRows && by_lists(span, a.stride) ? imax((2048 >> LG) >> (31 - __builtin_clz((uint32_t)imax(span, 1))), p.least) : p.least;
-  const int32_t blocks = key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG).count();
+  const int32_t least = PART != kPrefix && BM == kRows && by_lists(span, a.stride) ? imax((2048 >> LG) >> (31 - __builtin_clz((uint32_t)imax(span, 1))), p.least) : p.least;
+  const KeyList kl = PART == kPrefix ? key_list(kernel_mask(a), x0, x1, q.len, LG) : key_list(kernel_mask(a), q.len - span, q.len - 1, q.len, LG);
+  const int32_t blocks = kl.count() - (PART == kOwn ? kl.before(x0 >> LG) : 0);
   if (BM == kTileRows && rows <= p.row_min) return {0, 0, 1, blocks};
   return {(rows + BM - 1) / BM, blocks, least, 0};
 }
@@ -131,14 +143,23 @@ __device__ __forceinline__ float wave_total(float x) {
 
 // What q_start and lengths hold for request r0 + lane (past R: zeros).
 struct RawRequest {
-  int32_t s0, s1, len;
+  int32_t s0, s1, len, x0, x1;
 };
+template <int PART = kWhole>
 __device__ __forceinline__ RawRequest raw_request(const PagedK& a, int r0, int lane) {
-  RawRequest x{0, 0, 0};
-  if (r0 + lane < a.R) {
-    x.s0 = a.q_start[r0 + lane];
-    x.s1 = a.q_start[r0 + lane + 1];
-    x.len = a.lengths[r0 + lane];
+  RawRequest x{0, 0, 0, 0, 0};
+  const int r = r0 + lane;
+  if (r < a.R) {
+    const int32_t* start = PART == kPrefix ? a.share.start : a.q_start;
+    x.s0 = start[r];
+    x.s1 = start[r + 1];
+    x.len = PART == kPrefix ? a.share.prefix[r] : a.lengths[r];
+    if (PART == kPrefix) {
+      x.x0 = imin(imax(a.share.low[r], 0), kMaxPosition);
+      x.x1 = imin(imax(a.share.high[r], 0), kMaxPosition);
+    }
+    // (whole segments of 16 keys, as pages are)
+    if (PART == kOwn) x.x0 = imin(imax(a.share.first[r], 0), a.cols << a.page_lg) & ~15;
   }
   return x;
 }
@@ -162,17 +183,20 @@ __device__ __forceinline__ Request load_request(const PagedK& a, const RawReques
   return request_of(s0, s1, x.len, a.T, a.cols << a.page_lg);
 }
 
-template <int BM, int LG>
+template <int BM, int LG, int PART = kWhole>
 __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, const RawRequest& raw, int32_t id, int lane) {
   Unit u;
   u.found = false;
+  u.x0 = u.x1 = 0;
   Request q{0, 0, 0};
+  RawRequest x = raw;
   Work w{0, 0, 1, 0};
   float total = 0.f, few = 0.f;  // (a share needs no exact total)
   int32_t end = 0;
   for (int r0 = 0; r0 < a.R; r0 += 64) {
-    q = load_request(a, r0 == 0 ? raw : raw_request(a, r0, lane), r0, lane, end);
-    w = work_of<BM, LG>(a, p, q);
+    if (r0) x = raw_request<PART>(a, r0, lane);
+    q = load_request(a, x, r0, lane, end);
+    w = work_of<BM, LG, PART>(a, p, q, x.x0, x.x1);
     total += wave_total((float)w.tiles * (float)w.blocks);
     if (BM == kTileRows) few += wave_total((float)w.few);
   }
@@ -194,8 +218,9 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, c
   end = 0;
   for (int r0 = 0; r0 < a.R; r0 += 64) {
     if (a.R > 64) {
-      q = load_request(a, r0 == 0 ? raw : raw_request(a, r0, lane), r0, lane, end);
-      w = work_of<BM, LG>(a, p, q);
+      x = r0 ? raw_request<PART>(a, r0, lane) : raw;
+      q = load_request(a, x, r0, lane, end);
+      w = work_of<BM, LG, PART>(a, p, q, x.x0, x.x1);
     }
     // (to the nearest: a tile little longer than a share stays whole)
     const float b = (float)w.blocks, mine = fmaxf(fmaxf(share, (float)w.least), __builtin_amdgcn_sqrtf(b) * p.root_over);
@@ -211,10 +236,12 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, c
       u.r = r0 + l;
       u.rq = {get(q.start), get(q.n), get(q.len)};
       u.splits = get(splits);
+      if (PART != kWhole) u.x0 = get(x.x0);
+      if (PART == kPrefix) u.x1 = get(x.x1);
       // KV heads side by side, so that those of one head are Hkv units apart: with 8 of them a head's
       // work falls on one XCD (work-groups are dealt to the XCDs in turn) and shares its L2
-      const int32_t x = id - get(at), y = divide(x, a.by_Hkv);
-      u.h = x - y * a.Hkv;
+      const int32_t i = id - get(at), y = divide(i, a.by_Hkv);
+      u.h = i - y * a.Hkv;
       const int32_t tile = u.splits == 1 ? y : (int32_t)((uint32_t)y / (uint32_t)u.splits);
       u.split = y - tile * u.splits;
       u.slot = slot + get(s_in - slotted) + (tile * a.Hkv + u.h) * u.splits;
@@ -283,6 +310,39 @@ __device__ __forceinline__ bool last_share(const PagedPart& p, const Unit& u, in
 // so far; every score is -inf then).
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
+// The packed row of token `tok` of a unit's rows, and (kPrefix) its position.
+template <int PART>
+__device__ __forceinline__ int32_t row_of(const PagedK& a, const Unit& u, int32_t tok) {
+  return PART == kPrefix ? imin(imax(a.share.rows[u.rq.start + tok], 0), a.T - 1) : u.rq.start + tok;
+}
+template <int PART>
+__device__ __forceinline__ int32_t position_of(const PagedK& a, const Unit& u, int32_t tok) {
+  return PART == kPrefix ? imin(imax(a.share.positions[u.rq.start + tok], 0), kMaxPosition) : u.rq.len - u.rq.n + tok;
+}
+__device__ __forceinline__ int32_t lanes_min(int32_t x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) x = imin(x, __shfl_xor(x, o));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int32_t lanes_max(int32_t x) { return ~lanes_min(~x); }
+
+// What the rounding of m = x c left out (0 where m is not finite: nothing needs it there).
+__device__ __forceinline__ float rest_of(float x, float c, float m) {
+  return __builtin_fabsf(m) < INFINITY ? __builtin_fmaf(x, c, -m) : 0.f;
+}
+// Two states of a row, maxima m + rest in log2 units, as one: the factors of each side's sums.
+struct Merge {
+  float m, rest, f0, f1;
+};
+__device__ __forceinline__ Merge merge_of(float m0, float rest0, float m1, float rest1) {
+  Merge x;
+  x.rest = m0 > m1 ? rest0 : m1 > m0 ? rest1 : nan_max(rest0, rest1);
+  x.m = nan_max(m0, m1);
+  x.f0 = __builtin_amdgcn_exp2f((m0 - base_of(x.m)) + (rest0 - x.rest));
+  x.f1 = __builtin_amdgcn_exp2f((m1 - base_of(x.m)) + (rest1 - x.rest));
+  return x;
+}
+
 // floats of a slot: O of every row, then maximum and sum (and of a chunk's tile what the maximum lacks)
 constexpr int slot_floats(int BM, int D) { return BM * (D + (BM == kTileRows ? 3 : 2)); }
 
@@ -292,5 +352,10 @@ int check_pages(const char* who, int64_t n_pages, int32_t page_size, int* page_l
 int launch_paged_bf16(const PagedK& a, int D, hipStream_t s);
 int launch_paged_f16(const PagedK& a, int D, hipStream_t s);
 int launch_paged_f32(const PagedK& a, int D, hipStream_t s);
+
+// The same for requests that share prefixes: `pre` is a with the parts of the prefixes.
+int launch_shared_bf16(const PagedK& pre, const PagedK& a, int D, hipStream_t s);
+int launch_shared_f16(const PagedK& pre, const PagedK& a, int D, hipStream_t s);
+int launch_shared_f32(const PagedK& pre, const PagedK& a, int D, hipStream_t s);
 
 }  // namespace pa

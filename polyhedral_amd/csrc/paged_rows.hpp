@@ -95,7 +95,7 @@ struct RowsShape {
   static constexpr int SMEM = LIST_AT + kWaves * LIST * 4;
 };
 
-template <typename T, int D>
+template <typename T, int D, int PART = kWhole>
 __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* smem, int32_t* flag) {
   using S = RowsShape<T, D>;
   constexpr bool F32 = S::F32;
@@ -108,7 +108,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
   const int tid = threadIdx.x, lane = tid & 63, q16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const RawRequest raw = raw_request(a, 0, lane);
+  const RawRequest raw = raw_request<PART>(a, 0, lane);
   // (what depends on the lane alone, while these are on their way)
   const uint32_t koff = (uint32_t)(q16 * (int32_t)a.c_sn) + 16u * (uint32_t)g;
   uint32_t voff[F32 ? 4 : Rows<D>::NI];
@@ -137,7 +137,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
     }
   }
 
-  const Unit u = find_unit<kRows, S::LG>(a, part, raw, id, lane);
+  const Unit u = find_unit<kRows, S::LG, PART>(a, part, raw, id, lane);
   if (!u.found) return;
 
   // ---- the tile's rows -----------------------------------------------------------
@@ -147,22 +147,28 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
   const int i = imin(i0 + q16, rows - 1);          // (a lane past the rows repeats the last)
   const int tok = token_of(a, i), head = u.h * a.G + (i - tok * a.G);
   const int pos0 = u.rq.len - u.rq.n;
-  const int q_pos = pos0 + tok;
-  const int q_lo = pos0 + token_of(a, i0), q_hi = pos0 + token_of(a, i0 + n_rows - 1);
+  const int q_pos = PART == kPrefix ? position_of<PART>(a, u, tok) : pos0 + tok;
+  const int q_lo = PART == kPrefix ? lanes_min(q_pos) : pos0 + token_of(a, i0);
+  const int q_hi = PART == kPrefix ? lanes_max(q_pos) : pos0 + token_of(a, i0 + n_rows - 1);
   const int len = u.rq.len;
 
   u32x4 qf[NK];
   {
-    const char* qrow = a.q + (int64_t)(u.rq.start + tok) * a.q_st + (int64_t)head * a.q_sh + 16 * g;
+    const char* qrow = a.q + (int64_t)row_of<PART>(a, u, tok) * a.q_st + (int64_t)head * a.q_sh + 16 * g;
 #pragma unroll
     for (int kc = 0; kc < NK; ++kc) qf[kc] = *reinterpret_cast<const u32x4*>(qrow + 64 * kc);
   }
 
   // ---- the keys of this share ------------------------------------------------------
   const KernelMask mask = kernel_mask(a);
-  const KeyList kl = key_list(mask, q_lo, q_hi, len, S::LG);
+  const KeyList kl = PART == kPrefix ? key_list(mask, u.x0, u.x1, len, S::LG) : key_list(mask, q_lo, q_hi, len, S::LG);
+  const int32_t skip = PART == kOwn ? kl.before(u.x0 >> S::LG) : 0, from = PART == kOwn ? u.x0 : 0;
   int32_t j0, j1;
-  share_of(kl.count(), u.split, u.splits, &j0, &j1);
+  share_of(kl.count() - skip, u.split, u.splits, &j0, &j1);
+  if (PART == kOwn) {
+    j0 += skip;
+    j1 += skip;
+  }
   const int n_steps = j1 - j0 > w ? (j1 - j0 - w + kWaves - 1) / kWaves : 0;
   const int32_t* table = a.tables + (int64_t)u.r * a.pitch;
   const char* kbase = a.k + u.h * a.c_sh;
@@ -189,6 +195,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
     int v = mask_verdict(mask, q_lo, q_hi, key, key + 15);  // (does not wait for the pages)
     if (v == kFull && key + 15 >= len) v = kPartial;
     if (key >= len || page < 0) v = kDead;
+    if (PART == kOwn && key < from) v = kDead;
     c_live = __ballot(v != kDead);
     c_full = __ballot(v == kFull);
     c_key = key;
@@ -398,7 +405,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
   };
   const int n_tok = q_hi - q_lo + 1;
   if (n_steps > 0) load_raw(0);
-  if (!by_lists(n_tok, a.stride)) {
+  if (PART == kPrefix || !by_lists(n_tok, a.stride)) {
     // ---- block by block -------------------------------------------------------------
     Step s0{}, s1{};
     if (n_steps > 0) prefetch(0, 0, s0, d0);
@@ -427,7 +434,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
       const int st0 = c * (PL / NS);            // first step (block) of this list
       const int32_t key = lane < PL ? key_at(st0 + lane / NS) : len;
       const int32_t page = checked_page(r_page, a.n_pages);
-      const bool some = key < len && page >= 0;
+      const bool some = key < len && page >= 0 && (PART != kOwn || key >= from);
       c_off = (int64_t)imax(page, 0) * a.c_sp + (int64_t)(key & ((1 << a.page_lg) - 1)) * a.c_sn;
       if ((c + 1) * (PL / NS) < n_steps) {
         const int32_t next = lane < PL ? key_at(st0 + PL / NS + lane / NS) : len;
@@ -629,13 +636,39 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
   }
   if (row >= n_rows) return;
   const int ir = i0 + row, t_r = token_of(a, ir), h_r = u.h * a.G + (ir - t_r * a.G);
+  float m2 = 0.f, rest = 0.f;  // (kWhole has no use for them)
+  if constexpr (PART != kWhole) {
+    m2 = M * a.c;
+    rest = rest_of(M, a.c, m2);
+    const int64_t at = (int64_t)row_of<PART>(a, u, t_r) * (a.Hkv * a.G) + h_r;
+    f32x4* po = reinterpret_cast<f32x4*>(a.pre_o + at * D + c0);
+    f32x4* ml = reinterpret_cast<f32x4*>(a.pre_ml + 4 * at);
+    if constexpr (PART == kPrefix) {
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+      for (int e = 0; e < CPT; e += 4) po[e / 4] = f32x4{out[e], out[e + 1], out[e + 2], out[e + 3]} * inv;
+      if (c0 == 0) *ml = f32x4{m2, rest, L, 0.f};
+      return;
+    }
+    if (from > 0) {
+      const f32x4 p = *ml;
+      const Merge x = merge_of(m2, rest, p[0], p[1]);
+      const float f1 = x.f1 * p[2];
+#pragma unroll
+      for (int e = 0; e < CPT; ++e) out[e] = x.f0 * out[e] + f1 * po[e / 4][e % 4];
+      L = x.f0 * L + f1;
+      m2 = x.m;
+      rest = x.rest;
+    }
+  }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   char* orow = a.o + (int64_t)(u.rq.start + t_r) * a.o_st + (int64_t)h_r * a.o_sh;
 #pragma unroll
   for (int e = 0; e < CPT; e += 4)
     Mma<T>::store4(orow + (c0 + e) * ESZ, f32x4{out[e], out[e + 1], out[e + 2], out[e + 3]} * inv);
   if (a.lse && c0 == 0)
-    a.lse[(int64_t)(u.rq.start + t_r) * a.lse_st + (int64_t)h_r * a.lse_sh] = L == 0.f ? -INFINITY : (M * a.c + log2f(L)) * kLn2;
+    a.lse[(int64_t)(u.rq.start + t_r) * a.lse_st + (int64_t)h_r * a.lse_sh] =
+        L == 0.f ? -INFINITY : PART == kOwn && from > 0 ? (m2 + (log2f(L) + rest)) * kLn2 : __builtin_fmaf(M, a.c, log2f(L)) * kLn2;
 }
 
 }  // namespace

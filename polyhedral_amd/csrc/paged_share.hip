@@ -1,0 +1,198 @@
+// Which tokens of a step share a prefix (gfx950): the plan of pa_shared_attn, once for all layers.
+//
+// With own(r) the holder of request r where it has one, tokens in this step and whole pages to share,
+// a group is the requests of one holder, if they are two or more; its prefix is the least that they
+// share.  Each request sums over the others (R^2 comparisons, spread over the work-group: 64 requests
+// are 4 a thread), so no atomic gives an order, and the same step has the same plan always.
+//
+// What bounds it: latency, three trips to memory and the launch.
+#include "page_checks.hpp"
+
+namespace pa {
+namespace {
+
+constexpr int kShareThreads = 1024;
+constexpr int kShareRequests = 1024;  // requests whose state fits the LDS
+
+struct ShareK {
+  const int32_t* lengths;
+  const int32_t* q_start;
+  const int32_t* holders;
+  const int32_t* shared;
+  int32_t R, T, page_lg;
+  int32_t* start;
+  int32_t* rows;
+  int32_t* positions;
+  int32_t* prefix;
+  int32_t* low;
+  int32_t* high;
+  int32_t* first;
+  int32_t* workspace;
+};
+
+template <bool LDS>
+__global__ __launch_bounds__(kShareThreads) void share_kernel(const ShareK a) {
+  constexpr int NW = kShareThreads / 64;
+  __shared__ int32_t lds[LDS ? 8 * kShareRequests : 1];
+  __shared__ int32_t wave_n[NW];
+  __shared__ int32_t falls;
+  int32_t* at = LDS ? lds : a.workspace;
+  int32_t *s0 = at, *n = at + a.R, *len = at + 2 * (int64_t)a.R, *own = at + 3 * (int64_t)a.R, *some = at + 4 * (int64_t)a.R,
+          *off = at + 5 * (int64_t)a.R, *cut = at + 6 * (int64_t)a.R, *tot = at + 7 * (int64_t)a.R;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  if (tid == 0) falls = 0;
+  __syncthreads();
+
+  // ---- the requests: starts that fall back are taken as the largest before (as in pa_paged_attn) ------
+  for (int r = tid; r < a.R; r += kShareThreads) {
+    const int32_t x = imin(imax(a.q_start[r], 0), a.T), y = imin(imax(a.q_start[r + 1], 0), a.T);
+    s0[r] = x;
+    n[r] = y - x;
+    if (y < x) falls = 1;
+    len[r] = imin(imax(a.lengths[r], 0), kMaxPosition);
+    own[r] = a.holders[r];
+    some[r] = a.shared[r];
+  }
+  __syncthreads();
+  if (falls) {
+    if (tid == 0) {
+      int32_t end = 0;
+      for (int r = 0; r < a.R; ++r) {
+        const int32_t y = s0[r] + n[r], x = imax(s0[r], end);
+        s0[r] = x;
+        end = imax(x, y);
+        n[r] = end - x;
+      }
+    }
+    __syncthreads();
+  }
+  for (int r = tid; r < a.R; r += kShareThreads) {
+    some[r] = imin(imax(some[r], 0), len[r]) >> a.page_lg << a.page_lg;
+    if (!((uint32_t)own[r] < (uint32_t)a.R) || n[r] == 0 || some[r] == 0) own[r] = -1;
+  }
+  __syncthreads();
+
+  // ---- a request among those of its holder: `per` lanes to a request -----------------------------------
+  int per = 1;
+  while (per < 64 && 2 * per * a.R <= kShareThreads) per *= 2;
+  for (int r0 = 0; r0 < a.R; r0 += kShareThreads / per) {
+    const int r = r0 + tid / per;
+    const int32_t mine = r < a.R ? own[r] : -1;
+    int32_t count = 0, before = 0, least = kMaxPosition;
+    if (mine >= 0)
+      for (int x = tid % per; x < a.R; x += per)
+        if (own[x] == mine) {
+          ++count;
+          if (x < r) before += n[x];
+          least = imin(least, some[x]);
+        }
+    for (int o = 1; o < per; o <<= 1) {
+      count += __shfl_xor(count, o);
+      before += __shfl_xor(before, o);
+      least = imin(least, __shfl_xor(least, o));
+    }
+    if (r < a.R && tid % per == 0) {
+      const bool group = count > 1;
+      off[r] = before;
+      cut[r] = group ? least : 0;
+      a.first[r] = group ? least : 0;
+    }
+  }
+  __syncthreads();
+  // ---- the groups, by holder -------------------------------------------------------------------------
+  for (int r0 = 0; r0 < a.R; r0 += kShareThreads / per) {
+    const int g = r0 + tid / per;
+    int32_t sum = 0, lo = kMaxPosition, hi = 0, pre = 0;
+    if (g < a.R)
+      for (int x = tid % per; x < a.R; x += per)
+        if (own[x] == g && cut[x] > 0) {
+          sum += n[x];
+          lo = imin(lo, len[x] - n[x]);
+          hi = imax(hi, len[x] - 1);
+          pre = cut[x];
+        }
+    for (int o = 1; o < per; o <<= 1) {
+      sum += __shfl_xor(sum, o);
+      lo = imin(lo, __shfl_xor(lo, o));
+      hi = imax(hi, __shfl_xor(hi, o));
+      pre = imax(pre, __shfl_xor(pre, o));
+    }
+    if (g < a.R && tid % per == 0) {
+      tot[g] = sum;
+      a.prefix[g] = pre;
+      a.low[g] = sum ? lo : 0;
+      a.high[g] = sum ? hi : 0;
+    }
+  }
+  __syncthreads();
+  // ---- exclusive sums of the groups' rows, in place (at most T in all) ---------------------------------
+  int32_t total = 0;
+  for (int r0 = 0; r0 < a.R; r0 += kShareThreads) {
+    const int g = r0 + tid;
+    const int32_t x = g < a.R ? tot[g] : 0;
+    int32_t in = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int32_t up = __shfl_up(in, o);
+      if (lane >= o) in += up;
+    }
+    if (lane == 63) wave_n[w] = in;
+    __syncthreads();
+    int32_t base = total;
+#pragma unroll
+    for (int y = 0; y < NW; ++y) {
+      if (y < w) base += wave_n[y];
+      total += wave_n[y];
+    }
+    if (g < a.R) {
+      tot[g] = base + in - x;
+      a.start[g] = base + in - x;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) a.start[a.R] = total;
+  // ---- the rows: a wave to a request -------------------------------------------------------------------
+  for (int r = w; r < a.R; r += NW) {
+    if (cut[r] == 0) continue;
+    const int32_t to = tot[own[r]] + off[r], from = s0[r], m = n[r], p0 = len[r] - m;
+    for (int i = lane; i < m; i += 64) {
+      a.rows[to + i] = from + i;
+      a.positions[to + i] = p0 + i;
+    }
+  }
+  for (int i = total + tid; i < a.T; i += kShareThreads) a.rows[i] = a.positions[i] = -1;
+}
+
+}  // namespace
+}  // namespace pa
+
+extern "C" int pa_share_rows(const pa_share_args* x, void* stream) {
+  using namespace pa;
+  PA_CHECK_ARG(x, "pa_share_rows: null arguments");
+  int lg;
+  if (int rc = check_pages("pa_share_rows", 0, x->page_size, &lg)) return rc;
+  PA_CHECK_ARG(x->R >= 0 && x->R < (1 << 24), "pa_share_rows: R=%d (below 2^24)", x->R);
+  PA_CHECK_ARG(x->T >= 0 && x->T <= kMaxPosition, "pa_share_rows: T=%lld", (long long)x->T);
+  PA_CHECK_ARG(x->start && x->q_start, "pa_share_rows: null start / q_start");
+  PA_CHECK_ARG(x->R == 0 || (x->lengths && x->holders && x->shared && x->prefix && x->low && x->high && x->first && x->workspace),
+               "pa_share_rows: null lengths / holders / shared / prefix / low / high / first / workspace");
+  PA_CHECK_ARG(x->T == 0 || (x->rows && x->positions), "pa_share_rows: null rows / positions");
+  const int64_t R = x->R;
+  if (int rc = check_apart("pa_share_rows",
+                           {{"lengths", flat(x->lengths, 4 * R)}, {"q_start", flat(x->q_start, 4 * (R + 1))},
+                            {"holders", flat(x->holders, 4 * R)}, {"shared", flat(x->shared, 4 * R)}},
+                           {{"start", flat(x->start, 4 * (R + 1))}, {"rows", flat(x->rows, 4 * x->T)},
+                            {"positions", flat(x->positions, 4 * x->T)}, {"prefix", flat(x->prefix, 4 * R)},
+                            {"low", flat(x->low, 4 * R)}, {"high", flat(x->high, 4 * R)}, {"first", flat(x->first, 4 * R)},
+                            {"workspace", flat(x->workspace, 32 * R)}}))
+    return rc;
+  const ShareK a{x->lengths, x->q_start, x->holders, x->shared, x->R, (int32_t)x->T, lg, x->start, x->rows, x->positions,
+                 x->prefix, x->low, x->high, x->first, x->workspace};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (x->R <= kShareRequests)
+    hipLaunchKernelGGL(share_kernel<true>, dim3(1), dim3(kShareThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(share_kernel<false>, dim3(1), dim3(kShareThreads), 0, s, a);
+  PA_LAUNCH_CHECK("share_kernel");
+  return PA_OK;
+}

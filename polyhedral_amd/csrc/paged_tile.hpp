@@ -62,7 +62,7 @@ struct TileShape {
   static constexpr int SMEM = 4 * SLOT;            // aligned to two slots
 };
 
-template <typename T, int D>
+template <typename T, int D, int PART = kWhole>
 __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* smem, int32_t* flag) {
   using Frag = typename Mma<T>::frag;
   using R = Rows<D>;
@@ -75,7 +75,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   const int tid = threadIdx.x, lane = tid & 63, G = lane >> 5, m = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const RawRequest raw = raw_request(a, 0, lane);
+  const RawRequest raw = raw_request<PART>(a, 0, lane);
   // (what depends on the lane alone, while these are on their way)
   uint32_t doff[R::NI];
   dma_offsets<D>(doff, a.c_sn, lane);
@@ -84,7 +84,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   // (K reads are on the slot of the step ahead, V reads on that of the current one; a slot is one bit
   // of an address, as the rings are aligned to two slots)
   TileReads<D> rd = tile_reads<D>((lds_cptr)smem, lane);
-  const Unit u = find_unit<kTileRows, kTileLg>(a, part, raw, id, lane);
+  const Unit u = find_unit<kTileRows, kTileLg, PART>(a, part, raw, id, lane);
   if (!u.found) return;
 
   // ---- rows ------------------------------------------------------------------------
@@ -92,13 +92,24 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   const int i0 = u.tile * kTileRows;
   const int n_rows = imin(rows - i0, kTileRows);
   const int w0 = imin(i0 + 32 * w, rows - 1), w1 = imin(i0 + 32 * w + 31, rows - 1);  // this wave's rows
-  const int q_lo = pos0 + token_of(a, w0), q_hi = pos0 + token_of(a, w1);
+  int q_lo = pos0 + token_of(a, w0), q_hi = pos0 + token_of(a, w1);
+  if (PART == kPrefix) {
+    const int32_t p = position_of<PART>(a, u, token_of(a, imin(i0 + 32 * w + m, rows - 1)));
+    q_lo = lanes_min(p);
+    q_hi = lanes_max(p);
+  }
 
   // ---- the keys of this share ---------------------------------------------------------
   const KernelMask mask = kernel_mask(a);
-  const KeyList kl = key_list(mask, pos0 + token_of(a, i0), pos0 + token_of(a, i0 + n_rows - 1), len, kTileLg);
+  const KeyList kl = PART == kPrefix ? key_list(mask, u.x0, u.x1, len, kTileLg)
+                                     : key_list(mask, pos0 + token_of(a, i0), pos0 + token_of(a, i0 + n_rows - 1), len, kTileLg);
+  const int32_t skip = PART == kOwn ? kl.before(u.x0 >> kTileLg) : 0;
   int32_t j0, j1;
-  share_of(kl.count(), u.split, u.splits, &j0, &j1);
+  share_of(kl.count() - skip, u.split, u.splits, &j0, &j1);
+  if (PART == kOwn) {
+    j0 += skip;
+    j1 += skip;
+  }
   const int n_steps = j1 - j0;
   const int32_t* table = a.tables + (int64_t)u.r * a.pitch;
   const char* kbase = a.k + u.h * a.c_sh;
@@ -123,6 +134,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
     int v = mask_verdict(mask, q_lo, q_hi, key, key + 15);  // (does not wait for the pages)
     if (v == kFull && key + 15 >= len) v = kPartial;
     if (key >= len || page < 0) v = kDead;
+    if (PART == kOwn && key < u.x0) v = kDead;
     c_live = __ballot(v != kDead);
     c_full = __ballot(v == kFull);
     // (keys without a page read the cache's first one, and are dead)
@@ -135,8 +147,8 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   Frag qf[NQF];
   {
     const int i = imin(i0 + 32 * w + m, rows - 1), tok = token_of(a, i), head = u.h * a.G + (i - tok * a.G);
-    q_pos = pos0 + tok;
-    const char* qrow = a.q + (int64_t)(u.rq.start + tok) * a.q_st + (int64_t)head * a.q_sh;
+    q_pos = PART == kPrefix ? position_of<PART>(a, u, tok) : pos0 + tok;
+    const char* qrow = a.q + (int64_t)row_of<PART>(a, u, tok) * a.q_st + (int64_t)head * a.q_sh;
 #pragma unroll
     for (int kc = 0; kc < NQF; ++kc)
       qf[kc] = __builtin_bit_cast(Frag, *reinterpret_cast<const uint4*>(qrow + (16 * kc + 8 * G) * ESZ));
@@ -468,11 +480,45 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
           for (int z = 0; z < 4; ++z) acc[db][4 * e + z] += f * x[db][e][z];
     }
   }
+  if constexpr (PART != kWhole) {
+    // (a lane has columns 32 db + 8 e + 4 G .. + 3 of its row, as floats 16 bytes)
+    const int ir = imin(i0 + 32 * w + m_e, rows - 1), tok = token_of(a, ir), head = u.h * a.G + (ir - tok * a.G);
+    const int64_t at = (int64_t)row_of<PART>(a, u, tok) * (a.Hkv * a.G) + head;
+    f32x4* po = reinterpret_cast<f32x4*>(a.pre_o + at * D) + G_e;
+    f32x4* ml = reinterpret_cast<f32x4*>(a.pre_ml + 4 * at);
+    if constexpr (PART == kPrefix) {
+      const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
+      if (!mine) return;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          po[8 * db + 2 * e] = f32x4{acc[db][4 * e], acc[db][4 * e + 1], acc[db][4 * e + 2], acc[db][4 * e + 3]} * inv;
+      if (G_e == 0) *ml = f32x4{m_run, m_rest, l_tot, 0.f};
+      return;
+    }
+    if (u.x0 > 0) {
+      const f32x4 p = *ml;
+      const Merge x = merge_of(m_run, m_rest, p[0], p[1]);
+      const float f1 = x.f1 * p[2];
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f32x4 y = po[8 * db + 2 * e];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) acc[db][4 * e + z] = x.f0 * acc[db][4 * e + z] + f1 * y[z];
+        }
+      l_tot = x.f0 * l_tot + f1;
+      m_run = x.m;
+      m_rest = x.rest;
+    }
+  }
   const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
   if (a.lse && G_e == 0 && mine) {
     const int ir = i0 + 32 * w + m_e, tok = token_of(a, ir), head = u.h * a.G + (ir - tok * a.G);
     a.lse[(int64_t)(u.rq.start + tok) * a.lse_st + (int64_t)head * a.lse_sh] =
-        l_tot == 0.f ? -INFINITY : (m_run + log2f(l_tot)) * kLn2;
+        l_tot == 0.f ? -INFINITY : (m_run + (PART == kOwn && u.x0 > 0 ? log2f(l_tot) + m_rest : log2f(l_tot))) * kLn2;
   }
   // Through LDS (32 rows a wave, 16-byte units swizzled), so that they are stored as whole rows.
   // (every wave is past its last read of the rings: the sums' check was a barrier)

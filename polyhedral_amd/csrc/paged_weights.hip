@@ -1,0 +1,378 @@
+// The attention weight that cached keys receive, over a paged cache (gfx950): for every key and KV head
+// the sum over its request's new tokens and the heads of the group of exp(scale q . k - lse).
+//
+// The keys are cut into blocks (64 keys of one KV head, f32: 32) whose sums are independent.  A wave
+// takes a run of consecutive blocks, an equal share of all blocks times the row tiles each meets: K
+// rows go straight into the A operand's registers of 16x16 MFMAs (S^T = K Q^T, as in paged_rows.hpp),
+// once for all rows of the request, the next block's loads ahead of this one's products.  Lane (q = l %
+// 16, g = l / 16) holds scores of keys 4 g + 0..3 of each 16 keys for row q; their exponentials are
+// added up over the row tiles, and over the 16 rows at the end, in a fixed order.
+//
+// Scores, exponentials and sums are float32.  A dead pair adds 0 whatever its key holds, by selection.
+#include <math.h>
+
+#include "page_checks.hpp"
+#include "paged_rows.hpp"
+
+namespace pa {
+namespace {
+
+struct WeightsK {
+  const char* q;
+  int64_t q_st, q_sh;  // bytes, as every stride of q and k
+  const char* k;
+  int64_t c_sp, c_sh, c_sn;
+  int64_t n_pages;
+  int32_t page_lg, cols;
+  const int32_t* tables;
+  int64_t pitch;
+  const int32_t* lengths;
+  const int32_t* q_start;
+  const int32_t* first;
+  int32_t R, T, Hkv, G;
+  Divisor by_G;
+  float c;  // scale * log2(e)
+  int32_t n_include, n_exclude;
+  pa_term terms[PA_MAX_TERMS];
+  const float* lse;
+  int64_t lse_st, lse_sh;  // elements
+  float* scores;
+  int64_t s_sp, s_sh;  // elements
+};
+
+__device__ __forceinline__ KernelMask weights_mask(const WeightsK& a) {
+  typedef const __attribute__((address_space(4))) char cchar;
+  cchar* args = (cchar*)__builtin_amdgcn_kernarg_segment_ptr();
+  return {a.n_include, a.n_exclude, a.terms[0], (cterm*)(args + offsetof(WeightsK, terms))};
+}
+
+template <typename T, int D>
+struct WeightsShape {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int NS = F32 ? 2 : 4;           // 16-key segments of a block
+  static constexpr int LG = F32 ? 5 : 6;           // log2 keys of a block
+  static constexpr int NK = F32 ? D / 16 : D / 32; // 16-byte units of a row that a lane holds
+  static constexpr int PER = 64 / NS;              // blocks whose pages are held at a time
+};
+
+// One request's share of the work: blocks first >> LG .. of each head, `cost` each.
+struct WeighedRequest {
+  Request rq;
+  int32_t first, block0, blocks, cost;
+};
+template <int LG>
+__device__ __forceinline__ WeighedRequest weighed(const WeightsK& a, int r0, int lane, int32_t& end) {
+  WeighedRequest x{{0, 0, 0}, 0, 0, 0, 0};
+  const int r = r0 + lane;
+  int32_t s0 = 0, s1 = 0, len = 0, first = 0;
+  if (r < a.R) {
+    s0 = a.q_start[r];
+    s1 = a.q_start[r + 1];
+    len = a.lengths[r];
+    first = a.first ? a.first[r] : 0;
+  }
+  s0 = imin(imax(s0, 0), a.T);
+  s1 = imin(imax(s1, 0), a.T);
+  // (starts that fall back are taken as the largest so far, as in load_request)
+  if (__ballot(r < a.R && (s1 < s0 || s0 < end)) != 0ull) {
+    s0 = imax(s0, end);
+#pragma unroll 1
+    for (int o = 1; o < 64; o <<= 1) {
+      const int32_t y = __shfl_up(s0, o);
+      if (lane >= o) s0 = imax(s0, y);
+    }
+    s1 = imax(s1, s0);
+  }
+  end = __builtin_amdgcn_readlane(s1, imin(a.R - 1 - r0, 63));
+  x.rq = request_of(s0, s1, len, a.T, a.cols << a.page_lg);
+  x.first = imin(imax(first, 0), x.rq.len);
+  x.block0 = x.first >> LG;
+  // (without new tokens nothing changes)
+  x.blocks = r < a.R && x.rq.n > 0 ? ((x.rq.len + (1 << LG) - 1) >> LG) - x.block0 : 0;
+  x.cost = 2 + (x.rq.n * a.G + kRows - 1) / kRows;
+  return x;
+}
+
+__device__ __forceinline__ int64_t wave_scan64(int64_t x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)x, o);
+    const int32_t hi = __shfl_up((int)(x >> 32), o);
+    if (lane >= o) x += (int64_t)((uint64_t)lo | (uint64_t)(uint32_t)hi << 32);
+  }
+  return x;
+}
+__device__ __forceinline__ int64_t readlane64(int64_t x, int l) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, l);
+  const int32_t hi = __builtin_amdgcn_readlane((int)(x >> 32), l);
+  return (int64_t)((uint64_t)lo | (uint64_t)(uint32_t)hi << 32);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void weights_kernel(const WeightsK a) {
+  using S = WeightsShape<T, D>;
+  constexpr int NS = S::NS, NK = S::NK, LG = S::LG, PER = S::PER;
+  const int tid = threadIdx.x, lane = tid & 63, q16 = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const KernelMask mask = weights_mask(a);
+  const uint32_t koff = (uint32_t)(q16 * (int32_t)a.c_sn) + 16u * (uint32_t)g;
+
+  // ---- this wave's share of all blocks, by their cost --------------------------------------
+  int64_t total = 0;
+  int32_t end = 0;
+  WeighedRequest x{};
+  for (int r0 = 0; r0 < a.R; r0 += 64) {
+    x = weighed<LG>(a, r0, lane, end);
+    total += readlane64(wave_scan64((int64_t)x.blocks * a.Hkv * x.cost, lane), 63);
+  }
+  const int64_t waves = (int64_t)gridDim.x * 4, me = (int64_t)blockIdx.x * 4 + w;
+  const int64_t per = total / waves, more = total - per * waves;
+  const int64_t lo = per * me + (me < more ? me : more), hi = lo + per + (me < more ? 1 : 0);
+  if (lo >= hi) return;
+
+  int64_t before = 0;
+  end = 0;
+  for (int r0 = 0; r0 < a.R && before < hi; r0 += 64) {
+    if (a.R > 64) x = weighed<LG>(a, r0, lane, end);
+    if (a.R <= 64) end = 0;
+    const int64_t mine = (int64_t)x.blocks * a.Hkv * x.cost, in = wave_scan64(mine, lane), at = before + in - mine;
+    uint64_t hit = __ballot(at < hi && at + mine > lo);
+    before += readlane64(in, 63);
+    while (hit) {
+      const int l = (int)__builtin_ctzll(hit);
+      hit &= hit - 1;
+      auto get = [&](int32_t y) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(y, l); };
+      const int r = r0 + l;
+      const Request rq{get(x.rq.start), get(x.rq.n), get(x.rq.len)};
+      const int32_t first = get(x.first), block0 = get(x.block0), blocks = get(x.blocks), cost = get(x.cost);
+      const int64_t from = readlane64(at, l);
+      // the blocks that begin within the share (all heads of the request one after the other)
+      const int64_t all = (int64_t)blocks * a.Hkv;
+      int64_t b0 = lo <= from ? 0 : (lo - from + cost - 1) / cost, b1 = (hi - from + cost - 1) / cost;
+      if (b1 > all) b1 = all;
+      const int32_t* table = a.tables + (int64_t)r * a.pitch;
+      const int rows = rq.n * a.G, pos0 = rq.len - rq.n, tiles = (rows + kRows - 1) / kRows;
+      while (b0 < b1) {
+        const int h = (int)((uint64_t)b0 / (uint32_t)blocks);
+        const int32_t i0 = (int32_t)(b0 - (int64_t)h * blocks);
+        const int n_blocks = (int)(b1 - b0 < blocks - i0 ? b1 - b0 : blocks - i0);
+        b0 += n_blocks;
+        const char* kbase = a.k + h * a.c_sh;
+        float* sbase = a.scores + h * a.s_sh;
+
+        // rows of a tile: this lane's, its -lse in log2 units, its position (a lane past the rows: none)
+        u32x4 qf[NK];
+        float neg = 0.f;
+        int32_t q_pos = 0, q_lo = 0, q_hi = 0;
+        bool row_ok = false;
+        auto take_rows = [&](int tile) __attribute__((always_inline)) {
+          const int i = imin(tile * kRows + q16, rows - 1), tok = divide(i, a.by_G), head = h * a.G + (i - tok * a.G);
+          const char* qrow = a.q + (int64_t)(rq.start + tok) * a.q_st + (int64_t)head * a.q_sh + 16 * g;
+#pragma unroll
+          for (int kc = 0; kc < NK; ++kc) qf[kc] = *reinterpret_cast<const u32x4*>(qrow + 64 * kc);
+          const float z = a.lse[(int64_t)(rq.start + tok) * a.lse_st + (int64_t)head * a.lse_sh];
+          neg = -z * 1.4426950408889634f;
+          row_ok = tile * kRows + q16 < rows && z != -INFINITY;
+          q_pos = pos0 + tok;
+          q_lo = pos0 + divide(tile * kRows, a.by_G);
+          q_hi = pos0 + divide(imin(tile * kRows + kRows, rows) - 1, a.by_G);
+        };
+        if (tiles == 1) take_rows(0);
+
+        // ---- PER blocks at a time: lane l holds segment l's page --------------------------------
+        int32_t c_page = -1;
+        auto key_of = [&](int c) __attribute__((always_inline)) -> int32_t {
+          const int b = c * PER + lane / NS;
+          return b < n_blocks ? ((block0 + i0 + b) << LG) + 16 * (lane % NS) : rq.len;
+        };
+        auto take_pages = [&](int c) __attribute__((always_inline)) {
+          const int32_t key = key_of(c);
+          c_page = key < rq.len ? checked_page(table[key >> a.page_lg], a.n_pages) : -1;
+        };
+        struct Data {
+          u32x4 k[NS][NK];
+          float old;       // score of key 16 (q16 / 4) + 4 g + q16 % 4 of the block (NS = 2: of q16 < 8)
+          float* to;       // its place, null where it is none of ours
+          int32_t key;     // the block's first
+          uint32_t there;  // segments with a page
+        };
+        auto fetch = [&](int b, Data& d) __attribute__((always_inline)) {
+          if (b % PER == 0) take_pages(b / PER);
+          const int l0 = NS * (b % PER);
+          d.key = (block0 + i0 + b) << LG;
+          d.there = 0u;
+#pragma unroll
+          for (int t = 0; t < NS; ++t) {
+            const int32_t page = __builtin_amdgcn_readlane(c_page, l0 + t);
+            d.there |= page >= 0 ? 1u << t : 0u;
+            const int64_t off = (int64_t)imax(page, 0) * a.c_sp + (int64_t)((d.key + 16 * t) & ((1 << a.page_lg) - 1)) * a.c_sn;
+#pragma unroll
+            for (int kc = 0; kc < NK; ++kc) d.k[t][kc] = *reinterpret_cast<const u32x4*>(kbase + off + koff + 64 * kc);
+          }
+          const int seg = (q16 >> 2) % NS;
+          const int32_t page = __shfl(c_page, l0 + seg), key = d.key + 16 * seg + 4 * g + (q16 & 3);
+          d.to = nullptr;
+          d.old = 0.f;
+          if (q16 < 4 * NS && page >= 0 && key >= first && key < rq.len) {
+            d.to = sbase + (int64_t)page * a.s_sp + (key & ((1 << a.page_lg) - 1));
+            if (key < pos0) d.old = *d.to;
+          }
+        };
+        auto compute = [&](const Data& d) __attribute__((always_inline)) {
+          float sum[4 * NS];
+#pragma unroll
+          for (int e = 0; e < 4 * NS; ++e) sum[e] = 0.f;
+          for (int tile = 0; tile < tiles; ++tile) {
+            if (tiles > 1) take_rows(tile);
+            int v = mask_verdict(mask, q_lo, q_hi, d.key, d.key + 16 * NS - 1);
+            if (v == kDead) continue;
+            if (v == kFull && d.key + 16 * NS > rq.len) v = kPartial;
+            uint64_t word = ~0ull;
+            if (v != kFull) {
+              word = mask_word(mask, q_pos, d.key, rq.len);
+              if (NS == 4) word |= (uint64_t)mask_word(mask, q_pos, d.key + 32, rq.len) << 32;
+            }
+            if (!row_ok) word = 0ull;
+#pragma unroll
+            for (int t = 0; t < NS; ++t) {
+              f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int kc = 0; kc < NK; ++kc) {
+                if constexpr (S::F32) {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    const uint32_t kx = d.k[t][kc][j], qx = qf[kc][j];
+                    s = mma16x4(__builtin_bit_cast(float, kx), __builtin_bit_cast(float, qx), s);
+                  }
+                } else {
+                  using Frag = typename Mma<T>::frag;
+                  s = mma16x32<T>(__builtin_bit_cast(Frag, d.k[t][kc]), __builtin_bit_cast(Frag, qf[kc]), s);
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.c, neg));
+                sum[4 * t + e] += (word >> (16 * t + 4 * g + e)) & 1ull ? p : 0.f;
+              }
+            }
+          }
+          // over the 16 rows, halving: lane q16 ends with the sum of key 16 (q16 / 4) + 4 g + q16 % 4
+          float total = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4 * NS; ++e) {
+            float y = sum[e];
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) y += __shfl_xor(y, o);
+            if (q16 == e) total = y;
+          }
+          if (d.to) *d.to = d.old + total;
+        };
+        Data d0{}, d1{};
+        fetch(0, d0);
+        int b = 0;
+        for (; b + 1 < n_blocks; b += 2) {
+          fetch(b + 1, d1);
+          compute(d0);
+          if (b + 2 < n_blocks) fetch(b + 2, d0);
+          compute(d1);
+        }
+        if (b < n_blocks) compute(d0);
+      }
+    }
+  }
+}
+
+template <typename T, int D>
+int launch_weights(const WeightsK& a, hipStream_t s) {
+  hipLaunchKernelGGL((weights_kernel<T, D>), dim3(1024), dim3(256), 0, s, a);
+  PA_LAUNCH_CHECK("weights_kernel");
+  return PA_OK;
+}
+
+}  // namespace
+}  // namespace pa
+
+extern "C" int pa_paged_weights(const pa_weights_args* x, void* stream) {
+  using namespace pa;
+  const char* who = "pa_paged_weights";
+  PA_CHECK_ARG(x, "%s: null arguments", who);
+  int lg;
+  if (int rc = check_pages(who, x->n_pages, x->page_size, &lg)) return rc;
+  PA_CHECK_ARG(x->dtype == PA_BF16 || x->dtype == PA_F16 || x->dtype == PA_F32, "%s: dtype %d", who, x->dtype);
+  PA_CHECK_ARG(x->D == 64 || x->D == 128, "%s: D=%d (64 or 128)", who, x->D);
+  PA_CHECK_ARG(x->Hkv >= 1 && x->Hq >= x->Hkv && x->Hq % x->Hkv == 0 && x->Hq <= 65535,
+               "%s: %d query heads and %d KV heads (a multiple, at most 65535)", who, x->Hq, x->Hkv);
+  PA_CHECK_ARG(x->R >= 0 && x->T >= 0 && x->T <= kMaxPosition && x->T * x->Hq <= kMaxPosition, "%s: R=%d T=%lld Hq=%d (T Hq < 2^30)", who,
+               x->R, (long long)x->T, x->Hq);
+  PA_CHECK_ARG(x->max_fresh >= 0, "%s: max_fresh=%lld", who, (long long)x->max_fresh);
+  PA_CHECK_ARG(x->cols >= 0 && ((int64_t)x->cols << lg) <= kMaxPosition && x->pitch >= x->cols, "%s: %d columns of %d, pitch %lld", who,
+               x->cols, x->page_size, (long long)x->pitch);
+  PA_CHECK_ARG(!x->mask.perm_q && !x->mask.perm_kv, "%s: the mask takes no permutation tables", who);
+  for (int i = 0; i < x->mask.n_include + x->mask.n_exclude && i < PA_MAX_TERMS; ++i)
+    PA_CHECK_ARG(x->mask.terms[i].kind != PA_DENSE, "%s: PA_DENSE has no meaning here", who);
+  if (int rc = check_mask(&x->mask, 0)) return rc;
+  PA_CHECK_ARG(x->scale > 0.f && x->scale < INFINITY, "%s: scale=%g must be positive", who, (double)x->scale);
+  if (x->R == 0 || x->T == 0 || x->n_pages == 0 || x->cols == 0) return PA_OK;
+  PA_CHECK_ARG(x->q && x->k && x->lse && x->scores && x->tables && x->lengths && x->q_start, "%s: null pointer", who);
+  const int64_t esz = x->dtype == PA_F32 ? 4 : 2, row = x->D * esz, R = x->R;
+  auto al = [&](const void* p, int64_t s0, int64_t s1, int64_t s2) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (s0 * esz) % 16 == 0 && (s1 * esz) % 16 == 0 && (s2 * esz) % 16 == 0;
+  };
+  PA_CHECK_ARG(al(x->q, x->q_st, x->q_sh, 0) && al(x->k, x->c_sp, x->c_sh, x->c_sn), "%s: rows must be 16-byte aligned", who);
+  PA_CHECK_ARG(x->q_st >= 0 && x->q_sh >= 0 && x->c_sp >= 0 && x->c_sh >= 0 && x->c_sn >= x->D && x->c_sn <= (1 << 21),
+               "%s: negative strides, or cache rows closer than D or further than 2^21", who);
+  PA_CHECK_ARG(x->s_sp >= 0 && x->s_sh >= 0, "%s: negative strides of scores", who);
+  // scores are written while the inputs are read, a page's by different waves
+  const Strided<2> scores = strided<2>(x->scores, 4ll * x->page_size, {x->n_pages, x->Hkv}, {x->s_sp, x->s_sh}, 4);
+  PA_CHECK_ARG(nested(scores), "%s: rows of scores overlap", who);
+  const char* other = overlap(scores, strided<2>(x->q, row, {x->T, x->Hq}, {x->q_st, x->q_sh}, (int)esz)) ? "q"
+                      : overlap(scores, strided<3>(x->k, row, {x->n_pages, x->Hkv, x->page_size}, {x->c_sp, x->c_sh, x->c_sn}, (int)esz)) ? "k"
+                      : overlap(scores, strided<2>(x->lse, 4, {x->T, x->Hq}, {x->lse_st, x->lse_sh}, 4)) ? "lse"
+                      : overlap(scores, tables_span(x->tables, x->R, x->pitch, x->cols)) ? "tables"
+                      : overlap(scores, flat(x->lengths, 4 * R)) ? "lengths"
+                      : overlap(scores, flat(x->q_start, 4 * (R + 1))) ? "q_start"
+                      : overlap(scores, flat(x->first, x->first ? 4 * R : 0)) ? "first" : nullptr;
+  PA_CHECK_ARG(!other, "%s: scores and %s overlap", who, other);
+  WeightsK a;
+  a.q = static_cast<const char*>(x->q);
+  a.q_st = x->q_st * esz;
+  a.q_sh = x->q_sh * esz;
+  a.k = static_cast<const char*>(x->k);
+  a.c_sp = x->c_sp * esz;
+  a.c_sh = x->c_sh * esz;
+  a.c_sn = x->c_sn * esz;
+  a.n_pages = x->n_pages;
+  a.page_lg = lg;
+  a.cols = x->cols;
+  a.tables = x->tables;
+  a.pitch = x->pitch;
+  a.lengths = x->lengths;
+  a.q_start = x->q_start;
+  a.first = x->first;
+  a.R = x->R;
+  a.T = (int32_t)x->T;
+  a.Hkv = x->Hkv;
+  a.G = x->Hq / x->Hkv;
+  a.by_G = divisor_of((uint32_t)a.G);
+  a.c = x->scale * 1.4426950408889634f;
+  a.n_include = x->mask.n_include;
+  a.n_exclude = x->mask.n_exclude;
+  for (int i = 0; i < PA_MAX_TERMS; ++i) {
+    pa_term t = x->mask.terms[i];
+    // (no distance reaches the clamp)
+    t.p0 = imin(t.p0, kMaxPosition);
+    t.p1 = imin(t.p1, kMaxPosition);
+    t.p2 = imin(t.p2, kMaxPosition);
+    a.terms[i] = t;
+  }
+  a.lse = x->lse;
+  a.lse_st = x->lse_st;
+  a.lse_sh = x->lse_sh;
+  a.scores = x->scores;
+  a.s_sp = x->s_sp;
+  a.s_sh = x->s_sh;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (x->D == 64)
+    return x->dtype == PA_F32 ? launch_weights<float, 64>(a, s) : x->dtype == PA_BF16 ? launch_weights<__bf16, 64>(a, s) : launch_weights<_Float16, 64>(a, s);
+  return x->dtype == PA_F32 ? launch_weights<float, 128>(a, s) : x->dtype == PA_BF16 ? launch_weights<__bf16, 128>(a, s) : launch_weights<_Float16, 128>(a, s);
+}

@@ -12,7 +12,16 @@ tables[r, t // page_size].  A step of a batch of requests, each with any number 
 3. ``attention``: every new token to all cached ones of its request, under any mask but an
    explicit matrix, query heads sharing KV heads in groups (pa_paged_attn).
 
-``release`` gives pages back (pa_page_release).  Lengths, tables and counts stay on the device:
+``release`` gives pages back (pa_page_release).
+
+Requests whose tables name the same pages in front share a prefix: ``sharing`` finds which of a step's
+tokens do (pa_share_rows), once for all layers, and ``shared_attention`` reads each prefix once for all
+of them (pa_shared_attn).  Keys can be given up one by one: ``weights`` adds up the attention that
+each has received (pa_paged_weights), ``choose`` picks those that stay (pa_choose_keys), and ``evict`` moves
+them to the front of their request's pages (pa_evict_rows), after which their places count as their
+positions.
+
+Lengths, tables and counts stay on the device:
 nothing here waits for it, and a step can be captured in a graph and replayed.  ``prepare_*``
 validate once and return a launch that a program keeps for its buffers; ``PagedKVCache`` holds
 the state of all this for a model's layers.
@@ -33,11 +42,24 @@ MAX_POSITION = (1 << 30) - 1   # lengths stay at or below it
 SHORT_OF_PAGES, TOO_LONG, TOO_MANY_TOKENS = 1, 2, 4
 LIST_FULL = 8   # in PagedKVCache.failed: a release that would have passed the free list's length
 
+SHARED = 16      # there too: a prefix that could not be shared, or its request finished before those that share it
+
 TableStep = namedtuple("TableStep", "lengths q_start slots positions free_count status")
 TableStep.__doc__ = """int32 device tensors of a step: tokens of each request with the new ones, the packed rows'
 starts [R + 1], each row's slot (page * page_size + row in the page) and position (-1 for rows of
 no request), pages left free [1], status [1] (0, or SHORT_OF_PAGES + TOO_LONG + TOO_MANY_TOKENS:
 nothing was taken then, and no row has a slot)."""
+
+
+Sharing = namedtuple("Sharing", "start rows positions prefix low high first")
+Sharing.__doc__ = """int32 device tensors: which of a step's tokens share a prefix.  The tokens of the requests that
+share request g's are rows[start[g]:start[g + 1]] of the packed step, at positions[..]; prefix[g] (tokens
+of the prefix), low[g] and high[g] (the least and largest position) are 0 where there is no group;
+first[r] is prefix[g] for the requests of a group, 0 for others."""
+
+Choice = namedtuple("Choice", "kept lengths")
+Choice.__doc__ = """int32 device tensors: the places that stay [layers,] requests, heads, keep], ascending (-1: the request
+keeps all), and each request's length after their move."""
 
 
 class PagedLaunch:
@@ -244,21 +266,15 @@ def _paged_mask(mask):
     return mask
 
 
-def prepare_attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_fresh=None, out=None, lse=None):
-    """A PagedLaunch of the requests' newest tokens against all their cached ones.
+def _scale(scale, D):
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < math.inf:
+        raise ValueError(f"scale={scale} must be positive")
+    return scale
 
-    q [tokens, Hq, D]: rows q_start[r] .. q_start[r + 1] - 1 are request r's newest tokens, at
-    positions lengths[r] - n .. lengths[r] - 1 (their keys and values appended already).  k, v
-    [pages, Hkv, page_size, D]; query head h reads KV head h // (Hq // Hkv).  tables int32 [R,
-    columns], lengths int32 [R], q_start int32 [R + 1], on the device.  mask: a polyattn mask
-    object, a MaskSpec or a DeviceMask without tables, evaluated at positions; keys
-    past a request's length are never live, and neither are keys whose table entry names no page.
-    scale: positive, 1/sqrt(D) by default.  max_fresh: the most new tokens of a request, where the
-    program knows it (it selects kernels; any value gives right results).  out: [tokens, Hq, D];
-    lse: None or float32 [tokens, Hq], the natural-log sum-exp; neither shares memory with an
-    input, the other or itself (a call that does is refused when it is launched).  A row with no
-    live key gives 0 and -inf; rows of no request are left as they are (in a new ``out``: as its
-    memory was).  The result is out."""
+
+def _attention_launch(entry, q, k, v, tables, lengths, q_start, sharing, mask, scale, max_fresh, out, lse):
+    """The PagedLaunch of prepare_attention and prepare_shared_attention."""
     pages, Hkv, P, D = _cache(k, v)
     if q.dim() != 3:
         raise ValueError("q must be [tokens, heads, D]")
@@ -272,9 +288,7 @@ def prepare_attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_f
     _ints(q_start, "q_start", (R + 1,), dev)
     pitch = _tables(tables, R, P, dev)
     dm = _paged_mask(mask)
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < math.inf:
-        raise ValueError(f"scale={scale} must be positive")
+    scale = _scale(scale, D)
     max_fresh = T if max_fresh is None else int(max_fresh)
     if max_fresh < 0:
         raise ValueError(f"max_fresh={max_fresh} < 0")
@@ -296,17 +310,255 @@ def prepare_attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_f
         if lse.dtype != torch.float32 or lse.shape != (T, Hq) or lse.device != dev:
             raise ValueError(f"lse must be float32 [{T}, {Hq}] on {dev}")
         a.lse, a.lse_st, a.lse_sh = ptr(lse), lse.stride(0), lse.stride(1)
+    call, sizes = (ctypes.byref(a),), entry + "_workspace"
+    if sharing is not None:
+        s = _sharing_struct(sharing, R, T, dev)
+        call += (ctypes.byref(s),)
     nbytes, zero = ctypes.c_int64(0), ctypes.c_int64(0)
-    _lib.check(_lib.lib().pa_paged_workspace(ctypes.byref(a), ctypes.byref(nbytes), ctypes.byref(zero)), "pa_paged_workspace")
+    _lib.check(getattr(_lib.lib(), sizes)(ctypes.byref(a), ctypes.byref(nbytes), ctypes.byref(zero)), sizes)
     ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
     a.workspace, a.workspace_bytes = ptr(ws), nbytes.value
-    return PagedLaunch("pa_paged_attn", (ctypes.byref(a),), [a, q, k, v, tables, lengths, q_start, dm, o, lse, ws], k, o,
+    return PagedLaunch(entry + "_attn", call, [call, a, q, k, v, tables, lengths, q_start, sharing, dm, o, lse, ws], k, o,
                        zero=ws[:zero.value])
+
+
+def prepare_attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_fresh=None, out=None, lse=None):
+    """A PagedLaunch of the requests' newest tokens against all their cached ones.
+
+    q [tokens, Hq, D]: rows q_start[r] .. q_start[r + 1] - 1 are request r's newest tokens, at
+    positions lengths[r] - n .. lengths[r] - 1 (their keys and values appended already).  k, v
+    [pages, Hkv, page_size, D]; query head h reads KV head h // (Hq // Hkv).  tables int32 [R,
+    columns], lengths int32 [R], q_start int32 [R + 1], on the device.  mask: a polyattn mask
+    object, a MaskSpec or a DeviceMask without tables, evaluated at positions; keys
+    past a request's length are never live, and neither are keys whose table entry names no page.
+    scale: positive, 1/sqrt(D) by default.  max_fresh: the most new tokens of a request, where the
+    program knows it (it selects kernels; any value gives right results).  out: [tokens, Hq, D];
+    lse: None or float32 [tokens, Hq], the natural-log sum-exp; neither shares memory with an
+    input, the other or itself (a call that does is refused when it is launched).  A row with no
+    live key gives 0 and -inf; rows of no request are left as they are (in a new ``out``: as its
+    memory was).  The result is out."""
+    return _attention_launch("pa_paged", q, k, v, tables, lengths, q_start, None, mask, scale, max_fresh, out, lse)
 
 
 def attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_fresh=None, out=None, lse=None):
     """o [tokens, Hq, D]: see prepare_attention."""
     return prepare_attention(q, k, v, tables, lengths, q_start, mask, scale, max_fresh, out, lse)()
+
+
+def prepare_sharing(lengths, q_start, holders, shared, page_size, tokens, out=None):
+    """A PagedLaunch that finds which tokens of a step share a prefix; its result is a Sharing, which
+    holds for all layers of the step.
+
+    lengths, q_start: as in prepare_attention.  holders, shared: int32 [R], the request whose first
+    shared[r] tokens request r shares (-1: none), with that request's pages in its own table; only whole
+    pages are shared.  A request may be its own holder.  A prefix that one request alone has tokens for
+    is no group.  tokens: rows of the packed step.  out: a Sharing to write into."""
+    _page_size(page_size)
+    R = lengths.shape[0] if lengths.dim() == 1 else -1
+    _ints(lengths, "lengths", (R,) if R >= 0 else (0,))
+    dev = lengths.device
+    _ints(q_start, "q_start", (R + 1,), dev)
+    _ints(holders, "holders", (R,), dev)
+    _ints(shared, "shared", (R,), dev)
+    tokens = int(tokens)
+    if not 0 <= tokens <= MAX_POSITION:
+        raise ValueError(f"tokens={tokens} outside 0..{MAX_POSITION}")
+    sizes = (R + 1, tokens, tokens, R, R, R, R)
+    if out is None:
+        out = Sharing(*(torch.empty(n, dtype=torch.int32, device=dev) for n in sizes))
+    else:
+        for t, n, name in zip(out, sizes, Sharing._fields):
+            _ints(t, f"out.{name}", (n,), dev)
+        out = Sharing(*out)
+    ws = torch.empty(max(8 * R, 1), dtype=torch.int32, device=dev)
+    a = _lib.PaShareArgs()
+    ptr = _lib.address
+    a.lengths, a.q_start, a.holders, a.shared = ptr(lengths), ptr(q_start), ptr(holders), ptr(shared)
+    a.R, a.page_size, a.T, a.workspace = R, page_size, tokens, ptr(ws)
+    for name, t in zip(Sharing._fields, out):
+        setattr(a, name, ptr(t))
+    return PagedLaunch("pa_share_rows", (ctypes.byref(a),), [a, lengths, q_start, holders, shared, ws, out], lengths, out)
+
+
+def sharing(lengths, q_start, holders, shared, page_size, tokens, out=None):
+    """Which tokens of a step share a prefix: see prepare_sharing."""
+    return prepare_sharing(lengths, q_start, holders, shared, page_size, tokens, out)()
+
+
+def _sharing_struct(sharing, R, T, device):
+    s = _lib.PaSharing()
+    for t, n, name in zip(sharing, (R + 1, T, T, R, R, R, R), Sharing._fields):
+        _ints(t, f"sharing.{name}", (n,), device)
+        setattr(s, name, _lib.address(t))
+    return s
+
+
+def prepare_shared_attention(q, k, v, tables, lengths, q_start, sharing, mask, scale=None, max_fresh=None, out=None, lse=None):
+    """A PagedLaunch of prepare_attention's result where requests share prefixes: the keys of a shared
+    prefix are read once for all rows of its group, from its holder's table, and each request's own from
+    its.  sharing: the Sharing of this step; the other arguments and the result as in prepare_attention."""
+    return _attention_launch("pa_shared", q, k, v, tables, lengths, q_start, sharing, mask, scale, max_fresh, out, lse)
+
+
+def shared_attention(q, k, v, tables, lengths, q_start, sharing, mask, scale=None, max_fresh=None, out=None, lse=None):
+    """o [tokens, Hq, D]: see prepare_shared_attention."""
+    return prepare_shared_attention(q, k, v, tables, lengths, q_start, sharing, mask, scale, max_fresh, out, lse)()
+
+
+def _scores(t, shape, device):
+    """The checked strides of scores of all dimensions but the last."""
+    _lib.require_device(t)
+    if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape) or t.device != device:
+        raise ValueError(f"scores must be float32 {list(shape)} on {device}, got {list(t.shape)} {t.dtype} on {t.device}")
+    if t.numel() and t.stride(-1) != 1:
+        raise ValueError("scores need a unit stride in their last dimension")
+    return _strides(t)
+
+
+def _first(t, R, device):
+    return None if t is None else _ints(t, "first", (R,), device)
+
+
+def prepare_weights(q, k, tables, lengths, q_start, lse, scores, mask, scale=None, first=None, max_fresh=None):
+    """A PagedLaunch that adds to every cached key's score the attention weight it has from the step's
+    tokens: over the tokens of its request and the query heads that read its head, the sum of exp(scale
+    q . k - lse) where the key is live.
+
+    q, k, tables, lengths, q_start, mask, scale, max_fresh: as in prepare_attention.  lse: float32 [tokens, Hq], of
+    that attention (a row with -inf has no weight).  scores: float32 [pages, Hkv, page_size], as the
+    cache's rows, updated in place: the keys of this step's tokens start from 0, whatever their score
+    was.  first: int32 [R], places whose scores stay as they are are those below it (default: none); pages
+    that requests share lie below it.  The result is scores."""
+    pages, Hkv, P, D = _cache(k, k)
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, heads, D]")
+    T, Hq = q.shape[0], q.shape[1]
+    _rows(q, "q", (T, Hq, D), k)
+    if Hq < 1 or Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads are no multiple of {Hkv} KV heads")
+    dev = k.device
+    R = lengths.shape[0] if lengths.dim() == 1 else -1
+    _ints(lengths, "lengths", (R,) if R >= 0 else (0,), dev)
+    _ints(q_start, "q_start", (R + 1,), dev)
+    pitch = _tables(tables, R, P, dev)
+    first = _first(first, R, dev)
+    dm = _paged_mask(mask)
+    scale = _scale(scale, D)
+    max_fresh = T if max_fresh is None else int(max_fresh)
+    if max_fresh < 0:
+        raise ValueError(f"max_fresh={max_fresh} < 0")
+    _lib.require_device(lse)
+    if lse.dtype != torch.float32 or lse.shape != (T, Hq) or lse.device != dev:
+        raise ValueError(f"lse must be float32 [{T}, {Hq}] on {dev}")
+    a = _lib.PaWeightsArgs()
+    ptr = _lib.address
+    a.q, (a.q_st, a.q_sh) = ptr(q), _strides(q)
+    a.k, (a.c_sp, a.c_sh, a.c_sn) = ptr(k), _strides(k)
+    a.n_pages, a.page_size = pages, P
+    a.tables, a.pitch, a.cols = ptr(tables), pitch, tables.shape[1]
+    a.lengths, a.q_start, a.first, a.R = ptr(lengths), ptr(q_start), ptr(first), R
+    a.T, a.max_fresh, a.Hq, a.Hkv, a.D, a.dtype, a.scale = T, min(max_fresh, T), Hq, Hkv, D, _lib.dtype_code(q), scale
+    a.mask = dm.struct()
+    a.lse, a.lse_st, a.lse_sh = ptr(lse), lse.stride(0), lse.stride(1)
+    a.scores, (a.s_sp, a.s_sh) = ptr(scores), _scores(scores, (pages, Hkv, P), dev)
+    return PagedLaunch("pa_paged_weights", (ctypes.byref(a),), [a, q, k, tables, lengths, q_start, lse, scores, first, dm], k, scores)
+
+
+def weights(q, k, tables, lengths, q_start, lse, scores, mask, scale=None, first=None, max_fresh=None):
+    """Attention weights added to scores: see prepare_weights."""
+    return prepare_weights(q, k, tables, lengths, q_start, lse, scores, mask, scale, first, max_fresh)()
+
+
+def _layered(t, dims, name):
+    """(layers, stride of the layer) of a tensor of ``dims`` dimensions or, before them, layers."""
+    _lib.require_device(t)
+    if t.dim() not in (dims, dims + 1):
+        raise ValueError(f"{name} must have {dims} dimensions, or layers before them, got {list(t.shape)}")
+    return (1, 0) if t.dim() == dims else (t.shape[0], t.stride(0) if t.shape[0] > 1 else 0)
+
+
+def prepare_choose(scores, tables, lengths, keep, recent, limit=None, first=None, out=None):
+    """A PagedLaunch that says which cached keys stay; its result is a Choice.
+
+    scores: float32 [pages, heads, page_size], or [layers, ...]: every layer, request and head chooses by
+    its own.  tables int32 [R, columns], lengths int32 [R].  first: int32 [R], the tokens in front that
+    always stay (sinks, a shared prefix; default none).  A request of more than ``limit`` (default
+    keep) tokens behind those keeps ``keep`` of them: the ``recent`` newest, and of the others those with
+    the largest scores (of equal ones those in front; NaN is above every number).  out: a Choice to
+    write into; its lengths are not the given ones."""
+    layers, s_sl = _layered(scores, 3, "scores")
+    pages, Hkv, P = scores.shape[-3:]
+    _page_size(P)
+    dev = scores.device
+    s_sp, s_sh = _scores(scores, scores.shape, dev)[-2:]
+    R = lengths.shape[0] if lengths.dim() == 1 else -1
+    _ints(lengths, "lengths", (R,) if R >= 0 else (0,), dev)
+    pitch = _tables(tables, R, P, dev)
+    first = _first(first, R, dev)
+    keep, recent = int(keep), int(recent)
+    limit = keep if limit is None else int(limit)
+    if not 0 <= recent <= keep <= limit <= MAX_POSITION or keep < 1:
+        raise ValueError(f"recent={recent}, keep={keep}, limit={limit}: 0 <= recent <= keep <= limit <= {MAX_POSITION}, keep >= 1")
+    shape = (R, Hkv, keep) if scores.dim() == 3 else (layers, R, Hkv, keep)
+    if out is None:
+        out = Choice(torch.empty(shape, dtype=torch.int32, device=dev), torch.empty(R, dtype=torch.int32, device=dev))
+    else:
+        out = Choice(*out)
+        if not _ints(out.kept, "out.kept", shape, dev).is_contiguous():
+            raise ValueError("out.kept must be contiguous")
+        _ints(out.lengths, "out.lengths", (R,), dev)
+    a = _lib.PaChooseArgs()
+    ptr = _lib.address
+    a.scores, a.s_sl, a.s_sp, a.s_sh = ptr(scores), s_sl, s_sp, s_sh
+    a.n_pages, a.page_size, a.tables, a.pitch, a.cols = pages, P, ptr(tables), pitch, tables.shape[1]
+    a.lengths, a.first, a.layers, a.R, a.Hkv = ptr(lengths), ptr(first), layers, R, Hkv
+    a.keep, a.recent, a.limit, a.kept, a.after = keep, recent, limit, ptr(out.kept), ptr(out.lengths)
+    return PagedLaunch("pa_choose_keys", (ctypes.byref(a),), [a, scores, tables, lengths, first, out], scores, out)
+
+
+def choose(scores, tables, lengths, keep, recent, limit=None, first=None, out=None):
+    """Which cached keys stay: see prepare_choose."""
+    return prepare_choose(scores, tables, lengths, keep, recent, limit, first, out)()
+
+
+def prepare_evict(kept, k, v, scores, tables, lengths, first=None):
+    """A PagedLaunch that moves the rows of the keys that stay to the front, in place: in every layer and
+    head, row kept[.., r, h, j] of request r goes to place first[r] + j.
+
+    kept: int32 [R, heads, keep], or [layers, ...], as choose gives it (entries below their own place, as
+    -1, move nothing).  k, v [pages, heads, page_size, D] and scores [pages, heads, page_size] (or None), or
+    [layers, ...].  tables, lengths (before the move), first: as choose was given them.  The result is (k,
+    v, scores)."""
+    layers, c_sl = _layered(k, 4, "k")
+    _lib.require_device(v)
+    lead = k.shape[:-4]
+    if v.shape != k.shape or _strides(v) != _strides(k):
+        raise ValueError("k and v must share shape and strides")
+    pages, Hkv, P, D = _cache(*((k, v) if not lead else (k[0], v[0]) if layers else (k.new_empty(k.shape[1:]),) * 2))
+    dev = k.device
+    R = lengths.shape[0] if lengths.dim() == 1 else -1
+    _ints(lengths, "lengths", (R,) if R >= 0 else (0,), dev)
+    pitch = _tables(tables, R, P, dev)
+    first = _first(first, R, dev)
+    keep = kept.shape[-1] if kept.dim() else 0
+    if not _ints(kept, "kept", (*lead, R, Hkv, keep), dev).is_contiguous():
+        raise ValueError("kept must be contiguous")
+    a = _lib.PaEvictArgs()
+    ptr = _lib.address
+    if scores is not None:
+        a.scores, (a.s_sp, a.s_sh) = ptr(scores), _scores(scores, (*lead, pages, Hkv, P), dev)[-2:]
+        a.s_sl = scores.stride(0) if lead and layers > 1 else 0
+    a.kept, a.layers, a.R, a.Hkv, a.keep = ptr(kept), layers, R, Hkv, keep
+    a.k, a.v, a.c_sl = ptr(k), ptr(v), c_sl
+    a.c_sp, a.c_sh, a.c_sn = _strides(k)[-3:]
+    a.n_pages, a.page_size, a.tables, a.pitch, a.cols = pages, P, ptr(tables), pitch, tables.shape[1]
+    a.lengths, a.first, a.D, a.dtype = ptr(lengths), ptr(first), D, _lib.dtype_code(k)
+    return PagedLaunch("pa_evict_rows", (ctypes.byref(a),), [a, kept, k, v, scores, tables, lengths, first], k, (k, v, scores))
+
+
+def evict(kept, k, v, scores, tables, lengths, first=None):
+    """The rows that stay moved to the front: see prepare_evict."""
+    return prepare_evict(kept, k, v, scores, tables, lengths, first)()
 
 
 def _on_device(values, dtype, device):
@@ -325,11 +577,19 @@ class PagedKVCache:
     A step: ``step = cache.begin(fresh)``, then for each layer ``cache.append(k_new, v_new, step,
     layer)`` and ``cache.attend(q, mask, step, layer)``, before the next begin, trim or finish.
     ``trim`` gives back what a window has left behind, ``finish`` all of some requests' pages (their
-    rows then start anew).  All state is in tensors on the device that stay where they are, so a
+    rows then start anew).
+
+    ``share`` gives requests the first tokens of another one, whose pages they then read with it.  With
+    ``weigh``, scores [layers, pages, heads, page_size] are held too: ``cache.weigh(q, lse, mask, step, layer)``
+    after a layer's attend adds to them the attention that its keys have received, and ``evict`` gives
+    up the keys that had least, between steps.
+
+    All state is in tensors on the device that stay where they are, so a
     whole step with counts on the device can be captured in a graph, and every replay is a step;
     only ``check`` waits for the device."""
 
-    def __init__(self, requests, max_length, pages, heads, D, dtype=torch.bfloat16, page_size=64, layers=1, device=None):
+    def __init__(self, requests, max_length, pages, heads, D, dtype=torch.bfloat16, page_size=64, layers=1, device=None,
+                 weigh=False):
         _page_size(page_size)
         if requests < 1 or max_length < 1 or pages < 1 or heads < 1 or layers < 1:
             raise ValueError("requests, max_length, pages, heads and layers must be at least 1")
@@ -351,7 +611,11 @@ class PagedKVCache:
         self.free_list = torch.arange(pages - 1, -1, -1, **i32)   # page 0 is taken first
         self.free_count = torch.full((1,), pages, **i32)
         self.failed = torch.zeros(1, **i32)    # the status bits of all steps so far
-        self._last = (None, None)              # the newest step and its most new tokens of a request
+        self.holders = torch.full((requests,), -1, **i32)   # the request whose prefix each shares (itself: its own is shared)
+        self.shared = torch.zeros(requests, **i32)          # tokens of that
+        self.scores = torch.zeros(self.k.shape[:-1], dtype=torch.float32, device=dev) if weigh else None
+        self._shares = False                   # whether requests may share prefixes
+        self._last = (None, None, None)        # the newest step, its most new tokens of a request, its Sharing
 
     def begin(self, fresh, tokens=None):
         """Room for fresh[r] more tokens of every request (int32 [requests] on the device, or a list
@@ -373,7 +637,8 @@ class PagedKVCache:
         step = build_tables(self.lengths, fresh, self.tables, self.free_list, self.free_count, self.page_size, tokens, out)
         with torch.cuda.device(self.device):
             self.failed |= step.status
-        self._last = (step, most)
+        which = sharing(self.lengths, step.q_start, self.holders, self.shared, self.page_size, tokens) if self._shares else None
+        self._last = (step, most, which)
         return step
 
     def append(self, k_new, v_new, step, layer=0):
@@ -382,11 +647,76 @@ class PagedKVCache:
 
     def attend(self, q, mask, step, layer=0, scale=None, max_fresh=None, out=None, lse=None):
         """o [tokens, Hq, D] of a step's tokens against a layer's pages (see prepare_attention; of the
-        newest step max_fresh is known where its counts were a list)."""
-        if max_fresh is None and step is self._last[0]:
+        newest step max_fresh is known where its counts were a list, and shared prefixes are read once)."""
+        newest = step is self._last[0]
+        if max_fresh is None and newest:
             max_fresh = self._last[1]
+        if newest and self._last[2] is not None:
+            return shared_attention(q, self.k[layer], self.v[layer], self.tables, step.lengths, step.q_start, self._last[2],
+                                    mask, scale, max_fresh, out, lse)
         return attention(q, self.k[layer], self.v[layer], self.tables, step.lengths, step.q_start, mask, scale, max_fresh,
                          out, lse)
+
+    def share(self, holder, members, tokens):
+        """Requests ``members`` (a list; without tokens so far) begin with the first ``tokens`` tokens of
+        request ``holder``, whole pages that they read and do not copy.  The holder may go on; it keeps
+        these pages until the members have finished.  Where that cannot be (the holder has fewer tokens, or
+        begins with more of another's itself; a member is not empty) nothing happens, and ``check`` says
+        so."""
+        members = [int(m) for m in members]
+        holder, tokens = int(holder), int(tokens)
+        if not all(0 <= m < self.requests for m in members + [holder]) or holder in members:
+            raise ValueError(f"members {members} and holder {holder}: different ones of {self.requests} requests")
+        if not 0 < tokens <= self.max_length or tokens % self.page_size:
+            raise ValueError(f"tokens={tokens}: whole pages of {self.page_size}, up to {self.max_length}")
+        if not members:
+            return
+        at = _on_device(members + [holder], torch.int64, self.device)
+        n = tokens // self.page_size
+        with torch.cuda.device(self.device):
+            m, h = at[:-1], at[-1:]
+            of = self.holders[h]
+            second = (of >= 0) & (of != h)       # the holder shares another's prefix itself
+            root = torch.where(second, of, h)    # .. which is then theirs too
+            ok = ((self.lengths[h] >= tokens) & (~second | (self.shared[h] >= tokens))
+                  & (self.lengths[m] == 0) & (self.holders[m] < 0))
+            i32 = lambda x: x.to(torch.int32)  # noqa: E731
+            self.tables[m, :n] = torch.where(ok[:, None], self.tables[root, :n], self.tables[m, :n])
+            for state, new in ((self.lengths, torch.full_like(m, tokens)), (self.shared, torch.full_like(m, tokens)),
+                               (self.holders, root.expand(len(members)))):
+                state[m] = torch.where(ok, i32(new), state[m])
+            some = ok.any()
+            self.holders[root] = torch.where(some, i32(root), self.holders[root])
+            self.shared[root] = torch.where(some, self.shared[root].clamp(min=tokens), self.shared[root])
+            self.failed |= i32((~ok).any()) * SHARED
+        self._shares = True
+
+    def weigh(self, q, lse, mask, step, layer=0, scale=None):
+        """Adds the attention that a step's tokens have paid to a layer's keys to their scores (see
+        prepare_weights; lse: what attend wrote).  A shared prefix is not weighed."""
+        if self.scores is None:
+            raise RuntimeError("the cache holds no scores: make it with weigh=True")
+        most = self._last[1] if step is self._last[0] else None
+        weights(q, self.k[layer], self.tables, step.lengths, step.q_start, lse, self.scores[layer], mask, scale, self.shared, most)
+
+    def evict(self, keep, recent, limit=None, sinks=0):
+        """Every request of more than ``limit`` (default keep) tokens behind its first ``sinks`` ones (and
+        those that it shares) keeps ``keep`` of them, in each layer and head the ``recent`` newest and those
+        with the largest scores, moved together in their order; pages that this leaves go back.  From then
+        on a token's position is its place among those kept: a mask that counts distances counts them
+        there."""
+        if self.scores is None:
+            raise RuntimeError("the cache holds no scores: make it with weigh=True")
+        if sinks < 0:
+            raise ValueError(f"sinks={sinks} < 0")
+        P = self.page_size
+        with torch.cuda.device(self.device):
+            first = self.shared.clamp(min=min(int(sinks), self.max_length))
+            choice = choose(self.scores, self.tables, self.lengths, keep, recent, limit, first)
+            evict(choice.kept, self.k, self.v, self.scores, self.tables, self.lengths, first)
+            pages = lambda n: ((n + (P - 1)) // P).to(torch.int32)  # noqa: E731
+            self._release(pages(choice.lengths), pages(self.lengths))
+            self.lengths.copy_(choice.lengths)
 
     def _release(self, first, last):
         status = torch.empty(1, dtype=torch.int32, device=self.device)
@@ -396,16 +726,29 @@ class PagedKVCache:
 
     def finish(self, done):
         """Gives back the pages of the requests where done (bool [requests], on the device, or a list,
-        which a graph's capture does not take) is true and sets their lengths to 0."""
+        which a graph's capture does not take) is true and sets their lengths to 0.  One whose tokens
+        others share that are not done stays as it is, and ``check`` says so."""
         if not (isinstance(done, torch.Tensor) and done.is_cuda):
             done = _on_device(done, torch.bool, self.device)
         done = done.to(device=self.device, dtype=torch.bool)
         if done.shape != (self.requests,):
             raise ValueError(f"done must be [{self.requests}], got {list(done.shape)}")
         with torch.cuda.device(self.device):
+            self_ = torch.arange(self.requests, dtype=torch.int32, device=self.device)
+            member = (self.holders >= 0) & (self.holders != self_)
+            busy = torch.zeros(self.requests + 1, dtype=torch.bool, device=self.device)
+            busy.scatter_(0, torch.where(member & ~done, self.holders, self.requests).long(), True)
+            self.failed |= (done & busy[:-1]).any().to(torch.int32) * SHARED
+            done = done & ~busy[:-1]
+            # (a shared prefix's pages are its holder's)
+            first = torch.where(member, self.shared // self.page_size, 0).to(torch.int32)
             last = done.to(torch.int32) * self.tables.shape[1]
-            self._release(torch.zeros_like(last), last)
+            self._release(first, last)
+            col = torch.arange(self.tables.shape[1], dtype=torch.int32, device=self.device)
+            self.tables.masked_fill_(done[:, None] & (col < first[:, None]), -1)
             self.lengths.masked_fill_(done, 0)
+            self.shared.masked_fill_(done, 0)
+            self.holders.masked_fill_(done, -1)
 
     def trim(self, window, sinks=0):
         """Gives back the pages that neither the next token's window nor the first ``sinks`` tokens
@@ -415,7 +758,8 @@ class PagedKVCache:
         P = self.page_size
         with torch.cuda.device(self.device):
             last = ((self.lengths - int(min(window, MAX_POSITION)) + 1).clamp(min=0) // P).to(torch.int32)
-            first = torch.full_like(last, min(-(-int(sinks) // P), self.tables.shape[1]))
+            # (nor what requests share)
+            first = (self.shared // P).clamp(min=min(-(-int(sinks) // P), self.tables.shape[1])).to(torch.int32)
             self._release(first, last)
 
     def check(self):
@@ -424,5 +768,7 @@ class PagedKVCache:
         if bits:
             why = [w for b, w in ((SHORT_OF_PAGES, "too few free pages"), (TOO_LONG, f"a request past {self.max_length} tokens"),
                                   (TOO_MANY_TOKENS, "more new tokens than rows"),
-                                  (LIST_FULL, "more pages given back than there are")) if bits & b]
+                                  (LIST_FULL, "more pages given back than there are"),
+                                  (SHARED, "a prefix that could not be shared, or was finished before those that share it"))
+                   if bits & b]
             raise RuntimeError("a step did not fit: " + ", ".join(why))
