@@ -1,12 +1,13 @@
 // Which cached keys stay, and their move to the front of their request's pages (gfx950).
 //
 // pa_choose_keys: a work-group for the keys of one layer, request and KV head.  Their scores become
-// unsigned numbers of the same order and stay in registers (beyond 32768 of them they are read again for
-// every pass); the keep - recent-th largest is found bit by bit from the top, each pass counting by
-// ballots how many are not below the bound tried (no histogram: scores that are equal, as those of
-// keys that were never looked at, would queue for one LDS word).  Where a bound passes just the
-// number wanted the search ends, else the keys equal to it go by place; ranks among the kept are the
-// same ballots' counts, summed over waves.
+// unsigned numbers of the same order and stay in registers, four keys side by side a load (beyond 16384
+// they are read again for every pass).  The keep - recent-th largest is found 11, 11 and 10 bits at a
+// time, each from counts in LDS of the keys that agree so far; where a bin's keys just make up the number the
+// search ends, else the keys equal to the bound go by place.  Ranks among the kept are sums over the waves.
+// What bounds it: for one layer of a few requests the launch and its trips to memory (4 requests of 1000, 4
+// heads: 5.3 us), for many the counts' and ranks' instructions beside the barriers of three work-groups a CU
+// (8 layers of 32 requests of 1500 to 16384, 8 heads, 51 MB: 43 us, of which the loads 16).
 //
 // pa_evict_rows: kept[j] >= first + j, so the row that place first + j gives up was read for some j' <= j: a
 // work-group that takes the rows of one layer, request, KV head and tensor in order, a batch into
@@ -14,6 +15,7 @@
 #include <limits.h>
 
 #include "page_checks.hpp"
+#include "paged_attn.hpp"
 
 namespace pa {
 namespace {
@@ -34,11 +36,12 @@ __device__ __forceinline__ Held held_of(const Pages& p, int r) {
 }
 
 // ---- which stay ---------------------------------------------------------------------------------
-constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
+constexpr int kChooseThreads = 512, kChooseWaves = kChooseThreads / 64, kMostQuads = 8;
 
 struct ChooseK {
   const float* scores;
   int64_t s_sl, s_sp, s_sh;
+  uint32_t s_bytes;  // of a head's scores from its first to its last (0: not by 32-bit offsets of 16 bytes)
   Pages pages;
   int32_t R, Hkv, keep, recent, limit;
   int32_t* kept;
@@ -52,115 +55,170 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// The counts of the upper 11 bits are kept kCopies times, lane l adding to the l % kCopies-th: scores that are
+// equal (keys that nothing has looked at) or near queue for a word otherwise, some 6 cycles a lane (2048 lists
+// of 1500 to 16384, a fifth of them 0: the counts alone 33 us with one copy).  A copy's pitch puts a bin's
+// words on different banks.
+constexpr int kBins = 2048, kCopies = 4, kPitch = kBins + 64 / kCopies;
 struct ChooseShared {
-  int32_t n[2][kChooseWaves];
-  uint64_t pre[32 * kChooseWaves];
-  uint64_t wave[kChooseWaves];
+  __attribute__((aligned(16))) int32_t bins[kCopies * kPitch + kBins + kBins / 2];  // .. then those of the next bits
+  int32_t pre[2][kMostQuads * kChooseWaves];
+  int32_t wave[3][kChooseWaves];
+  int32_t bin[3], above[3], held[3];
 };
 
-template <int ITEMS>
+// The keys first .. first + n - 1 of a list, `want` of which stay.  Thread t holds QUADS times 4 of them side by
+// side (a page is a multiple of 16 rows, so they are in one), from the multiple of 4 at or below first.
+template <int QUADS, bool ANY>
 __device__ __forceinline__ void choose_body(const ChooseK& a, const float* scores, const int32_t* table, int32_t first,
                                             int32_t n, int32_t want, int32_t* kept, ChooseShared& s) {
-  constexpr int SPAN = ITEMS * kChooseThreads;
+  constexpr int SPAN = 4 * QUADS * kChooseThreads;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int chunks = (n + SPAN - 1) / SPAN;
-  uint32_t u[ITEMS];
+  const int32_t base = first & ~3, end = first + n;
+  const int chunks = QUADS == kMostQuads ? (end - base + SPAN - 1) / SPAN : 1;
+  const int one = (1 << a.pages.page_lg) - 1;
+  uint32_t u[QUADS][4];
+  auto at = [&](int c, int i) __attribute__((always_inline)) { return base + c * SPAN + 4 * (i * kChooseThreads + tid); };
   auto load = [&](int c) __attribute__((always_inline)) {
+    // All pages on their way at once, then all scores.  (A place past the table reads page 0, and what has no
+    // page the first scores; neither is used.)
+    const __amdgpu_buffer_rsrc_t pages = __builtin_amdgcn_make_buffer_rsrc((void*)table, 0, 4 * a.pages.cols, 0x00027000);
+    const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc((void*)scores, 0, (int)a.s_bytes, 0x00027000);
+    int32_t page[QUADS];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int x = c * SPAN + i * kChooseThreads + tid;
-      u[i] = 0u;
-      if (x < n) {
-        const int32_t t = first + x, page = checked_page(table[t >> a.pages.page_lg], a.pages.n_pages);
-        u[i] = page < 0 ? 1u : rank_of(scores[(int64_t)page * a.s_sp + (t & ((1 << a.pages.page_lg) - 1))]);
+    for (int i = 0; i < QUADS; ++i) page[i] = (int32_t)__builtin_amdgcn_raw_buffer_load_b32(pages, (at(c, i) >> a.pages.page_lg) << 2, 0, 0);
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) {
+      page[i] = checked_page(page[i], a.pages.n_pages);
+      u32x4 x;
+      if constexpr (ANY) {
+        x = u32x4{0u, 0u, 0u, 0u};
+        if (page[i] >= 0) {
+          const float* y = scores + (int64_t)page[i] * a.s_sp + (at(c, i) & one);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = __builtin_bit_cast(uint32_t, y[e]);
+        }
+      } else {
+        const uint32_t off = (uint32_t)page[i] * (uint32_t)a.s_sp + (uint32_t)(at(c, i) & one);
+        x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, page[i] < 0 ? 0u : off << 2, 0, 0));
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[i][e] = x[e];
     }
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = at(c, i) + e;
+        u[i][e] = t < first || t >= end ? 0u : page[i] < 0 ? 1u : rank_of(__builtin_bit_cast(float, u[i][e]));
+      }
   };
+#pragma unroll
+  for (int i = tid; i < (int)(sizeof(s.bins) / 16); i += kChooseThreads) reinterpret_cast<u32x4*>(s.bins)[i] = u32x4{0u, 0u, 0u, 0u};
   load(0);
-  // ---- the largest bound that `want` of them are not below ----
+  __syncthreads();
+  // ---- the bound: its upper 11 bits, the next 11, the last 10, each by the counts of the keys that have
+  // the bits so far (what is no key is 0, below all) ----
   uint32_t bound = 0u;
-  int buf = 0;
-  bool just = false;
+  int32_t rest = want;  // of the keys at the bound's bits so far that many stay
+  bool just = false;    // all of them do
 #pragma unroll 1
-  for (uint32_t bit = 0x80000000u; bit && !just; bit >>= 1) {
-    const uint32_t x = bound | bit;
-    int32_t mine = 0;
+  for (int round = 0; round < 3 && !just; ++round) {
+    const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 10 : 11;
+    const uint32_t mask = (1u << bits) - 1u;
+    int32_t* bins = s.bins + (round == 0 ? 0 : round == 1 ? kCopies * kPitch : kCopies * kPitch + kBins);
+    int32_t* mine_of = round == 0 ? bins + lane % kCopies * kPitch : bins;
     for (int c = 0; c < chunks; ++c) {
       if (chunks > 1) load(c);
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) mine += __builtin_popcountll(__ballot(u[i] >= x));
+      for (int i = 0; i < QUADS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          // (largest first)
+          if (round == 0 || (u[i][e] ^ bound) >> (shift + bits) == 0u) atomicAdd(&mine_of[mask - ((u[i][e] >> shift) & mask)], 1);
     }
-    if (lane == 0) s.n[buf][w] = mine;
     __syncthreads();
-    int32_t all = 0;
+    constexpr int PER = kBins / kChooseThreads;
+    static_assert(PER == 4, "16 bytes a thread");
+    u32x4 mine = u32x4{0u, 0u, 0u, 0u};
+    if (round < 2 || tid < kChooseThreads / 2)
+      for (int z = 0; z < (round == 0 ? kCopies : 1); ++z) mine += *reinterpret_cast<const u32x4*>(bins + z * kPitch + PER * tid);
+    const int32_t sum = (int32_t)((mine[0] + mine[1]) + (mine[2] + mine[3])), in = wave_scan(sum);
+    if (lane == 63) s.wave[round][w] = in;
+    __syncthreads();
+    int32_t above = in - sum;
 #pragma unroll
-    for (int y = 0; y < kChooseWaves; ++y) all += s.n[buf][y];
-    buf ^= 1;
-    if (all >= want) bound = x;
-    just = all == want;
-  }
-  // `above` of them are past the bound (just: not below it), and the first of those at it make up the rest
-  const uint32_t past = just ? bound : bound + 1u;  // (bound is no 0xffffffff unless just: it is below)
-  const bool top = !just && bound == 0xffffffffu;   // (NaNs beyond the number wanted)
-  int32_t above = want;
-  if (!just) {
-    int32_t mine = 0;
-    for (int c = 0; c < chunks; ++c) {
-      if (chunks > 1) load(c);
+    for (int y = 0; y < kChooseWaves; ++y) above += y < w ? s.wave[round][y] : 0;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) mine += __builtin_popcountll(__ballot(!top && u[i] >= past));
+    for (int i = 0; i < PER; ++i) {
+      if (above < rest && rest <= above + (int32_t)mine[i]) {
+        s.bin[round] = PER * tid + i;
+        s.above[round] = above;
+        s.held[round] = (int32_t)mine[i];
+      }
+      above += (int32_t)mine[i];
     }
-    if (lane == 0) s.n[buf][w] = mine;
     __syncthreads();
-    above = 0;
-#pragma unroll
-    for (int y = 0; y < kChooseWaves; ++y) above += s.n[buf][y];
+    bound |= (mask - (uint32_t)s.bin[round]) << shift;
+    rest -= s.above[round];
+    just = rest == s.held[round];
   }
-  const int32_t at_bound = want - above;
-  // ---- their ranks, in order of place: item, wave, lane ----
-  uint64_t done = 0ull;  // of earlier chunks: past the bound, at it (high half)
+  // Those above the bound stay (just: those not below it), and of those at it the first `rest`.
+  const uint32_t least = just ? bound : bound + 1u;
+  const bool top = !just && bound == 0xffffffffu;  // (NaNs beyond the number wanted: nothing is above)
+  int32_t ties = 0, done = 0;
+  // Ranks of the keys for which `is` holds, in order of place: quad, thread, key.  rank(i): of the first key of
+  // this thread's quad i; from: those of earlier chunks, and of this one after it.
+  int32_t in[QUADS];
+  auto ranks = [&](auto is, int32_t* from, int32_t* counts) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) {
+      const int32_t x = (is(u[i][0]) + is(u[i][1])) + (is(u[i][2]) + is(u[i][3]));
+      in[i] = wave_scan(x);
+      if (lane == 63) counts[i * kChooseWaves + w] = in[i];
+      in[i] -= x;
+    }
+    __syncthreads();
+    static_assert(kMostQuads * kChooseWaves <= 64, "one entry a lane");
+    const int32_t one_of = lane < QUADS * kChooseWaves ? counts[lane] : 0, upto = wave_scan(one_of);
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) in[i] += *from + __builtin_amdgcn_readlane(upto - one_of, i * kChooseWaves + w);
+    *from += __builtin_amdgcn_readlane(upto, 63);
+  };
   for (int c = 0; c < chunks; ++c) {
-    if (chunks > 1) load(c);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const uint64_t g = __ballot(!top && u[i] >= past), e = __ballot(!just && u[i] == bound);
-      if (lane == 0)
-        s.pre[i * kChooseWaves + w] = (uint64_t)__builtin_popcountll(g) | (uint64_t)__builtin_popcountll(e) << 32;
+    if (chunks > 1) {
+      __syncthreads();  // (the last one's counts have been read)
+      load(c);
     }
-    __syncthreads();
-    // exclusive sums of ITEMS x waves entries, one a thread
-    const uint64_t own = tid < ITEMS * kChooseWaves ? s.pre[tid] : 0ull;
-    uint64_t in = own;
+    if (!just) {
+      ranks([&](uint32_t x) __attribute__((always_inline)) { return x == bound ? 1 : 0; }, &ties, s.pre[0]);
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)in, o), hi = (uint32_t)__shfl_up((int)(in >> 32), o);
-      if (lane >= o) in += (uint64_t)lo | (uint64_t)hi << 32;
-    }
-    if (lane == 63) s.wave[w] = in;
-    __syncthreads();
-    uint64_t base = done;
+      for (int i = 0; i < QUADS; ++i)
 #pragma unroll
-    for (int y = 0; y < kChooseWaves; ++y) {
-      if (y < w) base += s.wave[y];
-      done += s.wave[y];
-    }
-    if (tid < ITEMS * kChooseWaves) s.pre[tid] = base + in - own;
-    __syncthreads();
+        for (int e = 0; e < 4; ++e) {
+          const bool tie = u[i][e] == bound;
+          u[i][e] = (!top && u[i][e] >= least) || (tie && in[i] < rest) ? 1u : 0u;
+          in[i] += tie ? 1 : 0;
+        }
+    } else {
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const bool gt = !top && u[i] >= past, eq = !just && u[i] == bound;
-      const uint64_t g = __ballot(gt), e = __ballot(eq), below = (1ull << lane) - 1ull;
-      const uint64_t p = s.pre[i * kChooseWaves + w];
-      const int32_t gr = (int32_t)(uint32_t)p + (int32_t)__builtin_popcountll(g & below);
-      const int32_t er = (int32_t)(p >> 32) + (int32_t)__builtin_popcountll(e & below);
-      if (gt || (eq && er < at_bound)) kept[gr + imin(er, at_bound)] = first + c * SPAN + i * kChooseThreads + tid;
+      for (int i = 0; i < QUADS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[i][e] = u[i][e] >= least ? 1u : 0u;
     }
+    ranks([&](uint32_t x) __attribute__((always_inline)) { return (int32_t)x; }, &done, s.pre[1]);
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (u[i][e]) kept[in[i]++] = at(c, i) + e;
   }
 }
 
-__global__ __launch_bounds__(kChooseThreads) void choose_kernel(const ChooseK a) {
+// ANY: scores that are not aligned to 16 bytes, or span more than 32 bits of bytes.
+template <bool ANY>
+__global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(6))) void choose_kernel(const ChooseK a) {
   __shared__ ChooseShared s;
   const int tid = threadIdx.x;
   const int h = (int)(blockIdx.x % (unsigned)a.Hkv), lr = (int)(blockIdx.x / (unsigned)a.Hkv);
@@ -178,12 +236,15 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(const ChooseK a)
   if (want == 0) return;
   const float* scores = a.scores + layer * a.s_sl + h * a.s_sh;
   const int32_t* table = a.pages.tables + r * a.pages.pitch;
-  if (n <= 4 * kChooseThreads)
-    choose_body<4>(a, scores, table, q.first, n, want, kept, s);
-  else if (n <= 16 * kChooseThreads)
-    choose_body<16>(a, scores, table, q.first, n, want, kept, s);
+  const int32_t held = n + (q.first & 3);
+  if (held <= 4 * kChooseThreads)
+    choose_body<1, ANY>(a, scores, table, q.first, n, want, kept, s);
+  else if (held <= 8 * kChooseThreads)
+    choose_body<2, ANY>(a, scores, table, q.first, n, want, kept, s);
+  else if (held <= 16 * kChooseThreads)
+    choose_body<4, ANY>(a, scores, table, q.first, n, want, kept, s);
   else
-    choose_body<32>(a, scores, table, q.first, n, want, kept, s);
+    choose_body<kMostQuads, ANY>(a, scores, table, q.first, n, want, kept, s);
 }
 
 // ---- their move -----------------------------------------------------------------------------------
@@ -299,6 +360,9 @@ extern "C" int pa_choose_keys(const pa_choose_args* x, void* stream) {
   a.s_sl = x->s_sl;
   a.s_sp = x->s_sp;
   a.s_sh = x->s_sh;
+  const wide bytes = x->n_pages ? span(strided<1>(x->scores, 4ll * x->page_size, {x->n_pages}, {x->s_sp}, 4)) : 4;
+  const bool aligned = reinterpret_cast<uintptr_t>(x->scores) % 16 == 0 && x->s_sl % 4 == 0 && x->s_sp % 4 == 0 && x->s_sh % 4 == 0;
+  a.s_bytes = x->n_pages && aligned && bytes < (1ll << 32) ? (uint32_t)bytes : 0u;
   a.R = x->R;
   a.Hkv = x->Hkv;
   a.keep = x->keep;
@@ -306,8 +370,11 @@ extern "C" int pa_choose_keys(const pa_choose_args* x, void* stream) {
   a.limit = x->limit;
   a.kept = x->kept;
   a.after = x->after;
-  hipLaunchKernelGGL(choose_kernel, dim3((unsigned)(x->layers * R * x->Hkv)), dim3(kChooseThreads), 0,
-                     static_cast<hipStream_t>(stream), a);
+  const dim3 grid((unsigned)(x->layers * R * x->Hkv));
+  if (a.s_bytes)
+    hipLaunchKernelGGL(choose_kernel<false>, grid, dim3(kChooseThreads), 0, static_cast<hipStream_t>(stream), a);
+  else
+    hipLaunchKernelGGL(choose_kernel<true>, grid, dim3(kChooseThreads), 0, static_cast<hipStream_t>(stream), a);
   PA_LAUNCH_CHECK("choose_kernel");
   return PA_OK;
 }

@@ -158,10 +158,12 @@ def _pool(rng, lengths, P, spare=3):
 
 def _choose(gpu, scores, tables, lengths, keep, recent, limit, first=None):
     """scores: numpy float32 [(layers,) pages, H, P]."""
-    wide = torch.full((*scores.shape[:-1], scores.shape[-1] + 3), NAN, device=gpu)
+    wide = torch.full((*scores.shape[:-1], scores.shape[-1] + 3), NAN, device=gpu)    # rows of any alignment
     wide[..., :scores.shape[-1]] = torch.as_tensor(scores, device=gpu)
-    got = paged.choose(wide[..., :scores.shape[-1]], dev(tables, gpu), dev(lengths, gpu), keep, recent, limit,
-                       None if first is None else dev(first, gpu))
+    rest = dev(tables, gpu), dev(lengths, gpu), keep, recent, limit, None if first is None else dev(first, gpu)
+    got = paged.choose(wide[..., :scores.shape[-1]], *rest)
+    again = paged.choose(torch.as_tensor(scores, device=gpu), *rest)
+    assert torch.equal(got.kept, again.kept) and torch.equal(got.lengths, again.lengths)
     f = np.zeros(len(lengths), dtype=int) if first is None else first
     for i, s in enumerate(scores if scores.ndim == 4 else scores[None]):
         kept, after = so.choose(s, tables, lengths, keep, recent, keep if limit is None else limit, f)
