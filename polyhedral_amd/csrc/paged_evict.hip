@@ -11,7 +11,9 @@
 //
 // pa_evict_rows: kept[j] >= first + j, so the row that place first + j gives up was read for some j' <= j: a
 // work-group that takes the rows of one layer, request, KV head and tensor in order, a batch into
-// registers before any of it is stored, moves them in place with no scratch memory.
+// registers before any of it is stored and the next one's on their way meanwhile, moves them in place with
+// no scratch memory.  What bounds it: HBM (1.8 GB in 375 us, 4.9 TB/s, where a copy reaches 5.0), and for
+// a few heads four trips to memory.
 #include <limits.h>
 
 #include "page_checks.hpp"
@@ -248,7 +250,9 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
 }
 
 // ---- their move -----------------------------------------------------------------------------------
-constexpr int kEvictThreads = 256;
+// Heads from which there are work-groups enough with 512 threads (1024: 4 layers of 32 requests, 8 heads, 1.8 GB
+// 389 us and 375; a layer of 2 requests, 4 heads, 4 MB 7.1 us and 7.6).
+constexpr int64_t kManyHeads = 512;
 
 struct EvictK {
   const int32_t* kept;
@@ -261,43 +265,76 @@ struct EvictK {
   int32_t R, Hkv, keep, row_lg;    // row_lg: log2 of the 16-byte units of a row
 };
 
-// Units of type U (1 << lg of them a row) of the kept rows of one head, in order.
-template <typename U, int UNROLL, typename At>
+// Units of type U (1 << lg of them a row) of the kept rows of one head, in order, by THREADS threads.  A batch's
+// rows are loaded before the last one's are stored: they come from places past those.
+template <typename U, int UNROLL, int THREADS, typename At>
 __device__ __forceinline__ void move_rows(const EvictK& a, const int32_t* kept, const int32_t* table, const Held& q, int lg, At at) {
-  const int tid = threadIdx.x;
-  const int per = kEvictThreads >> lg;  // rows that one load of the work-group takes
+  const int tid = threadIdx.x, unit = tid & ((1 << lg) - 1);
+  const int per = THREADS >> lg;  // rows that one load of the work-group takes
   const int one = (1 << a.pages.page_lg) - 1;
   const int32_t reach = a.pages.cols << a.pages.page_lg;
-  for (int j0 = 0; j0 < a.keep; j0 += per * UNROLL) {
+  if (reach == 0) return;
+  struct Batch {
     U x[UNROLL];
-    U* to[UNROLL];
+    U* from[UNROLL];
+    U* to[UNROLL];  // null where nothing moves
+  };
+  auto places = [&](int j0, Batch& b) __attribute__((always_inline)) {
+    int32_t of[UNROLL], p[UNROLL], d[UNROLL];
+    if (j0 >= a.keep) {
+#pragma unroll
+      for (int i = 0; i < UNROLL; ++i) b.to[i] = nullptr;
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) of[i] = kept[imin(j0 + i * per + (tid >> lg), a.keep - 1)];
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
-      const int j = j0 + i * per + (tid >> lg);
-      to[i] = nullptr;
-      x[i] = U{};
-      if (j >= a.keep) continue;
-      const int32_t of = kept[j], dst = q.first + j;
-      if (of <= dst || of >= reach) continue;
-      const int32_t p = checked_page(table[of >> a.pages.page_lg], a.pages.n_pages);
-      const int32_t d = checked_page(table[dst >> a.pages.page_lg], a.pages.n_pages);
-      if (p < 0 || d < 0) continue;
-      to[i] = at(d, dst & one) + (tid & ((1 << lg) - 1));
-      x[i] = *(at(p, of & one) + (tid & ((1 << lg) - 1)));
+      const int32_t dst = imin(q.first + j0 + i * per + (tid >> lg), reach - 1);
+      p[i] = table[imin(imax(of[i], 0), reach - 1) >> a.pages.page_lg];
+      d[i] = table[dst >> a.pages.page_lg];
     }
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) {
+      const int j = j0 + i * per + (tid >> lg), dst = q.first + j;
+      p[i] = checked_page(p[i], a.pages.n_pages);
+      d[i] = checked_page(d[i], a.pages.n_pages);
+      b.from[i] = at(imax(p[i], 0), of[i] & one) + unit;
+      b.to[i] = j < a.keep && of[i] > dst && of[i] < reach && p[i] >= 0 && d[i] >= 0 ? at(d[i], dst & one) + unit : nullptr;
+    }
+  };
+  auto fetch = [&](Batch& b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) {
+      b.x[i] = U{};
+      if (b.to[i]) b.x[i] = *b.from[i];
+    }
+  };
+  auto step = [&](int j0, Batch& b, Batch& next) __attribute__((always_inline)) {
     // (all of the batch has been read, by every wave, before any of it is written)
 #pragma unroll
-    for (int i = 0; i < UNROLL; ++i) asm volatile("" ::"v"(x[i]));
+    for (int i = 0; i < UNROLL; ++i) asm volatile("" ::"v"(b.x[i]));
     __syncthreads();
+    fetch(next);
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i)
-      if (to[i]) *to[i] = x[i];
+      if (b.to[i]) *b.to[i] = b.x[i];
+    places(j0 + 2 * per * UNROLL, b);
+  };
+  Batch b0, b1;
+  places(0, b0);
+  fetch(b0);
+  places(per * UNROLL, b1);
+  for (int j0 = 0; j0 < a.keep; j0 += 2 * per * UNROLL) {
+    step(j0, b0, b1);
+    step(j0 + per * UNROLL, b1, b0);
   }
 }
 
 typedef uint32_t unit16 __attribute__((ext_vector_type(4)));
 
-__global__ __launch_bounds__(kEvictThreads) void evict_kernel(const EvictK a) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void evict_kernel(const EvictK a) {
   const int h = (int)(blockIdx.x % (unsigned)a.Hkv), lr = (int)(blockIdx.x / (unsigned)a.Hkv);
   const int r = lr % a.R, layer = lr / a.R;
   const Held q = held_of(a.pages, r);
@@ -305,12 +342,12 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const EvictK a) {
   const int32_t* table = a.pages.tables + r * a.pages.pitch;
   if (blockIdx.y < 2) {
     char* base = (blockIdx.y ? a.v : a.k) + layer * a.c_sl + h * a.c_sh;
-    move_rows<unit16, 8>(a, kept, table, q, a.row_lg, [&](int32_t page, int32_t row) __attribute__((always_inline)) {
+    move_rows<unit16, 4, THREADS>(a, kept, table, q, a.row_lg, [&](int32_t page, int32_t row) __attribute__((always_inline)) {
       return reinterpret_cast<unit16*>(base + page * a.c_sp + row * a.c_sn);
     });
   } else {
     float* base = a.scores + layer * a.s_sl + h * a.s_sh;
-    move_rows<float, 8>(a, kept, table, q, 0, [&](int32_t page, int32_t row) __attribute__((always_inline)) {
+    move_rows<float, 4, THREADS>(a, kept, table, q, 0, [&](int32_t page, int32_t row) __attribute__((always_inline)) {
       return base + page * a.s_sp + row;
     });
   }
@@ -442,8 +479,12 @@ extern "C" int pa_evict_rows(const pa_evict_args* x, void* stream) {
   a.Hkv = x->Hkv;
   a.keep = x->keep;
   a.row_lg = row == 128 ? 3 : row == 256 ? 4 : 5;
-  hipLaunchKernelGGL(evict_kernel, dim3((unsigned)(x->layers * R * x->Hkv), x->scores ? 3 : 2), dim3(kEvictThreads), 0,
-                     static_cast<hipStream_t>(stream), a);
+  const int64_t heads = x->layers * R * x->Hkv;
+  const dim3 grid((unsigned)heads, x->scores ? 3 : 2);
+  if (heads < kManyHeads)
+    hipLaunchKernelGGL(evict_kernel<1024>, grid, dim3(1024), 0, static_cast<hipStream_t>(stream), a);
+  else
+    hipLaunchKernelGGL(evict_kernel<512>, grid, dim3(512), 0, static_cast<hipStream_t>(stream), a);
   PA_LAUNCH_CHECK("evict_kernel");
   return PA_OK;
 }
