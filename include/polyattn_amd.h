@@ -614,8 +614,9 @@ int pa_paged_attn(const pa_paged_args* args, void* stream);
  * with lse [T, Hq] of their attention (-inf: the row has no weight).  Key t's score is row t %
  * page_size of page tables[r][t / page_size]: float at scores + page * s_sp + head * s_sh + row.  Keys
  * without a page and scores of no request's keys are left as they are; no key from first[r] on is
- * in two requests' tables.  first may be NULL (0).  One token or many: every key's sum is taken by
- * one wave in a fixed order.  scores shares no memory with an input or itself.
+ * in two requests' tables.  first may be NULL (0).  max_fresh: the most new tokens of a request (a hint, as
+ * in pa_paged_attn).  Every key's sum is taken in a fixed order.  scores shares no memory with an input or
+ * itself.  workspace as in pa_paged_attn, its sizes (which may be 0) from pa_weights_workspace.
  *
  * pa_choose_keys: for each of `layers` layers, request and KV head the keys that stay.  With m =
  * lengths[r] - first[r] (first may be NULL: 0; clamped to 0 .. lengths[r]): where m > limit, the `recent`
@@ -684,8 +685,11 @@ typedef struct pa_weights_args {
   int64_t lse_st, lse_sh;
   float* scores;
   int64_t s_sp, s_sh;
+  void* workspace;
+  int64_t workspace_bytes;
 } pa_weights_args;
 
+int pa_weights_workspace(const pa_weights_args* args, int64_t* bytes, int64_t* zero_bytes);
 int pa_paged_weights(const pa_weights_args* args, void* stream);
 
 typedef struct pa_choose_args {

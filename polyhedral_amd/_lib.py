@@ -107,7 +107,7 @@ class PaWeightsArgs(ctypes.Structure):
                 ("cols", c_i32), ("lengths", c_vp), ("q_start", c_vp), ("first", c_vp), ("R", c_i32), ("T", c_i64),
                 ("max_fresh", c_i64), ("Hq", c_i32), ("Hkv", c_i32), ("D", c_i32), ("dtype", c_i32), ("scale", c_f32),
                 ("mask", PaMask), ("lse", c_vp), ("lse_st", c_i64), ("lse_sh", c_i64), ("scores", c_vp), ("s_sp", c_i64),
-                ("s_sh", c_i64)]
+                ("s_sh", c_i64), ("workspace", c_vp), ("workspace_bytes", c_i64)]
 
 
 class PaChooseArgs(ctypes.Structure):
@@ -166,6 +166,7 @@ SIGNATURES = {
     "pa_share_rows": (ctypes.c_int, [ctypes.POINTER(PaShareArgs), c_vp]),
     "pa_shared_workspace": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), ctypes.POINTER(c_i64), ctypes.POINTER(c_i64)]),
     "pa_shared_attn": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), ctypes.POINTER(PaSharing), c_vp]),
+    "pa_weights_workspace": (ctypes.c_int, [ctypes.POINTER(PaWeightsArgs), ctypes.POINTER(c_i64), ctypes.POINTER(c_i64)]),
     "pa_paged_weights": (ctypes.c_int, [ctypes.POINTER(PaWeightsArgs), c_vp]),
     "pa_choose_keys": (ctypes.c_int, [ctypes.POINTER(PaChooseArgs), c_vp]),
     "pa_evict_rows": (ctypes.c_int, [ctypes.POINTER(PaEvictArgs), c_vp]),

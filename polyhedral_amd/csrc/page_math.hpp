@@ -199,6 +199,44 @@ PA_HD KeyList key_list(const PageMask<Ptr>& m, int32_t q0, int32_t q1, int32_t l
   return l;
 }
 
+// Queries that may see a key of k0 .. k1: positions lo .. hi.
+struct QueryRange {
+  int32_t lo, hi;
+};
+template <typename Ptr>
+PA_HD QueryRange query_range(const PageMask<Ptr>& m, int32_t k0, int32_t k1) {
+  QueryRange r{kMaxPosition, -1};
+#pragma unroll 1
+  for (int i = 0; i < m.n_include; ++i) {
+    const pa_term t = m.term(i);
+    int32_t lo = k0, hi = kMaxPosition;
+    switch (t.kind) {
+      case PA_WINDOW:
+        hi = imin(k1, kMaxPosition - t.p0) + t.p0 - 1;
+        break;
+      case PA_SINKS:
+        if (k0 >= t.p1) hi = imin(k1, kMaxPosition - t.p0) + t.p0 - 1;
+        break;
+      case PA_TWOBAND: {
+        const int32_t far = imax(t.p0, t.p2 > 0 ? imin(t.p1, kMaxPosition - t.p2) + t.p2 : 0);
+        hi = imin(k1, kMaxPosition - far) + far - 1;
+        break;
+      }
+      case PA_PREFIX_LM:
+        if (k0 < t.p0) lo = 0;
+        break;
+      case PA_FULL:
+        lo = 0;
+        break;
+      default:
+        break;
+    }
+    r.lo = imin(r.lo, lo);
+    r.hi = imax(r.hi, hi);
+  }
+  return r;
+}
+
 // Page of a request's table, or -1 where it names none of the cache.
 PA_HD int32_t checked_page(int32_t page, int64_t n_pages) {
   return (uint32_t)page < (uint64_t)n_pages ? page : -1;

@@ -9,6 +9,7 @@
 // added up over the row tiles, and over the 16 rows at the end, in a fixed order.
 //
 // Scores, exponentials and sums are float32.  A dead pair adds 0 whatever its key holds, by selection.
+#include <limits.h>
 #include <math.h>
 
 #include "page_checks.hpp"
@@ -38,6 +39,12 @@ struct WeightsK {
   int64_t lse_st, lse_sh;  // elements
   float* scores;
   int64_t s_sp, s_sh;  // elements
+  // requests with more rows (new tokens times heads of a group) than row_max are taken by the first tile_grid
+  // work-groups, the others by the rest
+  int32_t row_max, tile_grid;
+  float by_shares;     // 1 / the shares that the former's work is cut into
+  float* part;         // [slots][256] sums of split groups' shares
+  int32_t* count;      // [slots] shares done, at a group's first slot; zero between calls
 };
 
 __device__ __forceinline__ KernelMask weights_mask(const WeightsK& a) {
@@ -88,7 +95,7 @@ __device__ __forceinline__ WeighedRequest weighed(const WeightsK& a, int r0, int
   x.first = imin(imax(first, 0), x.rq.len);
   x.block0 = x.first >> LG;
   // (without new tokens nothing changes)
-  x.blocks = r < a.R && x.rq.n > 0 ? ((x.rq.len + (1 << LG) - 1) >> LG) - x.block0 : 0;
+  x.blocks = r < a.R && x.rq.n > 0 && x.rq.n * a.G <= a.row_max ? ((x.rq.len + (1 << LG) - 1) >> LG) - x.block0 : 0;
   x.cost = 2 + (x.rq.n * a.G + kRows - 1) / kRows;
   return x;
 }
@@ -108,8 +115,9 @@ __device__ __forceinline__ int64_t readlane64(int64_t x, int l) {
   return (int64_t)((uint64_t)lo | (uint64_t)(uint32_t)hi << 32);
 }
 
+// Few rows a request: blocks of keys, a wave each.
 template <typename T, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void weights_kernel(const WeightsK a) {
+__device__ __forceinline__ void weigh_blocks(const WeightsK& a, int32_t id, int32_t grid) {
   using S = WeightsShape<T, D>;
   constexpr int NS = S::NS, NK = S::NK, LG = S::LG, PER = S::PER;
   const int tid = threadIdx.x, lane = tid & 63, q16 = lane & 15, g = lane >> 4;
@@ -125,7 +133,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void w
     x = weighed<LG>(a, r0, lane, end);
     total += readlane64(wave_scan64((int64_t)x.blocks * a.Hkv * x.cost, lane), 63);
   }
-  const int64_t waves = (int64_t)gridDim.x * 4, me = (int64_t)blockIdx.x * 4 + w;
+  const int64_t waves = (int64_t)grid * 4, me = (int64_t)id * 4 + w;
   const int64_t per = total / waves, more = total - per * waves;
   const int64_t lo = per * me + (me < more ? me : more), hi = lo + per + (me < more ? 1 : 0);
   if (lo >= hi) return;
@@ -134,7 +142,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void w
   end = 0;
   for (int r0 = 0; r0 < a.R && before < hi; r0 += 64) {
     if (a.R > 64) x = weighed<LG>(a, r0, lane, end);
-    if (a.R <= 64) end = 0;
     const int64_t mine = (int64_t)x.blocks * a.Hkv * x.cost, in = wave_scan64(mine, lane), at = before + in - mine;
     uint64_t hit = __ballot(at < hi && at + mine > lo);
     before += readlane64(in, 63);
@@ -282,22 +289,300 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void w
   }
 }
 
+// ---- many rows a request ------------------------------------------------------------------------
+// A unit is 256 keys of one KV head and one of `splits` equal shares of the 64-row steps that may see them.  A
+// wave holds 64 keys in registers, as the A operand of 32x32 MFMAs; the rows of Q come by LDS DMA, 64 a step in
+// two slots, and are read as the B operand by all four waves.  Lane l then has row l % 32 and 16 of 32 keys,
+// whose exponentials it adds up over all steps, those of one 32 rows beside the MFMAs of the next; at the end
+// the 32 lanes' sums are added by halves.  Shares of a group leave their sums in the workspace, and the last
+// one adds them in order.
+constexpr int kKeysLg = 8, kKeys = 1 << kKeysLg, kStepRows = 64;
+
+template <typename T, int D>
+struct WeighTile {
+  static constexpr int ROW = 2 * D, SLOT = kStepRows * ROW;
+};
+
+struct KeyUnit {
+  Request rq;
+  int32_t r, first, h, group, share, splits, slot;
+};
+struct KeyWork {
+  Request rq;
+  int32_t first, group0, groups, steps;
+};
+__device__ __forceinline__ KeyWork key_work(const WeightsK& a, int r0, int lane, int32_t& end) {
+  const WeighedRequest x = weighed<kKeysLg>(a, r0, lane, end);
+  KeyWork k{x.rq, x.first, x.block0, 0, 0};
+  const int32_t rows = x.rq.n * a.G;
+  if (r0 + lane < a.R && rows > a.row_max) {
+    k.groups = ((x.rq.len + kKeys - 1) >> kKeysLg) - x.block0;
+    k.steps = (rows + kStepRows - 1) / kStepRows;
+  }
+  return k;
+}
+// Unit `id`, false past the last.  share: steps of a share (0 at first).
+__device__ __forceinline__ bool find_keys(const WeightsK& a, int32_t id, int lane, float& share, KeyUnit& u) {
+  KeyWork k{};
+  int32_t end = 0;
+  if (share == 0.f || a.R <= 64) {
+    float total = 0.f;
+    for (int r0 = 0; r0 < a.R; r0 += 64) {
+      k = key_work(a, r0, lane, end);
+      total += wave_total((float)k.groups * (float)k.steps);
+    }
+    share = fmaxf(total * (float)a.Hkv * a.by_shares, 8.f);
+  }
+  int64_t before = 0;
+  int32_t slot = 0;
+  end = 0;
+  for (int r0 = 0; r0 < a.R; r0 += 64) {
+    if (a.R > 64) k = key_work(a, r0, lane, end);
+    const int32_t splits = imax((int32_t)((float)k.steps / share + 0.5f), 1);
+    const int64_t units = (int64_t)k.groups * a.Hkv * splits;
+    const int32_t slotted = splits > 1 ? (int32_t)units : 0;
+    const int64_t n_in = wave_scan64(units, lane), at = before + n_in - units;
+    const int32_t s_in = wave_scan(slotted);
+    const uint64_t hit = __ballot(at <= id && id < at + units);
+    if (hit) {
+      const int l = (int)__builtin_ctzll(hit);
+      auto get = [&](int32_t y) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(y, l); };
+      u.rq = {get(k.rq.start), get(k.rq.n), get(k.rq.len)};
+      u.r = r0 + l;
+      u.first = get(k.first);
+      u.splits = get(splits);
+      // heads side by side, as in find_unit
+      const uint32_t i = (uint32_t)(id - readlane64(at, l)), y = i / (uint32_t)a.Hkv;
+      u.h = (int32_t)(i - y * (uint32_t)a.Hkv);
+      const int32_t group = (int32_t)(y / (uint32_t)u.splits);
+      u.share = (int32_t)y - group * u.splits;
+      u.group = get(k.group0) + group;
+      u.slot = slot + get(s_in - slotted) + (group * a.Hkv + u.h) * u.splits;
+      return true;
+    }
+    before += readlane64(n_in, 63);
+    slot += __builtin_amdgcn_readlane(s_in, 63);
+  }
+  return false;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, char* smem, int32_t* flag) {
+  using Frag = typename Mma<T>::frag;
+  using R = Rows<D>;
+  constexpr int NQF = D / 16, SLOT = WeighTile<T, D>::SLOT;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, m = lane & 31;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char_t*)smem;
+  const KernelMask mask = weights_mask(a);
+  const int32_t len = u.rq.len, pos0 = len - u.rq.n, rows = u.rq.n * a.G;
+  const int32_t key0 = (u.group << kKeysLg) + 64 * w;  // this wave's first key
+  const int32_t* table = a.tables + (int64_t)u.r * a.pitch;
+  const int one = (1 << a.page_lg) - 1;
+
+  // ---- the keys (one past the length or without a page: some row of page 0, whose sum goes nowhere) ----
+  Frag kf[2][NQF];
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int32_t key = key0 + 32 * b + m;
+    const int32_t page = key < len ? checked_page(table[key >> a.page_lg], a.n_pages) : -1;
+    const char* row = a.k + (int64_t)imax(page, 0) * a.c_sp + u.h * a.c_sh + (int64_t)(key & one) * a.c_sn + 16 * half;
+#pragma unroll
+    for (int kc = 0; kc < NQF; ++kc) kf[b][kc] = __builtin_bit_cast(Frag, *reinterpret_cast<const u32x4*>(row + 32 * kc));
+  }
+
+  // ---- the steps: rows of tokens that may see one of the group's keys ----
+  const QueryRange q = query_range(mask, u.group << kKeysLg, imin((u.group << kKeysLg) + kKeys, len) - 1);
+  const int32_t t0 = imin(imax(q.lo - pos0, 0), u.rq.n), t1 = imin(imax(imin(q.hi, len) - pos0 + 1, t0), u.rq.n);
+  const int32_t first_step = t0 * a.G / kStepRows, n_steps = t1 > t0 ? (t1 * a.G + kStepRows - 1) / kStepRows - first_step : 0;
+  int32_t j0, j1;
+  share_of(n_steps, u.share, u.splits, &j0, &j1);
+  j0 += first_step;
+  j1 += first_step;
+
+  lds_cptr rd[NQF];  // row m of 32 staged ones, units 2 kc + half
+#pragma unroll
+  for (int kc = 0; kc < NQF; ++kc) rd[kc] = (lds_cptr)smem + m * R::ROW + 16 * ((2 * kc + half) ^ R::swz(m));
+  auto stage = [&](int32_t j, int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < R::NI; ++x) {
+      const int row = 16 * w + R::RPI * x + lane / R::UPR;
+      const int32_t i = imin(j * kStepRows + row, rows - 1), tok = divide(i, a.by_G);
+      dma_x4_va(lds0 + slot * SLOT + 16 * w * R::ROW + x * 1024,
+                a.q + (int64_t)(u.rq.start + tok) * a.q_st + (int64_t)(u.h * a.G + (i - tok * a.G)) * a.q_sh +
+                    16 * ((lane % R::UPR) ^ R::swz(R::RPI * x + lane / R::UPR)));
+    }
+  };
+  // -lse in log2 units of row j kStepRows + lane (no row, or one without weight: +inf, told by `none`)
+  auto load_lse = [&](int32_t j) __attribute__((always_inline)) -> float {
+    const int32_t i = j * kStepRows + lane, ic = imin(i, rows - 1), tok = divide(ic, a.by_G);
+    const float z = a.lse[(int64_t)(u.rq.start + tok) * a.lse_st + (int64_t)(u.h * a.G + (ic - tok * a.G)) * a.lse_sh];
+    return i < rows ? z : -INFINITY;
+  };
+
+  f32x16 sum0 = f32x16{0}, sum1 = f32x16{0};
+  float c_exp = a.c;
+  asm volatile("" : "+s"(c_exp));
+  auto add = [&](const f32x16& x, float neg, f32x16& sum) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c_exp, neg));
+  };
+  auto mask_block = [&](f32x16& x, uint32_t word) __attribute__((always_inline)) {
+    word >>= 4 * half;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float xv = x[e];
+      const int32_t keep = __builtin_amdgcn_sbfe((int32_t)word, 8 * (e >> 2) + (e & 3), 1);
+      x[e] = __builtin_bit_cast(float, (__builtin_bit_cast(int32_t, xv) & keep) | (int32_t)(0xff800000u & ~(uint32_t)keep));
+    }
+  };
+  f32x16 x0 = f32x16{0}, x1 = f32x16{0};
+  float neg = 0.f;
+  bool have = false;  // x0, x1: scores whose exponentials are still to be added
+  if (j0 < j1) {
+    stage(j0, 0);
+    float z = load_lse(j0);
+#pragma unroll 1
+    for (int32_t j = j0; j < j1; ++j) {
+      const int slot = (j - j0) & 1;
+      dma_wait_all();
+      asm volatile("" ::"v"(z));
+      __syncthreads();
+      const float z_now = z;
+      if (j + 1 < j1) {
+        stage(j + 1, 1 - slot);
+        z = load_lse(j + 1);
+      }
+      const uint64_t ok = __ballot(z_now != -INFINITY);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int32_t i0 = j * kStepRows + 32 * b;
+        if (i0 >= rows) break;
+        const int32_t q_lo = pos0 + divide(i0, a.by_G), q_hi = pos0 + divide(imin(i0 + 31, rows - 1), a.by_G);
+        int v = mask_verdict(mask, q_lo, q_hi, key0, key0 + 63);
+        if (v == kDead) continue;
+        const uint32_t rows_ok = (uint32_t)(ok >> (32 * b));
+        if (rows_ok != ~0u || (v == kFull && key0 + 63 >= len)) v = kPartial;
+        const float zb = __shfl(z_now, 32 * b + m);
+        f32x16 y0, y1;
+        u32x4 qf[NQF];
+#pragma unroll
+        for (int kc = 0; kc < NQF; ++kc) qf[kc] = *(lds_u4*)(rd[kc] + slot * SLOT + 32 * b * R::ROW);
+        y0 = Mma<T>::mma(kf[0][0], __builtin_bit_cast(Frag, qf[0]), f32x16{0});
+#pragma unroll
+        for (int kc = 1; kc < NQF; ++kc) y0 = Mma<T>::mma(kf[0][kc], __builtin_bit_cast(Frag, qf[kc]), y0);
+        y1 = Mma<T>::mma(kf[1][0], __builtin_bit_cast(Frag, qf[0]), f32x16{0});
+#pragma unroll
+        for (int kc = 1; kc < NQF; ++kc) y1 = Mma<T>::mma(kf[1][kc], __builtin_bit_cast(Frag, qf[kc]), y1);
+        if (have) {
+          add(x0, neg, sum0);
+          add(x1, neg, sum1);
+        }
+        if (v != kFull) {
+          const bool row = (rows_ok >> m) & 1u;
+          const int32_t pos = pos0 + divide(imin(i0 + m, rows - 1), a.by_G);
+          mask_block(y0, row ? mask_word(mask, pos, key0, len) : 0u);
+          mask_block(y1, row ? mask_word(mask, pos, key0 + 32, len) : 0u);
+        }
+        x0 = y0;
+        x1 = y1;
+        neg = (rows_ok >> m) & 1u ? -zb * 1.4426950408889634f : 0.f;
+        have = true;
+      }
+    }
+    if (have) {
+      add(x0, neg, sum0);
+      add(x1, neg, sum1);
+    }
+  }
+
+  // ---- over the 32 rows: lane l ends with the sum of key 32 (l / 16 % 2) + 8 (l / 4 % 4) + 4 half + l % 4 ----
+  float v32[32];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    v32[e] = sum0[e];
+    v32[16 + e] = sum1[e];
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int e = 0; e < o; ++e) {
+      const float give = up ? v32[e] : v32[e + o];
+      v32[e] = (up ? v32[e + o] : v32[e]) + __shfl_xor(give, o);
+    }
+  }
+  float total = v32[0];
+  const int in_wave = 32 * ((lane >> 4) & 1) + 8 * ((lane >> 2) & 3) + 4 * half + (lane & 3);
+  if (u.splits > 1) {
+    float* first = a.part + (int64_t)u.slot * kKeys + 64 * w + lane;
+    share_store(first + u.share * kKeys, total);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+      const int32_t n = __hip_atomic_fetch_add(a.count + u.slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      *flag = n == u.splits - 1;
+      if (n == u.splits - 1) __hip_atomic_store(a.count + u.slot, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (*flag == 0) return;
+    total = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < u.splits; ++s) total += __hip_atomic_load(first + s * kKeys, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  const int32_t key = key0 + in_wave;
+  if (key < u.first || key >= len) return;
+  const int32_t page = checked_page(table[key >> a.page_lg], a.n_pages);
+  if (page < 0) return;
+  float* to = a.scores + page * a.s_sp + u.h * a.s_sh + (key & one);
+  *to = (key < pos0 ? *to : 0.f) + total;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void weights_kernel(const WeightsK a) {
+  if constexpr (sizeof(T) == 2) {
+    __shared__ __attribute__((aligned(256))) char smem[2 * WeighTile<T, D>::SLOT];
+    __shared__ int32_t flag;
+    if ((int32_t)blockIdx.x < a.tile_grid) {
+      float share = 0.f;
+      KeyUnit u;
+      for (int32_t id = (int32_t)blockIdx.x; find_keys(a, id, (int)threadIdx.x & 63, share, u); id += a.tile_grid) {
+        weigh_keys<T, D>(a, u, smem, &flag);
+        __syncthreads();  // (the slots and the flag have been read)
+      }
+      return;
+    }
+  }
+  weigh_blocks<T, D>(a, (int32_t)blockIdx.x - a.tile_grid, (int32_t)gridDim.x - a.tile_grid);
+}
+
+// The requests' rows from which they are taken by 256 keys, and the work-groups and shares of those.
+constexpr int kFewRows = 32, kTileGroups = 512, kTileShares = 1536;
+
+struct WeightsPlan {
+  bool tile;
+  int64_t slots, zero, bytes;
+};
+WeightsPlan weights_plan(const pa_weights_args* x) {
+  const int64_t most = x->max_fresh < x->T ? x->max_fresh : x->T;
+  WeightsPlan p;
+  p.tile = x->dtype != PA_F32 && most * (x->Hq / x->Hkv) > kFewRows;
+  p.slots = p.tile ? 2 * kTileShares : 0;  // (a group that is split has at most 4/3 of the shares that its work fills)
+  p.zero = (4 * p.slots + 255) / 256 * 256;
+  p.bytes = p.zero + 4 * p.slots * kKeys;
+  return p;
+}
+
 template <typename T, int D>
 int launch_weights(const WeightsK& a, hipStream_t s) {
-  hipLaunchKernelGGL((weights_kernel<T, D>), dim3(1024), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((weights_kernel<T, D>), dim3((unsigned)(a.tile_grid + 1024)), dim3(256), 0, s, a);
   PA_LAUNCH_CHECK("weights_kernel");
   return PA_OK;
 }
 
-}  // namespace
-}  // namespace pa
-
-extern "C" int pa_paged_weights(const pa_weights_args* x, void* stream) {
-  using namespace pa;
-  const char* who = "pa_paged_weights";
+int check_weights(const char* who, const pa_weights_args* x, int* page_lg) {
   PA_CHECK_ARG(x, "%s: null arguments", who);
-  int lg;
-  if (int rc = check_pages(who, x->n_pages, x->page_size, &lg)) return rc;
+  if (int rc = check_pages(who, x->n_pages, x->page_size, page_lg)) return rc;
   PA_CHECK_ARG(x->dtype == PA_BF16 || x->dtype == PA_F16 || x->dtype == PA_F32, "%s: dtype %d", who, x->dtype);
   PA_CHECK_ARG(x->D == 64 || x->D == 128, "%s: D=%d (64 or 128)", who, x->D);
   PA_CHECK_ARG(x->Hkv >= 1 && x->Hq >= x->Hkv && x->Hq % x->Hkv == 0 && x->Hq <= 65535,
@@ -305,13 +590,35 @@ extern "C" int pa_paged_weights(const pa_weights_args* x, void* stream) {
   PA_CHECK_ARG(x->R >= 0 && x->T >= 0 && x->T <= kMaxPosition && x->T * x->Hq <= kMaxPosition, "%s: R=%d T=%lld Hq=%d (T Hq < 2^30)", who,
                x->R, (long long)x->T, x->Hq);
   PA_CHECK_ARG(x->max_fresh >= 0, "%s: max_fresh=%lld", who, (long long)x->max_fresh);
-  PA_CHECK_ARG(x->cols >= 0 && ((int64_t)x->cols << lg) <= kMaxPosition && x->pitch >= x->cols, "%s: %d columns of %d, pitch %lld", who,
+  PA_CHECK_ARG(x->cols >= 0 && ((int64_t)x->cols << *page_lg) <= kMaxPosition && x->pitch >= x->cols, "%s: %d columns of %d, pitch %lld", who,
                x->cols, x->page_size, (long long)x->pitch);
   PA_CHECK_ARG(!x->mask.perm_q && !x->mask.perm_kv, "%s: the mask takes no permutation tables", who);
   for (int i = 0; i < x->mask.n_include + x->mask.n_exclude && i < PA_MAX_TERMS; ++i)
     PA_CHECK_ARG(x->mask.terms[i].kind != PA_DENSE, "%s: PA_DENSE has no meaning here", who);
   if (int rc = check_mask(&x->mask, 0)) return rc;
   PA_CHECK_ARG(x->scale > 0.f && x->scale < INFINITY, "%s: scale=%g must be positive", who, (double)x->scale);
+  return PA_OK;
+}
+
+}  // namespace
+}  // namespace pa
+
+extern "C" int pa_weights_workspace(const pa_weights_args* x, int64_t* bytes, int64_t* zero) {
+  using namespace pa;
+  int lg;
+  if (int rc = check_weights("pa_paged_weights", x, &lg)) return rc;
+  PA_CHECK_ARG(bytes && zero, "pa_paged_weights: null output");
+  const WeightsPlan p = weights_plan(x);
+  *bytes = p.bytes;
+  *zero = p.zero;
+  return PA_OK;
+}
+
+extern "C" int pa_paged_weights(const pa_weights_args* x, void* stream) {
+  using namespace pa;
+  const char* who = "pa_paged_weights";
+  int lg;
+  if (int rc = check_weights(who, x, &lg)) return rc;
   if (x->R == 0 || x->T == 0 || x->n_pages == 0 || x->cols == 0) return PA_OK;
   PA_CHECK_ARG(x->q && x->k && x->lse && x->scores && x->tables && x->lengths && x->q_start, "%s: null pointer", who);
   const int64_t esz = x->dtype == PA_F32 ? 4 : 2, row = x->D * esz, R = x->R;
@@ -325,14 +632,24 @@ extern "C" int pa_paged_weights(const pa_weights_args* x, void* stream) {
   // scores are written while the inputs are read, a page's by different waves
   const Strided<2> scores = strided<2>(x->scores, 4ll * x->page_size, {x->n_pages, x->Hkv}, {x->s_sp, x->s_sh}, 4);
   PA_CHECK_ARG(nested(scores), "%s: rows of scores overlap", who);
-  const char* other = overlap(scores, strided<2>(x->q, row, {x->T, x->Hq}, {x->q_st, x->q_sh}, (int)esz)) ? "q"
-                      : overlap(scores, strided<3>(x->k, row, {x->n_pages, x->Hkv, x->page_size}, {x->c_sp, x->c_sh, x->c_sn}, (int)esz)) ? "k"
-                      : overlap(scores, strided<2>(x->lse, 4, {x->T, x->Hq}, {x->lse_st, x->lse_sh}, 4)) ? "lse"
-                      : overlap(scores, tables_span(x->tables, x->R, x->pitch, x->cols)) ? "tables"
-                      : overlap(scores, flat(x->lengths, 4 * R)) ? "lengths"
-                      : overlap(scores, flat(x->q_start, 4 * (R + 1))) ? "q_start"
-                      : overlap(scores, flat(x->first, x->first ? 4 * R : 0)) ? "first" : nullptr;
+  auto in_of = [&](const auto& out) -> const char* {
+    return overlap(out, strided<2>(x->q, row, {x->T, x->Hq}, {x->q_st, x->q_sh}, (int)esz)) ? "q"
+           : overlap(out, strided<3>(x->k, row, {x->n_pages, x->Hkv, x->page_size}, {x->c_sp, x->c_sh, x->c_sn}, (int)esz)) ? "k"
+           : overlap(out, strided<2>(x->lse, 4, {x->T, x->Hq}, {x->lse_st, x->lse_sh}, 4)) ? "lse"
+           : overlap(out, tables_span(x->tables, x->R, x->pitch, x->cols)) ? "tables"
+           : overlap(out, flat(x->lengths, 4 * R)) ? "lengths"
+           : overlap(out, flat(x->q_start, 4 * (R + 1))) ? "q_start"
+           : overlap(out, flat(x->first, x->first ? 4 * R : 0)) ? "first" : nullptr;
+  };
+  const char* other = in_of(scores);
   PA_CHECK_ARG(!other, "%s: scores and %s overlap", who, other);
+  const WeightsPlan p = weights_plan(x);
+  PA_CHECK_ARG(p.bytes == 0 || (x->workspace && reinterpret_cast<uintptr_t>(x->workspace) % 256 == 0 && x->workspace_bytes >= p.bytes),
+               "%s: needs a 256-byte aligned workspace of %lld bytes", who, (long long)p.bytes);
+  const Strided<1> ws = flat(x->workspace, p.bytes);
+  other = in_of(ws);
+  PA_CHECK_ARG(!other, "%s: workspace and %s overlap", who, other);
+  PA_CHECK_ARG(!overlap(ws, scores), "%s: workspace and scores overlap", who);
   WeightsK a;
   a.q = static_cast<const char*>(x->q);
   a.q_st = x->q_st * esz;
@@ -371,6 +688,11 @@ extern "C" int pa_paged_weights(const pa_weights_args* x, void* stream) {
   a.scores = x->scores;
   a.s_sp = x->s_sp;
   a.s_sh = x->s_sh;
+  a.row_max = p.tile ? kFewRows : INT_MAX;
+  a.tile_grid = p.tile ? kTileGroups : 0;
+  a.by_shares = 1.f / (float)kTileShares;
+  a.count = reinterpret_cast<int32_t*>(x->workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(x->workspace) + p.zero);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (x->D == 64)
     return x->dtype == PA_F32 ? launch_weights<float, 64>(a, s) : x->dtype == PA_BF16 ? launch_weights<__bf16, 64>(a, s) : launch_weights<_Float16, 64>(a, s);

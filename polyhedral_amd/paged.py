@@ -273,6 +273,16 @@ def _scale(scale, D):
     return scale
 
 
+def _workspace(sizes, a, device):
+    """The workspace of the call with arguments ``a``, whose pointer is set, and the part of it that is zero
+    before the first run (None: none)."""
+    nbytes, zero = ctypes.c_int64(0), ctypes.c_int64(0)
+    _lib.check(getattr(_lib.lib(), sizes)(ctypes.byref(a), ctypes.byref(nbytes), ctypes.byref(zero)), sizes)
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+    a.workspace, a.workspace_bytes = _lib.address(ws), nbytes.value
+    return ws, ws[:zero.value] if zero.value else None
+
+
 def _attention_launch(entry, q, k, v, tables, lengths, q_start, sharing, mask, scale, max_fresh, out, lse):
     """The PagedLaunch of prepare_attention and prepare_shared_attention."""
     pages, Hkv, P, D = _cache(k, v)
@@ -314,12 +324,9 @@ def _attention_launch(entry, q, k, v, tables, lengths, q_start, sharing, mask, s
     if sharing is not None:
         s = _sharing_struct(sharing, R, T, dev)
         call += (ctypes.byref(s),)
-    nbytes, zero = ctypes.c_int64(0), ctypes.c_int64(0)
-    _lib.check(getattr(_lib.lib(), sizes)(ctypes.byref(a), ctypes.byref(nbytes), ctypes.byref(zero)), sizes)
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = ptr(ws), nbytes.value
+    ws, zero = _workspace(sizes, a, dev)
     return PagedLaunch(entry + "_attn", call, [call, a, q, k, v, tables, lengths, q_start, sharing, dm, o, lse, ws], k, o,
-                       zero=ws[:zero.value])
+                       zero=zero)
 
 
 def prepare_attention(q, k, v, tables, lengths, q_start, mask, scale=None, max_fresh=None, out=None, lse=None):
@@ -461,7 +468,9 @@ def prepare_weights(q, k, tables, lengths, q_start, lse, scores, mask, scale=Non
     a.mask = dm.struct()
     a.lse, a.lse_st, a.lse_sh = ptr(lse), lse.stride(0), lse.stride(1)
     a.scores, (a.s_sp, a.s_sh) = ptr(scores), _scores(scores, (pages, Hkv, P), dev)
-    return PagedLaunch("pa_paged_weights", (ctypes.byref(a),), [a, q, k, tables, lengths, q_start, lse, scores, first, dm], k, scores)
+    ws, zero = _workspace("pa_weights_workspace", a, dev)
+    return PagedLaunch("pa_paged_weights", (ctypes.byref(a),), [a, q, k, tables, lengths, q_start, lse, scores, first, dm, ws], k,
+                       scores, zero=zero)
 
 
 def weights(q, k, tables, lengths, q_start, lse, scores, mask, scale=None, first=None, max_fresh=None):
