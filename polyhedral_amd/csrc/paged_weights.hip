@@ -42,6 +42,7 @@ struct WeightsK {
   // requests with more rows (new tokens times heads of a group) than row_max are taken by the first tile_grid
   // work-groups, the others by the rest
   int32_t row_max, tile_grid;
+  int32_t even;        // a step's rows are whole tokens, whose offsets in q and lse fit 31 bits
   float by_shares;     // 1 / the shares that the former's work is cut into
   float* part;         // [slots][256] sums of split groups' shares
   int32_t* count;      // [slots] shares done, at a group's first slot; zero between calls
@@ -403,29 +404,59 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
   lds_cptr rd[NQF];  // row m of 32 staged ones, units 2 kc + half
 #pragma unroll
   for (int kc = 0; kc < NQF; ++kc) rd[kc] = (lds_cptr)smem + m * R::ROW + 16 * ((2 * kc + half) ^ R::swz(m));
-  auto stage = [&](int32_t j, int slot) __attribute__((always_inline)) {
+  // Step j's rows, 16 a wave, and -lse of row l for lane l (a row past the last: -inf).  Where a step is whole
+  // tokens it is one uniform pointer and the lanes' offsets, which stay.
+  uint32_t off[R::NI];
+#pragma unroll
+  for (int x = 0; x < R::NI; ++x) {
+    const int i = 16 * w + R::RPI * x + lane / R::UPR, tok = divide(i, a.by_G);
+    off[x] = (uint32_t)tok * (uint32_t)a.q_st + (uint32_t)(i - tok * a.G) * (uint32_t)a.q_sh +
+             16u * (uint32_t)((lane % R::UPR) ^ R::swz(R::RPI * x + lane / R::UPR));
+  }
+  const int lse_tok = divide(lane, a.by_G);
+  const int32_t lse_off = (int32_t)(lse_tok * (int32_t)a.lse_st + (lane - lse_tok * a.G) * (int32_t)a.lse_sh);
+  const int32_t whole = a.even ? rows / kStepRows : 0;  // steps that are
+  const char* q0 = a.q + (int64_t)u.rq.start * a.q_st + (int64_t)u.h * a.G * a.q_sh;
+  const float* lse0 = a.lse + (int64_t)u.rq.start * a.lse_st + (int64_t)u.h * a.G * a.lse_sh;
+  auto stage = [&](int32_t j, int slot) __attribute__((always_inline)) -> float {
+    const uint32_t to = lds0 + slot * SLOT + 16 * w * R::ROW;
+    if (j < whole) {
+      const int32_t tok = divide(j * kStepRows, a.by_G);
+      const char* base = q0 + (int64_t)tok * a.q_st;
+#pragma unroll
+      for (int x = 0; x < R::NI; ++x) dma_x4(to + x * 1024, base, off[x]);
+      return (lse0 + (int64_t)tok * a.lse_st)[lse_off];
+    }
 #pragma unroll
     for (int x = 0; x < R::NI; ++x) {
-      const int row = 16 * w + R::RPI * x + lane / R::UPR;
-      const int32_t i = imin(j * kStepRows + row, rows - 1), tok = divide(i, a.by_G);
-      dma_x4_va(lds0 + slot * SLOT + 16 * w * R::ROW + x * 1024,
-                a.q + (int64_t)(u.rq.start + tok) * a.q_st + (int64_t)(u.h * a.G + (i - tok * a.G)) * a.q_sh +
-                    16 * ((lane % R::UPR) ^ R::swz(R::RPI * x + lane / R::UPR)));
+      const int i = imin(j * kStepRows + 16 * w + R::RPI * x + lane / R::UPR, rows - 1), tok = divide(i, a.by_G);
+      dma_x4_va(to + x * 1024, q0 + (int64_t)tok * a.q_st + (int64_t)(i - tok * a.G) * a.q_sh +
+                                   16 * ((lane % R::UPR) ^ R::swz(R::RPI * x + lane / R::UPR)));
     }
+    const int32_t i = imin(j * kStepRows + lane, rows - 1), tok = divide(i, a.by_G);
+    const float z = lse0[(int64_t)tok * a.lse_st + (int64_t)(i - tok * a.G) * a.lse_sh];
+    return j * kStepRows + lane < rows ? z : -INFINITY;
   };
-  // -lse in log2 units of row j kStepRows + lane (no row, or one without weight: +inf, told by `none`)
-  auto load_lse = [&](int32_t j) __attribute__((always_inline)) -> float {
-    const int32_t i = j * kStepRows + lane, ic = imin(i, rows - 1), tok = divide(ic, a.by_G);
-    const float z = a.lse[(int64_t)(u.rq.start + tok) * a.lse_st + (int64_t)(u.h * a.G + (ic - tok * a.G)) * a.lse_sh];
-    return i < rows ? z : -INFINITY;
+  // 64 steps at a time: bit l of live / full: some pair of this wave's keys and step l's rows may be live / all are
+  uint64_t live = 0ull, full = 0ull;
+  auto verdicts = [&](int32_t j) __attribute__((always_inline)) {
+    const int32_t i0 = imin((j + lane) * kStepRows, rows - 1), i1 = imin(i0 + kStepRows, rows) - 1;
+    const int v = mask_verdict(mask, pos0 + divide(i0, a.by_G), pos0 + divide(i1, a.by_G), key0, key0 + 63);
+    live = __ballot(v != kDead);
+    full = key0 + 63 < len ? __ballot(v == kFull) : 0ull;
   };
 
-  f32x16 sum0 = f32x16{0}, sum1 = f32x16{0};
+  float sum[32] = {};
   float c_exp = a.c;
   asm volatile("" : "+s"(c_exp));
-  auto add = [&](const f32x16& x, float neg, f32x16& sum) __attribute__((always_inline)) {
+  auto add = [&](const f32x16& x, float neg, float* to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sum[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c_exp, neg));
+    for (int e = 0; e < 16; ++e) to[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c_exp, neg));
+    // (or they are moved behind the branches that follow, away from the MFMAs)
+#pragma unroll
+    for (int e = 0; e < 16; e += 8)
+      asm volatile("" : "+v"(to[e]), "+v"(to[e + 1]), "+v"(to[e + 2]), "+v"(to[e + 3]), "+v"(to[e + 4]), "+v"(to[e + 5]), "+v"(to[e + 6]),
+                   "+v"(to[e + 7]));
   };
   auto mask_block = [&](f32x16& x, uint32_t word) __attribute__((always_inline)) {
     word >>= 4 * half;
@@ -436,12 +467,26 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
       x[e] = __builtin_bit_cast(float, (__builtin_bit_cast(int32_t, xv) & keep) | (int32_t)(0xff800000u & ~(uint32_t)keep));
     }
   };
-  f32x16 x0 = f32x16{0}, x1 = f32x16{0};
-  float neg = 0.f;
-  bool have = false;  // x0, x1: scores whose exponentials are still to be added
+  // Scores of 32 keys and 32 rows, in two places in turn: the exponentials of one are added beside the MFMAs of
+  // the other.
+  f32x16 xa, xb;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) xb[e] = -INFINITY;  // (dead)
+  float neg = 0.f;  // of the rows of the scores that are still to be added
+  auto block = [&](const Frag* k, const u32x4* qf, f32x16& y, const f32x16& x, float neg_x, float* to) __attribute__((always_inline)) {
+    y = Mma<T>::mma(k[0], __builtin_bit_cast(Frag, qf[0]), f32x16{0});
+#pragma unroll
+    for (int kc = 1; kc < NQF; ++kc) y = Mma<T>::mma(k[kc], __builtin_bit_cast(Frag, qf[kc]), y);
+    add(x, neg_x, to);
+#pragma unroll
+    for (int z = 0; z < NQF; ++z) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 2);
+      __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 6 : 12, 2);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
   if (j0 < j1) {
-    stage(j0, 0);
-    float z = load_lse(j0);
+    float z = stage(j0, 0);
 #pragma unroll 1
     for (int32_t j = j0; j < j1; ++j) {
       const int slot = (j - j0) & 1;
@@ -449,70 +494,45 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
       asm volatile("" ::"v"(z));
       __syncthreads();
       const float z_now = z;
-      if (j + 1 < j1) {
-        stage(j + 1, 1 - slot);
-        z = load_lse(j + 1);
-      }
-      const uint64_t ok = __ballot(z_now != -INFINITY);
+      if (j + 1 < j1) z = stage(j + 1, 1 - slot);
+      if (((j - j0) & 63) == 0) verdicts(j);
+      if (!((live >> ((j - j0) & 63)) & 1ull)) continue;
+      const int32_t i0 = j * kStepRows;
+      const uint64_t ok = __ballot(z_now != -INFINITY);  // (rows past the last have no weight)
+      const bool all = ok == ~0ull && ((full >> ((j - j0) & 63)) & 1ull);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const int32_t i0 = j * kStepRows + 32 * b;
-        if (i0 >= rows) break;
-        const int32_t q_lo = pos0 + divide(i0, a.by_G), q_hi = pos0 + divide(imin(i0 + 31, rows - 1), a.by_G);
-        int v = mask_verdict(mask, q_lo, q_hi, key0, key0 + 63);
-        if (v == kDead) continue;
-        const uint32_t rows_ok = (uint32_t)(ok >> (32 * b));
-        if (rows_ok != ~0u || (v == kFull && key0 + 63 >= len)) v = kPartial;
+        const bool row = (uint32_t)(ok >> (32 * b + m)) & 1u;
+        auto word = [&](int32_t key) __attribute__((always_inline)) -> uint32_t {
+          return row ? mask_word(mask, pos0 + divide(imin(i0 + 32 * b + m, rows - 1), a.by_G), key, len) : 0u;
+        };
         const float zb = __shfl(z_now, 32 * b + m);
-        f32x16 y0, y1;
         u32x4 qf[NQF];
 #pragma unroll
         for (int kc = 0; kc < NQF; ++kc) qf[kc] = *(lds_u4*)(rd[kc] + slot * SLOT + 32 * b * R::ROW);
-        y0 = Mma<T>::mma(kf[0][0], __builtin_bit_cast(Frag, qf[0]), f32x16{0});
-#pragma unroll
-        for (int kc = 1; kc < NQF; ++kc) y0 = Mma<T>::mma(kf[0][kc], __builtin_bit_cast(Frag, qf[kc]), y0);
-        y1 = Mma<T>::mma(kf[1][0], __builtin_bit_cast(Frag, qf[0]), f32x16{0});
-#pragma unroll
-        for (int kc = 1; kc < NQF; ++kc) y1 = Mma<T>::mma(kf[1][kc], __builtin_bit_cast(Frag, qf[kc]), y1);
-        if (have) {
-          add(x0, neg, sum0);
-          add(x1, neg, sum1);
-        }
-        if (v != kFull) {
-          const bool row = (rows_ok >> m) & 1u;
-          const int32_t pos = pos0 + divide(imin(i0 + m, rows - 1), a.by_G);
-          mask_block(y0, row ? mask_word(mask, pos, key0, len) : 0u);
-          mask_block(y1, row ? mask_word(mask, pos, key0 + 32, len) : 0u);
-        }
-        x0 = y0;
-        x1 = y1;
-        neg = (rows_ok >> m) & 1u ? -zb * 1.4426950408889634f : 0.f;
-        have = true;
+        __builtin_amdgcn_sched_barrier(0);
+        block(kf[0], qf, xa, xb, neg, sum + 16);
+        neg = row ? -zb * 1.4426950408889634f : 0.f;
+        if (!all) mask_block(xa, word(key0));
+        block(kf[1], qf, xb, xa, neg, sum);
+        if (!all) mask_block(xb, word(key0 + 32));
       }
     }
-    if (have) {
-      add(x0, neg, sum0);
-      add(x1, neg, sum1);
-    }
+    add(xb, neg, sum + 16);
   }
 
   // ---- over the 32 rows: lane l ends with the sum of key 32 (l / 16 % 2) + 8 (l / 4 % 4) + 4 half + l % 4 ----
-  float v32[32];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    v32[e] = sum0[e];
-    v32[16 + e] = sum1[e];
-  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const bool up = lane & o;
 #pragma unroll
     for (int e = 0; e < o; ++e) {
-      const float give = up ? v32[e] : v32[e + o];
-      v32[e] = (up ? v32[e + o] : v32[e]) + __shfl_xor(give, o);
+      float x = sum[e], y = sum[e + o];
+      asm("" : "+v"(x), "+v"(y));  // (or the index is selected, and the value by as many comparisons)
+      sum[e] = (up ? y : x) + __shfl_xor(up ? x : y, o);
     }
   }
-  float total = v32[0];
+  float total = sum[0];
   const int in_wave = 32 * ((lane >> 4) & 1) + 8 * ((lane >> 2) & 3) + 4 * half + (lane & 3);
   if (u.splits > 1) {
     float* first = a.part + (int64_t)u.slot * kKeys + 64 * w + lane;
@@ -557,7 +577,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void w
 }
 
 // The requests' rows from which they are taken by 256 keys, and the work-groups and shares of those.
-constexpr int kFewRows = 32, kTileGroups = 512, kTileShares = 1536;
+constexpr int kFewRows = 32, kTileGroups = 512, kTileShares = 1024;
 
 struct WeightsPlan {
   bool tile;
@@ -690,6 +710,8 @@ extern "C" int pa_paged_weights(const pa_weights_args* x, void* stream) {
   a.s_sh = x->s_sh;
   a.row_max = p.tile ? kFewRows : INT_MAX;
   a.tile_grid = p.tile ? kTileGroups : 0;
+  auto near = [&](int64_t st, int64_t sh) { return st <= (1 << 24) && sh <= (1 << 24) && st >= -(1 << 24) && sh >= -(1 << 24); };
+  a.even = kStepRows % a.G == 0 && near(a.q_st, a.q_sh) && near(a.lse_st, a.lse_sh);
   a.by_shares = 1.f / (float)kTileShares;
   a.count = reinterpret_cast<int32_t*>(x->workspace);
   a.part = reinterpret_cast<float*>(static_cast<char*>(x->workspace) + p.zero);
