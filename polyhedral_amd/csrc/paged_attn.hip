@@ -37,7 +37,7 @@ struct PagedPlan {
   PagedPart rows, tiles;
   PagedPart pre_rows, pre_tiles;  // of the prefixes that requests share
   int64_t zero, bytes;
-  int64_t pre_o, pre_ml;          // where their states begin
+  int64_t states, own, at;        // where the states of their shares begin, those of own keys, and their places
 };
 
 // A part whose requests have at most max_tiles tiles: its grid and slots.  (The shares of all tiles are
@@ -118,15 +118,20 @@ int plan_of(const char* who, const pa_paged_args* x, bool sharing, PagedPlan* p)
       p->pre_tiles.row_min = kFewRows;
       p->pre_tiles.row_max = INT_MAX;
     }
-    PA_CHECK_ARG((int64_t)p->pre_rows.grid + p->pre_tiles.grid <= kMaxGroups, "%s: %lld work-groups exceed the grid limit", who,
-                 (long long)p->pre_rows.grid + p->pre_tiles.grid);
+    PA_CHECK_ARG((int64_t)p->pre_rows.grid + p->pre_tiles.grid + p->rows.grid + p->tiles.grid <= kMaxGroups,
+                 "%s: %lld work-groups exceed the grid limit", who,
+                 (long long)p->pre_rows.grid + p->pre_tiles.grid + p->rows.grid + p->tiles.grid);
+    // every unit over a prefix has a slot
+    p->pre_rows.slots = p->pre_rows.grid;
+    p->pre_tiles.slots = p->pre_tiles.grid;
   }
-  const int64_t few_slots = (int64_t)p->rows.slots + p->pre_rows.slots, tile_slots = (int64_t)p->tiles.slots + p->pre_tiles.slots;
-  p->zero = (4 * (few_slots + tile_slots) + 255) / 256 * 256;
-  p->pre_o = p->zero + 4 * (few_slots * slot_floats(kRows, x->D) + tile_slots * slot_floats(kTileRows, x->D));
-  const int64_t rows = sharing ? x->T * x->Hq : 0;
-  p->pre_ml = p->pre_o + 4 * rows * x->D;
-  p->bytes = p->pre_ml + 16 * rows;
+  p->zero = (4 * ((int64_t)p->rows.slots + p->tiles.slots) + 255) / 256 * 256;
+  p->states = p->zero + 4ll * p->rows.slots * slot_floats(kRows, x->D) + 4ll * p->tiles.slots * slot_floats(kTileRows, x->D);
+  const int64_t state = 4 * state_floats(x->D), rows = sharing ? x->T * x->Hq : 0;
+  p->own = p->states + state * ((int64_t)p->pre_rows.slots * kRows + (int64_t)p->pre_tiles.slots * kTileRows);
+  p->at = p->own + state * rows;
+  p->bytes = p->at + (int64_t)sizeof(StatesAt) * rows;
+  PA_CHECK_ARG(p->own - p->states < (1ll << 36), "%s: %lld bytes of states", who, (long long)(p->own - p->states));
   return PA_OK;
 }
 
@@ -196,7 +201,7 @@ int run_paged(const char* who, const pa_paged_args* x, const pa_sharing* share, 
   PA_CHECK_ARG(x->workspace && reinterpret_cast<uintptr_t>(x->workspace) % 256 == 0 && x->workspace_bytes >= p.bytes,
                "%s: needs a 256-byte aligned workspace of %lld bytes", who, (long long)p.bytes);
   if (int rc = check_overlaps(who, x, share, (int)esz, p.bytes)) return rc;
-  PagedK a;
+  PagedK a{};
   a.q = static_cast<const char*>(x->q);
   a.q_st = x->q_st * esz;
   a.q_sh = x->q_sh * esz;
@@ -245,20 +250,19 @@ int run_paged(const char* who, const pa_paged_args* x, const pa_sharing* share, 
   a.tiles.count = a.rows.count + p.rows.slots;
   a.rows.part = ws + p.zero;
   a.tiles.part = a.rows.part + 4ll * p.rows.slots * slot_floats(kRows, x->D);
-  a.share = share ? *share : pa_sharing{};
-  a.pre_o = reinterpret_cast<float*>(ws + p.pre_o);
-  a.pre_ml = reinterpret_cast<float*>(ws + p.pre_ml);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (share && p.pre_rows.grid) {
-    PagedK pre = a;
-    pre.rows = p.pre_rows;
-    pre.tiles = p.pre_tiles;
-    pre.rows.count = a.tiles.count + p.tiles.slots;
-    pre.tiles.count = pre.rows.count + p.pre_rows.slots;
-    pre.rows.part = a.tiles.part + 4ll * p.tiles.slots * slot_floats(kTileRows, x->D);
-    pre.tiles.part = pre.rows.part + 4ll * p.pre_rows.slots * slot_floats(kRows, x->D);
-    if (x->dtype == PA_F32) return launch_shared_f32(pre, a, x->D, s);
-    return x->dtype == PA_BF16 ? launch_shared_bf16(pre, a, x->D, s) : launch_shared_f16(pre, a, x->D, s);
+    a.share = *share;
+    a.pre_rows = p.pre_rows;
+    a.pre_tiles = p.pre_tiles;
+    a.states = reinterpret_cast<float*>(ws + p.states);
+    a.n_states = (p.own - p.states) / 4;
+    a.pre_rows.part = ws + p.states;
+    a.pre_tiles.part = a.pre_rows.part + 4ll * p.pre_rows.slots * kRows * state_floats(x->D);
+    a.own = reinterpret_cast<float*>(ws + p.own);
+    a.at = reinterpret_cast<StatesAt*>(ws + p.at);
+    if (x->dtype == PA_F32) return launch_shared_f32(a, x->D, s);
+    return x->dtype == PA_BF16 ? launch_shared_bf16(a, x->D, s) : launch_shared_f16(a, x->D, s);
   }
   if (x->dtype == PA_F32) return launch_paged_f32(a, x->D, s);
   return x->dtype == PA_BF16 ? launch_paged_bf16(a, x->D, s) : launch_paged_f16(a, x->D, s);

@@ -25,9 +25,9 @@ constexpr int kTileRows = 128;  // and of a chunk's tile
 constexpr int kTileLg = 6;      // log2 keys of a step of a chunk's tile
 
 // Which rows and keys a body takes.  Requests that share a prefix are attended in two parts: the rows of
-// all of a group's requests against the prefix, whose states go to memory (kPrefix: "request" g is the
-// group of holder g, its rows found through a list, at positions of their own), and each request's rows
-// against its own keys, merged with those states (kOwn).
+// all of a group's requests against the prefix (kPrefix: "request" g is the group of holder g, its rows
+// found through a list, at positions of their own), and each request's rows against its own keys (kOwn).
+// Both leave the rows' states in memory, a prefix one for each share of it, and a second launch merges them.
 enum Part { kWhole = 0, kPrefix = 1, kOwn = 2 };
 
 // What one of the two kernels' bodies does in a call.
@@ -71,8 +71,19 @@ struct PagedK {
   PagedPart tiles, rows;
   // ---- requests that share prefixes (kPrefix, kOwn) ----
   pa_sharing share;
-  float* pre_o;   // [T, Hq, D]: the rows' outputs over their prefix
-  float* pre_ml;  // [T, Hq, 4]: maximum (log2 units), what its rounding left out, sum
+  PagedPart pre_tiles, pre_rows;
+  // States: D floats of O, then maximum (log2 units), what its rounding left out, sum, and one unused.
+  float* states;       // of the prefixes' shares, a slot of pre_tiles or pre_rows each, at their `part`
+  float* own;          // [T, Hq] states over the requests' own keys
+  struct StatesAt* at; // [T, Hq] by place among the groups' rows
+  int64_t n_states;    // floats of `states`, a multiple of 4
+};
+
+// Where a row's states over its prefix are: units of 4 floats.
+struct StatesAt {
+  uint32_t first, step;
+  int32_t n;
+  int32_t unused;
 };
 
 // The mask of a kernel whose first argument is a PagedK.
@@ -225,7 +236,7 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, c
     // (to the nearest: a tile little longer than a share stays whole)
     const float b = (float)w.blocks, mine = fmaxf(fmaxf(share, (float)w.least), __builtin_amdgcn_sqrtf(b) * p.root_over);
     const int32_t splits = imax((int32_t)(b * __builtin_amdgcn_rcpf(mine) + 0.5f), 1);
-    const int32_t units = w.tiles * a.Hkv * splits, slotted = splits > 1 ? units : 0;
+    const int32_t units = w.tiles * a.Hkv * splits, slotted = PART == kPrefix || splits > 1 ? units : 0;
     const int32_t n_in = wave_scan(units), s_in = wave_scan(slotted);
     const int32_t at = before + n_in - units;
     const uint64_t hit = __ballot(at <= id && id < at + units);
@@ -330,21 +341,21 @@ __device__ __forceinline__ int32_t lanes_max(int32_t x) { return ~lanes_min(~x);
 __device__ __forceinline__ float rest_of(float x, float c, float m) {
   return __builtin_fabsf(m) < INFINITY ? __builtin_fmaf(x, c, -m) : 0.f;
 }
-// Two states of a row, maxima m + rest in log2 units, as one: the factors of each side's sums.
-struct Merge {
-  float m, rest, f0, f1;
-};
-__device__ __forceinline__ Merge merge_of(float m0, float rest0, float m1, float rest1) {
-  Merge x;
-  x.rest = m0 > m1 ? rest0 : m1 > m0 ? rest1 : nan_max(rest0, rest1);
-  x.m = nan_max(m0, m1);
-  x.f0 = __builtin_amdgcn_exp2f((m0 - base_of(x.m)) + (rest0 - x.rest));
-  x.f1 = __builtin_amdgcn_exp2f((m1 - base_of(x.m)) + (rest1 - x.rest));
-  return x;
-}
-
 // floats of a slot: O of every row, then maximum and sum (and of a chunk's tile what the maximum lacks)
 constexpr int slot_floats(int BM, int D) { return BM * (D + (BM == kTileRows ? 3 : 2)); }
+
+// and of a slot of a prefix's share
+constexpr int state_floats(int D) { return D + 4; }
+
+// Where a row over a prefix leaves its state, row `row` of the unit's slot; the first share says where all are.
+template <int BM, int D>
+__device__ __forceinline__ float* prefix_state(const PagedK& a, const PagedPart& p, const Unit& u, int32_t row, int32_t tok, int32_t head, bool tell) {
+  constexpr int SLOT = BM * state_floats(D);
+  float* first = reinterpret_cast<float*>(p.part) + (int64_t)u.slot * SLOT + row * state_floats(D);
+  if (tell && u.split == 0)
+    a.at[(int64_t)(u.rq.start + tok) * (a.Hkv * a.G) + head] = StatesAt{(uint32_t)((first - a.states) / 4), SLOT / 4, u.splits, 0};
+  return first + (int64_t)u.split * SLOT;
+}
 
 int check_pages(const char* who, int64_t n_pages, int32_t page_size, int* page_lg);
 
@@ -353,9 +364,9 @@ int launch_paged_bf16(const PagedK& a, int D, hipStream_t s);
 int launch_paged_f16(const PagedK& a, int D, hipStream_t s);
 int launch_paged_f32(const PagedK& a, int D, hipStream_t s);
 
-// The same for requests that share prefixes: `pre` is a with the parts of the prefixes.
-int launch_shared_bf16(const PagedK& pre, const PagedK& a, int D, hipStream_t s);
-int launch_shared_f16(const PagedK& pre, const PagedK& a, int D, hipStream_t s);
-int launch_shared_f32(const PagedK& pre, const PagedK& a, int D, hipStream_t s);
+// The same for requests that share prefixes.
+int launch_shared_bf16(const PagedK& a, int D, hipStream_t s);
+int launch_shared_f16(const PagedK& a, int D, hipStream_t s);
+int launch_shared_f32(const PagedK& a, int D, hipStream_t s);
 
 }  // namespace pa

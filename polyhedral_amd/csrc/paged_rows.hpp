@@ -103,7 +103,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
   constexpr int NB = D / 16;                       // blocks of 16 output columns
   constexpr int NK = F32 ? D / 16 : D / 32;        // 16-byte units of a K or Q row that a lane holds
   constexpr int SEG = 16 * ROW, STAGE = 2 * SEG;
-  const PagedPart& part = a.rows;
+  const PagedPart& part = PART == kPrefix ? a.pre_rows : a.rows;
 
   const int tid = threadIdx.x, lane = tid & 63, q16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -139,6 +139,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
 
   const Unit u = find_unit<kRows, S::LG, PART>(a, part, raw, id, lane);
   if (!u.found) return;
+  if (PART == kPrefix && u.slot + u.splits > part.slots) return;  // (a sharing of another step)
 
   // ---- the tile's rows -----------------------------------------------------------
   const int rows = u.rq.n * a.G;
@@ -562,7 +563,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
     }
   };
   gather();
-  if (u.splits > 1) {
+  if (PART != kPrefix && u.splits > 1) {
     constexpr int SLOT_B = slot_floats(kRows, D) * 4, ML = kRows * D * 4;
     char* first = part.part + (int64_t)u.slot * SLOT_B;  // of the tile's shares
     if (row < n_rows) {
@@ -636,30 +637,14 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
   }
   if (row >= n_rows) return;
   const int ir = i0 + row, t_r = token_of(a, ir), h_r = u.h * a.G + (ir - t_r * a.G);
-  float m2 = 0.f, rest = 0.f;  // (kWhole has no use for them)
-  if constexpr (PART != kWhole) {
-    m2 = M * a.c;
-    rest = rest_of(M, a.c, m2);
-    const int64_t at = (int64_t)row_of<PART>(a, u, t_r) * (a.Hkv * a.G) + h_r;
-    f32x4* po = reinterpret_cast<f32x4*>(a.pre_o + at * D + c0);
-    f32x4* ml = reinterpret_cast<f32x4*>(a.pre_ml + 4 * at);
-    if constexpr (PART == kPrefix) {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
+  if (PART == kPrefix || (PART == kOwn && from > 0)) {
+    float* to = PART == kPrefix ? prefix_state<kRows, D>(a, part, u, row, t_r, h_r, c0 == 0)
+                                : a.own + ((int64_t)(u.rq.start + t_r) * (a.Hkv * a.G) + h_r) * state_floats(D);
 #pragma unroll
-      for (int e = 0; e < CPT; e += 4) po[e / 4] = f32x4{out[e], out[e + 1], out[e + 2], out[e + 3]} * inv;
-      if (c0 == 0) *ml = f32x4{m2, rest, L, 0.f};
-      return;
-    }
-    if (from > 0) {
-      const f32x4 p = *ml;
-      const Merge x = merge_of(m2, rest, p[0], p[1]);
-      const float f1 = x.f1 * p[2];
-#pragma unroll
-      for (int e = 0; e < CPT; ++e) out[e] = x.f0 * out[e] + f1 * po[e / 4][e % 4];
-      L = x.f0 * L + f1;
-      m2 = x.m;
-      rest = x.rest;
-    }
+    for (int e = 0; e < CPT; e += 4) *reinterpret_cast<f32x4*>(to + c0 + e) = f32x4{out[e], out[e + 1], out[e + 2], out[e + 3]};
+    const float m2 = M * a.c;
+    if (c0 == 0) *reinterpret_cast<f32x4*>(to + D) = f32x4{m2, rest_of(M, a.c, m2), L, 0.f};
+    return;
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   char* orow = a.o + (int64_t)(u.rq.start + t_r) * a.o_st + (int64_t)h_r * a.o_sh;
@@ -668,7 +653,7 @@ __device__ __forceinline__ void rows_body(const PagedK& a, int32_t id, char* sme
     Mma<T>::store4(orow + (c0 + e) * ESZ, f32x4{out[e], out[e + 1], out[e + 2], out[e + 3]} * inv);
   if (a.lse && c0 == 0)
     a.lse[(int64_t)(u.rq.start + t_r) * a.lse_st + (int64_t)h_r * a.lse_sh] =
-        L == 0.f ? -INFINITY : PART == kOwn && from > 0 ? (m2 + (log2f(L) + rest)) * kLn2 : __builtin_fmaf(M, a.c, log2f(L)) * kLn2;
+        L == 0.f ? -INFINITY : (M * a.c + log2f(L)) * kLn2;
 }
 
 }  // namespace

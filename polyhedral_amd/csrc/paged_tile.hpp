@@ -70,7 +70,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   constexpr int SLOT = TileShape<T, D>::SLOT;
   constexpr int VRING = 0, KRING = 2 * SLOT;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char_t*)smem;
-  const PagedPart& part = a.tiles;
+  const PagedPart& part = PART == kPrefix ? a.pre_tiles : a.tiles;
 
   const int tid = threadIdx.x, lane = tid & 63, G = lane >> 5, m = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -86,6 +86,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   TileReads<D> rd = tile_reads<D>((lds_cptr)smem, lane);
   const Unit u = find_unit<kTileRows, kTileLg, PART>(a, part, raw, id, lane);
   if (!u.found) return;
+  if (PART == kPrefix && u.slot + u.splits > part.slots) return;  // (a sharing of another step)
 
   // ---- rows ------------------------------------------------------------------------
   const int rows = u.rq.n * a.G, len = u.rq.len, pos0 = len - u.rq.n;
@@ -425,7 +426,7 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
   asm volatile("" : "+v"(lane_e));
   const int m_e = lane_e & 31, G_e = lane_e >> 5;
   const bool mine = 32 * w + m_e < n_rows;
-  if (u.splits > 1) {
+  if (PART != kPrefix && u.splits > 1) {
     // a slot is the waves' registers as they are: 16 bytes of O per lane, then maximum and sum, then
     // what the maximum lacks (which is as large as the difference of two shares' maxima, where these are
     // huge)
@@ -480,45 +481,26 @@ __device__ __forceinline__ void tile_body(const PagedK& a, int32_t id, char* sme
           for (int z = 0; z < 4; ++z) acc[db][4 * e + z] += f * x[db][e][z];
     }
   }
-  if constexpr (PART != kWhole) {
-    // (a lane has columns 32 db + 8 e + 4 G .. + 3 of its row, as floats 16 bytes)
-    const int ir = imin(i0 + 32 * w + m_e, rows - 1), tok = token_of(a, ir), head = u.h * a.G + (ir - tok * a.G);
-    const int64_t at = (int64_t)row_of<PART>(a, u, tok) * (a.Hkv * a.G) + head;
-    f32x4* po = reinterpret_cast<f32x4*>(a.pre_o + at * D) + G_e;
-    f32x4* ml = reinterpret_cast<f32x4*>(a.pre_ml + 4 * at);
-    if constexpr (PART == kPrefix) {
-      const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
-      if (!mine) return;
+  if (PART == kPrefix || (PART == kOwn && u.x0 > 0)) {
+    // (a lane has columns 32 db + 8 e + 4 G .. + 3 of its row)
+    if (!mine) return;
+    const int ir = i0 + 32 * w + m_e, tok = token_of(a, ir), head = u.h * a.G + (ir - tok * a.G);
+    float* to = PART == kPrefix ? prefix_state<kTileRows, D>(a, part, u, 32 * w + m_e, tok, head, G_e == 0)
+                                : a.own + ((int64_t)(u.rq.start + tok) * (a.Hkv * a.G) + head) * state_floats(D);
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
+    for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          po[8 * db + 2 * e] = f32x4{acc[db][4 * e], acc[db][4 * e + 1], acc[db][4 * e + 2], acc[db][4 * e + 3]} * inv;
-      if (G_e == 0) *ml = f32x4{m_run, m_rest, l_tot, 0.f};
-      return;
-    }
-    if (u.x0 > 0) {
-      const f32x4 p = *ml;
-      const Merge x = merge_of(m_run, m_rest, p[0], p[1]);
-      const float f1 = x.f1 * p[2];
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const f32x4 y = po[8 * db + 2 * e];
-#pragma unroll
-          for (int z = 0; z < 4; ++z) acc[db][4 * e + z] = x.f0 * acc[db][4 * e + z] + f1 * y[z];
-        }
-      l_tot = x.f0 * l_tot + f1;
-      m_run = x.m;
-      m_rest = x.rest;
-    }
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f32x4*>(to + 32 * db + 8 * e + 4 * G_e) =
+            f32x4{acc[db][4 * e], acc[db][4 * e + 1], acc[db][4 * e + 2], acc[db][4 * e + 3]};
+    if (G_e == 0) *reinterpret_cast<f32x4*>(to + D) = f32x4{m_run, m_rest, l_tot, 0.f};
+    return;
   }
   const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
   if (a.lse && G_e == 0 && mine) {
     const int ir = i0 + 32 * w + m_e, tok = token_of(a, ir), head = u.h * a.G + (ir - tok * a.G);
     a.lse[(int64_t)(u.rq.start + tok) * a.lse_st + (int64_t)head * a.lse_sh] =
-        l_tot == 0.f ? -INFINITY : (m_run + (PART == kOwn && u.x0 > 0 ? log2f(l_tot) + m_rest : log2f(l_tot))) * kLn2;
+        l_tot == 0.f ? -INFINITY : (m_run + log2f(l_tot)) * kLn2;
   }
   // Through LDS (32 rows a wave, 16-byte units swizzled), so that they are stored as whole rows.
   // (every wave is past its last read of the rings: the sums' check was a barrier)
