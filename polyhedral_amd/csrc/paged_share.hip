@@ -7,6 +7,7 @@
 //
 // What bounds it: latency, three trips to memory and the launch.
 #include "page_checks.hpp"
+#include "paged_attn.hpp"
 
 namespace pa {
 namespace {
@@ -35,26 +36,25 @@ __global__ __launch_bounds__(kShareThreads) void share_kernel(const ShareK a) {
   constexpr int NW = kShareThreads / 64;
   __shared__ int32_t lds[LDS ? 8 * kShareRequests : 1];
   __shared__ int32_t wave_n[NW];
-  __shared__ int32_t falls;
   int32_t* at = LDS ? lds : a.workspace;
   int32_t *s0 = at, *n = at + a.R, *len = at + 2 * (int64_t)a.R, *own = at + 3 * (int64_t)a.R, *some = at + 4 * (int64_t)a.R,
           *off = at + 5 * (int64_t)a.R, *cut = at + 6 * (int64_t)a.R, *tot = at + 7 * (int64_t)a.R;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  if (tid == 0) falls = 0;
-  __syncthreads();
 
   // ---- the requests: starts that fall back are taken as the largest before (as in pa_paged_attn) ------
+  bool falls = false;
   for (int r = tid; r < a.R; r += kShareThreads) {
     const int32_t x = imin(imax(a.q_start[r], 0), a.T), y = imin(imax(a.q_start[r + 1], 0), a.T);
+    const int32_t o = a.holders[r], l = imin(imax(a.lengths[r], 0), kMaxPosition);
+    const int32_t m = imin(imax(a.shared[r], 0), l) >> a.page_lg << a.page_lg;
     s0[r] = x;
     n[r] = y - x;
-    if (y < x) falls = 1;
-    len[r] = imin(imax(a.lengths[r], 0), kMaxPosition);
-    own[r] = a.holders[r];
-    some[r] = a.shared[r];
+    len[r] = l;
+    some[r] = m;
+    own[r] = (uint32_t)o < (uint32_t)a.R && y != x && m > 0 ? o : -1;
+    falls |= y < x;
   }
-  __syncthreads();
-  if (falls) {
+  if (__syncthreads_or(falls)) {
     if (tid == 0) {
       int32_t end = 0;
       for (int r = 0; r < a.R; ++r) {
@@ -62,66 +62,56 @@ __global__ __launch_bounds__(kShareThreads) void share_kernel(const ShareK a) {
         s0[r] = x;
         end = imax(x, y);
         n[r] = end - x;
+        const int32_t o = a.holders[r];
+        own[r] = (uint32_t)o < (uint32_t)a.R && n[r] > 0 && some[r] > 0 ? o : -1;
       }
     }
     __syncthreads();
   }
-  for (int r = tid; r < a.R; r += kShareThreads) {
-    some[r] = imin(imax(some[r], 0), len[r]) >> a.page_lg << a.page_lg;
-    if (!((uint32_t)own[r] < (uint32_t)a.R) || n[r] == 0 || some[r] == 0) own[r] = -1;
-  }
-  __syncthreads();
 
-  // ---- a request among those of its holder: `per` lanes to a request -----------------------------------
+  // ---- a request among those of its holder, and as a holder: `per` lanes to a request --------------------
   int per = 1;
   while (per < 64 && 2 * per * a.R <= kShareThreads) per *= 2;
+  const int sub = tid & (per - 1);
   for (int r0 = 0; r0 < a.R; r0 += kShareThreads / per) {
     const int r = r0 + tid / per;
     const int32_t mine = r < a.R ? own[r] : -1;
     int32_t count = 0, before = 0, least = kMaxPosition;
-    if (mine >= 0)
-      for (int x = tid % per; x < a.R; x += per)
-        if (own[x] == mine) {
-          ++count;
-          if (x < r) before += n[x];
-          least = imin(least, some[x]);
-        }
+    int32_t members = 0, sum = 0, lo = kMaxPosition, hi = 0, pre = kMaxPosition;
+    for (int x = sub; x < a.R; x += per) {
+      const int32_t o = own[x], nx = n[x], sx = some[x], lx = len[x];
+      if (o >= 0 && o == mine) {
+        ++count;
+        before += x < r ? nx : 0;
+        least = imin(least, sx);
+      }
+      if (o == r) {
+        ++members;
+        sum += nx;
+        lo = imin(lo, lx - nx);
+        hi = imax(hi, lx - 1);
+        pre = imin(pre, sx);
+      }
+    }
     for (int o = 1; o < per; o <<= 1) {
       count += __shfl_xor(count, o);
       before += __shfl_xor(before, o);
       least = imin(least, __shfl_xor(least, o));
-    }
-    if (r < a.R && tid % per == 0) {
-      const bool group = count > 1;
-      off[r] = before;
-      cut[r] = group ? least : 0;
-      a.first[r] = group ? least : 0;
-    }
-  }
-  __syncthreads();
-  // ---- the groups, by holder -------------------------------------------------------------------------
-  for (int r0 = 0; r0 < a.R; r0 += kShareThreads / per) {
-    const int g = r0 + tid / per;
-    int32_t sum = 0, lo = kMaxPosition, hi = 0, pre = 0;
-    if (g < a.R)
-      for (int x = tid % per; x < a.R; x += per)
-        if (own[x] == g && cut[x] > 0) {
-          sum += n[x];
-          lo = imin(lo, len[x] - n[x]);
-          hi = imax(hi, len[x] - 1);
-          pre = cut[x];
-        }
-    for (int o = 1; o < per; o <<= 1) {
+      members += __shfl_xor(members, o);
       sum += __shfl_xor(sum, o);
       lo = imin(lo, __shfl_xor(lo, o));
       hi = imax(hi, __shfl_xor(hi, o));
-      pre = imax(pre, __shfl_xor(pre, o));
+      pre = imin(pre, __shfl_xor(pre, o));
     }
-    if (g < a.R && tid % per == 0) {
-      tot[g] = sum;
-      a.prefix[g] = pre;
-      a.low[g] = sum ? lo : 0;
-      a.high[g] = sum ? hi : 0;
+    if (r < a.R && sub == 0) {
+      const bool in = count > 1, group = members > 1;
+      off[r] = before;
+      cut[r] = in ? least : 0;
+      tot[r] = group ? sum : 0;
+      a.first[r] = in ? least : 0;
+      a.prefix[r] = group ? pre : 0;
+      a.low[r] = group ? lo : 0;
+      a.high[r] = group ? hi : 0;
     }
   }
   __syncthreads();
@@ -129,20 +119,15 @@ __global__ __launch_bounds__(kShareThreads) void share_kernel(const ShareK a) {
   int32_t total = 0;
   for (int r0 = 0; r0 < a.R; r0 += kShareThreads) {
     const int g = r0 + tid;
-    const int32_t x = g < a.R ? tot[g] : 0;
-    int32_t in = x;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int32_t up = __shfl_up(in, o);
-      if (lane >= o) in += up;
-    }
+    const int32_t x = g < a.R ? tot[g] : 0, in = wave_scan(x);
     if (lane == 63) wave_n[w] = in;
     __syncthreads();
     int32_t base = total;
 #pragma unroll
     for (int y = 0; y < NW; ++y) {
-      if (y < w) base += wave_n[y];
-      total += wave_n[y];
+      const int32_t z = wave_n[y];
+      base += y < w ? z : 0;
+      total += z;
     }
     if (g < a.R) {
       tot[g] = base + in - x;
@@ -151,11 +136,12 @@ __global__ __launch_bounds__(kShareThreads) void share_kernel(const ShareK a) {
     __syncthreads();
   }
   if (tid == 0) a.start[a.R] = total;
-  // ---- the rows: a wave to a request -------------------------------------------------------------------
-  for (int r = w; r < a.R; r += NW) {
-    if (cut[r] == 0) continue;
+  // ---- the rows ----------------------------------------------------------------------------------------
+  for (int r0 = 0; r0 < a.R; r0 += kShareThreads / per) {
+    const int r = r0 + tid / per;
+    if (r >= a.R || cut[r] == 0) continue;
     const int32_t to = tot[own[r]] + off[r], from = s0[r], m = n[r], p0 = len[r] - m;
-    for (int i = lane; i < m; i += 64) {
+    for (int i = sub; i < m; i += per) {
       a.rows[to + i] = from + i;
       a.positions[to + i] = p0 + i;
     }

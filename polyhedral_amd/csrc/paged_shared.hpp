@@ -48,51 +48,61 @@ void shared_both_kernel(const PagedK a) {
     rows_body<T, D, kOwn>(a, id - a.pre_rows.grid, smem, &flag);
 }
 
-// D / 4 lanes to a row of the groups' rows.
-template <typename T, int D>
+// A row's state: D / 4 lanes with 4 columns each.
+struct MergeState {
+  float m, rest, l;
+  f32x4 x;
+  __device__ __forceinline__ void add(const f32x4& ml, const f32x4& y) {
+    const float top = nan_max(m, ml[0]);
+    const float r = ml[0] > m ? ml[1] : ml[0] == m ? nan_max(rest, ml[1]) : rest;
+    const float f0 = __builtin_amdgcn_exp2f((m - base_of(top)) + (rest - r)), f1 = __builtin_amdgcn_exp2f((ml[0] - base_of(top)) + (ml[1] - r));
+    m = top;
+    rest = r;
+    l = f0 * l + f1 * ml[2];
+    x = f0 * x + f1 * y;
+  }
+};
+
+// ONE: a work-group merges one row, its states dealt to 256 / (D / 4) lots of lanes and those in order; else each
+// lot a row.
+template <typename T, int D, bool ONE>
 __global__ __launch_bounds__(256) void shared_merge_kernel(const PagedK a) {
-  constexpr int LPR = D / 4, STATE = state_floats(D) / 4;
-  const int col = (int)threadIdx.x % LPR;
+  constexpr int LPR = D / 4, LOTS = 256 / LPR, STATE = state_floats(D) / 4;
+  __shared__ f32x4 part[ONE ? LOTS : 1][LPR + 1];
+  const int col = (int)threadIdx.x % LPR, lot = (int)threadIdx.x / LPR;
   const int Hq = a.Hkv * a.G;
-  const int64_t id = (int64_t)blockIdx.x * (256 / LPR) + (int)threadIdx.x / LPR;
+  const int64_t id = ONE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * LOTS + lot;
+  const int32_t i = imin((int32_t)(id / Hq), a.T - 1), head = (int32_t)(id % Hq);
+  // (all on their way at once)
+  const int32_t last = a.share.start[a.R], last_q = a.q_start[a.R], tok = a.share.rows[i];
+  StatesAt at = a.at[(int64_t)i * Hq + head];
   // (a sharing of another step: rows past the requests' last stay, and states are read from within their memory)
-  const int32_t rows = imin(imax(a.share.start[a.R], 0), a.T), end = imin(imax(a.q_start[a.R], 0), a.T);
-  const int32_t i = (int32_t)(id / Hq), head = (int32_t)(id - (int64_t)i * Hq);
-  if (i >= rows) return;
-  const int32_t tok = a.share.rows[i];
-  if (tok < 0 || tok >= end) return;
-  StatesAt at = a.at[id];
+  if (id >= (int64_t)imin(imax(last, 0), a.T) * Hq || tok < 0 || tok >= imin(imax(last_q, 0), a.T)) return;
   if (at.n < 0 || at.n > (1 << 20) || ((int64_t)at.first + (int64_t)at.step * imax(at.n - 1, 0) + STATE) * 4 > a.n_states) at.n = 0;
   const f32x4* state = reinterpret_cast<const f32x4*>(a.states) + at.first;
   const f32x4* own = reinterpret_cast<const f32x4*>(a.own) + ((int64_t)tok * Hq + head) * STATE;
-  const f32x4 oml = own[D / 4];
-  f32x4 x = own[col];
-  // the largest maximum, then the sums
-  float m = oml[0], rest = oml[1];
+  MergeState s{-INFINITY, 0.f, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
+  if (!ONE || lot == 0) s.add(own[D / 4], own[col]);
 #pragma unroll 4
-  for (int s = 0; s < at.n; ++s) {
-    const f32x4 ml = state[(int64_t)s * at.step + D / 4];
-    rest = ml[0] > m ? ml[1] : ml[0] == m ? nan_max(rest, ml[1]) : rest;
-    m = nan_max(m, ml[0]);
+  for (int j = ONE ? lot : 0; j < at.n; j += ONE ? LOTS : 1) {
+    const f32x4* y = state + (int64_t)j * at.step;
+    s.add(y[D / 4], y[col]);
   }
-  const float base = base_of(m);
-  const float f0 = __builtin_amdgcn_exp2f((oml[0] - base) + (oml[1] - rest));
-  f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < at.n; ++s) {
-    const f32x4 ml = state[(int64_t)s * at.step + D / 4], y = state[(int64_t)s * at.step + col];
-    const float f = __builtin_amdgcn_exp2f((ml[0] - base) + (ml[1] - rest));
-    l += f * ml[2];
-    sum += f * y;
+  if constexpr (ONE) {
+    part[lot][col] = s.x;
+    if (col == 0) part[lot][LPR] = f32x4{s.m, s.rest, s.l, 0.f};
+    __syncthreads();
+    if (lot) return;
+    for (int j = 1; j < imin(LOTS, at.n); ++j) s.add(part[j][LPR], part[j][col]);
   }
-  l += f0 * oml[2];
-  sum += f0 * x;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  Mma<T>::store4(a.o + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + 4 * (int)sizeof(T) * col, sum * inv);
+  const float inv = s.l == 0.f ? 0.f : 1.f / s.l;
+  Mma<T>::store4(a.o + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + 4 * (int)sizeof(T) * col, s.x * inv);
   if (a.lse && col == 0)
-    a.lse[(int64_t)tok * a.lse_st + (int64_t)head * a.lse_sh] = l == 0.f ? -INFINITY : (m + (log2f(l) + rest)) * kLn2;
+    a.lse[(int64_t)tok * a.lse_st + (int64_t)head * a.lse_sh] = s.l == 0.f ? -INFINITY : (s.m + (log2f(s.l) + s.rest)) * kLn2;
 }
+
+// Rows up to which each has a work-group of its own to merge it.
+constexpr int64_t kMergeRows = 8192;
 
 template <typename T, int D>
 int launch_shared_t(const PagedK& a, hipStream_t s) {
@@ -105,7 +115,10 @@ int launch_shared_t(const PagedK& a, hipStream_t s) {
   if (!both) hipLaunchKernelGGL((shared_rows_kernel<T, D>), dim3(grid), dim3(64 * kWaves), 0, s, a);
   PA_LAUNCH_CHECK("shared_kernel");
   const int64_t rows = (int64_t)a.T * a.Hkv * a.G;
-  hipLaunchKernelGGL((shared_merge_kernel<T, D>), dim3((unsigned)((rows * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
+  if (rows <= kMergeRows)
+    hipLaunchKernelGGL((shared_merge_kernel<T, D, true>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((shared_merge_kernel<T, D, false>), dim3((unsigned)((rows * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
   PA_LAUNCH_CHECK("shared_merge_kernel");
   return PA_OK;
 }
