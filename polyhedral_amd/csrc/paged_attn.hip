@@ -45,12 +45,15 @@ struct PagedPlan {
 // least, and then less than twice those that its blocks fill.  The work-groups without a unit each
 // hold a place on a CU for 1.5 us; a grid without them, whose groups loop over units, costs more: 276
 // -> 296 us of sinks in chunks, 15 -> 17 us of one token over 8000, by registers that the loop holds.)
-int part_of(const char* who, const pa_paged_args* x, int BM, int shares, int64_t max_tiles, PagedPart* p) {
+// blocks: the most that all its requests have, where the grid goes by that too (-1: not).
+int part_of(const char* who, const pa_paged_args* x, int BM, int shares, int32_t least, int64_t max_tiles, int64_t blocks, PagedPart* p) {
+  p->by_shares = 1.0001f / (float)shares;
+  if (blocks >= 0 && blocks / least < shares) shares = (int)(blocks / least);
   const int64_t most = shares + max_tiles * x->Hkv;
   PA_CHECK_ARG(most <= kMaxGroups, "%s: %lld work-groups exceed the grid limit", who, (long long)most);
   p->grid = (int32_t)most;
   p->slots = (int32_t)(2 * shares < most ? 2 * shares : most);
-  p->by_shares = 1.0001f / (float)shares;
+  p->least = least;
   const int G = x->Hq / x->Hkv;
   p->span = (BM + G - 1) / G + 1;
   return PA_OK;
@@ -83,17 +86,17 @@ int plan_of(const char* who, const pa_paged_args* x, bool sharing, PagedPlan* p)
   p->tile = x->dtype != PA_F32 && x->n_pages > 0 && most * G > few_rows;
   int64_t few = x->T * G / kRows + some;
   if (p->tile && few > some * ((few_rows + kRows - 1) / kRows)) few = some * ((few_rows + kRows - 1) / kRows);
+  // (a call that shares: the tables' reach in blocks of 16 or 32 keys, for each tile of few rows)
+  const int64_t row_blocks = sharing ? few * x->Hkv * (((int64_t)x->cols << p->page_lg) / (x->dtype == PA_F32 ? 16 : 32) + 1) : -1;
   // (beside chunks too: 61 requests of a token and 3 chunks with 256 shares 232 us, with 512 177, with 1024
   // 166; 36 requests of which most are chunks 53 with any)
-  if (int rc = part_of(who, x, kRows, 1024, few, &p->rows)) return rc;
-  p->rows.least = 4;
+  if (int rc = part_of(who, x, kRows, 1024, 4, few, row_blocks, &p->rows)) return rc;
   p->rows.root_over = 0.7f;
   p->rows.row_min = 0;
   p->rows.row_max = p->tile ? (int32_t)few_rows : INT_MAX;
   p->tiles = PagedPart{};
   if (p->tile) {
-    if (int rc = part_of(who, x, kTileRows, 512, x->T * G / kTileRows + some, &p->tiles)) return rc;
-    p->tiles.least = 8;
+    if (int rc = part_of(who, x, kTileRows, 512, 8, x->T * G / kTileRows + some, -1, &p->tiles)) return rc;
     p->tiles.root_over = 1.f;
     p->tiles.row_min = (int32_t)few_rows;
     p->tiles.row_max = INT_MAX;
@@ -107,13 +110,13 @@ int plan_of(const char* who, const pa_paged_args* x, bool sharing, PagedPlan* p)
     const int64_t groups = some / 2;
     few = x->T * G / kRows + groups;
     if (tile && few > groups * (kFewRows / kRows)) few = groups * (kFewRows / kRows);
-    if (int rc = part_of(who, x, kRows, 1024, few, &p->pre_rows)) return rc;
-    p->pre_rows.least = 4;
+    // (beside tiles fewer shares, as its work-groups are mostly without work: 64 requests behind 8192 tokens 64 us
+    // with 1024, 61 with 256)
+    if (int rc = part_of(who, x, kRows, tile ? 256 : 1024, 4, few, row_blocks, &p->pre_rows)) return rc;
     p->pre_rows.root_over = 0.7f;
     p->pre_rows.row_max = tile ? kFewRows : INT_MAX;
     if (tile) {
-      if (int rc = part_of(who, x, kTileRows, 512, x->T * G / kTileRows + groups, &p->pre_tiles)) return rc;
-      p->pre_tiles.least = 8;
+      if (int rc = part_of(who, x, kTileRows, 512, 8, x->T * G / kTileRows + groups, -1, &p->pre_tiles)) return rc;
       p->pre_tiles.root_over = 1.f;
       p->pre_tiles.row_min = kFewRows;
       p->pre_tiles.row_max = INT_MAX;
@@ -131,7 +134,8 @@ int plan_of(const char* who, const pa_paged_args* x, bool sharing, PagedPlan* p)
   p->own = p->states + state * ((int64_t)p->pre_rows.slots * kRows + (int64_t)p->pre_tiles.slots * kTileRows);
   p->at = p->own + state * rows;
   p->bytes = p->at + (int64_t)sizeof(StatesAt) * rows;
-  PA_CHECK_ARG(p->own - p->states < (1ll << 36), "%s: %lld bytes of states", who, (long long)(p->own - p->states));
+  PA_CHECK_ARG(p->own - p->states < (1ll << 36) && rows * (x->D / 4) <= kMaxGroups * 256,
+               "%s: %lld rows leave too many states (%lld bytes)", who, (long long)rows, (long long)(p->own - p->states));
   return PA_OK;
 }
 

@@ -2,9 +2,14 @@
 //
 // One grid takes the prefixes, each read once for the rows of all its requests, and every request's own keys:
 // the tiles of many rows first, whose MFMAs the loads of the others then run beside.  A second launch merges the
-// states that they leave, a row at a time, in the order of the prefix's shares and the own keys last.  (The two
-// parts one after the other, a part's shares merged by its last work-group and the prefix's state taken up
-// by the own part: 64 requests behind 8192 tokens 41 and 29 us, 87 with the plan.)
+// states that they leave, a row at a time, in the order of the prefix's shares.  (The two parts one after the
+// other, a part's shares merged by its last work-group and the prefix's state taken up by the own part: 64
+// requests behind 8192 tokens 41 and 29 us, and 24 us of one row's 64 shares behind 65536.)
+//
+// What bounds it, at 32 heads on 8 of 128 in bf16: behind long prefixes HBM (32 requests behind 65536, 358 MB: 90
+// us of 104, 4.0 TB/s), with chunks the tiles' MFMAs (12 of 100 to 600 tokens behind 12000 to 16384: 0.94 ms,
+// 0.96 PFLOP/s), else what is outside the steps: 64 requests behind 8192 tokens, whose prefix is 176 units of 12
+// steps, 43 us, then 7 of the merge, 5 of the plan and the launches' gaps, where its 128 MB take 26.
 #pragma once
 
 #include "paged_rows.hpp"
@@ -42,10 +47,11 @@ void shared_both_kernel(const PagedK a) {
     return;
   }
   id -= a.tiles.grid;
-  if (id < a.pre_rows.grid)
-    rows_body<T, D, kPrefix>(a, id, smem, &flag);
+  // (beside tiles a prefix of few rows is rare: its work-groups, mostly without work, last)
+  if (id < a.rows.grid)
+    rows_body<T, D, kOwn>(a, id, smem, &flag);
   else
-    rows_body<T, D, kOwn>(a, id - a.pre_rows.grid, smem, &flag);
+    rows_body<T, D, kPrefix>(a, id - a.rows.grid, smem, &flag);
 }
 
 // A row's state: D / 4 lanes with 4 columns each.

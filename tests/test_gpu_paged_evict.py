@@ -287,6 +287,59 @@ def test_evict_of_layouts(gpu):
         assert torch.equal(y, want), order
 
 
+def test_offsets_past_32_bits(gpu):
+    """Keys, and scores, whose bytes lie past 4 GiB."""
+    far, P, H, D = 8400, 256, 8, 128                    # pages of 512 KiB: 4.1 GiB
+    b = Batch(gpu, torch.bfloat16, D, P, 16, H, [(1, 900), (40, 600), (1, 30)])
+    t, n, s = b.dev()
+    lse = torch.empty(b.T, b.Hq, device=gpu)
+    paged.attention(b.q, b.k, b.v, t, n, s, pm.Causal(), lse=lse)
+    near = torch.zeros(b.pages, H, P, device=gpu)
+    paged.weights(b.q, b.k, t, n, s, lse, near, pm.Causal())
+    k, v = (torch.empty(far + b.pages, H, P, D, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+    k[far:], v[far:] = b.k, b.v
+    wide = torch.empty(far + b.pages, H, 64 * P, device=gpu)[:, :, :P]      # 4.1 GiB of scores
+    wide[far:] = 0
+    ft = torch.where(t >= 0, t + far, t)
+    paged.weights(b.q, k, ft, n, s, lse, wide, pm.Causal())
+    assert torch.equal(wide[far:], near)
+    kept, after = paged.choose(near, t, n, 300, 20)
+    got = paged.choose(wide, ft, n, 300, 20)
+    assert torch.equal(got.kept, kept) and torch.equal(got.lengths, after)
+    paged.evict(kept, b.k, b.v, near, t, n)
+    paged.evict(kept, k, v, wide, ft, n)
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in ((k[far:], b.k), (v[far:], b.v)))
+    assert torch.equal(wide[far:], near)
+
+
+def test_launches_that_run_again_and_at_once(gpu):
+    """Two launches of weights with shares to merge, each captured and replayed on a stream of its own."""
+    sizes = [(300, 2000), (1, 900), (90, 90)]
+    made = []
+    for seed in (1, 2):
+        b = Batch(gpu, torch.bfloat16, 128, 16, 8, 2, sizes, seed=seed)
+        lse = torch.empty(b.T, b.Hq, device=gpu)
+        paged.attention(b.q, b.k, b.v, *b.dev(), pm.Causal(), lse=lse)
+        scores = torch.zeros(b.pages, 2, 16, device=gpu)
+        launch = paged.prepare_weights(b.q, b.k, *b.dev(), lse, scores, pm.Causal())
+        want = launch().clone()
+        scores.zero_()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            launch()
+        made.append((graph, launch, scores, want, b, lse))
+    streams = [torch.cuda.Stream() for _ in made]
+    for _ in range(4):
+        torch.cuda.synchronize()
+        for s, (graph, *_) in zip(streams, made):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, _, scores, want, *_ in made:
+            assert torch.equal(scores, want)
+            scores.zero_()
+
+
 def test_refusals(gpu):
     k = torch.zeros(4, 2, 16, 64, dtype=torch.float16, device=gpu)
     v, s = torch.zeros_like(k), torch.zeros(4, 2, 16, device=gpu)

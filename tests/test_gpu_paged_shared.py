@@ -192,6 +192,24 @@ def test_many_requests_and_heads(gpu):
         Shared(gpu, torch.float16, 64, 16, Hq, Hkv, groups, _tokens(R // 5, 1, 90, 9), seed=R).check(pm.Causal())
 
 
+def test_more_requests_than_a_work_group_has_threads(gpu):
+    rng = np.random.default_rng(1)
+    groups = [(16 * int(rng.integers(1, 4)), _tokens(int(rng.integers(1, 40)), 1, 20, i)) for i in range(60)]
+    Shared(gpu, torch.float16, 64, 16, 2, 1, groups, _tokens(300, 1, 30, 9), seed=1).check(pm.Causal())
+
+
+def test_offsets_past_32_bits(gpu):
+    """Pages whose bytes lie past 4 GiB, for prefix and own keys."""
+    b = Shared(gpu, torch.bfloat16, 128, 256, 8, 8, [(2048, _tokens(8, 1, 600, 1)), (256, [(200, 300), (1, 9)])], [(1, 700)])
+    far = 8400                                  # pages of 512 KiB: 4.1 GiB
+    k, v = (torch.empty(far + b.pages, 8, 256, 128, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+    k[far:], v[far:] = b.k, b.v
+    want, wl = b.run(pm.Causal())
+    b.k, b.v, b.tables = k, v, np.where(b.tables >= 0, b.tables + far, b.tables)
+    o, lse = b.run(pm.Causal())
+    assert torch.equal(o, want) and torch.equal(lse, wl)
+
+
 @pytest.mark.parametrize("most", [0, 1, 40, 10000])
 def test_any_hint_gives_right_results(gpu, most):
     Shared(gpu, torch.bfloat16, 128, 32, 8, 2, [(320, [(1, 5), (90, 100), (3, 40)])], [(1, 90), (33, 33)]).check(pm.Causal(), max_fresh=most)
