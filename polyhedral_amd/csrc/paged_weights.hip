@@ -46,6 +46,7 @@ struct WeightsK {
   float by_shares;     // 1 / the shares that the former's work is cut into
   float* part;         // [slots][256] sums of split groups' shares
   int32_t* count;      // [slots] shares done, at a group's first slot; zero between calls
+  int32_t* queue;      // units drawn, 16 ints apart; zero between calls
 };
 
 __device__ __forceinline__ KernelMask weights_mask(const WeightsK& a) {
@@ -297,6 +298,7 @@ __device__ __forceinline__ void weigh_blocks(const WeightsK& a, int32_t id, int3
 // whose exponentials it adds up over all steps, those of one 32 rows beside the MFMAs of the next; at the end
 // the 32 lanes' sums are added by halves.  Shares of a group leave their sums in the workspace, and the last
 // one adds them in order.
+constexpr int kQueues = 8;
 constexpr int kKeysLg = 8, kKeys = 1 << kKeysLg, kStepRows = 64;
 
 template <typename T, int D>
@@ -322,8 +324,8 @@ __device__ __forceinline__ KeyWork key_work(const WeightsK& a, int r0, int lane,
   }
   return k;
 }
-// Unit `id`, false past the last.  share: steps of a share (0 at first).
-__device__ __forceinline__ bool find_keys(const WeightsK& a, int32_t id, int lane, float& share, KeyUnit& u) {
+// Unit `id`; past the last: false, and units is how many there are.  share: steps of a share (0 at first).
+__device__ __forceinline__ bool find_keys(const WeightsK& a, int32_t id, int lane, float& share, KeyUnit& u, int64_t& units_all) {
   KeyWork k{};
   int32_t end = 0;
   if (share == 0.f || a.R <= 64) {
@@ -364,6 +366,7 @@ __device__ __forceinline__ bool find_keys(const WeightsK& a, int32_t id, int lan
     before += readlane64(n_in, 63);
     slot += __builtin_amdgcn_readlane(s_in, 63);
   }
+  units_all = before;
   return false;
 }
 
@@ -499,11 +502,12 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
       if (!((live >> ((j - j0) & 63)) & 1ull)) continue;
       const int32_t i0 = j * kStepRows;
       const uint64_t ok = __ballot(z_now != -INFINITY);  // (rows past the last have no weight)
-      const bool all = ok == ~0ull && ((full >> ((j - j0) & 63)) & 1ull);
+      const bool is_full = (full >> ((j - j0) & 63)) & 1ull, all = is_full && ok == ~0ull;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const bool row = (uint32_t)(ok >> (32 * b + m)) & 1u;
         auto word = [&](int32_t key) __attribute__((always_inline)) -> uint32_t {
+          if (is_full) return row ? ~0u : 0u;  // (rows without weight alone)
           return row ? mask_word(mask, pos0 + divide(imin(i0 + 32 * b + m, rows - 1), a.by_G), key, len) : 0u;
         };
         const float zb = __shfl(z_now, 32 * b + m);
@@ -564,12 +568,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void w
     __shared__ __attribute__((aligned(256))) char smem[2 * WeighTile<T, D>::SLOT];
     __shared__ int32_t flag;
     if ((int32_t)blockIdx.x < a.tile_grid) {
+      // Units are of different lengths and go to whom has time: the first by the work-group's number, the
+      // others from a queue for each XCD (work-groups are dealt to those in turn), so that a head's rows stay in
+      // one L2.  Who draws its last number clears the queue.
+      const int32_t x = (int32_t)blockIdx.x % kQueues, of_x = a.tile_grid / kQueues;
       float share = 0.f;
       KeyUnit u;
-      for (int32_t id = (int32_t)blockIdx.x; find_keys(a, id, (int)threadIdx.x & 63, share, u); id += a.tile_grid) {
+      int32_t n = (int32_t)blockIdx.x / kQueues;
+      int64_t units = 0;
+      while (find_keys(a, n * kQueues + x, (int)threadIdx.x & 63, share, u, units)) {
         weigh_keys<T, D>(a, u, smem, &flag);
         __syncthreads();  // (the slots and the flag have been read)
+        if (threadIdx.x == 0)
+          flag = of_x + __hip_atomic_fetch_add(a.queue + 16 * x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        n = flag;
+        __syncthreads();
       }
+      // (a number is drawn after every unit)
+      if (threadIdx.x == 0 && n >= of_x && n - of_x == (int32_t)((units - x + kQueues - 1) / kQueues) - 1)
+        __hip_atomic_store(a.queue + 16 * x, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       return;
     }
   }
@@ -588,7 +606,7 @@ WeightsPlan weights_plan(const pa_weights_args* x) {
   WeightsPlan p;
   p.tile = x->dtype != PA_F32 && most * (x->Hq / x->Hkv) > kFewRows;
   p.slots = p.tile ? 2 * kTileShares : 0;  // (a group that is split has at most 4/3 of the shares that its work fills)
-  p.zero = (4 * p.slots + 255) / 256 * 256;
+  p.zero = p.tile ? (4 * (p.slots + 16 * kQueues) + 255) / 256 * 256 : 0;
   p.bytes = p.zero + 4 * p.slots * kKeys;
   return p;
 }
@@ -713,7 +731,8 @@ extern "C" int pa_paged_weights(const pa_weights_args* x, void* stream) {
   auto near = [&](int64_t st, int64_t sh) { return st <= (1 << 24) && sh <= (1 << 24) && st >= -(1 << 24) && sh >= -(1 << 24); };
   a.even = kStepRows % a.G == 0 && near(a.q_st, a.q_sh) && near(a.lse_st, a.lse_sh);
   a.by_shares = 1.f / (float)kTileShares;
-  a.count = reinterpret_cast<int32_t*>(x->workspace);
+  a.queue = reinterpret_cast<int32_t*>(x->workspace);
+  a.count = a.queue + 16 * kQueues;
   a.part = reinterpret_cast<float*>(static_cast<char*>(x->workspace) + p.zero);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (x->D == 64)
