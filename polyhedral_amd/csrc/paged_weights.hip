@@ -503,13 +503,22 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
       const int32_t i0 = j * kStepRows;
       const uint64_t ok = __ballot(z_now != -INFINITY);  // (rows past the last have no weight)
       const bool is_full = (full >> ((j - j0) & 63)) & 1ull, all = is_full && ok == ~0ull;
+      // words of this lane's rows and the wave's keys (rolled, for one copy of the mask's code)
+      uint32_t word[2][2] = {};
+      if (!all) {
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {
+          const int i = 32 * (x >> 1) + m;
+          uint32_t y = ~0u;  // (full: rows without weight alone are dead)
+          if (!is_full) y = mask_word(mask, pos0 + divide(imin(i0 + i, rows - 1), a.by_G), key0 + 32 * (x & 1), len);
+          y = (uint32_t)(ok >> i) & 1u ? y : 0u;
+#pragma unroll
+          for (int z = 0; z < 4; ++z) word[z >> 1][z & 1] = z == x ? y : word[z >> 1][z & 1];
+        }
+      }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const bool row = (uint32_t)(ok >> (32 * b + m)) & 1u;
-        auto word = [&](int32_t key) __attribute__((always_inline)) -> uint32_t {
-          if (is_full) return row ? ~0u : 0u;  // (rows without weight alone)
-          return row ? mask_word(mask, pos0 + divide(imin(i0 + 32 * b + m, rows - 1), a.by_G), key, len) : 0u;
-        };
         const float zb = __shfl(z_now, 32 * b + m);
         u32x4 qf[NQF];
 #pragma unroll
@@ -517,9 +526,9 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
         __builtin_amdgcn_sched_barrier(0);
         block(kf[0], qf, xa, xb, neg, sum + 16);
         neg = row ? -zb * 1.4426950408889634f : 0.f;
-        if (!all) mask_block(xa, word(key0));
+        if (!all) mask_block(xa, word[b][0]);
         block(kf[1], qf, xb, xa, neg, sum);
-        if (!all) mask_block(xb, word(key0 + 32));
+        if (!all) mask_block(xb, word[b][1]);
       }
     }
     add(xb, neg, sum + 16);
