@@ -470,19 +470,24 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
       x[e] = __builtin_bit_cast(float, (__builtin_bit_cast(int32_t, xv) & keep) | (int32_t)(0xff800000u & ~(uint32_t)keep));
     }
   };
-  // Scores of 32 keys and 32 rows, in two places in turn: the exponentials of one are added beside the MFMAs of
-  // the other.
-  f32x16 xa, xb;
+  // Scores of the wave's keys and 32 rows, in two places in turn: the exponentials of one are added beside the MFMAs
+  // of the other, which are two chains (one, of 32 keys at a time, waits for itself).
+  f32x16 xa[2], xb[2];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) xb[e] = -INFINITY;  // (dead)
+  for (int e = 0; e < 16; ++e) xb[0][e] = xb[1][e] = -INFINITY;  // (dead)
   float neg = 0.f;  // of the rows of the scores that are still to be added
-  auto block = [&](const Frag* k, const u32x4* qf, f32x16& y, const f32x16& x, float neg_x, float* to) __attribute__((always_inline)) {
-    y = Mma<T>::mma(k[0], __builtin_bit_cast(Frag, qf[0]), f32x16{0});
+  auto block = [&](const u32x4* qf, f32x16* y, const f32x16* x) __attribute__((always_inline)) {
+    y[0] = Mma<T>::mma(kf[0][0], __builtin_bit_cast(Frag, qf[0]), f32x16{0});
+    y[1] = Mma<T>::mma(kf[1][0], __builtin_bit_cast(Frag, qf[0]), f32x16{0});
 #pragma unroll
-    for (int kc = 1; kc < NQF; ++kc) y = Mma<T>::mma(k[kc], __builtin_bit_cast(Frag, qf[kc]), y);
-    add(x, neg_x, to);
+    for (int kc = 1; kc < NQF; ++kc) {
+      y[0] = Mma<T>::mma(kf[0][kc], __builtin_bit_cast(Frag, qf[kc]), y[0]);
+      y[1] = Mma<T>::mma(kf[1][kc], __builtin_bit_cast(Frag, qf[kc]), y[1]);
+    }
+    add(x[0], neg, sum);
+    add(x[1], neg, sum + 16);
 #pragma unroll
-    for (int z = 0; z < NQF; ++z) {
+    for (int z = 0; z < 2 * NQF; ++z) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 2);
       __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 6 : 12, 2);
     }
@@ -524,14 +529,17 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
 #pragma unroll
         for (int kc = 0; kc < NQF; ++kc) qf[kc] = *(lds_u4*)(rd[kc] + slot * SLOT + 32 * b * R::ROW);
         __builtin_amdgcn_sched_barrier(0);
-        block(kf[0], qf, xa, xb, neg, sum + 16);
+        f32x16* y = b ? xb : xa;
+        block(qf, y, b ? xa : xb);
         neg = row ? -zb * 1.4426950408889634f : 0.f;
-        if (!all) mask_block(xa, word[b][0]);
-        block(kf[1], qf, xb, xa, neg, sum);
-        if (!all) mask_block(xb, word[b][1]);
+        if (!all) {
+          mask_block(y[0], word[b][0]);
+          mask_block(y[1], word[b][1]);
+        }
       }
     }
-    add(xb, neg, sum + 16);
+    add(xb[0], neg, sum);
+    add(xb[1], neg, sum + 16);
   }
 
   // ---- over the 32 rows: lane l ends with the sum of key 32 (l / 16 % 2) + 8 (l / 4 % 4) + 4 half + l % 4 ----
