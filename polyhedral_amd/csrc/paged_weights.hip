@@ -1,12 +1,15 @@
 // The attention weight that cached keys receive, over a paged cache (gfx950): for every key and KV head
 // the sum over its request's new tokens and the heads of the group of exp(scale q . k - lse).
 //
-// The keys are cut into blocks (64 keys of one KV head, f32: 32) whose sums are independent.  A wave
-// takes a run of consecutive blocks, an equal share of all blocks times the row tiles each meets: K
-// rows go straight into the A operand's registers of 16x16 MFMAs (S^T = K Q^T, as in paged_rows.hpp),
-// once for all rows of the request, the next block's loads ahead of this one's products.  Lane (q = l %
-// 16, g = l / 16) holds scores of keys 4 g + 0..3 of each 16 keys for row q; their exponentials are
-// added up over the row tiles, and over the 16 rows at the end, in a fixed order.
+// Sums of different keys are independent, so the keys are what is cut.  Requests of few rows (new tokens times
+// heads of a group) are bound by the bytes of K: weigh_blocks, a wave for some blocks of 64 keys (f32: 32), K straight
+// into registers.  64 requests of 300..8192 tokens, a new one each (8 KV heads of 128, bf16, 317 MB of K): 75 us, 4.2
+// TB/s of the 5.0 that a copy reaches; one request of 1001 tokens, 4 heads of 64 in f32: 6.0 us, latency.  Requests of
+// many rows are bound by products and exponentials: weigh_keys, a work-group for 256 keys, which stay in registers
+// while rows of Q pass by.  8 chunks of 256..1500 tokens behind 1000..8000 (32 heads over 8 of 128, f16, 127
+// GFLOP of products and 0.5 G exponentials): 177 us, 0.72 PFLOP/s; matrix instructions run in a third of the
+// cycles and vector instructions, mostly the exponentials' chains, in near half, beside each other; about 40 us go to the units'
+// beginnings and ends (keys' loads, reduction over lanes).  By blocks alone it takes 610 us.
 //
 // Scores, exponentials and sums are float32.  A dead pair adds 0 whatever its key holds, by selection.
 #include <limits.h>
@@ -117,7 +120,12 @@ __device__ __forceinline__ int64_t readlane64(int64_t x, int l) {
   return (int64_t)((uint64_t)lo | (uint64_t)(uint32_t)hi << 32);
 }
 
-// Few rows a request: blocks of keys, a wave each.
+// ---- few rows a request -------------------------------------------------------------------------
+// A wave takes a run of consecutive blocks, an equal share of all blocks times the row tiles each meets: K rows go
+// straight into the A operand's registers of 16x16 MFMAs (S^T = K Q^T, as in paged_rows.hpp), once for all
+// rows of the request, the next block's loads ahead of this one's products.  Lane (q = l % 16, g = l / 16) holds
+// scores of keys 4 g + 0..3 of each 16 keys for row q; their exponentials are added up over the row tiles, and
+// over the 16 rows at the end, in a fixed order.
 template <typename T, int D>
 __device__ __forceinline__ void weigh_blocks(const WeightsK& a, int32_t id, int32_t grid) {
   using S = WeightsShape<T, D>;
@@ -489,7 +497,8 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
 #pragma unroll
     for (int z = 0; z < 2 * NQF; ++z) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 2);
-      __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 6 : 12, 2);
+      __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 4 : 8, 2);
+      __builtin_amdgcn_sched_group_barrier(0x400, D == 128 ? 2 : 4, 2);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -611,8 +620,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void w
   weigh_blocks<T, D>(a, (int32_t)blockIdx.x - a.tile_grid, (int32_t)gridDim.x - a.tile_grid);
 }
 
-// The requests' rows from which they are taken by 256 keys, and the work-groups and shares of those.
-constexpr int kFewRows = 32, kTileGroups = 512, kTileShares = 1024;
+// The most rows of a request that is taken by blocks.  32 requests of 300..8192 tokens (bf16, 8 KV heads of 128): by
+// blocks / by 256 keys 47 / 54 us at 24 rows, 48 / 54 at 32, 53 / 54 at 48, 59 / 52 at 64, 70 / 63 at 96; 4 requests of
+// 2000..16000: 16 / 16 at 12, 19 / 16 at 32, 25 / 15 at 64.
+constexpr int kFewRows = 32;
+// Work-groups of the others, two a CU, whose registers are full (one: 228 us of the chunks' 177), and the shares that
+// the work is cut into at least (512: 176, 768: 176, 1024: 178, 1536: 191, for each reads its keys anew).
+constexpr int kTileGroups = 512, kTileShares = 768;
 
 struct WeightsPlan {
   bool tile;
