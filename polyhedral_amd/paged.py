@@ -624,6 +624,7 @@ class PagedKVCache:
         self.shared = torch.zeros(requests, **i32)          # tokens of that
         self.scores = torch.zeros(self.k.shape[:-1], dtype=torch.float32, device=dev) if weigh else None
         self._shares = False                   # whether requests may share prefixes
+        self._trims = False                    # whether pages in front may be missing
         self._last = (None, None, None)        # the newest step, its most new tokens of a request, its Sharing
 
     def begin(self, fresh, tokens=None):
@@ -670,8 +671,9 @@ class PagedKVCache:
         """Requests ``members`` (a list; without tokens so far) begin with the first ``tokens`` tokens of
         request ``holder``, whole pages that they read and do not copy.  The holder may go on; it keeps
         these pages until the members have finished.  Where that cannot be (the holder has fewer tokens, or
-        begins with more of another's itself; a member is not empty) nothing happens, and ``check`` says
-        so."""
+        has given some of their pages back, or begins with fewer of another's itself; a member is not empty)
+        nothing happens, and ``check`` says so.  Not to be captured; steps captured before the first call read
+        a shared prefix as often as there are requests."""
         members = [int(m) for m in members]
         holder, tokens = int(holder), int(tokens)
         if not all(0 <= m < self.requests for m in members + [holder]) or holder in members:
@@ -687,7 +689,7 @@ class PagedKVCache:
             of = self.holders[h]
             second = (of >= 0) & (of != h)       # the holder shares another's prefix itself
             root = torch.where(second, of, h)    # .. which is then theirs too
-            ok = ((self.lengths[h] >= tokens) & (~second | (self.shared[h] >= tokens))
+            ok = ((self.lengths[h] >= tokens) & (~second | (self.shared[h] >= tokens)) & (self.tables[root, :n] >= 0).all()
                   & (self.lengths[m] == 0) & (self.holders[m] < 0))
             i32 = lambda x: x.to(torch.int32)  # noqa: E731
             self.tables[m, :n] = torch.where(ok[:, None], self.tables[root, :n], self.tables[m, :n])
@@ -702,7 +704,8 @@ class PagedKVCache:
 
     def weigh(self, q, lse, mask, step, layer=0, scale=None):
         """Adds the attention that a step's tokens have paid to a layer's keys to their scores (see
-        prepare_weights; lse: what attend wrote).  A shared prefix is not weighed."""
+        prepare_weights; lse: what attend wrote).  Called for every step: a step's own keys start from 0 there.  A
+        shared prefix is not weighed."""
         if self.scores is None:
             raise RuntimeError("the cache holds no scores: make it with weigh=True")
         most = self._last[1] if step is self._last[0] else None
@@ -713,9 +716,11 @@ class PagedKVCache:
         those that it shares) keeps ``keep`` of them, in each layer and head the ``recent`` newest and those
         with the largest scores, moved together in their order; pages that this leaves go back.  From then
         on a token's position is its place among those kept: a mask that counts distances counts them
-        there."""
+        there.  Not in a cache that is trimmed: there may be no page where they go."""
         if self.scores is None:
             raise RuntimeError("the cache holds no scores: make it with weigh=True")
+        if self._trims:
+            raise RuntimeError("the cache has been trimmed: its requests have no pages in front to move keys to")
         if sinks < 0:
             raise ValueError(f"sinks={sinks} < 0")
         P = self.page_size
@@ -733,6 +738,10 @@ class PagedKVCache:
         with torch.cuda.device(self.device):
             self.failed |= status * LIST_FULL
 
+    def _may_share(self):
+        # (a captured call may be replayed after the first prefix is shared)
+        return self._shares or torch.cuda.is_current_stream_capturing()
+
     def finish(self, done):
         """Gives back the pages of the requests where done (bool [requests], on the device, or a list,
         which a graph's capture does not take) is true and sets their lengths to 0.  One whose tokens
@@ -743,11 +752,19 @@ class PagedKVCache:
         if done.shape != (self.requests,):
             raise ValueError(f"done must be [{self.requests}], got {list(done.shape)}")
         with torch.cuda.device(self.device):
+            if not self._may_share():
+                last = done.to(torch.int32) * self.tables.shape[1]
+                self._release(torch.zeros_like(last), last)
+                self.lengths.masked_fill_(done, 0)
+                return
             self_ = torch.arange(self.requests, dtype=torch.int32, device=self.device)
             member = (self.holders >= 0) & (self.holders != self_)
             busy = torch.zeros(self.requests + 1, dtype=torch.bool, device=self.device)
             busy.scatter_(0, torch.where(member & ~done, self.holders, self.requests).long(), True)
-            self.failed |= (done & busy[:-1]).any().to(torch.int32) * SHARED
+            # (whether any is, without a reduction, which may clear memory in ways that a graph does not replay)
+            some = torch.zeros(2, dtype=torch.int32, device=self.device)
+            some.scatter_(0, (done & busy[:-1]).long(), SHARED)
+            self.failed |= some[1:]
             done = done & ~busy[:-1]
             # (a shared prefix's pages are its holder's)
             first = torch.where(member, self.shared // self.page_size, 0).to(torch.int32)
@@ -764,11 +781,13 @@ class PagedKVCache:
         need: with a SinksWindow(sinks, window) mask no later token sees them."""
         if window < 1 or sinks < 0:
             raise ValueError(f"window={window} must be at least 1 and sinks={sinks} at least 0")
+        self._trims = True
         P = self.page_size
         with torch.cuda.device(self.device):
             last = ((self.lengths - int(min(window, MAX_POSITION)) + 1).clamp(min=0) // P).to(torch.int32)
-            # (nor what requests share)
-            first = (self.shared // P).clamp(min=min(-(-int(sinks) // P), self.tables.shape[1])).to(torch.int32)
+            first = torch.full_like(last, min(-(-int(sinks) // P), self.tables.shape[1]))
+            if self._may_share():   # (nor what requests share)
+                torch.maximum(first, self.shared // P, out=first)
             self._release(first, last)
 
     def check(self):

@@ -442,6 +442,14 @@ def test_a_cache_without_scores_refuses(gpu):
         paged.PagedKVCache(2, 100, 20, 2, 64, torch.float16, 16, device=gpu, weigh=True).evict(10, 2, sinks=-1)
 
 
+def test_a_trimmed_cache_does_not_evict(gpu):
+    c = paged.PagedKVCache(2, 100, 20, 2, 64, torch.float16, 16, device=gpu, weigh=True)
+    c.begin([80, 3])
+    c.trim(window=20)
+    with pytest.raises(RuntimeError, match="trimmed"):
+        c.evict(10, 2)
+
+
 def test_captured_steps_and_evictions(gpu):
     """A step with its weights and an eviction in graphs, replayed, against a second cache without."""
     R, H, G, D, P = 4, 2, 2, 64, 16

@@ -436,3 +436,43 @@ def test_prefixes_that_cannot_be_shared_or_finished(gpu):
     assert int(c.free_count) == 57
     c.finish([True] * 5)
     assert int(c.free_count) == 60 and (c.tables == -1).all() and (c.holders == -1).all() and (c.shared == 0).all()
+
+
+def test_a_prefix_with_pages_given_back_is_not_shared(gpu):
+    c = paged.PagedKVCache(3, 200, 30, 2, 64, torch.float16, 16, device=gpu)
+    c.begin([100, 0, 0])
+    c.trim(window=20)
+    c.check()
+    c.share(0, [1], 32)
+    assert host(c.lengths).tolist() == [100, 0, 0] and host(c.holders).tolist() == [-1] * 3 and (c.tables[1] == -1).all()
+    with pytest.raises(RuntimeError, match="shared"):
+        c.check()
+
+
+def test_a_captured_finish_keeps_what_is_shared_later(gpu):
+    """finish and trim captured before the first prefix is shared, replayed after."""
+    c = paged.PagedKVCache(4, 200, 40, 2, 64, torch.float16, 16, device=gpu)
+    done = torch.zeros(4, dtype=torch.bool, device=gpu)
+    c.begin([100, 0, 0, 20])
+    end, cut = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(end):
+        c.finish(done)
+    with torch.cuda.graph(cut):
+        c.trim(window=20)
+    c.share(0, [1, 2], 64)
+    c.begin([0, 5, 9, 1])
+    prefix = host(c.tables)[0, :4]
+    for ended, free in (((), 30), ((1,), 31), ((0, 3), 33), ((2,), 34), ((0,), 40)):
+        done.zero_()
+        done[list(ended)] = True
+        end.replay()
+        cut.replay()
+        torch.cuda.synchronize()
+        tables = host(c.tables)
+        ids = np.concatenate([np.unique(tables[tables >= 0]), host(c.free_list)[:int(c.free_count)]])
+        assert sorted(ids.tolist()) == list(range(40)) and int(c.free_count) == free, ended
+        if ended != (0,):
+            assert np.array_equal(tables[0, :4], prefix)
+    with pytest.raises(RuntimeError, match="finished before"):   # (0, while 2 went on)
+        c.check()
