@@ -13,7 +13,7 @@
 // work-group that takes the rows of one layer, request, KV head and tensor in order, a batch into
 // registers before any of it is stored and the next one's on their way meanwhile, moves them in place with
 // no scratch memory.  What bounds it: HBM (1.8 GB in 375 us, 4.9 TB/s, where a copy reaches 5.0), and for
-// a few heads four trips to memory.
+// a few heads four trips to memory (2 requests of about 1000, 4 heads of 64 in f32: 4.8 us).
 #include <limits.h>
 
 #include "page_checks.hpp"
@@ -254,6 +254,13 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
 // 389 us and 375; a layer of 2 requests, 4 heads, 4 MB 7.1 us and 7.6).
 constexpr int64_t kManyHeads = 512;
 
+// Where heads times K and V are fewer than the CUs, a row is cut into slices of 64 bytes or more (each takes more rows
+// at a time then, and a head's columns move independently): one request of 7000, 4 heads of 128 in f16, to 2500:
+// 24.8 us whole, 14.6 in slices of 128 bytes, 9.6 of 64; 4 requests of 9000, 8 heads in f32, to 2048: 47 and
+// 26; two requests of about 1000, 4 heads of 64 in f32: 7.1 and 4.8; 16 requests of 8 heads are as fast whole.
+constexpr int kSliceLg = 2;
+constexpr int64_t kSliceGroups = 256;
+
 struct EvictK {
   const int32_t* kept;
   char* k;
@@ -263,6 +270,7 @@ struct EvictK {
   int64_t s_sl, s_sp, s_sh;        // floats
   Pages pages;
   int32_t R, Hkv, keep, row_lg;    // row_lg: log2 of the 16-byte units of a row
+  int32_t cut_lg;                  // and of the slices of a row that go to work-groups of their own
 };
 
 // Units of type U (1 << lg of them a row) of the kept rows of one head, in order, by THREADS threads.  A batch's
@@ -340,9 +348,10 @@ __global__ __launch_bounds__(THREADS) void evict_kernel(const EvictK a) {
   const Held q = held_of(a.pages, r);
   const int32_t* kept = a.kept + (((int64_t)layer * a.R + r) * a.Hkv + h) * a.keep;
   const int32_t* table = a.pages.tables + r * a.pages.pitch;
-  if (blockIdx.y < 2) {
-    char* base = (blockIdx.y ? a.v : a.k) + layer * a.c_sl + h * a.c_sh;
-    move_rows<unit16, 4, THREADS>(a, kept, table, q, a.row_lg, [&](int32_t page, int32_t row) __attribute__((always_inline)) {
+  if (blockIdx.y < 2u << a.cut_lg) {
+    const int lg = a.row_lg - a.cut_lg;
+    char* base = (blockIdx.y & 1 ? a.v : a.k) + layer * a.c_sl + h * a.c_sh + ((int)(blockIdx.y >> 1) << lg << 4);
+    move_rows<unit16, 4, THREADS>(a, kept, table, q, lg, [&](int32_t page, int32_t row) __attribute__((always_inline)) {
       return reinterpret_cast<unit16*>(base + page * a.c_sp + row * a.c_sn);
     });
   } else {
@@ -480,7 +489,9 @@ extern "C" int pa_evict_rows(const pa_evict_args* x, void* stream) {
   a.keep = x->keep;
   a.row_lg = row == 128 ? 3 : row == 256 ? 4 : 5;
   const int64_t heads = x->layers * R * x->Hkv;
-  const dim3 grid((unsigned)heads, x->scores ? 3 : 2);
+  a.cut_lg = 0;
+  while (a.row_lg - a.cut_lg > kSliceLg && heads << (a.cut_lg + 1) < kSliceGroups) ++a.cut_lg;
+  const dim3 grid((unsigned)heads, (2u << a.cut_lg) + (x->scores ? 1 : 0));
   if (heads < kManyHeads)
     hipLaunchKernelGGL(evict_kernel<1024>, grid, dim3(1024), 0, static_cast<hipStream_t>(stream), a);
   else
