@@ -7,7 +7,7 @@
 // TB/s of the 5.0 that a copy reaches; one request of 1001 tokens, 4 heads of 64 in f32: 6.0 us, latency.  Requests of
 // many rows are bound by products and exponentials: weigh_keys, a work-group for 256 keys, which stay in registers
 // while rows of Q pass by.  8 chunks of 256..1500 tokens behind 1000..8000 (32 heads over 8 of 128, f16, 127
-// GFLOP of products and 0.5 G exponentials): 177 us, 0.72 PFLOP/s; matrix instructions run in a third of the
+// GFLOP of products and 0.5 G exponentials): 172 to 178 us from card to card, 0.72 PFLOP/s; matrix instructions run in a third of the
 // cycles and vector instructions, mostly the exponentials' chains, in near half, beside each other; about 40 us go to the units'
 // beginnings and ends (keys' loads, reduction over lanes).  By blocks alone it takes 610 us.
 //
@@ -42,9 +42,10 @@ struct WeightsK {
   int64_t lse_st, lse_sh;  // elements
   float* scores;
   int64_t s_sp, s_sh;  // elements
-  // requests with more rows (new tokens times heads of a group) than row_max are taken by the first tile_grid
-  // work-groups, the others by the rest
+  // requests with more rows (new tokens times heads of a group) than row_max are taken by units of 256 keys, where
+  // the grid has tile_grid work-groups, the others by blocks
   int32_t row_max, tile_grid;
+  int32_t near;        // no token sees all before it
   int32_t even;        // a step's rows are whole tokens, whose offsets in q and lse fit 31 bits
   float by_shares;     // 1 / the shares that the former's work is cut into
   float* part;         // [slots][256] sums of split groups' shares
@@ -67,14 +68,22 @@ struct WeightsShape {
   static constexpr int PER = 64 / NS;              // blocks whose pages are held at a time
 };
 
-// One request's share of the work: blocks first >> LG .. of each head, `cost` each.
+// One request's share of the work: blocks of each head, `cost` each: those from the `first` key's on and, where a
+// window leaves some dead, which hold a key that may be live or a new token's (whose score begins), a list of two runs.
+// (32 requests of 16000 to 32000 under a window of 1024 and 64 sinks: 25 us, 311 of all blocks.)
+struct BlockList {
+  int32_t low, base0, base1;
+  __device__ __forceinline__ int32_t block(int32_t j) const { return j + (j < low ? base0 : base1); }
+};
 struct WeighedRequest {
   Request rq;
-  int32_t first, block0, blocks, cost;
+  int32_t first;
+  BlockList list;
+  int32_t blocks, cost;
 };
-template <int LG>
+template <int LG, bool LIST>
 __device__ __forceinline__ WeighedRequest weighed(const WeightsK& a, int r0, int lane, int32_t& end) {
-  WeighedRequest x{{0, 0, 0}, 0, 0, 0, 0};
+  WeighedRequest x{{0, 0, 0}, 0, {0, 0, 0}, 0, 0};
   const int r = r0 + lane;
   int32_t s0 = 0, s1 = 0, len = 0, first = 0;
   if (r < a.R) {
@@ -98,10 +107,29 @@ __device__ __forceinline__ WeighedRequest weighed(const WeightsK& a, int r0, int
   end = __builtin_amdgcn_readlane(s1, imin(a.R - 1 - r0, 63));
   x.rq = request_of(s0, s1, len, a.T, a.cols << a.page_lg);
   x.first = imin(imax(first, 0), x.rq.len);
-  x.block0 = x.first >> LG;
+  const int32_t block0 = x.first >> LG, end_block = (x.rq.len + (1 << LG) - 1) >> LG;
+  x.list = {0, block0, block0};
   // (without new tokens nothing changes)
-  x.blocks = r < a.R && x.rq.n > 0 && x.rq.n * a.G <= a.row_max ? ((x.rq.len + (1 << LG) - 1) >> LG) - x.block0 : 0;
+  x.blocks = r < a.R && x.rq.n > 0 ? end_block - block0 : 0;
+  if (LIST && a.near && x.blocks) {
+    const int32_t pos0 = x.rq.len - x.rq.n;
+    KeyList kl = key_list(weights_mask(a), pos0, x.rq.len - 1, x.rq.len, LG);
+    const int32_t fresh = imax(imax(pos0, 0) >> LG, kl.low);
+    kl.first = kl.high ? imin(kl.first, fresh) : fresh;
+    kl.high = imax(end_block - kl.first, 0);
+    const int32_t skip = kl.before(block0);
+    x.list = {kl.low - skip, skip, kl.first - kl.low + skip};
+    x.blocks = kl.count() - skip;
+  }
   x.cost = 2 + (x.rq.n * a.G + kRows - 1) / kRows;
+  return x;
+}
+
+// Those of few rows.
+template <int LG>
+__device__ __forceinline__ WeighedRequest few(const WeightsK& a, int r0, int lane, int32_t& end) {
+  WeighedRequest x = weighed<LG, true>(a, r0, lane, end);
+  if (x.rq.n * a.G > a.row_max) x.blocks = 0;
   return x;
 }
 
@@ -140,7 +168,7 @@ __device__ __forceinline__ void weigh_blocks(const WeightsK& a, int32_t id, int3
   int32_t end = 0;
   WeighedRequest x{};
   for (int r0 = 0; r0 < a.R; r0 += 64) {
-    x = weighed<LG>(a, r0, lane, end);
+    x = few<LG>(a, r0, lane, end);
     total += readlane64(wave_scan64((int64_t)x.blocks * a.Hkv * x.cost, lane), 63);
   }
   const int64_t waves = (int64_t)grid * 4, me = (int64_t)id * 4 + w;
@@ -151,7 +179,7 @@ __device__ __forceinline__ void weigh_blocks(const WeightsK& a, int32_t id, int3
   int64_t before = 0;
   end = 0;
   for (int r0 = 0; r0 < a.R && before < hi; r0 += 64) {
-    if (a.R > 64) x = weighed<LG>(a, r0, lane, end);
+    if (a.R > 64) x = few<LG>(a, r0, lane, end);
     const int64_t mine = (int64_t)x.blocks * a.Hkv * x.cost, in = wave_scan64(mine, lane), at = before + in - mine;
     uint64_t hit = __ballot(at < hi && at + mine > lo);
     before += readlane64(in, 63);
@@ -161,7 +189,8 @@ __device__ __forceinline__ void weigh_blocks(const WeightsK& a, int32_t id, int3
       auto get = [&](int32_t y) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(y, l); };
       const int r = r0 + l;
       const Request rq{get(x.rq.start), get(x.rq.n), get(x.rq.len)};
-      const int32_t first = get(x.first), block0 = get(x.block0), blocks = get(x.blocks), cost = get(x.cost);
+      const int32_t first = get(x.first), blocks = get(x.blocks), cost = get(x.cost);
+      const BlockList list{get(x.list.low), get(x.list.base0), get(x.list.base1)};
       const int64_t from = readlane64(at, l);
       // the blocks that begin within the share (all heads of the request one after the other)
       const int64_t all = (int64_t)blocks * a.Hkv;
@@ -200,7 +229,7 @@ __device__ __forceinline__ void weigh_blocks(const WeightsK& a, int32_t id, int3
         int32_t c_page = -1;
         auto key_of = [&](int c) __attribute__((always_inline)) -> int32_t {
           const int b = c * PER + lane / NS;
-          return b < n_blocks ? ((block0 + i0 + b) << LG) + 16 * (lane % NS) : rq.len;
+          return b < n_blocks ? (list.block(i0 + b) << LG) + 16 * (lane % NS) : rq.len;
         };
         auto take_pages = [&](int c) __attribute__((always_inline)) {
           const int32_t key = key_of(c);
@@ -216,7 +245,7 @@ __device__ __forceinline__ void weigh_blocks(const WeightsK& a, int32_t id, int3
         auto fetch = [&](int b, Data& d) __attribute__((always_inline)) {
           if (b % PER == 0) take_pages(b / PER);
           const int l0 = NS * (b % PER);
-          d.key = (block0 + i0 + b) << LG;
+          d.key = list.block(i0 + b) << LG;
           d.there = 0u;
 #pragma unroll
           for (int t = 0; t < NS; ++t) {
@@ -323,11 +352,11 @@ struct KeyWork {
   int32_t first, group0, groups, steps;
 };
 __device__ __forceinline__ KeyWork key_work(const WeightsK& a, int r0, int lane, int32_t& end) {
-  const WeighedRequest x = weighed<kKeysLg>(a, r0, lane, end);
-  KeyWork k{x.rq, x.first, x.block0, 0, 0};
+  const WeighedRequest x = weighed<kKeysLg, false>(a, r0, lane, end);
+  KeyWork k{x.rq, x.first, x.list.base1, 0, 0};
   const int32_t rows = x.rq.n * a.G;
   if (r0 + lane < a.R && rows > a.row_max) {
-    k.groups = ((x.rq.len + kKeys - 1) >> kKeysLg) - x.block0;
+    k.groups = x.blocks;
     k.steps = (rows + kStepRows - 1) / kStepRows;
   }
   return k;
@@ -391,6 +420,12 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
   const int32_t key0 = (u.group << kKeysLg) + 64 * w;  // this wave's first key
   const int32_t* table = a.tables + (int64_t)u.r * a.pitch;
   const int one = (1 << a.page_lg) - 1;
+
+  // (a group that a window leaves dead, with no score that begins)
+  if (a.near && (u.group + 1) << kKeysLg <= pos0) {
+    const QueryRange q = query_range(mask, u.group << kKeysLg, (u.group << kKeysLg) + kKeys - 1);
+    if (q.hi < pos0 || q.lo >= len) return;
+  }
 
   // ---- the keys (one past the length or without a page: some row of page 0, whose sum goes nowhere) ----
   Frag kf[2][NQF];
@@ -590,10 +625,13 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
 
 template <typename T, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void weights_kernel(const WeightsK a) {
+  // Equal shares of the blocks first, then units as there is time (work-groups of their own for the blocks, 1024
+  // behind these, mostly had none: 183 us of chunks that take 178).
+  weigh_blocks<T, D>(a, (int32_t)blockIdx.x, (int32_t)gridDim.x);
   if constexpr (sizeof(T) == 2) {
     __shared__ __attribute__((aligned(256))) char smem[2 * WeighTile<T, D>::SLOT];
     __shared__ int32_t flag;
-    if ((int32_t)blockIdx.x < a.tile_grid) {
+    if (a.tile_grid) {
       // Units are of different lengths and go to whom has time: the first by the work-group's number, the
       // others from a queue for each XCD (work-groups are dealt to those in turn), so that a head's rows stay in
       // one L2.  Who draws its last number clears the queue.
@@ -614,10 +652,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void w
       // (a number is drawn after every unit)
       if (threadIdx.x == 0 && n >= of_x && n - of_x == (int32_t)((units - x + kQueues - 1) / kQueues) - 1)
         __hip_atomic_store(a.queue + 16 * x, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      return;
     }
   }
-  weigh_blocks<T, D>(a, (int32_t)blockIdx.x - a.tile_grid, (int32_t)gridDim.x - a.tile_grid);
 }
 
 // The most rows of a request that is taken by blocks.  32 requests of 300..8192 tokens (bf16, 8 KV heads of 128): by
@@ -644,7 +680,7 @@ WeightsPlan weights_plan(const pa_weights_args* x) {
 
 template <typename T, int D>
 int launch_weights(const WeightsK& a, hipStream_t s) {
-  hipLaunchKernelGGL((weights_kernel<T, D>), dim3((unsigned)(a.tile_grid + 1024)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((weights_kernel<T, D>), dim3((unsigned)(a.tile_grid ? a.tile_grid : 1024)), dim3(256), 0, s, a);
   PA_LAUNCH_CHECK("weights_kernel");
   return PA_OK;
 }
@@ -757,6 +793,11 @@ extern "C" int pa_paged_weights(const pa_weights_args* x, void* stream) {
   a.scores = x->scores;
   a.s_sp = x->s_sp;
   a.s_sh = x->s_sh;
+  a.near = a.n_include > 0;
+  for (int i = 0; i < a.n_include; ++i) {
+    const int32_t kind = a.terms[i].kind;
+    a.near = a.near && (kind == PA_WINDOW || kind == PA_SINKS || kind == PA_TWOBAND);
+  }
   a.row_max = p.tile ? kFewRows : INT_MAX;
   a.tile_grid = p.tile ? kTileGroups : 0;
   auto near = [&](int64_t st, int64_t sh) { return st <= (1 << 24) && sh <= (1 << 24) && st >= -(1 << 24) && sh >= -(1 << 24); };

@@ -74,6 +74,19 @@ def test_weights_of_chunks(gpu, dtype, D, Hq, Hkv):
     _weigh(b, pm.LocalStrided(60, 16), max_fresh=3)
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)])
+@pytest.mark.parametrize("mask", [pm.SinksWindow(100, 300), pm.SinksWindow(1, 64), pm.SlidingWindow(5), pm.TwoBand(30, 700, 90),
+                                  pm.Union(pm.SlidingWindow(70), pm.SinksWindow(300, 2)),
+                                  pm.Difference(pm.SlidingWindow(400), pm.SlidingWindow(130))], ids=str)
+def test_weights_under_windows_that_leave_blocks_dead(gpu, dtype, D, mask):
+    """Blocks of keys that no new token sees keep their scores; new keys that nothing sees get 0."""
+    sizes = [(1, 3000), (2, 1025), (40, 2500), (1, 64), (9, 70), (7, 1400), (130, 1300), (1, 2049), (300, 300), (1, 511)]
+    b = Batch(gpu, dtype, D, 32, 8, 4, sizes, seed=9)
+    _weigh(b, mask)
+    _weigh(b, mask, first=np.array([64, 1000, 200, 64, 3, 1390, 900, 2040, 0, 400]))
+    _weigh(b, mask, first=np.array([2900, 3, 2400, 1, 65, 700, 100, 1, 256, 511]), max_fresh=1)
+
+
 def test_weights_of_many_requests_and_long_ones(gpu):
     rng = np.random.default_rng(1)
     for R in (63, 64, 65, 300):
