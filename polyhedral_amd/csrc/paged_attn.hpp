@@ -194,6 +194,12 @@ __device__ __forceinline__ Request load_request(const PagedK& a, const RawReques
   return request_of(s0, s1, x.len, a.T, a.cols << a.page_lg);
 }
 
+// A prefix's tiles are few, and the root of their blocks may leave places without work: then a third of the most
+// shares at least, as a row's states are merged by a work-group of their own.  (24 requests of a token, 4 heads over
+// one of 128, behind 6700 to 26800: 32.6 -> 28.5 us; 9 of up to 29 tokens behind three of up to 62000: 49 -> 44, with
+// half of the shares 37, but 64 behind 8192 then 56 -> 61.)
+constexpr float kFewShares = 3.f;
+
 template <int BM, int LG, int PART = kWhole>
 __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, const RawRequest& raw, int32_t id, int lane) {
   Unit u;
@@ -234,7 +240,8 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, c
       w = work_of<BM, LG, PART>(a, p, q, x.x0, x.x1);
     }
     // (to the nearest: a tile little longer than a share stays whole)
-    const float b = (float)w.blocks, mine = fmaxf(fmaxf(share, (float)w.least), __builtin_amdgcn_sqrtf(b) * p.root_over);
+    const float b = (float)w.blocks, root = __builtin_amdgcn_sqrtf(b) * p.root_over;
+    const float mine = fmaxf(fmaxf(share, (float)w.least), PART == kPrefix ? fminf(root, kFewShares * share) : root);
     const int32_t splits = imax((int32_t)(b * __builtin_amdgcn_rcpf(mine) + 0.5f), 1);
     const int32_t units = w.tiles * a.Hkv * splits, slotted = PART == kPrefix || splits > 1 ? units : 0;
     const int32_t n_in = wave_scan(units), s_in = wave_scan(slotted);
