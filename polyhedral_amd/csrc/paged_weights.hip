@@ -11,7 +11,9 @@
 // cycles and vector instructions, mostly the exponentials' chains, in near half, beside each other; about 40 us go to the units'
 // beginnings and ends (keys' loads, reduction over lanes).  By blocks alone it takes 610 us.
 //
-// Scores, exponentials and sums are float32.  A dead pair adds 0 whatever its key holds, by selection.
+// Scores, exponentials and sums are float32.  A dead pair adds 0 whatever its key or its row's lse holds: by selection
+// (of its exponential, or of its score, as -inf beside a base of the row that is neither NaN nor infinite above).
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 
@@ -148,6 +150,12 @@ __device__ __forceinline__ int64_t readlane64(int64_t x, int l) {
   return (int64_t)((uint64_t)lo | (uint64_t)(uint32_t)hi << 32);
 }
 
+// A row's -lse in log2 units, NaN where that is, and at most the largest number, so that beside it a dead score's -inf
+// stays what it is.
+__device__ __forceinline__ float neg_of(float lse) {
+  return __builtin_elementwise_minimum(-lse * 1.4426950408889634f, FLT_MAX);
+}
+
 // ---- few rows a request -------------------------------------------------------------------------
 // A wave takes a run of consecutive blocks, an equal share of all blocks times the row tiles each meets: K rows go
 // straight into the A operand's registers of 16x16 MFMAs (S^T = K Q^T, as in paged_rows.hpp), once for all
@@ -217,7 +225,7 @@ __device__ __forceinline__ void weigh_blocks(const WeightsK& a, int32_t id, int3
 #pragma unroll
           for (int kc = 0; kc < NK; ++kc) qf[kc] = *reinterpret_cast<const u32x4*>(qrow + 64 * kc);
           const float z = a.lse[(int64_t)(rq.start + tok) * a.lse_st + (int64_t)head * a.lse_sh];
-          neg = -z * 1.4426950408889634f;
+          neg = neg_of(z);
           row_ok = tile * kRows + q16 < rows && z != -INFINITY;
           q_pos = pos0 + tok;
           q_lo = pos0 + divide(tile * kRows, a.by_G);
@@ -551,6 +559,7 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
       if (!((live >> ((j - j0) & 63)) & 1ull)) continue;
       const int32_t i0 = j * kStepRows;
       const uint64_t ok = __ballot(z_now != -INFINITY);  // (rows past the last have no weight)
+      const float neg_now = z_now == -INFINITY ? 0.f : neg_of(z_now);
       const bool is_full = (full >> ((j - j0) & 63)) & 1ull, all = is_full && ok == ~0ull;
       // words of this lane's rows and the wave's keys (rolled, for one copy of the mask's code)
       uint32_t word[2][2] = {};
@@ -567,15 +576,19 @@ __device__ __forceinline__ void weigh_keys(const WeightsK& a, const KeyUnit& u, 
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const bool row = (uint32_t)(ok >> (32 * b + m)) & 1u;
-        const float zb = __shfl(z_now, 32 * b + m);
+        float neg_b = __shfl(neg_now, 32 * b + m);
         u32x4 qf[NQF];
 #pragma unroll
         for (int kc = 0; kc < NQF; ++kc) qf[kc] = *(lds_u4*)(rd[kc] + slot * SLOT + 32 * b * R::ROW);
+        // (a row whose lse is NaN: in its scores, of which the live ones keep it, and not in their base)
+        if (__ballot(neg_now != neg_now) && neg_b != neg_b) {
+          qf[0][0] = ~0u;
+          neg_b = 0.f;
+        }
         __builtin_amdgcn_sched_barrier(0);
         f32x16* y = b ? xb : xa;
         block(qf, y, b ? xa : xb);
-        neg = row ? -zb * 1.4426950408889634f : 0.f;
+        neg = neg_b;
         if (!all) {
           mask_block(y[0], word[b][0]);
           mask_block(y[1], word[b][1]);

@@ -145,6 +145,41 @@ def test_a_live_key_that_is_not_finite_has_its_own_weight(gpu):
     assert torch.equal(*scores)
 
 
+@pytest.mark.parametrize("mask", [pm.Causal(), pm.SinksWindow(3, 70), pm.LocalStrided(40, 16), pm.Full()], ids=str)
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_a_row_whose_lse_is_not_finite_weighs_its_live_keys_alone(gpu, dtype, D, mask):
+    """NaN, infinities and the largest numbers as lse of some rows, in requests of few and of many rows: a key
+    that such a row does not see has the other rows' weights."""
+    b = Batch(gpu, dtype, D, 16, 8, 2, [(300, 700), (1, 60), (40, 150), (3, 100), (64, 64), (129, 400)], seed=3, poison=0.0)
+    spec = paged._paged_mask(mask).spec
+    t, n, s = b.dev()
+    lse = torch.empty(b.T, b.Hq, device=gpu)
+    paged.attention(b.q, b.k, b.v, t, n, s, mask, lse=lse)
+    rng = np.random.default_rng(0)
+    odd = [NAN, INF, -INF, -3.4e38, 3.4e38, -2.5e38]
+    where = [(r, int(i), int(h), odd[int(rng.integers(len(odd)))]) for r in range(len(b.n))
+             for i, h in zip(rng.integers(0, b.n[r], 5), rng.integers(0, b.Hq, 5))]
+    for r, i, h, x in where:
+        lse[b.q_start[r] + i, h] = x
+    # (those without weight: the others' weights and what these may be off by)
+    plain = f64(lse)
+    plain[~(np.abs(plain) < 1e30)] = -INF
+    want, bound = so.weights(f64(b.q), f64(b.k), b.tables, b.lengths, b.q_start, plain, np.zeros((b.pages, b.Hkv, b.P)), spec.live,
+                             D ** -0.5, np.zeros(len(b.n), dtype=int))
+    for r, i, h, _ in where:
+        x = float(lse[b.q_start[r] + i, h])
+        if np.isnan(x) or x < -1e30 and x != -INF:
+            L = b.lengths[r]
+            p = np.flatnonzero(spec.live(np.array([[L - b.n[r] + i]]), np.arange(L)[None, :])[0])
+            want[b.tables[r, p // 16], h // 4, p % 16] += NAN if np.isnan(x) else INF
+    scores = torch.zeros(b.pages, b.Hkv, b.P, device=gpu)
+    got = f64(paged.weights(b.q, b.k, t, n, s, lse, scores, mask))
+    assert np.isnan(want).any() and np.isinf(want).any()
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), np.isinf(want))
+    ok = np.isfinite(want)
+    assert (np.abs(got[ok] - want[ok]) <= bound[ok]).all()
+
+
 def test_weights_with_nothing_to_weigh(gpu):
     q = torch.ones(3, 4, 64, dtype=torch.float16, device=gpu)
     k, s = torch.zeros(2, 2, 16, 64, dtype=torch.float16, device=gpu), torch.full((2, 2, 16), 7.0, device=gpu)
