@@ -623,8 +623,10 @@ int pa_paged_attn(const pa_paged_args* args, void* stream);
  * newest and of the others the keep - recent with the largest scores (equal ones: the lowest places; NaN
  * is above every number; a key without a page below every one), as places in ascending order,
  * kept [layers, R, Hkv, keep]; after[r] = first[r] + keep.  Else kept is -1 and after[r] =
- * lengths[r].  0 <= recent <= keep <= limit, keep >= 1.  scores as above, layers s_sl floats apart.  kept and
- * after share no memory with an input or each other.
+ * lengths[r].  0 <= recent <= keep <= limit, keep >= 1.  scores as above, layers s_sl floats apart.  missing: NULL,
+ * or one int32: then a request past the limit that has a key from first[r] on without a page keeps all, as there is no
+ * place for its keys to go, and missing_bits are set in it.  kept, after and missing share no memory with an input or each
+ * other.
  *
  * pa_evict_rows: in each layer and KV head, row (K, V and score) kept[j] of request r goes to place
  * first[r] + j, in place: kept as pa_choose_keys gives it, or any list with kept[j] >= first[r] + j;
@@ -705,6 +707,8 @@ typedef struct pa_choose_args {
   int32_t layers, R, Hkv, keep, recent, limit;
   int32_t* kept;
   int32_t* after;
+  int32_t* missing;
+  int32_t missing_bits;
 } pa_choose_args;
 
 int pa_choose_keys(const pa_choose_args* args, void* stream);

@@ -14,7 +14,7 @@ LIB_PATH = pathlib.Path(__file__).resolve().parent / "_lib" / "libpolyattn_amd.s
 PA_OK, PA_E_INVALID, PA_E_HIP, PA_E_UNSUPPORTED = 0, -1, -2, -3
 PA_F32, PA_F16, PA_BF16 = 0, 1, 2
 MAX_TERMS = 8
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 c_i32, c_i64, c_f32, c_vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
@@ -114,7 +114,7 @@ class PaChooseArgs(ctypes.Structure):
     _fields_ = [("scores", c_vp), ("s_sl", c_i64), ("s_sp", c_i64), ("s_sh", c_i64), ("n_pages", c_i64),
                 ("page_size", c_i32), ("tables", c_vp), ("pitch", c_i64), ("cols", c_i32), ("lengths", c_vp),
                 ("first", c_vp), ("layers", c_i32), ("R", c_i32), ("Hkv", c_i32), ("keep", c_i32), ("recent", c_i32),
-                ("limit", c_i32), ("kept", c_vp), ("after", c_vp)]
+                ("limit", c_i32), ("kept", c_vp), ("after", c_vp), ("missing", c_vp), ("missing_bits", c_i32)]
 
 
 class PaEvictArgs(ctypes.Structure):

@@ -48,6 +48,8 @@ struct ChooseK {
   int32_t R, Hkv, keep, recent, limit;
   int32_t* kept;
   int32_t* after;
+  int32_t* missing;      // null, or where a request that cannot be evicted for want of pages shows
+  int32_t missing_bits;
 };
 
 // A number of the order of the scores: NaN above all, -0 as 0, never 0.
@@ -228,8 +230,18 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
   const Held q = held_of(a.pages, r);
   const int32_t m = q.len - q.first;
   int32_t* kept = a.kept + (((int64_t)layer * a.R + r) * a.Hkv + h) * a.keep;
-  if (layer == 0 && h == 0 && tid == 0) a.after[r] = m > a.limit ? q.first + a.keep : a.pages.lengths[r];
-  if (m <= a.limit) {
+  const int32_t* table = a.pages.tables + r * a.pages.pitch;
+  // (all layers and heads of a request see the same table; a trip to memory more, where it is asked for)
+  bool whole = m <= a.limit;
+  if (a.missing && !whole) {
+    bool none = false;
+    for (int32_t c = (q.first >> a.pages.page_lg) + tid; c <= (q.len - 1) >> a.pages.page_lg; c += kChooseThreads)
+      none |= checked_page(table[c], a.pages.n_pages) < 0;
+    whole = __syncthreads_or(none);
+    if (whole && layer == 0 && h == 0 && tid == 0) atomicOr(a.missing, a.missing_bits);
+  }
+  if (layer == 0 && h == 0 && tid == 0) a.after[r] = whole ? a.pages.lengths[r] : q.first + a.keep;
+  if (whole) {
     for (int j = tid; j < a.keep; j += kChooseThreads) kept[j] = -1;
     return;
   }
@@ -237,7 +249,6 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
   for (int j = tid; j < a.recent; j += kChooseThreads) kept[want + j] = q.len - a.recent + j;
   if (want == 0) return;
   const float* scores = a.scores + layer * a.s_sl + h * a.s_sh;
-  const int32_t* table = a.pages.tables + r * a.pages.pitch;
   const int32_t held = n + (q.first & 3);
   if (held <= 4 * kChooseThreads)
     choose_body<1, ANY>(a, scores, table, q.first, n, want, kept, s);
@@ -399,9 +410,10 @@ extern "C" int pa_choose_keys(const pa_choose_args* x, void* stream) {
   if (int rc = check_apart("pa_choose_keys",
                            {{"lengths", flat(x->lengths, 4 * R)}, {"first", flat(x->first, x->first ? 4 * R : 0)},
                             {"tables", tables_span(x->tables, x->R, x->pitch, x->cols)}},
-                           {{"kept", kept}, {"after", flat(x->after, 4 * R)}}))
+                           {{"kept", kept}, {"after", flat(x->after, 4 * R)}, {"missing", flat(x->missing, x->missing ? 4 : 0)}}))
     return rc;
-  PA_CHECK_ARG(!overlap(kept, scores) && !overlap(flat(x->after, 4 * R), scores), "pa_choose_keys: kept or after and scores overlap");
+  PA_CHECK_ARG(!overlap(kept, scores) && !overlap(flat(x->after, 4 * R), scores) && !overlap(flat(x->missing, x->missing ? 4 : 0), scores),
+               "pa_choose_keys: kept, after or missing and scores overlap");
   a.scores = x->scores;
   a.s_sl = x->s_sl;
   a.s_sp = x->s_sp;
@@ -416,6 +428,8 @@ extern "C" int pa_choose_keys(const pa_choose_args* x, void* stream) {
   a.limit = x->limit;
   a.kept = x->kept;
   a.after = x->after;
+  a.missing = x->missing;
+  a.missing_bits = x->missing_bits;
   const dim3 grid((unsigned)(x->layers * R * x->Hkv));
   if (a.s_bytes)
     hipLaunchKernelGGL(choose_kernel<false>, grid, dim3(kChooseThreads), 0, static_cast<hipStream_t>(stream), a);

@@ -43,6 +43,7 @@ SHORT_OF_PAGES, TOO_LONG, TOO_MANY_TOKENS = 1, 2, 4
 LIST_FULL = 8   # in PagedKVCache.failed: a release that would have passed the free list's length
 
 SHARED = 16      # there too: a prefix that could not be shared, or its request finished before those that share it
+TRIMMED = 32     # there too: a request that was to be evicted had given back pages in front
 
 TableStep = namedtuple("TableStep", "lengths q_start slots positions free_count status")
 TableStep.__doc__ = """int32 device tensors of a step: tokens of each request with the new ones, the packed rows'
@@ -486,15 +487,17 @@ def _layered(t, dims, name):
     return (1, 0) if t.dim() == dims else (t.shape[0], t.stride(0) if t.shape[0] > 1 else 0)
 
 
-def prepare_choose(scores, tables, lengths, keep, recent, limit=None, first=None, out=None):
+def prepare_choose(scores, tables, lengths, keep, recent, limit=None, first=None, out=None, missing=None, missing_bits=1):
     """A PagedLaunch that says which cached keys stay; its result is a Choice.
 
     scores: float32 [pages, heads, page_size], or [layers, ...]: every layer, request and head chooses by
     its own.  tables int32 [R, columns], lengths int32 [R].  first: int32 [R], the tokens in front that
     always stay (sinks, a shared prefix; default none).  A request of more than ``limit`` (default
     keep) tokens behind those keeps ``keep`` of them: the ``recent`` newest, and of the others those with
-    the largest scores (of equal ones those in front; NaN is above every number).  out: a Choice to
-    write into; its lengths are not the given ones."""
+    the largest scores (of equal ones those in front; NaN is above every number; a key without a page is
+    below all).  out: a Choice to write into; its lengths are not the given ones.  missing: int32 [1]; given, a
+    request past the limit that lacks a page from first on keeps all its keys, which then have no place to
+    go to, and missing gets missing_bits."""
     layers, s_sl = _layered(scores, 3, "scores")
     pages, Hkv, P = scores.shape[-3:]
     _page_size(P)
@@ -516,18 +519,21 @@ def prepare_choose(scores, tables, lengths, keep, recent, limit=None, first=None
         if not _ints(out.kept, "out.kept", shape, dev).is_contiguous():
             raise ValueError("out.kept must be contiguous")
         _ints(out.lengths, "out.lengths", (R,), dev)
+    if missing is not None:
+        _ints(missing, "missing", (1,), dev)
     a = _lib.PaChooseArgs()
     ptr = _lib.address
     a.scores, a.s_sl, a.s_sp, a.s_sh = ptr(scores), s_sl, s_sp, s_sh
     a.n_pages, a.page_size, a.tables, a.pitch, a.cols = pages, P, ptr(tables), pitch, tables.shape[1]
     a.lengths, a.first, a.layers, a.R, a.Hkv = ptr(lengths), ptr(first), layers, R, Hkv
     a.keep, a.recent, a.limit, a.kept, a.after = keep, recent, limit, ptr(out.kept), ptr(out.lengths)
-    return PagedLaunch("pa_choose_keys", (ctypes.byref(a),), [a, scores, tables, lengths, first, out], scores, out)
+    a.missing, a.missing_bits = ptr(missing), int(missing_bits)
+    return PagedLaunch("pa_choose_keys", (ctypes.byref(a),), [a, scores, tables, lengths, first, missing, out], scores, out)
 
 
-def choose(scores, tables, lengths, keep, recent, limit=None, first=None, out=None):
+def choose(scores, tables, lengths, keep, recent, limit=None, first=None, out=None, missing=None, missing_bits=1):
     """Which cached keys stay: see prepare_choose."""
-    return prepare_choose(scores, tables, lengths, keep, recent, limit, first, out)()
+    return prepare_choose(scores, tables, lengths, keep, recent, limit, first, out, missing, missing_bits)()
 
 
 def prepare_evict(kept, k, v, scores, tables, lengths, first=None):
@@ -716,7 +722,8 @@ class PagedKVCache:
         those that it shares) keeps ``keep`` of them, in each layer and head the ``recent`` newest and those
         with the largest scores, moved together in their order; pages that this leaves go back.  From then
         on a token's position is its place among those kept: a mask that counts distances counts them
-        there.  Not in a cache that is trimmed: there may be no page where they go."""
+        there.  Not in a cache that is trimmed: there may be no page where they go.  (A replay of an eviction
+        that was captured before leaves requests with such places as they are, and ``check`` says so.)"""
         if self.scores is None:
             raise RuntimeError("the cache holds no scores: make it with weigh=True")
         if self._trims:
@@ -726,7 +733,7 @@ class PagedKVCache:
         P = self.page_size
         with torch.cuda.device(self.device):
             first = self.shared.clamp(min=min(int(sinks), self.max_length))
-            choice = choose(self.scores, self.tables, self.lengths, keep, recent, limit, first)
+            choice = choose(self.scores, self.tables, self.lengths, keep, recent, limit, first, None, self.failed, TRIMMED)
             evict(choice.kept, self.k, self.v, self.scores, self.tables, self.lengths, first)
             pages = lambda n: ((n + (P - 1)) // P).to(torch.int32)  # noqa: E731
             self._release(pages(choice.lengths), pages(self.lengths))
@@ -797,6 +804,7 @@ class PagedKVCache:
             why = [w for b, w in ((SHORT_OF_PAGES, "too few free pages"), (TOO_LONG, f"a request past {self.max_length} tokens"),
                                   (TOO_MANY_TOKENS, "more new tokens than rows"),
                                   (LIST_FULL, "more pages given back than there are"),
-                                  (SHARED, "a prefix that could not be shared, or was finished before those that share it"))
+                                  (SHARED, "a prefix that could not be shared, or was finished before those that share it"),
+                                  (TRIMMED, "a request without the pages in front was to be evicted"))
                    if bits & b]
             raise RuntimeError("a step did not fit: " + ", ".join(why))

@@ -498,6 +498,63 @@ def test_a_trimmed_cache_does_not_evict(gpu):
         c.evict(10, 2)
 
 
+def test_requests_that_lack_pages_stay_whole_where_asked(gpu):
+    """choose with missing: of requests past the limit those that lack a page from first on keep all."""
+    rng = np.random.default_rng(0)
+    P, lengths = 16, np.array([100, 100, 100, 100, 20, 0, 100])
+    tables, pages = _pool(rng, lengths, P)
+    first = np.array([0, 33, 32, 0, 0, 0, 48])
+    tables[1, 2], tables[2, 1], tables[3, 6], tables[4, 0], tables[6, 3] = -1, -1, 1 << 30, -1, -7
+    scores = rng.standard_normal((2, pages, 3, P)).astype(np.float32)
+    whole = np.array([1, 3, 6])                     # (2 lacks one in front of first, 4 is within the limit)
+    want = [so.choose(s, tables, lengths, 30, 4, 40, first) for s in scores]
+    s, t, n, f = torch.as_tensor(scores, device=gpu), dev(tables, gpu), dev(lengths, gpu), dev(first, gpu)
+    for layers in (slice(None), 0):
+        bits = dev([3], gpu)
+        got = paged.choose(s[layers], t, n, 30, 4, 40, f, missing=bits, missing_bits=64)
+        kept, after = (np.stack([k for k, _ in want]) if layers != 0 else want[0][0]).copy(), want[0][1].copy()
+        kept[..., whole, :, :], after[whole] = -1, lengths[whole]
+        assert np.array_equal(host(got.kept), kept) and np.array_equal(host(got.lengths), after) and int(bits) == 67
+        none = dev([3], gpu)
+        paged.choose(s[layers], t[[0, 2, 4, 5]], n[[0, 2, 4, 5]], 30, 4, 40, f[[0, 2, 4, 5]], missing=none)
+        assert int(none) == 3
+    with pytest.raises(ValueError):
+        paged.choose(s, t, n, 30, 4, 40, f, missing=n)
+    with pytest.raises(RuntimeError, match="overlap"):
+        paged.choose(s, t, n, 30, 4, 40, f, missing=n[:1])
+
+
+def test_an_eviction_captured_before_a_trim_and_replayed_after(gpu):
+    """Requests without pages in front stay as they are, the others are evicted, no page is lost, and check tells."""
+    g = torch.Generator().manual_seed(0)
+    c = paged.PagedKVCache(4, 200, 40, 2, 64, torch.float16, 16, 2, gpu, weigh=True)
+    c.begin([100, 40, 90, 30])
+    for x in (c.k, c.v, c.scores):
+        x.copy_(torch.rand(x.shape, generator=g))
+    out = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(out):
+        c.evict(30, 5)
+    c.trim(window=45)
+    tables, k, v, scores = host(c.tables), f64(c.k), f64(c.v), f64(c.scores)
+    assert (tables[[0, 2], 0] == -1).all() and (tables[1, :3] >= 0).all()
+    only, none = np.array([0, 40, 0, 0]), np.zeros(4, dtype=int)
+    kept = [so.choose(s, tables, only, 30, 5, 30, none)[0] for s in scores]
+    want = [[so.evict(kept[i], x[i], tables, only, none) for i in range(2)] for x in (k, v, scores)]
+    for i in range(2):                               # (the second has nothing left to do)
+        out.replay()
+        torch.cuda.synchronize()
+        assert host(c.lengths).tolist() == [100, 30, 90, 30]
+        tables[1, 2] = -1
+        assert np.array_equal(host(c.tables), tables)
+        ids = np.concatenate([tables[tables >= 0], host(c.free_list)[:int(c.free_count)]])
+        assert sorted(ids.tolist()) == list(range(40))
+    for x, w in zip((c.k, c.v, c.scores), want):
+        assert np.array_equal(f64(x), np.array(w))
+    with pytest.raises(RuntimeError, match="pages in front"):
+        c.check()
+
+
 def test_captured_steps_and_evictions(gpu):
     """A step with its weights and an eviction in graphs, replayed, against a second cache without."""
     R, H, G, D, P = 4, 2, 2, 64, 16

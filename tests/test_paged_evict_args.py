@@ -138,3 +138,9 @@ def test_a_null_sharing_is_refused():
     a = _lib.PaPagedArgs()
     assert _lib.lib().pa_shared_attn(ctypes.byref(a), None, None) == _lib.PA_E_INVALID
     assert "sharing" in _lib.lib().pa_last_error().decode()
+
+
+def test_a_flag_of_missing_pages_that_shares_memory_is_refused():
+    for i, (f, n) in enumerate(CHOOSE.items()):
+        for p in (AT + i * STEP, AT + i * STEP + (n - 1) // 4 * 4):
+            _refused("pa_choose_keys", choose(missing=p), "overlap")
