@@ -626,7 +626,7 @@ int pa_paged_attn(const pa_paged_args* args, void* stream);
  * lengths[r].  0 <= recent <= keep <= limit, keep >= 1.  scores as above, layers s_sl floats apart.  missing: NULL,
  * or one int32: then a request past the limit that has a key from first[r] on without a page keeps all, as there is no
  * place for its keys to go, and missing_bits are set in it.  kept, after and missing share no memory with an input or each
- * other.
+ * other.  With no layers nothing is written.
  *
  * pa_evict_rows: in each layer and KV head, row (K, V and score) kept[j] of request r goes to place
  * first[r] + j, in place: kept as pa_choose_keys gives it, or any list with kept[j] >= first[r] + j;

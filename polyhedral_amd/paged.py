@@ -521,14 +521,18 @@ def prepare_choose(scores, tables, lengths, keep, recent, limit=None, first=None
         _ints(out.lengths, "out.lengths", (R,), dev)
     if missing is not None:
         _ints(missing, "missing", (1,), dev)
+    held, kept = scores, out.kept
+    if not layers:   # (one layer and head stand for none: the lengths do not depend on them)
+        layers, Hkv, s_sp, s_sh = 1, 1, 0, 0
+        held, kept = torch.zeros(P, device=dev), torch.empty(R, keep, dtype=torch.int32, device=dev)
     a = _lib.PaChooseArgs()
     ptr = _lib.address
-    a.scores, a.s_sl, a.s_sp, a.s_sh = ptr(scores), s_sl, s_sp, s_sh
+    a.scores, a.s_sl, a.s_sp, a.s_sh = ptr(held), s_sl, s_sp, s_sh
     a.n_pages, a.page_size, a.tables, a.pitch, a.cols = pages, P, ptr(tables), pitch, tables.shape[1]
     a.lengths, a.first, a.layers, a.R, a.Hkv = ptr(lengths), ptr(first), layers, R, Hkv
-    a.keep, a.recent, a.limit, a.kept, a.after = keep, recent, limit, ptr(out.kept), ptr(out.lengths)
+    a.keep, a.recent, a.limit, a.kept, a.after = keep, recent, limit, ptr(kept), ptr(out.lengths)
     a.missing, a.missing_bits = ptr(missing), int(missing_bits)
-    return PagedLaunch("pa_choose_keys", (ctypes.byref(a),), [a, scores, tables, lengths, first, missing, out], scores, out)
+    return PagedLaunch("pa_choose_keys", (ctypes.byref(a),), [a, held, kept, tables, lengths, first, missing, out], scores, out)
 
 
 def choose(scores, tables, lengths, keep, recent, limit=None, first=None, out=None, missing=None, missing_bits=1):

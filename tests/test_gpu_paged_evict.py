@@ -269,6 +269,18 @@ def test_choose_with_nothing_to_choose(gpu):
     assert got.kept.shape == (0, 1, 1, 4)
 
 
+def test_choose_of_no_layers_says_how_long_requests_are(gpu):
+    s = torch.zeros(0, 20, 3, 16, device=gpu)
+    lengths, first = np.array([100, 40, 90, 0]), np.array([0, 3, 50, 0])
+    t, n = torch.zeros(4, 9, dtype=I32, device=gpu), dev(lengths, gpu)
+    want = so.choose(np.zeros((20, 1, 16)), host(t), lengths, 30, 5, 39, first)[1]
+    out = (torch.empty(0, 4, 3, 30, dtype=I32, device=gpu), dev([-7] * 4, gpu))
+    got = paged.choose(s, t, n, 30, 5, 39, dev(first, gpu), out=out)
+    assert got.lengths is out[1] and np.array_equal(host(got.lengths), want) and want.tolist() == [30, 40, 80, 0]
+    t[0, 3], flag = -1, dev([0], gpu)
+    assert host(paged.choose(s, t, n, 30, 5, 39, dev(first, gpu), missing=flag).lengths).tolist() == [100, 40, 80, 0] and int(flag) == 1
+
+
 # ---- their move ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,D", TYPES)
 @pytest.mark.parametrize("P,layers,keep,first", [(16, 2, 50, 0), (64, None, 300, 3), (32, 1, 129, 40), (256, 3, 1000, 1)])
