@@ -292,7 +292,9 @@ __device__ __forceinline__ void move_rows(const EvictK& a, const int32_t* kept, 
   const int per = THREADS >> lg;  // rows that one load of the work-group takes
   const int one = (1 << a.pages.page_lg) - 1;
   const int32_t reach = a.pages.cols << a.pages.page_lg;
-  if (reach == 0) return;
+  // (a place past the table takes nothing; and sums of places stay below 2^31, however long the list)
+  const int32_t most = imin(a.keep, reach - q.first);
+  if (most <= 0) return;
   struct Batch {
     U x[UNROLL];
     U* from[UNROLL];
@@ -300,13 +302,13 @@ __device__ __forceinline__ void move_rows(const EvictK& a, const int32_t* kept, 
   };
   auto places = [&](int j0, Batch& b) __attribute__((always_inline)) {
     int32_t of[UNROLL], p[UNROLL], d[UNROLL];
-    if (j0 >= a.keep) {
+    if (j0 >= most) {
 #pragma unroll
       for (int i = 0; i < UNROLL; ++i) b.to[i] = nullptr;
       return;
     }
 #pragma unroll
-    for (int i = 0; i < UNROLL; ++i) of[i] = kept[imin(j0 + i * per + (tid >> lg), a.keep - 1)];
+    for (int i = 0; i < UNROLL; ++i) of[i] = kept[imin(j0 + i * per + (tid >> lg), most - 1)];
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
       const int32_t dst = imin(q.first + j0 + i * per + (tid >> lg), reach - 1);
@@ -319,7 +321,7 @@ __device__ __forceinline__ void move_rows(const EvictK& a, const int32_t* kept, 
       p[i] = checked_page(p[i], a.pages.n_pages);
       d[i] = checked_page(d[i], a.pages.n_pages);
       b.from[i] = at(imax(p[i], 0), of[i] & one) + unit;
-      b.to[i] = j < a.keep && of[i] > dst && of[i] < reach && p[i] >= 0 && d[i] >= 0 ? at(d[i], dst & one) + unit : nullptr;
+      b.to[i] = j < most && of[i] > dst && of[i] < reach && p[i] >= 0 && d[i] >= 0 ? at(d[i], dst & one) + unit : nullptr;
     }
   };
   auto fetch = [&](Batch& b) __attribute__((always_inline)) {
@@ -344,7 +346,7 @@ __device__ __forceinline__ void move_rows(const EvictK& a, const int32_t* kept, 
   places(0, b0);
   fetch(b0);
   places(per * UNROLL, b1);
-  for (int j0 = 0; j0 < a.keep; j0 += 2 * per * UNROLL) {
+  for (int j0 = 0; j0 < most; j0 += 2 * per * UNROLL) {
     step(j0, b0, b1);
     step(j0 + per * UNROLL, b1, b0);
   }

@@ -328,6 +328,26 @@ def test_evict_of_odd_lists(gpu):
         assert np.array_equal(f64(x), w)
 
 
+def test_evict_of_lists_longer_than_the_table(gpu):
+    """The longest list there can be, 4 GiB, of a request at the largest positions: places past the table take
+    nothing."""
+    P, D, keep, cols = 256, 64, paged.MAX_POSITION, paged.MAX_POSITION // 256
+    x = torch.randn(2, 3, 1, P, D, device=gpu).half()
+    t = torch.full((1, cols), -1, dtype=I32, device=gpu)
+    t[0, -2:] = dev([2, 0], gpu)
+    reach, first = cols * P, cols * P - 300
+    kept = torch.zeros(1, 1, keep, dtype=I32, device=gpu)
+    kept[0, 0, :290] = torch.arange(first + 10, first + 300, dtype=I32, device=gpu)
+    kept[0, 0, 290:400] = torch.arange(reach - 55, reach + 55, dtype=I32, device=gpu)
+    kept[0, 0, -5000:] = reach - 1
+    want = x.clone()
+    flat = torch.cat([x[:, 2, 0], x[:, 0, 0]], dim=1)          # the last 512 places
+    flat[:, 212:502] = flat[:, 222:512].clone()
+    want[:, 2, 0], want[:, 0, 0] = flat[:, :P], flat[:, P:]
+    paged.evict(kept, x[0], x[1], None, t, dev([reach], gpu), dev([first], gpu))
+    assert torch.equal(x, want)
+
+
 def test_evict_of_layouts(gpu):
     """K and V in one buffer, rows before heads, layers innermost."""
     P, keep, H, D, layers = 16, 40, 3, 64, 2
