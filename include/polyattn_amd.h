@@ -615,7 +615,8 @@ int pa_paged_attn(const pa_paged_args* args, void* stream);
  * page_size of page tables[r][t / page_size]: float at scores + page * s_sp + head * s_sh + row.  Keys
  * without a page and scores of no request's keys are left as they are; no key from first[r] on is
  * in two requests' tables.  first may be NULL (0).  max_fresh: the most new tokens of a request (a hint, as
- * in pa_paged_attn).  Every key's sum is taken in a fixed order.  scores shares no memory with an input or
+ * in pa_paged_attn).  Every key's sum is taken in a fixed order.  (In 16 bits, with max_fresh of more than 32 rows:
+ * requests times heads times 256-key groups of a table's reach stay below 2^31.)  scores shares no memory with an input or
  * itself.  workspace as in pa_paged_attn, its sizes (which may be 0) from pa_weights_workspace.
  *
  * pa_choose_keys: for each of `layers` layers, request and KV head the keys that stay.  With m =

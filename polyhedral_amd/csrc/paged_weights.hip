@@ -17,6 +17,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <algorithm>
+
 #include "page_checks.hpp"
 #include "paged_rows.hpp"
 
@@ -738,6 +740,12 @@ extern "C" int pa_paged_weights(const pa_weights_args* x, void* stream) {
   int lg;
   if (int rc = check_weights(who, x, &lg)) return rc;
   if (x->R == 0 || x->T == 0 || x->n_pages == 0 || x->cols == 0) return PA_OK;
+  const WeightsPlan p = weights_plan(x);
+  // (units are counted in 32 bits: those of whole groups of keys, at most one to each of a table, and the shares)
+  const int64_t many = std::min<int64_t>(x->R, x->T * (x->Hq / x->Hkv) / (kFewRows + 1)), groups = ((int64_t)x->cols << lg >> kKeysLg) + 1;
+  PA_CHECK_ARG(!p.tile || (wide)many * groups * x->Hkv < INT_MAX - 4 * kTileShares,
+               "%s: %lld requests of %d heads and tables of %d pages of %d exceed the units that can be counted", who, (long long)many,
+               x->Hkv, x->cols, x->page_size);
   PA_CHECK_ARG(x->q && x->k && x->lse && x->scores && x->tables && x->lengths && x->q_start, "%s: null pointer", who);
   const int64_t esz = x->dtype == PA_F32 ? 4 : 2, row = x->D * esz, R = x->R;
   auto al = [&](const void* p, int64_t s0, int64_t s1, int64_t s2) {
@@ -761,7 +769,6 @@ extern "C" int pa_paged_weights(const pa_weights_args* x, void* stream) {
   };
   const char* other = in_of(scores);
   PA_CHECK_ARG(!other, "%s: scores and %s overlap", who, other);
-  const WeightsPlan p = weights_plan(x);
   PA_CHECK_ARG(p.bytes == 0 || (x->workspace && reinterpret_cast<uintptr_t>(x->workspace) % 256 == 0 && x->workspace_bytes >= p.bytes),
                "%s: needs a 256-byte aligned workspace of %lld bytes", who, (long long)p.bytes);
   const Strided<1> ws = flat(x->workspace, p.bytes);

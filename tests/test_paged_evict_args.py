@@ -144,3 +144,14 @@ def test_a_flag_of_missing_pages_that_shares_memory_is_refused():
     for i, (f, n) in enumerate(CHOOSE.items()):
         for p in (AT + i * STEP, AT + i * STEP + (n - 1) // 4 * 4):
             _refused("pa_choose_keys", choose(missing=p), "overlap")
+
+
+def test_more_units_than_can_be_counted_are_refused():
+    """Requests of many rows are taken by 256 keys and head, in numbers of 32 bits."""
+    many = dict(T=1 << 13, max_fresh=1 << 13, R=1 << 20, Hq=1 << 15, Hkv=1 << 15)
+    _refused("pa_paged_weights", weights(cols=1 << 25, pitch=1 << 25, **many), "units")
+    _refused("pa_paged_weights", weights(cols=1 << 24, pitch=1 << 24, T=100, max_fresh=40, R=4, Hq=4096, Hkv=4096), "units")
+    # (a token a request is taken by blocks; and so little of a table is no matter)
+    for some in (dict(max_fresh=1), dict(cols=64, pitch=64), dict(dtype=_lib.PA_F32)):
+        rc, message = _call("pa_paged_weights", weights(**{**many, "cols": 1 << 25, "pitch": 1 << 25, "q": None, **some}))
+        assert rc == _lib.PA_E_INVALID and "null pointer" in message, (some, message)
