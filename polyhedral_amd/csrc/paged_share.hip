@@ -3,10 +3,12 @@
 // With own(r) the holder of request r where it has one, tokens in this step and whole pages to share,
 // a group is the requests of one holder, if they are two or more; its prefix is the least that they
 // share.  Each request sums over the others (R^2 comparisons, spread over the work-group: 64 requests
-// are 4 a thread), so no atomic gives an order, and the same step has the same plan always.
+// are 4 a thread), so no atomic gives an order, and the same step has the same plan always.  More than 1024 are
+// taken 1024 at a time, each compared with those of its own time alone, so the work grows as their number.
 //
 // What bounds it: latency, three trips to memory, the exchanges over the LDS and the launch: 5.0 us for 65 requests of
-// 64 tokens, 5.5 for 45 of 110.
+// 64 tokens, 5.5 for 45 of 110; for many the comparisons: 256 requests 12 us, 1024 127, 4096 290 (all with all: 2.6 ms),
+// 2^20 73 ms.
 #include "page_checks.hpp"
 #include "paged_attn.hpp"
 
@@ -35,7 +37,7 @@ struct ShareK {
 template <bool LDS>
 __global__ __launch_bounds__(kShareThreads) void share_kernel(const ShareK a) {
   constexpr int NW = kShareThreads / 64;
-  __shared__ int32_t lds[LDS ? 8 * kShareRequests : 1];
+  __shared__ int32_t lds[LDS ? 8 * kShareRequests : 2 * kShareThreads];
   __shared__ int32_t wave_n[NW];
   int32_t* at = LDS ? lds : a.workspace;
   int32_t *s0 = at, *n = at + a.R, *len = at + 2 * (int64_t)a.R, *own = at + 3 * (int64_t)a.R, *some = at + 4 * (int64_t)a.R,
@@ -56,63 +58,127 @@ __global__ __launch_bounds__(kShareThreads) void share_kernel(const ShareK a) {
     falls |= y < x;
   }
   if (__syncthreads_or(falls)) {
-    if (tid == 0) {
-      int32_t end = 0;
-      for (int r = 0; r < a.R; ++r) {
-        const int32_t y = s0[r] + n[r], x = imax(s0[r], end);
-        s0[r] = x;
-        end = imax(x, y);
-        n[r] = end - x;
+    int32_t top = 0;
+    for (int r0 = 0; r0 < a.R; r0 += kShareThreads) {
+      const int r = r0 + tid;
+      const bool in = r < a.R;
+      const int32_t y = in ? s0[r] + n[r] : 0;
+      int32_t x = in ? s0[r] : 0;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int32_t u = __shfl_up(x, o);
+        x = lane >= o ? imax(x, u) : x;
+      }
+      if (lane == 63) wave_n[w] = x;
+      __syncthreads();
+      x = imax(x, top);
+#pragma unroll
+      for (int z = 0; z < NW; ++z) {
+        const int32_t u = wave_n[z];
+        x = z < w ? imax(x, u) : x;
+        top = imax(top, u);
+      }
+      if (in) {
         const int32_t o = a.holders[r];
+        s0[r] = x;
+        n[r] = imax(y, x) - x;
         own[r] = (uint32_t)o < (uint32_t)a.R && n[r] > 0 && some[r] > 0 ? o : -1;
       }
+      __syncthreads();
     }
-    __syncthreads();
   }
 
   // ---- a request among those of its holder, and as a holder: `per` lanes to a request --------------------
   int per = 1;
   while (per < 64 && 2 * per * a.R <= kShareThreads) per *= 2;
   const int sub = tid & (per - 1);
-  for (int r0 = 0; r0 < a.R; r0 += kShareThreads / per) {
-    const int r = r0 + tid / per;
-    const int32_t mine = r < a.R ? own[r] : -1;
-    int32_t count = 0, before = 0, least = kMaxPosition;
-    int32_t members = 0, sum = 0, lo = kMaxPosition, hi = 0, pre = kMaxPosition;
-    for (int x = sub; x < a.R; x += per) {
-      const int32_t o = own[x], nx = n[x], sx = some[x], lx = len[x];
-      if (o >= 0 && o == mine) {
-        ++count;
-        before += x < r ? nx : 0;
-        least = imin(least, sx);
+  if constexpr (LDS) {
+    for (int r0 = 0; r0 < a.R; r0 += kShareThreads / per) {
+      const int r = r0 + tid / per;
+      const int32_t mine = r < a.R ? own[r] : -1;
+      int32_t count = 0, before = 0, least = kMaxPosition;
+      int32_t members = 0, sum = 0, lo = kMaxPosition, hi = 0, pre = kMaxPosition;
+      for (int x = sub; x < a.R; x += per) {
+        const int32_t o = own[x], nx = n[x], sx = some[x], lx = len[x];
+        if (o >= 0 && o == mine) {
+          ++count;
+          before += x < r ? nx : 0;
+          least = imin(least, sx);
+        }
+        if (o == r) {
+          ++members;
+          sum += nx;
+          lo = imin(lo, lx - nx);
+          hi = imax(hi, lx - 1);
+          pre = imin(pre, sx);
+        }
       }
-      if (o == r) {
-        ++members;
-        sum += nx;
-        lo = imin(lo, lx - nx);
-        hi = imax(hi, lx - 1);
-        pre = imin(pre, sx);
+      for (int o = 1; o < per; o <<= 1) {
+        count += __shfl_xor(count, o);
+        before += __shfl_xor(before, o);
+        least = imin(least, __shfl_xor(least, o));
+        members += __shfl_xor(members, o);
+        sum += __shfl_xor(sum, o);
+        lo = imin(lo, __shfl_xor(lo, o));
+        hi = imax(hi, __shfl_xor(hi, o));
+        pre = imin(pre, __shfl_xor(pre, o));
+      }
+      if (r < a.R && sub == 0) {
+        const bool in = count > 1, group = members > 1;
+        off[r] = before;
+        cut[r] = in ? least : 0;
+        tot[r] = group ? sum : 0;
+        a.first[r] = in ? least : 0;
+        a.prefix[r] = group ? pre : 0;
+        a.low[r] = group ? lo : 0;
+        a.high[r] = group ? hi : 0;
       }
     }
-    for (int o = 1; o < per; o <<= 1) {
-      count += __shfl_xor(count, o);
-      before += __shfl_xor(before, o);
-      least = imin(least, __shfl_xor(least, o));
-      members += __shfl_xor(members, o);
-      sum += __shfl_xor(sum, o);
-      lo = imin(lo, __shfl_xor(lo, o));
-      hi = imax(hi, __shfl_xor(hi, o));
-      pre = imin(pre, __shfl_xor(pre, o));
+  } else {
+    // Many requests, in order, as many at a time as there are threads: a request's rows come after those that its
+    // holder's earlier ones have, which are the sum so far and what the LDS shows of these.  (Whole numbers, whose
+    // sums and least ones do not depend on the order of the atomics; these pass the L1, so the loads do too.)
+    int32_t *count = a.first, *sum = a.start, *pre = a.prefix, *lo = a.low, *hi = a.high;
+    int32_t *by = lds, *of = lds + kShareThreads;
+    auto get = [](const int32_t* p) __attribute__((always_inline)) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    for (int g = tid; g < a.R; g += kShareThreads) {
+      count[g] = sum[g] = hi[g] = 0;
+      pre[g] = lo[g] = kMaxPosition;
     }
-    if (r < a.R && sub == 0) {
-      const bool in = count > 1, group = members > 1;
-      off[r] = before;
-      cut[r] = in ? least : 0;
-      tot[r] = group ? sum : 0;
-      a.first[r] = in ? least : 0;
-      a.prefix[r] = group ? pre : 0;
-      a.low[r] = group ? lo : 0;
-      a.high[r] = group ? hi : 0;
+    for (int r0 = 0; r0 < a.R; r0 += kShareThreads) {
+      const int r = r0 + tid;
+      const int32_t o = r < a.R ? own[r] : -1, m = r < a.R ? n[r] : 0;
+      by[tid] = o;
+      of[tid] = m;
+      __threadfence();
+      __syncthreads();
+      int32_t before = o >= 0 ? get(sum + o) : 0;
+#pragma unroll 8
+      for (int x = 0; x < 64 * (w + 1); ++x) before += by[x] == o && x < tid ? of[x] : 0;
+      if (r < a.R) off[r] = before;
+      __syncthreads();
+      if (o >= 0) {
+        atomicAdd(count + o, 1);
+        atomicAdd(sum + o, m);
+        atomicMin(pre + o, some[r]);
+        atomicMin(lo + o, len[r] - m);
+        atomicMax(hi + o, len[r] - 1);
+      }
+    }
+    __threadfence();
+    __syncthreads();
+    for (int r = tid; r < a.R; r += kShareThreads) {
+      const int32_t o = own[r];
+      cut[r] = o >= 0 && get(count + o) > 1 ? get(pre + o) : 0;
+    }
+    __syncthreads();
+    for (int g = tid; g < a.R; g += kShareThreads) {
+      const bool group = get(count + g) > 1;
+      tot[g] = group ? get(sum + g) : 0;
+      pre[g] = group ? get(pre + g) : 0;
+      lo[g] = group ? get(lo + g) : 0;
+      hi[g] = group ? get(hi + g) : 0;
+      a.first[g] = cut[g];
     }
   }
   __syncthreads();

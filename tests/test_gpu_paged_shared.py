@@ -62,6 +62,77 @@ def test_sharing_of_odd_entries(gpu):
     _sharing(gpu, lengths, np.zeros(7, dtype=int), np.full(6, 2), np.full(6, 16), 16, 0)
 
 
+def _plan(lengths, q_start, holders, shared, P, T):
+    """so.sharing for many requests, all in range: a stable sort by holder."""
+    R, n = len(lengths), np.diff(q_start)
+    some = np.minimum(shared, lengths) // P * P
+    own = np.where((n > 0) & (some > 0), holders, -1)
+    big = 1 << 40
+    count, prefix, low, high = np.zeros(R, dtype=np.int64), np.full(R, big), np.full(R, big), np.zeros(R, dtype=np.int64)
+    who = np.flatnonzero(own >= 0)
+    np.add.at(count, own[who], 1)
+    np.minimum.at(prefix, own[who], some[who])
+    np.minimum.at(low, own[who], (lengths - n)[who])
+    np.maximum.at(high, own[who], lengths[who] - 1)
+    for x in (prefix, low, high):
+        x[count < 2] = 0
+    who = who[count[own[who]] > 1]
+    first = np.zeros(R, dtype=np.int64)
+    first[who] = prefix[own[who]]
+    who = who[np.argsort(own[who], kind="stable")]
+    start = np.zeros(R + 1, dtype=np.int64)
+    np.add.at(start, own[who] + 1, n[who])
+    i = np.arange(int(n[who].sum())) - np.repeat(np.cumsum(n[who]) - n[who], n[who])
+    fill = np.full(T - len(i), -1)
+    return (np.cumsum(start), np.concatenate([np.repeat(q_start[who], n[who]) + i, fill]),
+            np.concatenate([np.repeat((lengths - n)[who], n[who]) + i, fill]), prefix, low, high, first)
+
+
+def _many(R, groups, seed):
+    rng = np.random.default_rng(seed)
+    lengths = rng.integers(0, 300, R)
+    n = np.minimum(rng.integers(0, 3, R), lengths)
+    return lengths, np.concatenate([[0], np.cumsum(n)]), rng.integers(-1, groups, R) * (R // groups), rng.integers(0, 300, R)
+
+
+@pytest.mark.parametrize("R,groups", [(40, 7), (1025, 1), (2048, 2048), (20000, 300), (200000, 1), (200000, 50000), (1 << 20, 5)])
+def test_sharing_of_many_requests(gpu, R, groups):
+    """Work that does not grow with the square of the requests."""
+    for x, y in zip(_plan(*_many(300, 20, R), 16, 900), so.sharing(*_many(300, 20, R), 16, 900)):
+        assert np.array_equal(x, y)
+    args = _many(R, groups, R)
+    T = int(args[1][-1]) + 3
+    got = paged.sharing(*(dev(x, gpu) for x in args), 16, T)
+    for g, w, name in zip(got, _plan(*args, 16, T), paged.Sharing._fields):
+        assert np.array_equal(host(g), w), name
+
+
+def falling(q_start, n, rng):
+    """Starts that are the given ones once those that fall back are taken as the largest before."""
+    raw = q_start.copy()
+    at = 1 + np.flatnonzero(n == 0)
+    raw[at] -= rng.integers(0, 50, len(at))
+    raw[0] -= 4
+    assert np.array_equal(np.maximum.accumulate(np.maximum(raw, 0)), q_start) and (np.diff(raw) < 0).any()
+    return raw
+
+
+@pytest.mark.parametrize("R,groups", [(6, 2), (64, 3), (65, 9), (1000, 40), (1024, 5), (1025, 5), (5000, 99)])
+def test_sharing_of_starts_that_fall_back(gpu, R, groups):
+    lengths, q_start, holders, shared = _many(R, groups, R)
+    T, rng = int(q_start[-1]) + 2, np.random.default_rng(R)
+    raw = falling(q_start, np.diff(q_start), rng)
+    got = paged.sharing(dev(lengths, gpu), dev(raw, gpu), dev(holders, gpu), dev(shared, gpu), 16, T)
+    for g, w, name in zip(got, so.sharing(lengths, q_start, holders, shared, 16, T), paged.Sharing._fields):
+        assert np.array_equal(host(g), w), name
+    raw[R // 2:] = T + 9 - np.arange(R + 1 - R // 2)      # (and past the rows, falling from there)
+    want = np.maximum.accumulate(np.clip(raw, 0, T))
+    lengths = lengths + np.diff(want)
+    got = paged.sharing(dev(lengths, gpu), dev(raw, gpu), dev(holders, gpu), dev(shared, gpu), 16, T)
+    for g, w, name in zip(got, so.sharing(lengths, want, holders, shared, 16, T), paged.Sharing._fields):
+        assert np.array_equal(host(g), w), name
+
+
 # ---- attention ------------------------------------------------------------------------------------
 class Shared:
     """groups: (prefix tokens, [(new tokens, own tokens with them), ..]); alone: the same of requests without
