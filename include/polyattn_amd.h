@@ -601,6 +601,12 @@ int pa_paged_attn(const pa_paged_args* args, void* stream);
  * 1]; prefix, low, high, first [R]; rows, positions [T]; workspace int32 [8 R].  The outputs and the
  * workspace share no memory with each other or with an input.
  *
+ * pa_page_finish: which of the requests with done[r] != 0 can give their pages back, in a cache whose requests share
+ * prefixes (holders and shared as above): all but holders of another request that is not done, for which refused_bits
+ * are set in refused.  For one that can, the columns first[r] .. last[r] - 1 of its table are its own pages, which
+ * pa_page_release takes; the entries in front become -1, lengths[r] and shared[r] 0, holders[r] -1.  For others first[r]
+ * = last[r] = 0.  done [R] bytes; refused one int32; workspace int32 [R].  No two tensors share memory.
+ *
  * pa_shared_attn: pa_paged_attn of the same arguments, for requests that share prefixes as `sharing`
  * says, computed once for all rows of a group: the keys t < prefix[g] of request g's table under
  * the mask at the rows' positions, and the keys from first[r] on of each request's own table.  What
@@ -652,6 +658,23 @@ typedef struct pa_share_args {
 } pa_share_args;
 
 int pa_share_rows(const pa_share_args* args, void* stream);
+
+typedef struct pa_finish_args {
+  const uint8_t* done;
+  int32_t* holders;
+  int32_t* shared;
+  int32_t* lengths;
+  int32_t R, page_size;
+  int32_t* tables;
+  int64_t pitch;
+  int32_t cols, refused_bits;
+  int32_t* refused;
+  int32_t* first;
+  int32_t* last;
+  int32_t* workspace;
+} pa_finish_args;
+
+int pa_page_finish(const pa_finish_args* args, void* stream);
 
 typedef struct pa_sharing {
   const int32_t* start;

@@ -14,7 +14,7 @@ LIB_PATH = pathlib.Path(__file__).resolve().parent / "_lib" / "libpolyattn_amd.s
 PA_OK, PA_E_INVALID, PA_E_HIP, PA_E_UNSUPPORTED = 0, -1, -2, -3
 PA_F32, PA_F16, PA_BF16 = 0, 1, 2
 MAX_TERMS = 8
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 c_i32, c_i64, c_f32, c_vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
@@ -96,6 +96,12 @@ class PaShareArgs(ctypes.Structure):
                 ("low", c_vp), ("high", c_vp), ("first", c_vp), ("workspace", c_vp)]
 
 
+class PaFinishArgs(ctypes.Structure):
+    _fields_ = [("done", c_vp), ("holders", c_vp), ("shared", c_vp), ("lengths", c_vp), ("R", c_i32), ("page_size", c_i32),
+                ("tables", c_vp), ("pitch", c_i64), ("cols", c_i32), ("refused_bits", c_i32), ("refused", c_vp), ("first", c_vp),
+                ("last", c_vp), ("workspace", c_vp)]
+
+
 class PaSharing(ctypes.Structure):
     _fields_ = [("start", c_vp), ("rows", c_vp), ("positions", c_vp), ("prefix", c_vp), ("low", c_vp), ("high", c_vp),
                 ("first", c_vp)]
@@ -164,6 +170,7 @@ SIGNATURES = {
     "pa_paged_workspace": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), ctypes.POINTER(c_i64), ctypes.POINTER(c_i64)]),
     "pa_paged_attn": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), c_vp]),
     "pa_share_rows": (ctypes.c_int, [ctypes.POINTER(PaShareArgs), c_vp]),
+    "pa_page_finish": (ctypes.c_int, [ctypes.POINTER(PaFinishArgs), c_vp]),
     "pa_shared_workspace": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), ctypes.POINTER(c_i64), ctypes.POINTER(c_i64)]),
     "pa_shared_attn": (ctypes.c_int, [ctypes.POINTER(PaPagedArgs), ctypes.POINTER(PaSharing), c_vp]),
     "pa_weights_workspace": (ctypes.c_int, [ctypes.POINTER(PaWeightsArgs), ctypes.POINTER(c_i64), ctypes.POINTER(c_i64)]),

@@ -216,8 +216,78 @@ __global__ __launch_bounds__(kShareThreads) void share_kernel(const ShareK a) {
   for (int i = total + tid; i < a.T; i += kShareThreads) a.rows[i] = a.positions[i] = -1;
 }
 
+// Which requests give their pages back: one work-group marks the holders of requests that go on, then a thread per
+// request says what becomes of it, then a wave per request clears what its table names of its holder's pages.  What
+// bounds it: latency, two trips to memory and the launch.
+struct FinishK {
+  const uint8_t* done;
+  int32_t* holders;
+  int32_t* shared;
+  int32_t* lengths;
+  int32_t R, page_lg;
+  int32_t* tables;
+  int64_t pitch;
+  int32_t cols, refused_bits;
+  int32_t* refused;
+  int32_t* first;
+  int32_t* last;
+  int32_t* busy;
+};
+
+__global__ __launch_bounds__(kShareThreads) void finish_kernel(const FinishK a) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  for (int r = tid; r < a.R; r += kShareThreads) a.busy[r] = 0;
+  __syncthreads();
+  for (int r = tid; r < a.R; r += kShareThreads) {
+    const int32_t h = a.holders[r];
+    if ((uint32_t)h < (uint32_t)a.R && h != r && !a.done[r]) a.busy[h] = 1;
+  }
+  __syncthreads();
+  bool kept = false;
+  for (int r = tid; r < a.R; r += kShareThreads) {
+    const bool done = a.done[r], busy = a.busy[r];
+    const int32_t h = a.holders[r];
+    const bool member = (uint32_t)h < (uint32_t)a.R && h != r, go = done && !busy;
+    kept |= done && busy;
+    a.first[r] = go && member ? imin(imax(a.shared[r], 0) >> a.page_lg, a.cols) : 0;
+    a.last[r] = go ? a.cols : 0;
+    if (go) {
+      a.lengths[r] = a.shared[r] = 0;
+      a.holders[r] = -1;
+    }
+  }
+  if (__syncthreads_or(kept) && tid == 0) *a.refused |= a.refused_bits;
+  for (int r = w; r < a.R; r += kShareThreads / 64)
+    for (int32_t c = lane; c < a.first[r]; c += 64) a.tables[r * a.pitch + c] = -1;
+}
+
 }  // namespace
 }  // namespace pa
+
+extern "C" int pa_page_finish(const pa_finish_args* x, void* stream) {
+  using namespace pa;
+  PA_CHECK_ARG(x, "pa_page_finish: null arguments");
+  int lg;
+  if (int rc = check_pages("pa_page_finish", 0, x->page_size, &lg)) return rc;
+  PA_CHECK_ARG(x->R >= 0 && x->R < (1 << 24), "pa_page_finish: R=%d (below 2^24)", x->R);
+  PA_CHECK_ARG(x->cols >= 0 && ((int64_t)x->cols << lg) <= kMaxPosition && x->pitch >= x->cols,
+               "pa_page_finish: %d columns of %d, pitch %lld", x->cols, x->page_size, (long long)x->pitch);
+  if (x->R == 0) return PA_OK;
+  PA_CHECK_ARG(x->done && x->holders && x->shared && x->lengths && x->refused && x->first && x->last && x->workspace &&
+                   (x->cols == 0 || x->tables),
+               "pa_page_finish: null pointer");
+  const int64_t n = 4ll * x->R;
+  if (int rc = check_apart("pa_page_finish", {{"done", flat(x->done, x->R)}},
+                           {{"holders", flat(x->holders, n)}, {"shared", flat(x->shared, n)}, {"lengths", flat(x->lengths, n)},
+                            {"tables", tables_span(x->tables, x->R, x->pitch, x->cols)}, {"refused", flat(x->refused, 4)},
+                            {"first", flat(x->first, n)}, {"last", flat(x->last, n)}, {"workspace", flat(x->workspace, n)}}))
+    return rc;
+  const FinishK a{x->done, x->holders, x->shared, x->lengths, x->R, lg, x->tables, x->pitch, x->cols, x->refused_bits, x->refused,
+                  x->first, x->last, x->workspace};
+  hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(kShareThreads), 0, static_cast<hipStream_t>(stream), a);
+  PA_LAUNCH_CHECK("finish_kernel");
+  return PA_OK;
+}
 
 extern "C" int pa_share_rows(const pa_share_args* x, void* stream) {
   using namespace pa;

@@ -749,10 +749,6 @@ class PagedKVCache:
         with torch.cuda.device(self.device):
             self.failed |= status * LIST_FULL
 
-    def _may_share(self):
-        # (a captured call may be replayed after the first prefix is shared)
-        return self._shares or torch.cuda.is_current_stream_capturing()
-
     def finish(self, done):
         """Gives back the pages of the requests where done (bool [requests], on the device, or a list,
         which a graph's capture does not take) is true and sets their lengths to 0.  One whose tokens
@@ -762,30 +758,17 @@ class PagedKVCache:
         done = done.to(device=self.device, dtype=torch.bool)
         if done.shape != (self.requests,):
             raise ValueError(f"done must be [{self.requests}], got {list(done.shape)}")
-        with torch.cuda.device(self.device):
-            if not self._may_share():
-                last = done.to(torch.int32) * self.tables.shape[1]
-                self._release(torch.zeros_like(last), last)
-                self.lengths.masked_fill_(done, 0)
-                return
-            self_ = torch.arange(self.requests, dtype=torch.int32, device=self.device)
-            member = (self.holders >= 0) & (self.holders != self_)
-            busy = torch.zeros(self.requests + 1, dtype=torch.bool, device=self.device)
-            busy.scatter_(0, torch.where(member & ~done, self.holders, self.requests).long(), True)
-            # (whether any is, without a reduction, which may clear memory in ways that a graph does not replay)
-            some = torch.zeros(2, dtype=torch.int32, device=self.device)
-            some.scatter_(0, (done & busy[:-1]).long(), SHARED)
-            self.failed |= some[1:]
-            done = done & ~busy[:-1]
-            # (a shared prefix's pages are its holder's)
-            first = torch.where(member, self.shared // self.page_size, 0).to(torch.int32)
-            last = done.to(torch.int32) * self.tables.shape[1]
-            self._release(first, last)
-            col = torch.arange(self.tables.shape[1], dtype=torch.int32, device=self.device)
-            self.tables.masked_fill_(done[:, None] & (col < first[:, None]), -1)
-            self.lengths.masked_fill_(done, 0)
-            self.shared.masked_fill_(done, 0)
-            self.holders.masked_fill_(done, -1)
+        done = done.contiguous()
+        # (a step captured before the first prefix is shared is right after it too: the state is on the device)
+        first, last, busy = (torch.empty(self.requests, dtype=torch.int32, device=self.device) for _ in range(3))
+        a = _lib.PaFinishArgs()
+        ptr = _lib.address
+        a.done, a.holders, a.shared, a.lengths = ptr(done), ptr(self.holders), ptr(self.shared), ptr(self.lengths)
+        a.R, a.page_size = self.requests, self.page_size
+        a.tables, a.pitch, a.cols = ptr(self.tables), self.tables.stride(0), self.tables.shape[1]
+        a.refused, a.refused_bits, a.first, a.last, a.workspace = ptr(self.failed), SHARED, ptr(first), ptr(last), ptr(busy)
+        PagedLaunch("pa_page_finish", (ctypes.byref(a),), [a, done, first, last, busy], self.lengths, None)()
+        self._release(first, last)
 
     def trim(self, window, sinks=0):
         """Gives back the pages that neither the next token's window nor the first ``sinks`` tokens
@@ -795,10 +778,9 @@ class PagedKVCache:
         self._trims = True
         P = self.page_size
         with torch.cuda.device(self.device):
-            last = ((self.lengths - int(min(window, MAX_POSITION)) + 1).clamp(min=0) // P).to(torch.int32)
-            first = torch.full_like(last, min(-(-int(sinks) // P), self.tables.shape[1]))
-            if self._may_share():   # (nor what requests share)
-                torch.maximum(first, self.shared // P, out=first)
+            last = (self.lengths - int(min(window, MAX_POSITION) - 1)).clamp_(min=0) // P
+            # (nor what requests share)
+            first = (self.shared // P).clamp_(min=min(-(-int(sinks) // P), self.tables.shape[1]))
             self._release(first, last)
 
     def check(self):

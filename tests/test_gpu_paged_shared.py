@@ -3,6 +3,7 @@ tests/shared_oracle.py and tests/paged_oracle.py."""
 import numpy as np
 import pytest
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from polyhedral_amd import paged
 from polyhedral_amd.polyattn import masks as pm
@@ -547,3 +548,86 @@ def test_a_captured_finish_keeps_what_is_shared_later(gpu):
             assert np.array_equal(tables[0, :4], prefix)
     with pytest.raises(RuntimeError, match="finished before"):   # (0, while 2 went on)
         c.check()
+
+
+class _Count(TorchDispatchMode):
+    """Counts torch's operations but those that only make or view a tensor."""
+
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        name = func.overloadpacket.__name__
+        if name not in ("empty", "view", "detach", "slice", "select", "alias", "unsqueeze", "expand"):
+            self.names.append(name)
+        return func(*args, **(kwargs or {}))
+
+
+def test_a_cache_that_never_shares_gives_pages_back_in_few_launches(gpu):
+    """Captured or not, as many as before requests could share."""
+    c = paged.PagedKVCache(3, 200, 40, 2, 64, torch.float16, 16, device=gpu)
+    c.begin([100, 40, 90])
+    done = torch.zeros(3, dtype=torch.bool, device=gpu)
+    torch.cuda.synchronize()
+    for what, most in ((lambda: c.finish(done), 7), (lambda: c.trim(50), 8)):
+        for captured in (False, True):
+            count = _Count()
+            if captured:
+                with torch.cuda.graph(torch.cuda.CUDAGraph()), count:
+                    what()
+            else:
+                with count:
+                    what()
+            assert len(count.names) <= most, count.names
+
+
+@pytest.mark.parametrize("R,cols", [(1, 3), (7, 20), (64, 5), (1500, 70)])
+def test_finish_against_numpy(gpu, R, cols):
+    """Random members, holders and requests of their own, any of them done: twice, the second time captured."""
+    P, rng = 16, np.random.default_rng(R)
+    c = paged.PagedKVCache(R, cols * P, R * cols + 5, 1, 64, torch.float16, P, device=gpu)
+    for captured in (False, True):
+        held = rng.integers(0, cols + 1, R)
+        lengths, holders, shared = held * P - rng.integers(0, P, R) * (held > 0), np.full(R, -1), np.zeros(R, dtype=np.int64)
+        tables, next_page = np.full((R, cols), -1), 0
+        for r in range(R):
+            g = int(rng.integers(0, R))
+            n = int(rng.integers(1, cols + 1))
+            if g < r and holders[g] in (-1, g) and lengths[g] >= n * P and held[r] >= n and rng.random() < 0.7:
+                holders[r], holders[g], shared[r], shared[g] = g, g, n * P, max(shared[g], n * P)
+                tables[r, :n] = tables[g, :n]
+            else:
+                n = 0
+            tables[r, n:held[r]] = next_page + np.arange(held[r] - n)
+            next_page += held[r] - n
+        pages = rng.permutation(c.pages)
+        tables = np.where(tables < 0, -1, pages[tables])
+        for x, y in ((c.lengths, lengths), (c.holders, holders), (c.shared, shared), (c.tables, tables)):
+            x.copy_(dev(y, gpu))
+        c.free_list[:c.pages - next_page] = dev(pages[next_page:], gpu)
+        c.free_count.fill_(c.pages - next_page)
+        c.failed.zero_()
+        done = rng.random(R) < 0.6
+        self_ = np.arange(R)
+        member = (holders >= 0) & (holders != self_)
+        busy = np.zeros(R, dtype=bool)
+        busy[holders[member & ~done]] = True
+        go = done & ~busy
+        d = torch.as_tensor(done, device=gpu)
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph):
+                c.finish(d)
+            graph.replay()
+        else:
+            c.finish(done.tolist())
+        torch.cuda.synchronize()
+        assert np.array_equal(host(c.lengths), np.where(go, 0, lengths)) and np.array_equal(host(c.shared), np.where(go, 0, shared))
+        assert np.array_equal(host(c.holders), np.where(go, -1, holders))
+        assert np.array_equal(host(c.tables), np.where(go[:, None], -1, tables))
+        assert int(c.failed) == (paged.SHARED if (done & busy).any() else 0)
+        used = np.unique(host(c.tables)[host(c.tables) >= 0])
+        free = host(c.free_list)[:int(c.free_count)]
+        assert sorted(np.concatenate([used, free]).tolist()) == list(range(c.pages))

@@ -155,3 +155,25 @@ def test_more_units_than_can_be_counted_are_refused():
     for some in (dict(max_fresh=1), dict(cols=64, pitch=64), dict(dtype=_lib.PA_F32)):
         rc, message = _call("pa_paged_weights", weights(**{**many, "cols": 1 << 25, "pitch": 1 << 25, "q": None, **some}))
         assert rc == _lib.PA_E_INVALID and "null pointer" in message, (some, message)
+
+
+FINISH = {"done": 2, "holders": 8, "shared": 8, "lengths": 8, "tables": 32, "refused": 4, "first": 8, "last": 8, "workspace": 8}
+
+
+def finish(**change):
+    a = _place(_lib.PaFinishArgs(), FINISH)
+    a.R, a.page_size, a.pitch, a.cols, a.refused_bits = 2, 16, 4, 4, 16
+    return _set(a, change)
+
+
+def test_finishing_refuses_what_it_cannot_take():
+    for o, (p, n) in {f: (AT + i * STEP, n) for i, (f, n) in enumerate(FINISH.items())}.items():
+        for f, m in FINISH.items():
+            if f != o:
+                _refused("pa_page_finish", finish(**{f: p}), "overlap")
+                _refused("pa_page_finish", finish(**{f: p - (m - 1) // 4 * 4 if f != "done" else p}), "overlap")
+    for bad in (dict(R=-1), dict(R=1 << 24), dict(page_size=0), dict(cols=-1), dict(pitch=3), dict(cols=1 << 27, pitch=1 << 27),
+                *(dict([(f, None)]) for f in FINISH)):
+        rc, message = _call("pa_page_finish", finish(**bad))
+        assert rc == _lib.PA_E_INVALID and message.startswith("pa_page_finish"), (bad, message)
+    assert _call("pa_page_finish", finish(R=0))[0] == 0
