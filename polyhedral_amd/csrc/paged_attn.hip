@@ -37,7 +37,7 @@ struct PagedPlan {
   PagedPart rows, tiles;
   PagedPart pre_rows, pre_tiles;  // of the prefixes that requests share
   int64_t zero, bytes;
-  int64_t states, own, at;        // where the states of their shares begin, those of own keys, and their places
+  int64_t states, own, at, end;   // where the states of their shares begin, those of own keys, their places, and the last row's
 };
 
 // A part whose requests have at most max_tiles tiles: its grid and slots.  (The shares of all tiles are
@@ -133,7 +133,8 @@ int plan_of(const char* who, const pa_paged_args* x, bool sharing, PagedPlan* p)
   const int64_t state = 4 * state_floats(x->D), rows = sharing ? x->T * x->Hq : 0;
   p->own = p->states + state * ((int64_t)p->pre_rows.slots * kRows + (int64_t)p->pre_tiles.slots * kTileRows);
   p->at = p->own + state * rows;
-  p->bytes = p->at + (int64_t)sizeof(StatesAt) * rows;
+  p->end = p->at + (int64_t)sizeof(StatesAt) * rows;
+  p->bytes = p->end + (sharing ? 16 : 0);
   PA_CHECK_ARG(p->own - p->states < (1ll << 36) && rows * (x->D / 4) <= kMaxGroups * 256,
                "%s: %lld rows leave too many states (%lld bytes)", who, (long long)rows, (long long)(p->own - p->states));
   return PA_OK;
@@ -265,6 +266,7 @@ int run_paged(const char* who, const pa_paged_args* x, const pa_sharing* share, 
     a.pre_tiles.part = a.pre_rows.part + 4ll * p.pre_rows.slots * kRows * state_floats(x->D);
     a.own = reinterpret_cast<float*>(ws + p.own);
     a.at = reinterpret_cast<StatesAt*>(ws + p.at);
+    a.end = reinterpret_cast<int32_t*>(ws + p.end);
     if (x->dtype == PA_F32) return launch_shared_f32(a, x->D, s);
     return x->dtype == PA_BF16 ? launch_shared_bf16(a, x->D, s) : launch_shared_f16(a, x->D, s);
   }

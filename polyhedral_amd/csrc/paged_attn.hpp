@@ -77,6 +77,7 @@ struct PagedK {
   float* own;          // [T, Hq] states over the requests' own keys
   struct StatesAt* at; // [T, Hq] by place among the groups' rows
   int64_t n_states;    // floats of `states`, a multiple of 4
+  int32_t* end;        // rows of requests end here, for the merge (q_start's last entry may have fallen back)
 };
 
 // Where a row's states over its prefix are: units of 4 floats.
@@ -217,6 +218,7 @@ __device__ __forceinline__ Unit find_unit(const PagedK& a, const PagedPart& p, c
     total += wave_total((float)w.tiles * (float)w.blocks);
     if (BM == kTileRows) few += wave_total((float)w.few);
   }
+  if (PART == kOwn && BM == kRows && id == 0 && lane == 0) *a.end = end;
   // Blocks of a share: all of the part's work over `shares` (rounded up, so the units stay within shares
   // + tiles Hkv, which the grid is sized for).  Two work-groups run per CU, so 1024 shares of few rows are
   // two rounds, which suits long lists of uneven lengths (64 requests of 300 to 8192 in one round of

@@ -80,10 +80,10 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const PagedK a) {
   const int64_t id = ONE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * LOTS + lot;
   const int32_t i = imin((int32_t)(id / Hq), a.T - 1), head = (int32_t)(id % Hq);
   // (all on their way at once)
-  const int32_t last = a.share.start[a.R], last_q = a.q_start[a.R], tok = a.share.rows[i];
+  const int32_t last = a.share.start[a.R], end = *a.end, tok = a.share.rows[i];
   StatesAt at = a.at[(int64_t)i * Hq + head];
   // (a sharing of another step: rows past the requests' last stay, and states are read from within their memory)
-  if (id >= (int64_t)imin(imax(last, 0), a.T) * Hq || tok < 0 || tok >= imin(imax(last_q, 0), a.T)) return;
+  if (id >= (int64_t)imin(imax(last, 0), a.T) * Hq || tok < 0 || tok >= end) return;
   if (at.n < 0 || at.n > (1 << 20) || ((int64_t)at.first + (int64_t)at.step * imax(at.n - 1, 0) + STATE) * 4 > a.n_states) at.n = 0;
   const f32x4* state = reinterpret_cast<const f32x4*>(a.states) + at.first;
   const f32x4* own = reinterpret_cast<const f32x4*>(a.own) + ((int64_t)tok * Hq + head) * STATE;

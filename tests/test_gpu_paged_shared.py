@@ -282,6 +282,26 @@ def test_offsets_past_32_bits(gpu):
     assert torch.equal(o, want) and torch.equal(lse, wl)
 
 
+@pytest.mark.parametrize("dtype,D,fresh", [(torch.bfloat16, 128, 1), (torch.float16, 64, 40), (torch.float32, 64, 3)])
+@pytest.mark.parametrize("members", [9, 80, 1200])
+def test_starts_that_fall_back(gpu, dtype, D, fresh, members):
+    """Taken alike by the plan, both parts of the attention and the merge: as the starts that they stand for."""
+    if members == 1200 and fresh > 3:
+        fresh = 3
+    rng = np.random.default_rng(members)
+    rows = [(int(n), int(n) + int(x)) for n, x in zip(rng.integers(0, fresh + 1, members), rng.integers(1, 60, members))]
+    b = Shared(gpu, dtype, D, 16, 4, 2, [(96, rows[::2]), (32, rows[1::2])], [(fresh, 50), (0, 20), (1, 3)], seed=members)
+    want, wl = b.check(pm.Causal())
+    starts, b.q_start = b.q_start, falling(b.q_start, b.n, rng)
+    args = b.args()
+    sharing = paged.sharing(args[1], args[2], dev(b.holders, gpu), dev(b.shared, gpu), 16, b.T)
+    for g, w in zip(sharing, so.sharing(b.lengths, starts, b.holders, b.shared, 16, b.T)):
+        assert np.array_equal(host(g), w)
+    o, lse = torch.full_like(want, 7.0), torch.full_like(wl, 7.0)
+    paged.shared_attention(b.q, b.k, b.v, *args, sharing, pm.Causal(), out=o, lse=lse)
+    assert torch.equal(o, want) and torch.equal(lse, wl)
+
+
 @pytest.mark.parametrize("most", [0, 1, 40, 10000])
 def test_any_hint_gives_right_results(gpu, most):
     Shared(gpu, torch.bfloat16, 128, 32, 8, 2, [(320, [(1, 5), (90, 100), (3, 40)])], [(1, 90), (33, 33)]).check(pm.Causal(), max_fresh=most)
