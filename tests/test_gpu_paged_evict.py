@@ -9,7 +9,7 @@ from polyhedral_amd.polyattn import masks as pm
 from polyhedral_amd.spec import MaskSpec
 from tests import shared_oracle as so
 from tests.test_gpu_paged import RAGGED, TYPES, Batch
-from tests.test_gpu_paged_shared import MASKS, dev, f64, host
+from tests.test_gpu_paged_shared import MASKS, dev, f64, falling, host
 
 pytestmark = pytest.mark.gpu
 
@@ -94,6 +94,32 @@ def test_weights_of_many_requests_and_long_ones(gpu):
         _weigh(Batch(gpu, torch.bfloat16, 64, 16, 4, 2, sizes, seed=R), pm.Causal())
     _weigh(Batch(gpu, torch.bfloat16, 128, 64, 4, 1, [(1, 20001), (1, 3)]), pm.Causal())
     _weigh(Batch(gpu, torch.float16, 64, 64, 8, 2, [(300, 9000), (1, 3000)]), pm.Causal())
+
+
+@pytest.mark.parametrize("dtype,D", TYPES)
+@pytest.mark.parametrize("R", [65, 130, 300])
+def test_weights_of_chunks_among_many_requests(gpu, dtype, D, R):
+    """More requests than lanes: chunks before and behind the 64th, whose shares are merged, tokens beside them, some of
+    none; and the same bits again."""
+    rng = np.random.default_rng(R)
+    sizes = [(int(n), int(n + x)) for n, x in zip(rng.integers(0, 3, R), rng.integers(1, 60, R))]
+    for r in {0, 5, 63, 64, R - 1, int(rng.integers(65, R + 1)) - 1, int(rng.integers(R))}:
+        n = int(rng.integers(33, 90))
+        sizes[r] = (n, n + int(rng.integers(0, 300)))
+    sizes[62], sizes[R - 1] = (500, 700), (610, 610)
+    b = Batch(gpu, dtype, D, 16, 8, 2, sizes, seed=R)
+    first = np.where(rng.random(R) < 0.3, rng.integers(0, 50, R), 0)
+    got = _weigh(b, pm.Causal(), first=first)
+    assert torch.equal(_weigh(b, pm.Causal(), first=first), got)
+    _weigh(b, pm.SinksWindow(3, 100))
+    # starts that fall back are taken as the ones that they stand for
+    t, n, s = b.dev()
+    lse, scores = torch.empty(b.T, b.Hq, device=gpu), [torch.zeros(b.pages, b.Hkv, b.P, device=gpu) for _ in range(2)]
+    paged.attention(b.q, b.k, b.v, t, n, s, pm.Causal(), lse=lse)
+    lse[int(b.n.sum()):] = NAN
+    for x, at in zip(scores, (s, dev(falling(b.q_start, b.n, rng), gpu))):
+        paged.weights(b.q, b.k, t, n, at, lse, x, pm.Causal())
+    assert torch.equal(*scores)
 
 
 def test_weights_sum_to_the_rows(gpu):
@@ -304,6 +330,26 @@ def test_evict_against_numpy(gpu, dtype, D, P, layers, keep, first):
         assert np.array_equal(f64(x).reshape(np.array(w).shape), np.array(w))
     paged.evict(choice.kept, k2, v2, None, t, n, fd)        # without scores
     assert torch.equal(k2, k) and torch.equal(v2, v)
+
+
+@pytest.mark.parametrize("dtype,D", TYPES)
+@pytest.mark.parametrize("R,H,layers", [(16, 4, 2), (9, 7, 3), (16, 8, 2), (33, 8, 2), (64, 2, 4), (511, 1, 1), (43, 3, 4)])
+def test_evict_of_many_heads(gpu, dtype, D, R, H, layers):
+    """From work-groups that cut rows into slices to those of 512 threads: R H layers on both sides of each rule."""
+    P, keep = 16, 33
+    rng = np.random.default_rng(R)
+    g = torch.Generator().manual_seed(R)
+    lengths = rng.integers(1, 4 * keep, R)
+    tables, pages = _pool(rng, lengths, P)
+    k, v = (torch.randn(layers, pages, H, P, D, generator=g).to(dtype).to(gpu) for _ in range(2))
+    scores = torch.rand(layers, pages, H, P, generator=g).to(gpu)
+    f = rng.integers(0, 9, R)
+    t, n, fd = dev(tables, gpu), dev(lengths, gpu), dev(f, gpu)
+    choice = paged.choose(scores, t, n, keep, 5, None, fd)
+    kept = host(choice.kept)
+    want = [[so.evict(kept[i], x[i], tables, lengths, f) for i in range(layers)] for x in (f64(k), f64(v), f64(scores))]
+    for x, w in zip(paged.evict(choice.kept, k, v, scores, t, n, fd), want):
+        assert np.array_equal(f64(x), np.array(w))
 
 
 def test_evict_of_odd_lists(gpu):

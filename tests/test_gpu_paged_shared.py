@@ -282,6 +282,21 @@ def test_offsets_past_32_bits(gpu):
     assert torch.equal(o, want) and torch.equal(lse, wl)
 
 
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_steps_of_many_rows(gpu, dtype, D):
+    """More rows times heads than have a work-group each to merge them: tokens, drafts and chunks."""
+    groups = [(320, [(300, 300), (33, 40), (1, 7), (64, 300)]), (64, [(257, 260), (1, 1), (5, 5)]), (160, _tokens(20, 1, 90, 3))]
+    b = Shared(gpu, dtype, D, 32, 16, 4, groups, [(70, 90), (1, 400), (3, 3)])
+    assert b.T * b.Hq > 8192
+    o, lse = b.check(pm.Causal())
+    again = b.run(pm.Causal())
+    assert torch.equal(again[0], o) and torch.equal(again[1], lse)
+    b.check(pm.SinksWindow(20, 100))
+    b = Shared(gpu, dtype, D, 16, 16, 16, [(96, _tokens(700, 1, 30, 5)), (32, _tokens(3, 1, 9, 2))], seed=2)
+    assert b.T * b.Hq > 8192
+    b.check(pm.Causal())
+
+
 @pytest.mark.parametrize("dtype,D,fresh", [(torch.bfloat16, 128, 1), (torch.float16, 64, 40), (torch.float32, 64, 3)])
 @pytest.mark.parametrize("members", [9, 80, 1200])
 def test_starts_that_fall_back(gpu, dtype, D, fresh, members):
