@@ -250,17 +250,14 @@ __device__ __forceinline__ void weigh_blocks(const WeightsK& a, int32_t id, int3
           float old;       // score of key 16 (q16 / 4) + 4 g + q16 % 4 of the block (NS = 2: of q16 < 8)
           float* to;       // its place, null where it is none of ours
           int32_t key;     // the block's first
-          uint32_t there;  // segments with a page
         };
         auto fetch = [&](int b, Data& d) __attribute__((always_inline)) {
           if (b % PER == 0) take_pages(b / PER);
           const int l0 = NS * (b % PER);
           d.key = list.block(i0 + b) << LG;
-          d.there = 0u;
 #pragma unroll
           for (int t = 0; t < NS; ++t) {
             const int32_t page = __builtin_amdgcn_readlane(c_page, l0 + t);
-            d.there |= page >= 0 ? 1u << t : 0u;
             const int64_t off = (int64_t)imax(page, 0) * a.c_sp + (int64_t)((d.key + 16 * t) & ((1 << a.page_lg) - 1)) * a.c_sn;
 #pragma unroll
             for (int kc = 0; kc < NK; ++kc) d.k[t][kc] = *reinterpret_cast<const u32x4*>(kbase + off + koff + 64 * kc);
