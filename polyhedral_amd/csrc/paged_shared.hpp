@@ -7,8 +7,8 @@
 // requests behind 8192 tokens 41 and 29 us, and 24 us of one row's 64 shares behind 65536.)
 //
 // What bounds it, at 32 heads on 8 of 128 in bf16: behind long prefixes HBM (32 requests behind 65536, 358 MB: 90
-// us of 104, 4.0 TB/s), with chunks the tiles' MFMAs (12 of 100 to 600 tokens behind 12000 to 16384: 0.94 ms,
-// 0.96 PFLOP/s), else what is outside the steps: 64 requests behind 8192 tokens, whose prefix is 176 units of 12
+// us of 104, 4.0 TB/s), with chunks the tiles' MFMAs (12 of 100 to 600 tokens behind 12000 to 16384: the call
+// 0.95 to 0.98 ms, 0.92 to 0.96 PFLOP/s), else what is outside the steps: 64 requests behind 8192 tokens, whose prefix is 176 units of 12
 // steps, 43 us, then 7 of the merge, 5 of the plan and the launches' gaps, where its 128 MB take 26.
 #pragma once
 
@@ -107,8 +107,11 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const PagedK a) {
     a.lse[(int64_t)tok * a.lse_st + (int64_t)head * a.lse_sh] = s.l == 0.f ? -INFINITY : (s.m + (log2f(s.l) + s.rest)) * kLn2;
 }
 
-// Rows up to which each has a work-group of its own to merge it.
-constexpr int64_t kMergeRows = 8192;
+// Rows (of all heads) up to which each has a work-group of its own to merge it.  The call with one each / with several
+// rows to a work-group, tokens of 32 heads on 8 of 128 in bf16: 1024 rows 24.0 / 23.8 us behind 2048 tokens and 36.7 / 41
+// behind 16384, 2048 rows 32.9 / 32.8 and 54 / 57, 4096 rows 59.5 / 57.1 and 98.3 / 97.3, 8192 rows 130 / 123 and 184 /
+// 178, 32768 of chunks 103 / 77 and 313 / 286; 2192 of 16 heads of 64 in f16 27.7 / 28.0.
+constexpr int64_t kMergeRows = 2560;
 
 template <typename T, int D>
 int launch_shared_t(const PagedK& a, hipStream_t s) {
