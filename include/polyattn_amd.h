@@ -597,8 +597,10 @@ int pa_paged_attn(const pa_paged_args* args, void* stream);
  * of rows (their places in the packed step) and positions (lengths[r] - n + i); prefix[g] = the
  * least that they share, low[g] / high[g] = their least and largest position, first[r] = prefix[g]
  * for each of them.  A prefix that one request alone has tokens for is no group: start[g] = start[g +
- * 1], prefix[g] = low[g] = high[g] = 0, and first[r] = 0.  Rows from start[R] on are -1.  start [R +
- * 1]; prefix, low, high, first [R]; rows, positions [T]; workspace int32 [8 R].  The outputs and the
+ * 1], prefix[g] = low[g] = high[g] = 0, and first[r] = 0.  Rows from start[R] on are -1.  The length of a
+ * request that shares holds its new tokens and lies within its table (whose reach this call does not know, where
+ * pa_paged_attn takes a longer one as that).  start [R + 1]; prefix, low, high, first [R]; rows, positions [T];
+ * workspace int32 [8 R].  The outputs and the
  * workspace share no memory with each other or with an input.
  *
  * pa_page_finish: which of the requests with done[r] != 0 can give their pages back, in a cache whose requests share
@@ -620,7 +622,7 @@ int pa_paged_attn(const pa_paged_args* args, void* stream);
  * with lse [T, Hq] of their attention (-inf: the row has no weight).  Key t's score is row t %
  * page_size of page tables[r][t / page_size]: float at scores + page * s_sp + head * s_sh + row.  Keys
  * without a page and scores of no request's keys are left as they are; no key from first[r] on is
- * in two requests' tables.  first may be NULL (0).  max_fresh: the most new tokens of a request (a hint, as
+ * in two requests' tables, or twice in one.  first may be NULL (0).  max_fresh: the most new tokens of a request (a hint, as
  * in pa_paged_attn).  Every key's sum is taken in a fixed order.  (In 16 bits, with max_fresh of more than 32 rows:
  * requests times heads times 256-key groups of a table's reach stay below 2^31.)  scores shares no memory with an input or
  * itself.  workspace as in pa_paged_attn, its sizes (which may be 0) from pa_weights_workspace.
@@ -639,7 +641,8 @@ int pa_paged_attn(const pa_paged_args* args, void* stream);
  * first[r] + j, in place: kept as pa_choose_keys gives it, or any list with kept[j] >= first[r] + j;
  * entries below that or past the table or without a page at either place move nothing.  K and V of
  * layer l: l * c_sl elements on.  scores may be NULL.  Rows of k, v and scores share no memory with
- * each other or with an input; no place from first[r] on is in two requests' tables. */
+ * each other or with an input; no place from first[r] on is in two requests' tables, or
+ * twice in one. */
 typedef struct pa_share_args {
   const int32_t* lengths;
   const int32_t* q_start;

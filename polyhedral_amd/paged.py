@@ -359,7 +359,7 @@ def prepare_sharing(lengths, q_start, holders, shared, page_size, tokens, out=No
 
     lengths, q_start: as in prepare_attention.  holders, shared: int32 [R], the request whose first
     shared[r] tokens request r shares (-1: none), with that request's pages in its own table; only whole
-    pages are shared.  A request may be its own holder.  A prefix that one request alone has tokens for
+    pages are shared.  The length of a request that shares holds its new tokens and lies within its table.  A request may be its own holder.  A prefix that one request alone has tokens for
     is no group.  tokens: rows of the packed step.  out: a Sharing to write into."""
     _page_size(page_size)
     R = lengths.shape[0] if lengths.dim() == 1 else -1
@@ -680,7 +680,8 @@ class PagedKVCache:
     def share(self, holder, members, tokens):
         """Requests ``members`` (a list; without tokens so far) begin with the first ``tokens`` tokens of
         request ``holder``, whole pages that they read and do not copy.  The holder may go on; it keeps
-        these pages until the members have finished.  Where that cannot be (the holder has fewer tokens, or
+        these pages, neither weighed nor evicted, until it finishes, which it can once the members have.  Members of
+        one holder are read together as far as the one that shares least.  Where that cannot be (the holder has fewer tokens, or
         has given some of their pages back, or begins with fewer of another's itself; a member is not empty)
         nothing happens, and ``check`` says so.  Not to be captured; steps captured before the first call read
         a shared prefix as often as there are requests."""
