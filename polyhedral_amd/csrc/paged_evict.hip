@@ -6,7 +6,7 @@
 // time, each from counts in LDS of the keys that agree so far; where a bin's keys just make up the number the
 // search ends, else the keys equal to the bound go by place.  Ranks among the kept are sums over the waves.
 // What bounds it: for one layer of a few requests the launch and its trips to memory (4 requests of 1000, 4
-// heads: 5.3 us), for many the counts' and ranks' instructions beside the barriers of three work-groups a CU
+// heads: 5.5 us), for many the counts' and ranks' instructions beside the barriers of three work-groups a CU
 // (8 layers of 32 requests of 1500 to 16384, 8 heads, 51 MB: 43 us, of which the loads 16).
 //
 // pa_evict_rows: kept[j] >= first + j, so the row that place first + j gives up was read for some j' <= j: a

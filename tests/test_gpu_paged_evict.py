@@ -1,5 +1,7 @@
 """Keys that are weighed, chosen and evicted (paged.weights, choose, evict, PagedKVCache.weigh and evict)
 against tests/shared_oracle.py."""
+import random
+
 import numpy as np
 import pytest
 import torch
@@ -7,6 +9,7 @@ import torch
 from polyhedral_amd import paged
 from polyhedral_amd.polyattn import masks as pm
 from polyhedral_amd.spec import MaskSpec
+from tests import paged_oracle as po
 from tests import shared_oracle as so
 from tests.test_gpu_paged import RAGGED, TYPES, Batch
 from tests.test_gpu_paged_shared import MASKS, dev, f64, falling, host
@@ -673,3 +676,74 @@ def test_captured_steps_and_evictions(gpu):
         for name in ("lengths", "tables", "k", "v", "scores", "free_count"):
             assert torch.equal(getattr(a, name), getattr(e, name)), (i, name)
     e.check()
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_lives_of_a_cache_at_random(gpu, seed):
+    """Steps, shares (some refused), evictions and finishes in any order, against rows on the host: attention, scores,
+    keys, holders, what check knows, and no page twice or lost."""
+    rng = random.Random(seed)
+    for _ in range(10):
+        R, P, H, G, D = rng.randint(1, 9), rng.choice([16, 32]), rng.choice([1, 2]), rng.choice([1, 4]), 64
+        dtype, cap = rng.choice([torch.float32, torch.bfloat16]), rng.choice([100, 300])
+        c = paged.PagedKVCache(R, cap, R * -(-cap // P) + 2, H, D, dtype, P, 1, gpu, weigh=True)
+        rows, holder, shared, failed, log = [np.zeros((0, H, D))] * R, [-1] * R, [0] * R, 0, []
+        for _ in range(rng.randint(5, 25)):
+            what, n = rng.choice(["step"] * 5 + ["share"] * 2 + ["evict", "finish"]), [len(x) for x in rows]
+            if what == "step":
+                fresh = [min(rng.choice([0, 1, 1, 2, 5, rng.randint(0, 60)]), c.max_length - n[r]) for r in range(R)]
+                m, T = sum(fresh), sum(fresh) + rng.randint(1, 2)
+                step = c.begin(fresh, T)
+                kn, vn, q = (torch.randn(T, x, D, generator=torch.Generator().manual_seed(m)).to(dtype).to(gpu) for x in (H, H, H * G))
+                c.append(kn, vn, step)
+                lse = torch.zeros(T, H * G, device=gpu)
+                o = c.attend(q, pm.Causal(), step, lse=lse, out=torch.zeros_like(q))
+                at = host(c.tables), host(step.lengths), host(step.q_start)
+                want, _, eo, _ = po.attention(f64(q), f64(c.k[0]), f64(c.v[0]), *at, lambda x, y: y <= x, D ** -0.5, dtype)
+                assert (np.abs(f64(o)[:m] - want[:m]) <= eo[:m]).all(), log
+                want, bound = so.weights(f64(q), f64(c.k[0]), *at, f64(lse), f64(c.scores[0]), lambda x, y: y <= x, D ** -0.5,
+                                         np.array(shared))
+                c.weigh(q, lse, pm.Causal(), step)
+                assert (np.abs(f64(c.scores[0]) - want) <= bound).all(), log
+                rows = [np.concatenate([x, f64(kn)[a:b]]) for x, a, b in zip(rows, at[2], at[2][1:])]
+                log.append((what, fresh))
+            elif what == "share":
+                h, t = rng.randrange(R), P * rng.randint(1, max(c.max_length // P // 2, 1))
+                members = [x for x in range(R) if x != h and rng.random() < 0.4]
+                c.share(h, members, t)
+                root = holder[h] if holder[h] not in (-1, h) else h
+                can = n[h] >= t and (root == h or shared[h] >= t)
+                for m in members:
+                    if can and n[m] == 0 and holder[m] < 0:
+                        rows[m], holder[m], shared[m] = rows[h][:t], root, t
+                        holder[root], shared[root] = root, max(shared[root], t)
+                    else:
+                        failed |= paged.SHARED
+                log.append((what, h, members, t))
+            elif what == "evict":
+                keep, sinks = rng.randint(1, 60), rng.randint(0, 20)
+                recent, limit = rng.randint(0, keep), keep + rng.randint(0, 30)
+                first = np.maximum(shared, sinks)
+                kept, after = so.choose(f64(c.scores[0]), host(c.tables), np.array(n), keep, recent, limit, first)
+                c.evict(keep, recent, limit, sinks)
+                for r in np.flatnonzero(after != n):
+                    rows[r] = np.concatenate([rows[r][:first[r]], np.stack([rows[r][kept[r, h], h] for h in range(H)], axis=1)])
+                log.append((what, keep, recent, limit, sinks))
+            else:
+                done = [rng.random() < 0.4 for _ in range(R)]
+                busy = [any(holder[m] == r != m and not done[m] for m in range(R)) for r in range(R)]
+                c.finish(done)
+                for r in np.flatnonzero(done):
+                    if busy[r]:
+                        failed |= paged.SHARED
+                    else:
+                        rows[r], holder[r], shared[r] = rows[r][:0], -1, 0
+                log.append((what, done))
+            tables, lengths = host(c.tables), host(c.lengths)
+            assert lengths.tolist() == [len(x) for x in rows], log
+            assert host(c.holders).tolist() == holder and host(c.shared).tolist() == shared and int(c.failed) == failed, log
+            for r, L in enumerate(lengths):
+                t = np.arange(L)
+                assert np.array_equal(f64(c.k[0])[tables[r, t // P], :, t % P], rows[r]), log
+            free = host(c.free_list)[:int(c.free_count)]
+            assert sorted(np.concatenate([np.unique(tables[tables >= 0]), free]).tolist()) == list(range(c.pages)), log
